@@ -1,0 +1,410 @@
+// Segment attention: plans and C entry points (declarations: include/gatgpu.h).
+#include "attention.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <memory>
+#include <new>
+#include <numeric>
+#include <string>
+
+struct gatgpu_attention {
+    gatgpu_ctx* ctx = nullptr;
+    gatgpu_attention_shape shape{};
+    std::vector<gatgpu::AttnSeg> segs;
+    uint64_t rows = 0, dist_bytes = 0;
+    bool shared_keys = false;  // key rows of two segments overlap
+    // Tables on the device: segments; tiles of the forward, the query and the key pass; joined tiles.
+    gatgpu::DevBuf dsegs, dfwd, dbwd_q, dbwd_kv, djoin;
+    uint64_t nfwd = 0, nbwd_q = 0, nbwd_kv = 0, njoin = 0;
+    int wfwd = 1, wbwd_q = 1, wbwd_kv = 1;  // waves a block
+    bool split = false;
+    bool spread = false;
+};
+
+namespace gatgpu {
+
+DeviceGuard::DeviceGuard(int device) {
+    if (hipGetDevice(&before) != hipSuccess) before = -1;
+    if (before != device) ok = hipSetDevice(device) == hipSuccess;
+    else before = -1;
+}
+DeviceGuard::~DeviceGuard() {
+    if (before >= 0) (void)hipSetDevice(before);
+}
+
+// A call must not reach a kernel with an array of the host or of another GPU.
+int check_device_array(gatgpu_ctx* c, const void* p, const char* name) {
+    hipPointerAttribute_t at{};
+    if (hipPointerGetAttributes(&at, p) != hipSuccess || (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged)) {
+        (void)hipGetLastError();
+        return fail(c, GATGPU_EINVAL, std::string(name) + " is not device memory");
+    }
+    if (at.type == hipMemoryTypeDevice && at.device != c->device)
+        return fail(c, GATGPU_EINVAL, std::string(name) + " is not on the context's device");
+    return GATGPU_OK;
+}
+
+}  // namespace gatgpu
+
+namespace {
+
+using namespace gatgpu;
+
+constexpr uint64_t kMaxLen = uint64_t(1) << 30, kMaxRow = uint64_t(1) << 44, kMaxTasks = uint64_t(1) << 30;
+
+// Keys that query i of a segment sees by position.
+uint32_t seen(const gatgpu_attention_shape& sh, const AttnSeg& s, int64_t i) {
+    if (sh.mask == GATGPU_MASK_FULL) return s.k_len;
+    const int64_t pos = i + int64_t(s.k_len) - int64_t(s.q_len);
+    return uint32_t(std::min<int64_t>(s.k_len, std::max<int64_t>(pos + 1, s.prefix)));
+}
+
+// True if two of the ranges [begin, begin + len) share a row.
+bool overlap(const std::vector<AttnSeg>& segs, bool keys) {
+    std::vector<std::pair<uint64_t, uint64_t>> r;
+    for (const AttnSeg& s : segs) {
+        const uint64_t at = keys ? s.k_begin : s.q_begin, len = keys ? s.k_len : s.q_len;
+        if (len) r.emplace_back(at, at + len);
+    }
+    std::sort(r.begin(), r.end());
+    for (size_t i = 1; i < r.size(); ++i)
+        if (r[i].first < r[i - 1].second) return true;
+    return false;
+}
+
+int upload(gatgpu_ctx* c, DevBuf& b, const void* p, size_t bytes) {
+    HIPCHECK(c, b.ensure(bytes));
+    if (bytes) HIPCHECK(c, hipMemcpyAsync(b.p, p, bytes, hipMemcpyHostToDevice, c->stream));
+    return GATGPU_OK;
+}
+
+// Long tiles first: the last blocks to start are then short ones.
+void longest_first(std::vector<AttnTask>& t) {
+    std::stable_sort(t.begin(), t.end(), [](const AttnTask& x, const AttnTask& y) { return x.hi - x.lo > y.hi - y.lo; });
+}
+
+int build(gatgpu_attention* P) {
+    gatgpu_ctx* c = P->ctx;
+    const gatgpu_attention_shape& sh = P->shape;
+    const uint64_t group = uint64_t(sh.heads / sh.kv_heads), kvh = uint64_t(sh.kv_heads), cus = uint64_t(c->cus);
+    uint64_t q4 = 0, k4 = 0, longest = 0;  // blocks of four waves, by rows and by keys
+    for (const AttnSeg& s : P->segs) {
+        q4 += (s.q_len * group + 127) / 128;
+        k4 += (uint64_t(s.k_len) + 127) / 128;
+        if (s.q_len) longest = std::max<uint64_t>(longest, s.k_len);
+    }
+    const auto full = [&](uint64_t total, uint64_t tiles) {
+        // Four waves a block where the chip is filled all the same and three of four waves have rows.
+        return tiles * kvh >= 2 * cus && total >= tiles * 96;
+    };
+    uint64_t rows = 0, keys = 0;
+    for (const AttnSeg& s : P->segs) rows += s.q_len * group, keys += s.k_len;
+    P->wfwd = P->wbwd_q = full(rows, q4) ? 4 : 1;
+    P->wbwd_kv = full(keys, k4) ? 4 : 1;
+
+    std::vector<AttnTask> fwd, bq, bk, join;
+    const auto q_tiles = [&](std::vector<AttnTask>& out, uint32_t tile) {
+        for (size_t s = 0; s < P->segs.size(); ++s) {
+            const AttnSeg& g = P->segs[s];
+            const uint64_t n = g.q_len * group;
+            for (uint64_t r = 0; r < n; r += tile) {
+                const uint64_t last = std::min<uint64_t>(n, r + tile) - 1;
+                out.push_back({uint32_t(s), uint32_t(r), 0, seen(sh, g, int64_t(last / group))});
+            }
+        }
+    };
+    q_tiles(fwd, 32u * uint32_t(P->wfwd));
+    q_tiles(bq, 32u * uint32_t(P->wbwd_q));
+    // Few tiles over long rows of keys: each tile's keys are cut into ranges that fill the chip.
+    uint64_t work = 0;
+    for (const AttnTask& t : fwd) work += t.hi;
+    if (P->wfwd == 1 && !fwd.empty() && fwd.size() * kvh < 4 * cus && longest > 256) {
+        const uint64_t want = std::max<uint64_t>(1, 8 * cus / kvh);  // tasks
+        const uint64_t chunk = std::max<uint64_t>(128, (work / want + 31) / 32 * 32);
+        std::vector<AttnTask> cut;
+        for (const AttnTask& t : fwd) {
+            join.push_back({t.seg, t.at, uint32_t(cut.size()), 0});
+            uint64_t lo = 0;
+            do {
+                const uint64_t hi = std::min<uint64_t>(t.hi, lo + chunk);
+                cut.push_back({t.seg, t.at, uint32_t(lo), uint32_t(hi)});
+                lo = hi;
+            } while (lo < t.hi);
+            join.back().hi = uint32_t(cut.size()) - join.back().lo;
+        }
+        if (cut.size() > fwd.size()) {
+            fwd.swap(cut);
+            P->split = true;
+        } else {
+            join.clear();
+        }
+    }
+    for (size_t s = 0; s < P->segs.size(); ++s) {
+        const AttnSeg& g = P->segs[s];
+        const uint32_t n = uint32_t(g.q_len * group);
+        for (uint64_t k = 0; k < g.k_len; k += 32u * uint32_t(P->wbwd_kv)) {
+            uint32_t lo = 0;  // first row that sees key k
+            if (sh.mask != GATGPU_MASK_FULL && k >= g.prefix) {
+                const int64_t first = int64_t(k) - (int64_t(g.k_len) - int64_t(g.q_len));
+                lo = uint32_t(std::min<int64_t>(g.q_len, std::max<int64_t>(0, first)) * int64_t(group));
+            }
+            bk.push_back({uint32_t(s), uint32_t(k), lo, n});
+        }
+    }
+    if (std::max({fwd.size(), bq.size(), bk.size(), join.size()}) * kvh >= kMaxTasks)
+        return fail(c, GATGPU_EOVERFLOW, "too many tiles");
+    if (!P->split) longest_first(fwd);
+    longest_first(bq);
+    longest_first(bk);
+    // Rows of long segments: an XCD keeps few heads' keys in its L2; short segments: whole lines.
+    P->spread = longest > 256;
+    P->nfwd = fwd.size();
+    P->nbwd_q = bq.size();
+    P->nbwd_kv = bk.size();
+    P->njoin = join.size();
+    if (int r = upload(c, P->dsegs, P->segs.data(), P->segs.size() * sizeof(AttnSeg))) return r;
+    if (int r = upload(c, P->dfwd, fwd.data(), fwd.size() * sizeof(AttnTask))) return r;
+    if (int r = upload(c, P->dbwd_q, bq.data(), bq.size() * sizeof(AttnTask))) return r;
+    if (int r = upload(c, P->dbwd_kv, bk.data(), bk.size() * sizeof(AttnTask))) return r;
+    if (int r = upload(c, P->djoin, join.data(), join.size() * sizeof(AttnTask))) return r;
+    HIPCHECK(c, hipStreamSynchronize(c->stream));
+    return GATGPU_OK;
+}
+
+uint64_t pad256(uint64_t b) { return (b + 255) / 256 * 256; }
+uint64_t part_bytes(const gatgpu_attention* P) {
+    return P->split ? pad256(P->nfwd * uint64_t(P->shape.kv_heads) * 32 * uint64_t(attention_width(P->shape.dim)) * 4) : 0;
+}
+uint64_t forward_bytes(const gatgpu_attention* P) {
+    return P->split ? part_bytes(P) + P->nfwd * uint64_t(P->shape.kv_heads) * 32 * 8 : 0;
+}
+uint64_t delta_bytes(const gatgpu_attention* P) { return pad256(P->rows * uint64_t(P->shape.heads) * 4); }
+uint64_t backward_bytes(const gatgpu_attention* P) {
+    const gatgpu_attention_shape& sh = P->shape;
+    return delta_bytes(P) + (sh.bias == GATGPU_BIAS_TABLE ? P->nbwd_q * uint64_t(sh.heads) * uint64_t(sh.buckets) * 4 : 0);
+}
+
+// A matrix of rows: there, aligned, wide enough, on the device.
+int check_rows(gatgpu_ctx* c, const char* name, const void* p, uint64_t stride, uint64_t width, int size) {
+    if (!p) return fail(c, GATGPU_EINVAL, std::string("null ") + name);
+    if (reinterpret_cast<uintptr_t>(p) % 16 || stride * uint64_t(size) % 16)
+        return fail(c, GATGPU_EINVAL, std::string(name) + " and its stride must be 16-byte aligned");
+    if (stride < width || stride > kMaxRow) return fail(c, GATGPU_EINVAL, std::string(name) + " has a bad row stride");
+    return check_device_array(c, p, name);
+}
+int check_floats(gatgpu_ctx* c, const char* name, const void* p) {
+    if (!p) return fail(c, GATGPU_EINVAL, std::string("null ") + name);
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(c, GATGPU_EINVAL, std::string(name) + " must be 4-byte aligned");
+    return check_device_array(c, p, name);
+}
+
+int check_call(gatgpu_attention* P, const gatgpu_attention_io* io, void* ws, uint64_t bytes, uint64_t need) {
+    gatgpu_ctx* c = P->ctx;
+    if (!io) return fail(c, GATGPU_EINVAL, "null arrays");
+    const gatgpu_attention_shape& sh = P->shape;
+    const int size = sh.precision == GATGPU_BF16 ? 2 : 4;
+    const uint64_t qw = uint64_t(sh.heads) * uint64_t(sh.dim), kw = uint64_t(sh.kv_heads) * uint64_t(sh.dim);
+    if (int r = check_rows(c, "q", io->q, io->q_stride, qw, size)) return r;
+    if (int r = check_rows(c, "k", io->k, io->k_stride, kw, size)) return r;
+    if (int r = check_rows(c, "v", io->v, io->v_stride, kw, size)) return r;
+    if (int r = check_rows(c, "out", io->out, io->out_stride, qw, size)) return r;
+    if (sh.bias != GATGPU_BIAS_NONE)
+        if (int r = check_floats(c, "bias", io->bias)) return r;
+    if (sh.bias == GATGPU_BIAS_TABLE && P->dist_bytes)
+        if (int r = check_rows(c, "dist", io->dist, 16, 16, 1)) return r;
+    if (io->rest) {
+        if (sh.precision != GATGPU_BF16) return fail(c, GATGPU_EINVAL, "rest belongs to bf16 outputs");
+        if (int r = check_rows(c, "rest", io->rest, io->out_stride, qw, size)) return r;
+    }
+    if (need) {
+        if (bytes < need) return fail(c, GATGPU_EINVAL, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
+        if (int r = check_rows(c, "workspace", ws, 16, 16, 1)) return r;
+    }
+    return GATGPU_OK;
+}
+
+AttnArgs make_args(const gatgpu_attention* P, const gatgpu_attention_io* io) {
+    const gatgpu_attention_shape& sh = P->shape;
+    AttnArgs a;
+    a.segs = P->dsegs.as<AttnSeg>();
+    a.heads = sh.heads;
+    a.kv_heads = sh.kv_heads;
+    a.group = sh.heads / sh.kv_heads;
+    a.dim = sh.dim;
+    a.causal = sh.mask == GATGPU_MASK_PREFIX;
+    a.bias_kind = sh.bias;
+    a.buckets = sh.buckets;
+    a.spread = P->spread;
+    a.scale = sh.scale;
+    a.cap = sh.cap;
+    a.q = io->q;
+    a.k = io->k;
+    a.v = io->v;
+    a.qs = io->q_stride;
+    a.ks = io->k_stride;
+    a.vs = io->v_stride;
+    a.bias = sh.bias == GATGPU_BIAS_NONE ? nullptr : io->bias;
+    a.dist = sh.bias == GATGPU_BIAS_TABLE ? io->dist : nullptr;
+    a.out = io->out;
+    a.rest = io->rest;
+    a.os = io->out_stride;
+    a.lse = io->lse;
+    return a;
+}
+
+int create(gatgpu_ctx* c, const gatgpu_attention_shape* sh, uint64_t n, const uint64_t* q_begin, const uint32_t* q_len,
+           const uint64_t* k_begin, const uint32_t* k_len, const uint32_t* prefix, gatgpu_attention** out) {
+    if (!out) return fail(c, GATGPU_EINVAL, "null output pointer");
+    *out = nullptr;
+    if (!sh) return fail(c, GATGPU_EINVAL, "null shape");
+    if (sh->precision != GATGPU_FP32 && sh->precision != GATGPU_BF16) return fail(c, GATGPU_EINVAL, "bad precision");
+    if (sh->heads < 1 || sh->heads > 64 || sh->kv_heads < 1 || sh->heads % sh->kv_heads)
+        return fail(c, GATGPU_EINVAL, "heads must be 1 to 64 and a multiple of kv_heads");
+    if (sh->dim < 8 || sh->dim > kAttnMaxDim || sh->dim % 8) return fail(c, GATGPU_EINVAL, "dim must be a multiple of 8, at most 128");
+    if (sh->mask != GATGPU_MASK_FULL && sh->mask != GATGPU_MASK_PREFIX) return fail(c, GATGPU_EINVAL, "bad mask");
+    if (sh->bias < GATGPU_BIAS_NONE || sh->bias > GATGPU_BIAS_TABLE) return fail(c, GATGPU_EINVAL, "bad bias");
+    if (sh->bias == GATGPU_BIAS_TABLE && (sh->buckets < 1 || sh->buckets > kAttnMaxBuckets))
+        return fail(c, GATGPU_EINVAL, "a bias table has 1 to 64 buckets");
+    if (!(sh->scale > 0.0f) || !std::isfinite(sh->scale)) return fail(c, GATGPU_EINVAL, "scale must be positive and finite");
+    if (!(sh->cap >= 0.0f) || !std::isfinite(sh->cap)) return fail(c, GATGPU_EINVAL, "cap must be 0 or positive and finite");
+    if (n && (!q_begin || !q_len || !k_begin || !k_len)) return fail(c, GATGPU_EINVAL, "null segment array");
+    if (n > kMaxTasks) return fail(c, GATGPU_EOVERFLOW, "too many segments");
+    const uint64_t group = uint64_t(sh->heads / sh->kv_heads);
+    std::unique_ptr<gatgpu_attention> P(new gatgpu_attention);
+    P->ctx = c;
+    P->shape = *sh;
+    if (sh->bias != GATGPU_BIAS_TABLE) P->shape.buckets = 0;
+    P->segs.resize(n);
+    for (uint64_t s = 0; s < n; ++s) {
+        AttnSeg& g = P->segs[s];
+        g.q_begin = q_begin[s];
+        g.k_begin = k_begin[s];
+        g.q_len = q_len[s];
+        g.k_len = k_len[s];
+        g.prefix = prefix ? std::min(prefix[s], k_len[s]) : 0;
+        g.dist_ld = (g.k_len + 15) / 16 * 16;
+        if (g.q_len * group > kMaxLen || g.k_len > kMaxLen)
+            return fail(c, GATGPU_EOVERFLOW, "segment " + std::to_string(s) + " is longer than 2^30 rows");
+        if (g.q_begin > kMaxRow || g.k_begin > kMaxRow)
+            return fail(c, GATGPU_EOVERFLOW, "segment " + std::to_string(s) + " begins beyond 2^44 rows");
+        g.base = P->rows;
+        g.dist = P->dist_bytes;
+        P->rows += g.q_len;
+        if (sh->bias == GATGPU_BIAS_TABLE) P->dist_bytes += uint64_t(g.q_len) * g.dist_ld;
+    }
+    if (overlap(P->segs, false)) return fail(c, GATGPU_EINVAL, "query rows of two segments overlap");
+    P->shared_keys = overlap(P->segs, true);
+    if (int r = build(P.get())) return r;
+    *out = P.release();
+    return GATGPU_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gatgpu_attention_create(gatgpu_ctx* c, const gatgpu_attention_shape* shape, uint64_t segments, const uint64_t* q_begin,
+                            const uint32_t* q_len, const uint64_t* k_begin, const uint32_t* k_len, const uint32_t* prefix,
+                            gatgpu_attention** out) {
+    if (!c) return fail(nullptr, GATGPU_EINVAL, "null context");
+    DeviceGuard on(c->device);
+    if (!on.ok) return fail(c, GATGPU_EDEVICE, "cannot select the context's device");
+    try {
+        return create(c, shape, segments, q_begin, q_len, k_begin, k_len, prefix, out);
+    } catch (const std::exception&) {
+        return fail(c, GATGPU_ENOMEM, "host allocation failed");
+    }
+}
+
+int gatgpu_attention_destroy(gatgpu_attention* P) {
+    if (!P) return GATGPU_OK;
+    DeviceGuard on(P->ctx->device);
+    (void)hipStreamSynchronize(P->ctx->stream);
+    delete P;
+    return GATGPU_OK;
+}
+
+int gatgpu_attention_workspace(const gatgpu_attention* P, uint64_t* forward, uint64_t* backward) {
+    if (!P) return fail(nullptr, GATGPU_EINVAL, "null plan");
+    if (forward) *forward = forward_bytes(P);
+    if (backward) *backward = backward_bytes(P);
+    return GATGPU_OK;
+}
+
+int gatgpu_attention_distances(const gatgpu_attention* P, uint64_t* bytes, uint64_t* offset, uint32_t* ld) {
+    if (!P) return fail(nullptr, GATGPU_EINVAL, "null plan");
+    if (P->shape.bias != GATGPU_BIAS_TABLE) return fail(P->ctx, GATGPU_EINVAL, "the plan has no bias table");
+    if (bytes) *bytes = P->dist_bytes;
+    for (size_t s = 0; s < P->segs.size(); ++s) {
+        if (offset) offset[s] = P->segs[s].dist;
+        if (ld) ld[s] = P->segs[s].dist_ld;
+    }
+    return GATGPU_OK;
+}
+
+int gatgpu_attention_forward(gatgpu_attention* P, const gatgpu_attention_io* io, void* ws, uint64_t bytes) {
+    if (!P) return fail(nullptr, GATGPU_EINVAL, "null plan");
+    gatgpu_ctx* c = P->ctx;
+    DeviceGuard on(c->device);
+    if (!on.ok) return fail(c, GATGPU_EDEVICE, "cannot select the context's device");
+    if (int r = check_call(P, io, ws, bytes, forward_bytes(P))) return r;
+    if (io->lse)
+        if (int r = check_floats(c, "lse", io->lse)) return r;
+    AttnArgs a = make_args(P, io);
+    const bool bf16 = P->shape.precision == GATGPU_BF16;
+    a.tasks = P->dfwd.as<AttnTask>();
+    a.ntasks = P->nfwd;
+    if (!a.ntasks) return GATGPU_OK;
+    if (P->split) {
+        a.part = static_cast<float*>(ws);
+        a.stat = reinterpret_cast<float*>(static_cast<char*>(ws) + part_bytes(P));
+    }
+    HIPCHECK(c, launch_attention_forward(a, bf16, P->wfwd, c->stream));
+    if (P->split) HIPCHECK(c, launch_attention_join(a, bf16, P->djoin.as<AttnTask>(), P->njoin, c->stream));
+    return GATGPU_OK;
+}
+
+int gatgpu_attention_backward(gatgpu_attention* P, const gatgpu_attention_io* io, void* ws, uint64_t bytes) {
+    if (!P) return fail(nullptr, GATGPU_EINVAL, "null plan");
+    gatgpu_ctx* c = P->ctx;
+    DeviceGuard on(c->device);
+    if (!on.ok) return fail(c, GATGPU_EDEVICE, "cannot select the context's device");
+    if (P->shared_keys) return fail(c, GATGPU_EINVAL, "key rows of two segments overlap: no backward pass");
+    if (int r = check_call(P, io, ws, bytes, backward_bytes(P))) return r;
+    const gatgpu_attention_shape& sh = P->shape;
+    const bool bf16 = sh.precision == GATGPU_BF16;
+    const int size = bf16 ? 2 : 4;
+    const uint64_t qw = uint64_t(sh.heads) * uint64_t(sh.dim), kw = uint64_t(sh.kv_heads) * uint64_t(sh.dim);
+    if (int r = check_floats(c, "lse", io->lse)) return r;
+    if (int r = check_rows(c, "dout", io->dout, io->dout_stride, qw, size)) return r;
+    if (int r = check_rows(c, "dq", io->dq, io->dq_stride, qw, size)) return r;
+    if (int r = check_rows(c, "dk", io->dk, io->dk_stride, kw, size)) return r;
+    if (int r = check_rows(c, "dv", io->dv, io->dv_stride, kw, size)) return r;
+    if (io->dbias) {
+        if (sh.bias != GATGPU_BIAS_TABLE) return fail(c, GATGPU_EINVAL, "dbias without a bias table");
+        if (bf16 && !io->rest) return fail(c, GATGPU_EINVAL, "dbias of bf16 rows needs rest");
+        if (int r = check_floats(c, "dbias", io->dbias)) return r;
+    }
+    AttnArgs a = make_args(P, io);
+    a.dout = io->dout;
+    a.dos = io->dout_stride;
+    a.dq = io->dq;
+    a.dk = io->dk;
+    a.dv = io->dv;
+    a.dqs = io->dq_stride;
+    a.dks = io->dk_stride;
+    a.dvs = io->dv_stride;
+    a.delta = static_cast<float*>(ws);
+    a.dbias = io->dbias ? reinterpret_cast<float*>(static_cast<char*>(ws) + delta_bytes(P)) : nullptr;
+    a.tasks = P->dbwd_q.as<AttnTask>();
+    a.ntasks = P->nbwd_q;
+    if (a.ntasks) HIPCHECK(c, launch_attention_backward_q(a, bf16, P->wbwd_q, c->stream));
+    if (io->dbias) HIPCHECK(c, launch_attention_bias_sum(a, io->dbias, c->stream));
+    a.tasks = P->dbwd_kv.as<AttnTask>();
+    a.ntasks = P->nbwd_kv;
+    if (a.ntasks) HIPCHECK(c, launch_attention_backward_kv(a, bf16, P->wbwd_kv, c->stream));
+    return GATGPU_OK;
+}
+
+}  // extern "C"

@@ -62,6 +62,10 @@ struct LayerState {
     // fixed-p fixture: p in degree-sorted edge order [e][heads], den [n][heads]
     DevBuf fixp, fixden;
     bool fixed_set = false;
+    // layer norm of the layer's output (gatgpu_set_norm)
+    bool norm = false;
+    DevBuf gamma, beta;
+    float norm_eps = 0.0f;
     double prepare_ms = 0;  // wall time of the last set_layer
     int width() const { return heads * dim; }
 };
@@ -207,6 +211,21 @@ struct TfDone {
 // fixed: the fixed-p operator (the layer's fixture p and den).
 int run_tf(gatgpu_ctx* c, int l, int precision, bool hidden, const float* src32, const uint16_t* srcbf,
            int ev_base, bool fixed, const TfBufs& b, TfDone* done);
+
+// The layer's norm over n FP32 rows at `stride`, in place, through ELU if hidden.
+int run_norm(gatgpu_ctx* c, const LayerState& Ls, float* rows, uint64_t n, uint64_t stride, bool hidden);
+
+// Makes `device` current for a scope and the caller's device current again after it.
+struct DeviceGuard {
+    int before = -1;
+    bool ok = true;
+    explicit DeviceGuard(int device);
+    ~DeviceGuard();
+    DeviceGuard(const DeviceGuard&) = delete;
+    DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
+// GATGPU_EINVAL unless p is memory of the context's device.
+int check_device_array(gatgpu_ctx* c, const void* p, const char* name);
 
 // Resolves the device address of the static scratch array of c->device
 // (layer_static.hip) once per device; the device must be current.

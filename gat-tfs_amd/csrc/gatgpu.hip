@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "context.hpp"
+#include "norm.hpp"
 
 using namespace gatgpu;
 
@@ -274,7 +275,8 @@ int download_rows_dense(gatgpu_ctx* c, float* host, const void* src, uint64_t st
 int run_layer_af(gatgpu_ctx* c, int l, bool hidden, const float* src32, const uint16_t* srcbf, int ev_base,
                  int dataflow, bool fixed) {
     LayerState& Ls = c->L[l];
-    if (fixed) hidden = false;
+    const bool normed = Ls.norm && !fixed, elu = hidden;
+    if (fixed || normed) hidden = false;
     const uint64_t n = c->n;
     const int K = Ls.heads, W = Ls.width(), D = Ls.in, xs = af_input_stride();
     HIPCHECK(c, Ls.left.ensure(n * K * 4));
@@ -408,6 +410,8 @@ int run_layer_af(gatgpu_ctx* c, int l, bool hidden, const float* src32, const ui
     a.fixden = fixed ? Ls.fixden.as<float>() : nullptr;
     HIPCHECK(c, launch_aggregate_af(a, c->stream, c->cus));
     }
+    if (normed)
+        if (int r = run_norm(c, Ls, Ls.out32.as<float>(), n, uint64_t(W), elu)) return r;
     if (ev_base >= 0) HIPCHECK(c, hipEventRecord(c->ev[ev_base + 3], c->stream));
     Ls.out_original = false;
     Ls.out_stride = W;
@@ -478,6 +482,7 @@ bool can_fuse_next(const gatgpu_ctx* c, int l, int precision, const int (&flows)
     if (flows[l] != GATGPU_TRANSFORM_FIRST || flows[l + 1] != GATGPU_TRANSFORM_FIRST) return false;
     const LayerState& A = c->L[l];
     const LayerState& B = c->L[l + 1];
+    if (A.norm) return false;
     const bool a_fast = A.groups == 1 && ((A.ksteps >= 1 && A.ksteps <= 8) || A.ksteps == 16);
     bool r_in_z = false;
     (void)z_stride(precision, B.heads, B.width(), &r_in_z);
@@ -520,6 +525,9 @@ int run_layer(gatgpu_ctx* c, int l, int precision, int dataflow, bool hidden, co
     }
     if (dataflow == GATGPU_AGGREGATE_FIRST || dataflow == GATGPU_TFS_B1)
         return run_layer_af(c, l, hidden, src32, srcbf, ev_base, dataflow, fixed);
+    // A layer with a norm aggregates to FP32 rows, which the norm and ELU then take in place.
+    const bool normed = Ls.norm && !fixed, elu = hidden;
+    if (normed) hidden = false;
     // ---- outputs
     HIPCHECK(c, Ls.left.ensure(n * K * 4));
     HIPCHECK(c, Ls.right.ensure(n * K * 4));
@@ -583,6 +591,10 @@ int run_layer(gatgpu_ctx* c, int l, int precision, int dataflow, bool hidden, co
     b.projected = fuse == kProjected;
     TfDone done;
     if (int r = run_tf(c, l, precision, hidden, src32, srcbf, ev_base, fixed, b, &done)) return r;
+    if (normed) {
+        if (int r = run_norm(c, Ls, b.out32, n, uint64_t(done.out_perm_used ? ostride : W), elu)) return r;
+        if (ev_base >= 0) HIPCHECK(c, hipEventRecord(c->ev[ev_base + 3], c->stream));
+    }
     Ls.ran = true;
     Ls.precision = precision;
     Ls.dataflow = GATGPU_TRANSFORM_FIRST;
@@ -775,6 +787,20 @@ int run_tf(gatgpu_ctx* c, int l, int precision, bool hidden, const float* src32,
     return GATGPU_OK;
 }
 
+int run_norm(gatgpu_ctx* c, const LayerState& Ls, float* rows, uint64_t n, uint64_t stride, bool hidden) {
+    NormArgs a;
+    a.rows = n;
+    a.width = uint32_t(Ls.width());
+    a.elu = hidden;
+    a.eps = Ls.norm_eps;
+    a.gamma = Ls.gamma.as<float>();
+    a.beta = Ls.beta.as<float>();
+    a.x = a.y = rows;
+    a.xs = a.ys = stride;
+    HIPCHECK(c, launch_norm_forward(a, false, c->stream));
+    return GATGPU_OK;
+}
+
 }  // namespace gatgpu
 
 namespace {
@@ -911,7 +937,7 @@ int gatgpu_set_layer(gatgpu_ctx* c, int layer, int in, int heads, int dim, const
     if (!all_finite(ar, W, &bad)) return fail(c, GATGPU_ENONFINITE, "nonfinite aR index=" + std::to_string(bad));
     LayerState& L = c->L[layer];
     L.set = false;
-    L.ran = L.fixed_set = false;
+    L.ran = L.fixed_set = L.norm = false;
     L.in = in;
     L.heads = heads;
     L.dim = dim;
@@ -945,6 +971,32 @@ int gatgpu_set_layer(gatgpu_ctx* c, int layer, int in, int heads, int dim, const
     c->st.model_prepare_ms = 0;
     for (const auto& q : c->L)
         if (q.set) c->st.model_prepare_ms += q.prepare_ms;
+    return GATGPU_OK;
+}
+
+int gatgpu_set_norm(gatgpu_ctx* c, int layer, const float* gamma, const float* beta, float eps) {
+    if (int r = check_ctx(c)) return r;
+    if (layer < 0 || layer > 2) return fail(c, GATGPU_EINVAL, "layer must be 0, 1 or 2");
+    LayerState& L = c->L[layer];
+    if (!gamma && !beta) {
+        L.norm = false;
+        return GATGPU_OK;
+    }
+    if (!gamma || !beta) return fail(c, GATGPU_EINVAL, "null norm weights");
+    if (!L.set) return fail(c, GATGPU_ESTATE, "layer weights not set");
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(c, GATGPU_EINVAL, "eps must be finite and not negative");
+    const uint64_t W = uint64_t(L.width());
+    uint64_t bad = 0;
+    if (!all_finite(gamma, W, &bad)) return fail(c, GATGPU_ENONFINITE, "nonfinite gamma index=" + std::to_string(bad));
+    if (!all_finite(beta, W, &bad)) return fail(c, GATGPU_ENONFINITE, "nonfinite beta index=" + std::to_string(bad));
+    HIPCHECK(c, hipStreamSynchronize(c->stream));  // a static layer in flight may still read the old ones
+    L.norm = false;
+    HIPCHECK(c, L.gamma.ensure(W * 4));
+    HIPCHECK(c, L.beta.ensure(W * 4));
+    HIPCHECK(c, hipMemcpy(L.gamma.p, gamma, W * 4, hipMemcpyHostToDevice));
+    HIPCHECK(c, hipMemcpy(L.beta.p, beta, W * 4, hipMemcpyHostToDevice));
+    L.norm_eps = eps;
+    L.norm = true;
     return GATGPU_OK;
 }
 

@@ -106,7 +106,7 @@ extern "C" {
 int gatgpu_static_scratch_need(gatgpu_ctx* c, int layer, int precision, int hidden, uint64_t* bytes) {
     if (int r = check_static_args(c, layer, precision)) return r;
     if (!bytes) return gatgpu::fail(c, GATGPU_EINVAL, "null output");
-    *bytes = plan_static(c, layer, precision, hidden != 0).bytes;
+    *bytes = plan_static(c, layer, precision, hidden != 0 && !c->L[layer].norm).bytes;
     return GATGPU_OK;
 }
 
@@ -115,7 +115,9 @@ int gatgpu_layer_forward_static(gatgpu_ctx* c, int layer, int precision, int hid
     if (int r = check_static_args(c, layer, precision)) return r;
     if (!x || !out) return fail(c, GATGPU_EINVAL, "null device pointer");
     if (!c->scratch) return fail(c, GATGPU_ESTATE, "static scratch array not resolved on this device");
-    const StaticPlan p = plan_static(c, layer, precision, hidden != 0);
+    const bool normed = c->L[layer].norm;
+    const bool raw = normed || !hidden;  // FP32 rows without ELU leave the aggregation
+    const StaticPlan p = plan_static(c, layer, precision, !raw);
     if (p.bytes > kScratchBytes)
         return fail(c, GATGPU_EOVERFLOW,
                     "layer needs " + std::to_string(p.bytes) + " bytes of static scratch; the array holds " +
@@ -150,7 +152,9 @@ int gatgpu_layer_forward_static(gatgpu_ctx* c, int layer, int precision, int hid
     // (20K rows of 4 x 16 41.7 -> 38.9 us, 30K of 8 x 32 66.0 -> 63.2, 60K of one head
     // 59.3 -> 57.0).
     b.clear = p.chunks;
-    if (int r = run_tf(c, layer, precision, hidden != 0, x, nullptr, -1, false, b, nullptr)) return r;
+    if (int r = run_tf(c, layer, precision, !raw, x, nullptr, -1, false, b, nullptr)) return r;
+    if (normed)
+        if (int r = run_norm(c, Ls, b.out32, n, W, hidden != 0)) return r;
     if (direct) return GATGPU_OK;
     if (b.outbf) HIPCHECK(c, launch_widen_bf16(b.outbf, out, n * W, c->stream));
     else HIPCHECK(c, hipMemcpyAsync(out, b.out32, n * W * 4, hipMemcpyDeviceToDevice, c->stream));

@@ -1,0 +1,572 @@
+// Layer norm, forward and backward.
+//
+//   h = x (+ residual, rounded to the storage type),  mean and var over the row's columns,
+//   r = 1 / sqrt(var + eps),  n = (h - mean) r,  t = n gamma + beta,  y = t or ELU(t)
+//   dt = dy (ELU'(t)),  dgamma = sum dt n,  dbeta = sum dt,  g = dt gamma,
+//   dx = r (g - mean(g) - n mean(g n)) (+ dsum)
+//
+// Bound by bytes: a row is read once into registers (TPR threads a row, ITEMS chunks of
+// VEC elements a thread), its mean and then its centred squares are summed from there, and
+// it is written once.  The backward pass gives each block a fixed set of rows and keeps its
+// columns' sums of dgamma and dbeta in registers over them; blocks leave one partial row
+// each, which a second launch adds in one fixed order.  Sums are FP32.
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "context.hpp"
+#include "norm.hpp"
+
+namespace gatgpu {
+namespace {
+
+template <class T, int VEC>
+__device__ inline void load_vec(const T* p, float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        if constexpr (sizeof(T) == 2) v[0] = bf16_widen(p[0]);
+        else v[0] = p[0];
+    } else if constexpr (sizeof(T) == 2) {  // 8
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(u[i] << 16);
+            v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+    } else {  // 4
+        const float4 w = *reinterpret_cast<const float4*>(p);
+        v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+    }
+}
+template <class T, int VEC>
+__device__ inline void store_vec(T* p, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        if constexpr (sizeof(T) == 2) p[0] = bf16_rne(v[0]);
+        else p[0] = v[0];
+    } else if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7]));
+    } else {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
+// FP32 weights of VEC columns.
+template <int VEC>
+__device__ inline void load_weights(const float* p, uint64_t at, float none, float (&v)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = p ? p[at + e] : none;
+}
+template <class T>
+__device__ inline float round_to(float x) {
+    if constexpr (sizeof(T) == 2) return bf16_widen(bf16_rne(x));
+    else return x;
+}
+// The sum of x over the TPR threads of a row, in every one of them.
+template <int TPR>
+__device__ inline float row_sum(float x, float* lds) {
+#pragma unroll
+    for (int d = (TPR < 64 ? TPR : 64) / 2; d; d /= 2) x += __shfl_xor(x, d);
+    if constexpr (TPR > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < TPR / 64; ++w) x += lds[w];
+    }
+    return x;
+}
+template <int TPR>
+__device__ inline float2 row_sum2(float2 x, float2* lds) {
+#pragma unroll
+    for (int d = (TPR < 64 ? TPR : 64) / 2; d; d /= 2) {
+        x.x += __shfl_xor(x.x, d);
+        x.y += __shfl_xor(x.y, d);
+    }
+    if constexpr (TPR > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < TPR / 64; ++w) {
+            x.x += lds[w].x;
+            x.y += lds[w].y;
+        }
+    }
+    return x;
+}
+template <class T>
+__device__ inline float elu_to(float t) {
+    if constexpr (sizeof(T) == 2) return elu_bf16(t);
+    else return elu(t);
+}
+
+template <class T, int VEC, int TPR, int ITEMS>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const NormArgs a) {
+    constexpr int BLOCK = TPR < 256 ? 256 : TPR;
+    __shared__ float lds[BLOCK / 64];
+    const uint64_t row = uint64_t(blockIdx.x) * (BLOCK / TPR) + threadIdx.x / TPR;
+    if (TPR <= 64 && row >= a.rows) return;  // (whole row groups; wider rows are whole blocks)
+    const uint32_t t = threadIdx.x % TPR, W = a.width;
+    const T* x = static_cast<const T*>(a.x) + row * a.xs;
+    float v[ITEMS][VEC];
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t c = (i * TPR + t) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[i][e] = 0.0f;
+        if (c < W) load_vec<T, VEC>(x + c, v[i]);
+    }
+    if (a.residual) {
+        const T* res = static_cast<const T*>(a.residual) + row * a.rs;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t c = (i * TPR + t) * VEC;
+            if (c < W) {
+                float r[VEC];
+                load_vec<T, VEC>(res + c, r);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[i][e] = round_to<T>(v[i][e] + r[e]);
+                if (a.sum) store_vec<T, VEC>(static_cast<T*>(a.sum) + row * a.ss + c, v[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum += v[i][e];
+    const float inv = 1.0f / float(W), mean = row_sum<TPR>(sum, lds) * inv;
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+        if ((i * TPR + t) * VEC < W)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum = fmaf(v[i][e] - mean, v[i][e] - mean, sum);
+    const float rstd = 1.0f / sqrtf(row_sum<TPR>(sum, lds) * inv + a.eps);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t c = (i * TPR + t) * VEC;
+        if (c >= W) continue;
+        float g[VEC], b[VEC];
+        load_weights<VEC>(a.gamma, c, 1.0f, g);
+        load_weights<VEC>(a.beta, c, 0.0f, b);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float y = fmaf((v[i][e] - mean) * rstd, g[e], b[e]);
+            v[i][e] = a.elu ? elu_to<T>(y) : y;
+        }
+        store_vec<T, VEC>(static_cast<T*>(a.y) + row * a.ys + c, v[i]);
+    }
+    if (t == 0) {
+        if (a.mean) a.mean[row] = mean;
+        if (a.rstd) a.rstd[row] = rstd;
+    }
+}
+
+// Rows of any width, a block a row: passes over the row where it lies.
+template <class T>
+__global__ __launch_bounds__(1024) void k_norm_fwd_any(const NormArgs a) {
+    __shared__ float lds[16];
+    const uint64_t row = blockIdx.x;
+    const uint32_t W = a.width;
+    const T* x = static_cast<const T*>(a.x) + row * a.xs;
+    const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.rs : nullptr;
+    const auto h = [&](uint32_t c) {
+        float v[1], r[1] = {0.0f};
+        load_vec<T, 1>(x + c, v);
+        if (!res) return v[0];
+        load_vec<T, 1>(res + c, r);
+        return round_to<T>(v[0] + r[0]);
+    };
+    float sum = 0.0f;
+    for (uint32_t c = threadIdx.x; c < W; c += 1024) sum += h(c);
+    const float mean = row_sum<1024>(sum, lds) / float(W);
+    sum = 0.0f;
+    for (uint32_t c = threadIdx.x; c < W; c += 1024) sum = fmaf(h(c) - mean, h(c) - mean, sum);
+    const float rstd = 1.0f / sqrtf(row_sum<1024>(sum, lds) / float(W) + a.eps);
+    for (uint32_t c = threadIdx.x; c < W; c += 1024) {
+        const float v[1] = {h(c)}, g = a.gamma ? a.gamma[c] : 1.0f, b = a.beta ? a.beta[c] : 0.0f;
+        if (a.sum) store_vec<T, 1>(static_cast<T*>(a.sum) + row * a.ss + c, v);
+        const float y = fmaf((v[0] - mean) * rstd, g, b), o[1] = {a.elu ? elu_to<T>(y) : y};
+        store_vec<T, 1>(static_cast<T*>(a.y) + row * a.ys + c, o);
+    }
+    if (threadIdx.x == 0) {
+        if (a.mean) a.mean[row] = mean;
+        if (a.rstd) a.rstd[row] = rstd;
+    }
+}
+
+template <class T, int VEC, int TPR, int ITEMS>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormArgs a) {
+    constexpr int BLOCK = TPR < 256 ? 256 : TPR, GROUPS = BLOCK / TPR;
+    __shared__ float2 lds[BLOCK / 64];
+    __shared__ float cols[GROUPS > 1 ? GROUPS * TPR * VEC : 1];
+    const uint32_t t = threadIdx.x % TPR, group = threadIdx.x / TPR, W = a.width;
+    const float inv = 1.0f / float(W);
+    float dg[ITEMS][VEC], db[ITEMS][VEC];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) dg[i][e] = db[i][e] = 0.0f;
+    // (Rows beyond the last leave a row group's lanes idle, not its reductions: all threads make
+    // the same rounds.)
+    const uint64_t step = uint64_t(gridDim.x) * GROUPS, first = uint64_t(blockIdx.x) * GROUPS;
+    for (uint64_t r0 = first; r0 < a.rows; r0 += step) {
+        const uint64_t row = r0 + group;
+        const bool in = row < a.rows;
+        float n[ITEMS][VEC], g[ITEMS][VEC];
+        float2 s = make_float2(0.0f, 0.0f);
+        const float mean = in ? a.mean[row] : 0.0f, rstd = in ? a.rstd[row] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t c = (i * TPR + t) * VEC;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) n[i][e] = g[i][e] = 0.0f;
+            if (in && c < W) {
+                load_vec<T, VEC>(static_cast<const T*>(a.h) + row * a.hs + c, n[i]);
+                load_vec<T, VEC>(static_cast<const T*>(a.dy) + row * a.dys + c, g[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t c = (i * TPR + t) * VEC;
+            if (!in || c >= W) continue;
+            float w[VEC], b[VEC];
+            load_weights<VEC>(a.gamma, c, 1.0f, w);
+            if (a.elu) load_weights<VEC>(a.beta, c, 0.0f, b);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                n[i][e] = (n[i][e] - mean) * rstd;
+                if (a.elu) {
+                    const float y = fmaf(n[i][e], w[e], b[e]);
+                    if (y < 0.0f) g[i][e] *= exp_w(y);
+                }
+                dg[i][e] = fmaf(g[i][e], n[i][e], dg[i][e]);
+                db[i][e] += g[i][e];
+                g[i][e] *= w[e];
+                s.x += g[i][e];
+                s.y = fmaf(g[i][e], n[i][e], s.y);
+            }
+        }
+        s = row_sum2<TPR>(s, lds);
+        s.x *= inv;
+        s.y *= inv;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t c = (i * TPR + t) * VEC;
+            if (!in || c >= W) continue;
+            float add[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) add[e] = 0.0f;
+            if (a.dsum) load_vec<T, VEC>(static_cast<const T*>(a.dsum) + row * a.dss + c, add);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) g[i][e] = fmaf(rstd, g[i][e] - s.x - n[i][e] * s.y, add[e]);
+            store_vec<T, VEC>(static_cast<T*>(a.dx) + row * a.dxs + c, g[i]);
+        }
+    }
+    if (!a.part) return;
+    // The block's column sums: row groups added in order.
+    float* to = a.part + uint64_t(blockIdx.x) * 2 * W;
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t c = (i * TPR + t) * VEC;
+            float v[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = which ? db[i][e] : dg[i][e];
+            if constexpr (GROUPS > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) cols[(group * VEC + e) * TPR + t] = v[e];
+                __syncthreads();
+                if (group == 0)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        for (int q = 1; q < GROUPS; ++q) v[e] += cols[(q * VEC + e) * TPR + t];
+            }
+            if (group == 0 && c < W)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) to[uint64_t(which) * W + c + e] = v[e];
+        }
+}
+
+template <class T>
+__global__ __launch_bounds__(1024) void k_norm_bwd_any(const NormArgs a) {
+    __shared__ float2 lds[16];
+    const uint64_t row = blockIdx.x;
+    const uint32_t W = a.width;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    const T* h = static_cast<const T*>(a.h) + row * a.hs;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.dys;
+    const auto terms = [&](uint32_t c, float& n, float& dt) {
+        float v[1], d[1];
+        load_vec<T, 1>(h + c, v);
+        load_vec<T, 1>(dy + c, d);
+        n = (v[0] - mean) * rstd;
+        dt = d[0];
+        if (a.elu) {
+            const float y = fmaf(n, a.gamma ? a.gamma[c] : 1.0f, a.beta ? a.beta[c] : 0.0f);
+            if (y < 0.0f) dt *= exp_w(y);
+        }
+    };
+    float2 s = make_float2(0.0f, 0.0f);
+    for (uint32_t c = threadIdx.x; c < W; c += 1024) {
+        float n, dt;
+        terms(c, n, dt);
+        dt *= a.gamma ? a.gamma[c] : 1.0f;
+        s.x += dt;
+        s.y = fmaf(dt, n, s.y);
+    }
+    s = row_sum2<1024>(s, lds);
+    for (uint32_t c = threadIdx.x; c < W; c += 1024) {
+        float n, dt, add[1] = {0.0f};
+        terms(c, n, dt);
+        if (a.dsum) load_vec<T, 1>(static_cast<const T*>(a.dsum) + row * a.dss + c, add);
+        dt *= a.gamma ? a.gamma[c] : 1.0f;
+        const float o[1] = {fmaf(rstd, dt - s.x / float(W) - n * (s.y / float(W)), add[0])};
+        store_vec<T, 1>(static_cast<T*>(a.dx) + row * a.dxs + c, o);
+    }
+}
+// Column sums of rows of any width: block (columns, row strip), a thread a column.  It runs
+// before k_norm_bwd_any, whose dx may take dy's place.
+template <class T>
+__global__ __launch_bounds__(256) void k_norm_cols_any(const NormArgs a) {
+    const uint32_t c = blockIdx.x * 256 + threadIdx.x, W = a.width;
+    if (c >= W) return;
+    const float w = a.gamma ? a.gamma[c] : 1.0f, b = a.beta ? a.beta[c] : 0.0f;
+    float dg = 0.0f, db = 0.0f;
+    for (uint64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        float v[1], d[1];
+        load_vec<T, 1>(static_cast<const T*>(a.h) + row * a.hs + c, v);
+        load_vec<T, 1>(static_cast<const T*>(a.dy) + row * a.dys + c, d);
+        const float n = (v[0] - a.mean[row]) * a.rstd[row];
+        if (a.elu) {
+            const float y = fmaf(n, w, b);
+            if (y < 0.0f) d[0] *= exp_w(y);
+        }
+        dg = fmaf(d[0], n, dg);
+        db += d[0];
+    }
+    a.part[uint64_t(blockIdx.y) * 2 * W + c] = dg;
+    a.part[uint64_t(blockIdx.y) * 2 * W + W + c] = db;
+}
+
+// dgamma, dbeta: 64 columns a block, 4 waves over the partial rows, added in one fixed order.
+__global__ __launch_bounds__(256) void k_norm_sum(const float* __restrict__ part, uint32_t blocks, uint32_t W, float* dgamma,
+                                                  float* dbeta) {
+    const uint64_t c = uint64_t(blockIdx.x) * 64 + (threadIdx.x & 63);
+    __shared__ float lds[256];
+    float sum = 0.0f;
+    if (c < 2 * uint64_t(W))
+        for (uint32_t b = threadIdx.x >> 6; b < blocks; b += 4) sum += part[uint64_t(b) * 2 * W + c];
+    lds[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x >= 64 || c >= 2 * uint64_t(W)) return;
+    sum = lds[threadIdx.x] + lds[threadIdx.x + 64] + lds[threadIdx.x + 128] + lds[threadIdx.x + 192];
+    if (c < W) {
+        if (dgamma) dgamma[c] = sum;
+    } else if (dbeta) dbeta[c - W] = sum;
+}
+
+// Threads a row and chunks a thread for a row of `chunks` chunks: the fewest threads that keep
+// a thread at 4 chunks, 0 where no kernel holds the row.
+struct NormShape {
+    int tpr, items;
+};
+NormShape norm_shape(uint64_t chunks) {
+    const NormShape all[] = {{16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}};
+    for (const NormShape& s : all)
+        if (chunks <= uint64_t(s.tpr) * s.items) return s;
+    return {0, 0};
+}
+bool aligned(const void* p, uint64_t stride, int size) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * uint64_t(size) % 16 == 0;
+}
+
+#define GATGPU_NORM_SHAPES(F) \
+    F(16, 1) F(16, 2) F(64, 1) F(64, 2) F(64, 4) F(256, 2) F(256, 4) F(1024, 2) F(1024, 4)
+
+template <class T, int VEC>
+hipError_t forward(const NormArgs& a, NormShape s, hipStream_t st) {
+    const uint64_t per = s.tpr < 256 ? 256 / s.tpr : 1;
+    const dim3 grid{uint32_t((a.rows + per - 1) / per)};
+#define F(TPR, ITEMS) \
+    if (s.tpr == TPR && s.items == ITEMS) k_norm_fwd<T, VEC, TPR, ITEMS><<<grid, TPR < 256 ? 256 : TPR, 0, st>>>(a);
+    GATGPU_NORM_SHAPES(F)
+#undef F
+    if (!s.tpr) k_norm_fwd_any<T><<<uint32_t(a.rows), 1024, 0, st>>>(a);
+    return hipGetLastError();
+}
+template <class T, int VEC>
+hipError_t backward(const NormArgs& a, NormShape s, uint32_t blocks, hipStream_t st) {
+#define F(TPR, ITEMS) \
+    if (s.tpr == TPR && s.items == ITEMS) k_norm_bwd<T, VEC, TPR, ITEMS><<<blocks, TPR < 256 ? 256 : TPR, 0, st>>>(a);
+    GATGPU_NORM_SHAPES(F)
+#undef F
+    if (!s.tpr) {
+        if (a.part) k_norm_cols_any<T><<<dim3((a.width + 255) / 256, blocks), 256, 0, st>>>(a);
+        if (a.rows) k_norm_bwd_any<T><<<uint32_t(a.rows), 1024, 0, st>>>(a);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+uint32_t norm_blocks(uint64_t rows, uint64_t width) {
+    // Two blocks a CU, fewer where rows are few; wide rows one a CU (a partial row costs 8 bytes a column).
+    const uint64_t most = width > 4096 ? 256 : 512;
+    return uint32_t(std::max<uint64_t>(1, std::min(most, (rows + 3) / 4)));
+}
+
+hipError_t launch_norm_forward(const NormArgs& a, bool bf16, hipStream_t s) {
+    const int size = bf16 ? 2 : 4, vec = 16 / size;
+    const bool wide = a.width % uint32_t(vec) == 0 && aligned(a.x, a.xs, size) && aligned(a.y, a.ys, size) &&
+                      (!a.residual || aligned(a.residual, a.rs, size)) && (!a.sum || aligned(a.sum, a.ss, size));
+    const NormShape shape = norm_shape(wide ? a.width / uint32_t(vec) : a.width);
+    if (bf16) return wide ? forward<uint16_t, 8>(a, shape, s) : forward<uint16_t, 1>(a, shape, s);
+    return wide ? forward<float, 4>(a, shape, s) : forward<float, 1>(a, shape, s);
+}
+
+hipError_t launch_norm_backward(const NormArgs& a, bool bf16, uint32_t blocks, float* dgamma, float* dbeta, hipStream_t s) {
+    const int size = bf16 ? 2 : 4, vec = 16 / size;
+    const bool wide = a.width % uint32_t(vec) == 0 && aligned(a.h, a.hs, size) && aligned(a.dy, a.dys, size) &&
+                      aligned(a.dx, a.dxs, size) && (!a.dsum || aligned(a.dsum, a.dss, size));
+    const NormShape shape = norm_shape(wide ? a.width / uint32_t(vec) : a.width);
+    hipError_t e;
+    if (bf16) e = wide ? backward<uint16_t, 8>(a, shape, blocks, s) : backward<uint16_t, 1>(a, shape, blocks, s);
+    else e = wide ? backward<float, 4>(a, shape, blocks, s) : backward<float, 1>(a, shape, blocks, s);
+    if (e != hipSuccess || !a.part) return e;
+    k_norm_sum<<<uint32_t((2 * uint64_t(a.width) + 63) / 64), 256, 0, s>>>(a.part, blocks, a.width, dgamma, dbeta);
+    return hipGetLastError();
+}
+
+}  // namespace gatgpu
+
+namespace {
+
+using namespace gatgpu;
+
+// Rows of the call's storage type: there, aligned to its elements, wide enough, on the device.
+int check_rows(gatgpu_ctx* c, const gatgpu_norm_io* io, const char* name, const void* p, uint64_t stride) {
+    if (!p) return fail(c, GATGPU_EINVAL, std::string("null ") + name);
+    if (reinterpret_cast<uintptr_t>(p) % (io->precision == GATGPU_BF16 ? 2 : 4))
+        return fail(c, GATGPU_EINVAL, std::string(name) + " is not aligned to its elements");
+    if (stride < io->width || stride > (uint64_t(1) << 44)) return fail(c, GATGPU_EINVAL, std::string(name) + " has a bad row stride");
+    return check_device_array(c, p, name);
+}
+int check_floats(gatgpu_ctx* c, const char* name, const void* p) {
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(c, GATGPU_EINVAL, std::string(name) + " must be 4-byte aligned");
+    return check_device_array(c, p, name);
+}
+int check_call(gatgpu_ctx* c, const gatgpu_norm_io* io) {
+    if (!io) return fail(c, GATGPU_EINVAL, "null arrays");
+    if (io->precision != GATGPU_FP32 && io->precision != GATGPU_BF16) return fail(c, GATGPU_EINVAL, "bad precision");
+    if (io->width == 0 || io->width > (1u << 30)) return fail(c, GATGPU_EINVAL, "width must be 1 to 2^30");
+    if (io->rows >= (uint64_t(1) << 31)) return fail(c, GATGPU_EOVERFLOW, "more than 2^31 - 1 rows");
+    if (!(io->eps >= 0.0f) || !std::isfinite(io->eps)) return fail(c, GATGPU_EINVAL, "eps must be finite and not negative");
+    if (io->gamma)
+        if (int r = check_floats(c, "gamma", io->gamma)) return r;
+    if (io->beta)
+        if (int r = check_floats(c, "beta", io->beta)) return r;
+    return GATGPU_OK;
+}
+NormArgs make_args(const gatgpu_norm_io* io) {
+    NormArgs a;
+    a.rows = io->rows;
+    a.width = io->width;
+    a.elu = io->elu != 0;
+    a.eps = io->eps;
+    a.gamma = io->gamma;
+    a.beta = io->beta;
+    a.mean = io->mean;
+    a.rstd = io->rstd;
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gatgpu_norm_forward(gatgpu_ctx* c, const gatgpu_norm_io* io) {
+    if (!c) return fail(nullptr, GATGPU_EINVAL, "null context");
+    DeviceGuard on(c->device);
+    if (!on.ok) return fail(c, GATGPU_EDEVICE, "cannot select the context's device");
+    if (int r = check_call(c, io)) return r;
+    if (!io->rows) return GATGPU_OK;
+    if (int r = check_rows(c, io, "x", io->x, io->x_stride)) return r;
+    if (int r = check_rows(c, io, "y", io->y, io->y_stride)) return r;
+    if (io->residual)
+        if (int r = check_rows(c, io, "residual", io->residual, io->residual_stride)) return r;
+    if (io->sum) {
+        if (!io->residual) return fail(c, GATGPU_EINVAL, "sum without a residual");
+        if (int r = check_rows(c, io, "sum", io->sum, io->sum_stride)) return r;
+    }
+    if (io->mean)
+        if (int r = check_floats(c, "mean", io->mean)) return r;
+    if (io->rstd)
+        if (int r = check_floats(c, "rstd", io->rstd)) return r;
+    NormArgs a = make_args(io);
+    a.x = io->x;
+    a.xs = io->x_stride;
+    a.residual = io->residual;
+    a.rs = io->residual_stride;
+    a.sum = io->sum;
+    a.ss = io->sum_stride;
+    a.y = io->y;
+    a.ys = io->y_stride;
+    HIPCHECK(c, launch_norm_forward(a, io->precision == GATGPU_BF16, c->stream));
+    return GATGPU_OK;
+}
+
+int gatgpu_norm_workspace(gatgpu_ctx* c, uint64_t rows, uint32_t width, uint64_t* bytes) {
+    if (!c) return fail(nullptr, GATGPU_EINVAL, "null context");
+    if (!bytes) return fail(c, GATGPU_EINVAL, "null output");
+    *bytes = uint64_t(norm_blocks(rows, width)) * 2 * uint64_t(width) * 4;
+    return GATGPU_OK;
+}
+
+int gatgpu_norm_backward(gatgpu_ctx* c, const gatgpu_norm_io* io, void* ws, uint64_t bytes) {
+    if (!c) return fail(nullptr, GATGPU_EINVAL, "null context");
+    DeviceGuard on(c->device);
+    if (!on.ok) return fail(c, GATGPU_EDEVICE, "cannot select the context's device");
+    if (int r = check_call(c, io)) return r;
+    NormArgs a = make_args(io);
+    a.h = io->residual ? io->sum : io->x;
+    a.hs = io->residual ? io->sum_stride : io->x_stride;
+    a.dy = io->dy;
+    a.dys = io->dy_stride;
+    a.dsum = io->dsum;
+    a.dss = io->dsum_stride;
+    a.dx = io->dx;
+    a.dxs = io->dx_stride;
+    if (io->rows) {
+        if (int r = check_rows(c, io, io->residual ? "sum" : "x", a.h, a.hs)) return r;
+        if (int r = check_rows(c, io, "dy", io->dy, io->dy_stride)) return r;
+        if (int r = check_rows(c, io, "dx", io->dx, io->dx_stride)) return r;
+        if (io->dsum)
+            if (int r = check_rows(c, io, "dsum", io->dsum, io->dsum_stride)) return r;
+        if (!io->mean || !io->rstd) return fail(c, GATGPU_EINVAL, "null mean or rstd");
+        if (int r = check_floats(c, "mean", io->mean)) return r;
+        if (int r = check_floats(c, "rstd", io->rstd)) return r;
+    }
+    const uint32_t blocks = norm_blocks(io->rows, io->width);
+    if (io->dgamma || io->dbeta) {
+        if (io->dgamma)
+            if (int r = check_floats(c, "dgamma", io->dgamma)) return r;
+        if (io->dbeta)
+            if (int r = check_floats(c, "dbeta", io->dbeta)) return r;
+        const uint64_t need = uint64_t(blocks) * 2 * uint64_t(io->width) * 4;
+        if (bytes < need)
+            return fail(c, GATGPU_EINVAL, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
+        if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return fail(c, GATGPU_EINVAL, "workspace must be 16-byte aligned device memory");
+        if (int r = check_device_array(c, ws, "workspace")) return r;
+        a.part = static_cast<float*>(ws);
+    }
+    if (!io->rows && !a.part) return GATGPU_OK;
+    HIPCHECK(c, launch_norm_backward(a, io->precision == GATGPU_BF16, blocks, io->dgamma, io->dbeta, c->stream));
+    return GATGPU_OK;
+}
+
+}  // extern "C"

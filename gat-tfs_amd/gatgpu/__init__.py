@@ -22,6 +22,9 @@ AUTO, TRANSFORM_FIRST, AGGREGATE_FIRST, TFS_B1 = 0, 1, 2, 3
 STAGE_Z, STAGE_LEFT, STAGE_RIGHT, STAGE_MAX, STAGE_DEN, STAGE_OUT, STAGE_XBF = range(7)
 OPT_BLOCK_ROW_MIN_DEGREE, OPT_SPLIT_ROW_MIN_DEGREE, OPT_SPLIT_CHUNK_EDGES, OPT_KEEP_INPUT_BF16 = 1, 2, 3, 5
 OPT_FUSE_NEXT_PROJECTION = 6
+MASK_FULL, MASK_PREFIX = 0, 1
+BIAS_NONE, BIAS_LINEAR, BIAS_TABLE = 0, 1, 2
+HIDDEN = 255  # GATGPU_HIDDEN: the distance of a pair that does not see each other
 
 STATIC_SCRATCH_BYTES = 64 << 20  # GATGPU_STATIC_SCRATCH_BYTES
 
@@ -35,7 +38,10 @@ EXPORTS = (
     "gatgpu_layer_forward", "gatgpu_model_forward", "gatgpu_get_stage", "gatgpu_stage_size",
     "gatgpu_set_option", "gatgpu_synchronize", "gatgpu_stream", "gatgpu_set_fixed_p", "gatgpu_fixed_p_forward",
     "gatgpu_get_static_times", "gatgpu_validate_graph", "gatgpu_layer_forward_static",
-    "gatgpu_static_scratch_need",
+    "gatgpu_static_scratch_need", "gatgpu_attention_create", "gatgpu_attention_destroy",
+    "gatgpu_attention_workspace", "gatgpu_attention_distances", "gatgpu_attention_forward",
+    "gatgpu_attention_backward", "gatgpu_norm_forward", "gatgpu_norm_backward", "gatgpu_norm_workspace",
+    "gatgpu_set_norm",
 )
 
 
@@ -57,6 +63,36 @@ class StaticTimes(ctypes.Structure):
 
     def as_dict(self):
         return {name: getattr(self, name) for name, _ in self._fields_}
+
+
+class AttentionShape(ctypes.Structure):
+    """gatgpu_attention_shape."""
+    _fields_ = [(name, ctypes.c_int) for name in ("precision", "heads", "kv_heads", "dim", "mask", "bias", "buckets")]
+    _fields_ += [("scale", ctypes.c_float), ("cap", ctypes.c_float)]
+
+
+class AttentionIO(ctypes.Structure):
+    """gatgpu_attention_io: the device arrays of a call, pointers as ints and
+    row strides in elements.  Fields not given are 0 (NULL)."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_stride", ctypes.c_uint64),
+                ("k_stride", ctypes.c_uint64), ("v_stride", ctypes.c_uint64), ("bias", ctypes.c_void_p),
+                ("dist", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_uint64),
+                ("lse", ctypes.c_void_p), ("rest", ctypes.c_void_p), ("dout", ctypes.c_void_p),
+                ("dout_stride", ctypes.c_uint64), ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p),
+                ("dv", ctypes.c_void_p), ("dq_stride", ctypes.c_uint64), ("dk_stride", ctypes.c_uint64),
+                ("dv_stride", ctypes.c_uint64), ("dbias", ctypes.c_void_p)]
+
+
+class NormIO(ctypes.Structure):
+    """gatgpu_norm_io: shape and device arrays of a layer norm call."""
+    _fields_ = [("precision", ctypes.c_int), ("elu", ctypes.c_int), ("rows", ctypes.c_uint64), ("width", ctypes.c_uint32),
+                ("eps", ctypes.c_float), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_uint64),
+                ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_uint64), ("sum", ctypes.c_void_p),
+                ("sum_stride", ctypes.c_uint64), ("gamma", ctypes.c_void_p), ("beta", ctypes.c_void_p),
+                ("y", ctypes.c_void_p), ("y_stride", ctypes.c_uint64), ("mean", ctypes.c_void_p),
+                ("rstd", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_uint64),
+                ("dsum", ctypes.c_void_p), ("dsum_stride", ctypes.c_uint64), ("dx", ctypes.c_void_p),
+                ("dx_stride", ctypes.c_uint64), ("dgamma", ctypes.c_void_p), ("dbeta", ctypes.c_void_p)]
 
 
 class GatGpuError(RuntimeError):
@@ -102,6 +138,16 @@ def load_library(path: os.PathLike | None = None):
     L.gatgpu_validate_graph.argtypes = [u64, u64, P, P]
     L.gatgpu_layer_forward_static.argtypes = [P, i32, i32, i32, P, P]
     L.gatgpu_static_scratch_need.argtypes = [P, i32, i32, i32, ctypes.POINTER(u64)]
+    L.gatgpu_attention_create.argtypes = [P, ctypes.POINTER(AttentionShape), u64, P, P, P, P, P, ctypes.POINTER(P)]
+    L.gatgpu_attention_destroy.argtypes = [P]
+    L.gatgpu_attention_workspace.argtypes = [P, ctypes.POINTER(u64), ctypes.POINTER(u64)]
+    L.gatgpu_attention_distances.argtypes = [P, ctypes.POINTER(u64), P, P]
+    L.gatgpu_attention_forward.argtypes = [P, ctypes.POINTER(AttentionIO), P, u64]
+    L.gatgpu_attention_backward.argtypes = [P, ctypes.POINTER(AttentionIO), P, u64]
+    L.gatgpu_norm_forward.argtypes = [P, ctypes.POINTER(NormIO)]
+    L.gatgpu_norm_backward.argtypes = [P, ctypes.POINTER(NormIO), P, u64]
+    L.gatgpu_norm_workspace.argtypes = [P, u64, ctypes.c_uint32, ctypes.POINTER(u64)]
+    L.gatgpu_set_norm.argtypes = [P, i32, P, P, ctypes.c_float]
     for name in EXPORTS:
         if name not in ("gatgpu_last_error", "gatgpu_stream"):
             getattr(L, name).restype = i32
@@ -181,6 +227,14 @@ class Context:
     def set_model(self, model):
         for l, p in enumerate(model):
             self.set_layer(l, p)
+
+    def set_norm(self, layer, gamma, beta, eps=1e-5):
+        """Layer norm of the layer's output (before ELU); gamma None: no norm any more."""
+        if gamma is not None:
+            gamma, beta = (np.ascontiguousarray(a, np.float32) for a in (gamma, beta))
+            if self.layers[layer] is not None and not gamma.size == beta.size == self.layers[layer][1] * self.layers[layer][2]:
+                raise ValueError("gamma and beta have one value per output column of the layer")
+        self._check(self.lib.gatgpu_set_norm(self.h, layer, _ptr(gamma), _ptr(beta) if gamma is not None else None, eps))
 
     def set_input(self, x):
         x = np.ascontiguousarray(x, np.float32)
@@ -270,6 +324,19 @@ class Context:
         self._check(self.lib.gatgpu_static_scratch_need(self.h, layer, precision, int(hidden), ctypes.byref(b)))
         return b.value
 
+    # -- layer norm on device rows
+    def norm_forward(self, io):
+        """gatgpu_norm_forward of a NormIO.  Enqueued on the context's stream."""
+        self._check(self.lib.gatgpu_norm_forward(self.h, io))
+
+    def norm_backward(self, io, workspace=None, workspace_bytes=0):
+        self._check(self.lib.gatgpu_norm_backward(self.h, io, workspace, workspace_bytes))
+
+    def norm_workspace(self, rows, width):
+        b = ctypes.c_uint64()
+        self._check(self.lib.gatgpu_norm_workspace(self.h, rows, width, ctypes.byref(b)))
+        return b.value
+
     def static_times(self):
         t = StaticTimes()
         self._check(self.lib.gatgpu_get_static_times(self.h, ctypes.byref(t)))
@@ -277,3 +344,73 @@ class Context:
 
     def synchronize(self):
         self._check(self.lib.gatgpu_synchronize(self.h))
+
+    def stream(self):
+        """The context's HIP stream as an int (gatgpu_stream), e.g. for torch.cuda.ExternalStream."""
+        return self.lib.gatgpu_stream(self.h)
+
+
+class Attention:
+    """A plan of attention among the rows of segments (gatgpu_attention).
+
+    q_len, k_len: rows per segment; q_begin, k_begin: their first rows (by default
+    packed one after another); prefix: keys every query sees (MASK_PREFIX).
+    forward and backward take an AttentionIO of device pointers and enqueue on
+    the context's stream."""
+
+    def __init__(self, ctx, q_len, k_len, *, heads, kv_heads=None, dim, precision=BF16, mask=MASK_FULL, prefix=None,
+                 bias=BIAS_NONE, buckets=0, scale=None, cap=0.0, q_begin=None, k_begin=None):
+        self.h = None
+        self.ctx = ctx
+        self.lib = ctx.lib
+        lens = [np.ascontiguousarray(a, np.uint32) for a in (q_len, k_len)]
+        begins = []
+        for begin, length in zip((q_begin, k_begin), lens):
+            if begin is None:
+                begin = np.cumsum(length, dtype=np.uint64) - length
+            begins.append(np.ascontiguousarray(begin, np.uint64))
+        prefix = None if prefix is None else np.ascontiguousarray(prefix, np.uint32)
+        self.segments = lens[0].size
+        if any(a.shape != (self.segments,) for a in (*lens, *begins)) or (prefix is not None and prefix.shape != (self.segments,)):
+            raise ValueError("one length, begin and prefix per segment")
+        shape = AttentionShape(precision, heads, heads if kv_heads is None else kv_heads, dim, mask, bias, buckets,
+                               dim ** -0.5 if scale is None else scale, cap)
+        h = ctypes.c_void_p()
+        ctx._check(self.lib.gatgpu_attention_create(ctx.h, ctypes.byref(shape), self.segments, _ptr(begins[0]), _ptr(lens[0]),
+                                                    _ptr(begins[1]), _ptr(lens[1]), _ptr(prefix), ctypes.byref(h)))
+        self.h = h
+
+    def close(self):
+        if self.h and self.ctx.h:  # (a context that is gone has taken its stream with it)
+            self.lib.gatgpu_attention_destroy(self.h)
+        self.h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def workspace_bytes(self, backward=False):
+        f, b = ctypes.c_uint64(), ctypes.c_uint64()
+        self.ctx._check(self.lib.gatgpu_attention_workspace(self.h, ctypes.byref(f), ctypes.byref(b)))
+        return b.value if backward else f.value
+
+    def distance_layout(self):
+        """(bytes, offsets, row strides) of the pair distances, per segment."""
+        n = ctypes.c_uint64()
+        off, ld = np.empty(self.segments, np.uint64), np.empty(self.segments, np.uint32)
+        self.ctx._check(self.lib.gatgpu_attention_distances(self.h, ctypes.byref(n), _ptr(off), _ptr(ld)))
+        return n.value, off, ld
+
+    def forward(self, io, workspace=None, workspace_bytes=0):
+        self.ctx._check(self.lib.gatgpu_attention_forward(self.h, io, workspace, workspace_bytes))
+
+    def backward(self, io, workspace=None, workspace_bytes=0):
+        self.ctx._check(self.lib.gatgpu_attention_backward(self.h, io, workspace, workspace_bytes))

@@ -301,6 +301,153 @@ int gatgpu_layer_forward_static(gatgpu_ctx* ctx, int layer, int precision, int h
  * the graph or the layer's weights are not set. */
 int gatgpu_static_scratch_need(gatgpu_ctx* ctx, int layer, int precision, int hidden, uint64_t* bytes);
 
+/* ---- attention among the rows of segments ------------------------------ */
+/* No counterpart in the reference.  Beside the attention over a graph's edges:
+ * softmax attention in which every row of a segment (a graph or document of a
+ * packed batch, or one sequence with its cached keys) attends to the keys of
+ * its own segment, on device-resident rows, with its gradient.
+ *
+ * Segment s has q_len[s] query rows from q_begin[s] and k_len[s] key rows from
+ * k_begin[s] of the caller's arrays.  Query i stands at position
+ * pos = i + k_len - q_len among the keys.  For head h and the key/value head
+ * h / (heads / kv_heads):
+ *   x = scale q.k      y = cap > 0 ? cap tanh(x / cap) : x      s = y + bias
+ *   out = sum_j p_j v_j,  p = softmax of s over the keys that the query sees
+ *   lse = log sum exp s
+ * GATGPU_MASK_FULL: every key is seen.  GATGPU_MASK_PREFIX: key j is seen if
+ * j <= pos or j < prefix[s] (causal with a visible prefix).
+ * GATGPU_BIAS_LINEAR: bias = -slope[h] |pos - j|, slope constant.
+ * GATGPU_BIAS_TABLE: bias = table[h][min(d, buckets - 1)] with one byte d of
+ * distance per pair (a shortest path, say); d = GATGPU_HIDDEN: not seen.  A
+ * table entry of -infinity hides its pairs as well.
+ * A row that sees no key of finite score gets out = 0, lse = -infinity, and no
+ * gradient.  Keys that are not seen add nothing, whatever they hold (NaN
+ * included); a NaN or infinity in a seen value reaches that row's output.
+ *
+ * Storage: GATGPU_FP32 (products in FP32) or GATGPU_BF16 (bf16 rows, FP32
+ * scores, softmax state and sums; the weights and, backward, the score
+ * gradients are rounded to bf16 as operands of their products).  dim: a
+ * multiple of 8, at most 128.  heads <= 64.
+ *
+ * All work is enqueued on the context's stream (gatgpu_stream) and calls return
+ * without waiting; neither forward nor backward allocates, waits or copies, so
+ * both can be captured into a HIP graph.  A captured call refers to its plan's
+ * tables, the buffers and the workspace: keep them until the last replay, and
+ * give graphs that may run at once workspaces of their own.  The same holds for
+ * calls: two that overlap need two workspaces.  Arrays must lie on the context's
+ * device.  Rows that belong to no segment are neither read nor written. */
+enum { GATGPU_MASK_FULL = 0, GATGPU_MASK_PREFIX = 1 };
+enum { GATGPU_BIAS_NONE = 0, GATGPU_BIAS_LINEAR = 1, GATGPU_BIAS_TABLE = 2 };
+#define GATGPU_HIDDEN 255
+
+typedef struct gatgpu_attention gatgpu_attention; /* a plan: shape and segments */
+typedef struct gatgpu_attention_shape {
+    int precision;        /* GATGPU_FP32 or GATGPU_BF16                          */
+    int heads, kv_heads;  /* heads is a multiple of kv_heads                     */
+    int dim;
+    int mask, bias;
+    int buckets;          /* GATGPU_BIAS_TABLE: 1 to 64                          */
+    float scale;          /* > 0                                                 */
+    float cap;            /* 0: none                                             */
+} gatgpu_attention_shape;
+
+/* Plans the segments (a host array each; prefix NULL: 0) and uploads the
+ * tables of tiles.  Query rows of two segments must not overlap
+ * (GATGPU_EINVAL); key rows may (a shared prefix in a cache), but such a plan
+ * has no backward pass.  Lengths may be 0; q_len * heads / kv_heads and k_len
+ * are at most 2^30.  The plan belongs to ctx and is destroyed before it. */
+int gatgpu_attention_create(gatgpu_ctx* ctx, const gatgpu_attention_shape* shape, uint64_t segments,
+                            const uint64_t* q_begin, const uint32_t* q_len, const uint64_t* k_begin,
+                            const uint32_t* k_len, const uint32_t* prefix, gatgpu_attention** out);
+/* Waits for the context's stream and frees the plan; accepts NULL. */
+int gatgpu_attention_destroy(gatgpu_attention* plan);
+/* Bytes of device workspace (16-byte aligned) a forward / backward call needs;
+ * either may be NULL. */
+int gatgpu_attention_workspace(const gatgpu_attention* plan, uint64_t* forward, uint64_t* backward);
+/* Layout of the pair distances: segment s has q_len[s] rows of ld[s] bytes
+ * (k_len rounded up to 16) from offset[s] on, `bytes` in all; any may be NULL.
+ * (Offsets are those of tight packing in the order of the segments.) */
+int gatgpu_attention_distances(const gatgpu_attention* plan, uint64_t* bytes, uint64_t* offset, uint32_t* ld);
+
+/* Device arrays of one call.  Rows of `heads` (or kv_heads) vectors of dim
+ * elements side by side; strides in elements, 16-byte aligned like the bases,
+ * at least the row's width (so q, k and v may be parts of one array's rows). */
+typedef struct gatgpu_attention_io {
+    const void *q, *k, *v;
+    uint64_t q_stride, k_stride, v_stride;
+    const float* bias;    /* LINEAR: slope[heads]; TABLE: table[heads][buckets]  */
+    const uint8_t* dist;  /* TABLE: pair distances, 16-byte aligned              */
+    void* out;
+    uint64_t out_stride;
+    float* lse;           /* [row][heads], row as in out; forward: may be NULL   */
+    void* rest;           /* bf16, may be NULL: what rounding took from out, as
+                             bf16, in rows like out's.  With it the backward
+                             pass forms dout.out to FP32 accuracy, which dbias
+                             needs: required when dbias is given              */
+    const void* dout;
+    uint64_t dout_stride;
+    void *dq, *dk, *dv;
+    uint64_t dq_stride, dk_stride, dv_stride;
+    float* dbias;         /* TABLE: [heads][buckets], may be NULL                */
+} gatgpu_attention_io;
+
+/* Reads q, k, v, bias, dist; writes out, and lse and rest where given. */
+int gatgpu_attention_forward(gatgpu_attention* plan, const gatgpu_attention_io* io, void* workspace, uint64_t bytes);
+/* Gradients of a forward call: reads what it read, its out, lse and rest, and
+ * dout; writes dq, dk and dv of every row of a segment, and dbias.  Sums run in
+ * one fixed order: equal inputs give equal bits. */
+int gatgpu_attention_backward(gatgpu_attention* plan, const gatgpu_attention_io* io, void* workspace, uint64_t bytes);
+
+/* ---- layer norm -------------------------------------------------------- */
+/* No counterpart in the reference (which has no norm between layers).
+ *   h = x + residual, rounded to the storage type and written to sum (without
+ *   a residual: h = x);  n = (h - mean) rstd over the row's columns, rstd =
+ *   1 / sqrt(variance + eps);  y = n gamma + beta, through ELU if elu != 0
+ * and the gradients of x (= residual), gamma and beta.  Device arrays; rows of
+ * `width` elements at strides in elements, any alignment (16-byte aligned rows of
+ * whole 16 bytes are faster); gamma, beta, mean, rstd and their gradients are
+ * FP32.  Stream, capture, device and workspace: as gatgpu_attention_forward.
+ * y may be x or residual, sum x or residual, dx dy or dsum (same stride). */
+typedef struct gatgpu_norm_io {
+    int precision;        /* of the rows: GATGPU_FP32 or GATGPU_BF16             */
+    int elu;
+    uint64_t rows;
+    uint32_t width;
+    float eps;            /* >= 0                                                */
+    const void* x;
+    uint64_t x_stride;
+    const void* residual; /* NULL: none                                          */
+    uint64_t residual_stride;
+    void* sum;            /* with a residual: h, may be NULL in a forward call
+                             that no backward follows                            */
+    uint64_t sum_stride;
+    const float *gamma, *beta; /* NULL: 1 and 0                                  */
+    void* y;
+    uint64_t y_stride;
+    float *mean, *rstd;   /* [rows]; forward: may be NULL                        */
+    const void* dy;
+    uint64_t dy_stride;
+    const void* dsum;     /* gradient that reaches h beside y's, NULL: none      */
+    uint64_t dsum_stride;
+    void* dx;
+    uint64_t dx_stride;
+    float *dgamma, *dbeta; /* [width], may be NULL                               */
+} gatgpu_norm_io;
+
+int gatgpu_norm_forward(gatgpu_ctx* ctx, const gatgpu_norm_io* io);
+/* Reads h (sum where a residual is given, else x), mean, rstd, gamma, beta, dy
+ * and dsum; writes dx, dgamma and dbeta (sums in one fixed order). */
+int gatgpu_norm_backward(gatgpu_ctx* ctx, const gatgpu_norm_io* io, void* workspace, uint64_t bytes);
+/* Bytes of workspace of a backward call that gives dgamma or dbeta. */
+int gatgpu_norm_workspace(gatgpu_ctx* ctx, uint64_t rows, uint32_t width, uint64_t* bytes);
+/* Layer norm of the model's own layers: from now on the output of `layer` is
+ * norm(aggregation), through ELU where the layer is hidden, in every forward of
+ * the layer (gatgpu_layer_forward, gatgpu_model_forward,
+ * gatgpu_layer_forward_static); its OUT stage is that, in FP32.  gamma, beta:
+ * host FP32 [heads*dim], finite.  gamma and beta NULL: no norm any more.  The
+ * fixed-p operator has none.  set_layer(layer) drops it. */
+int gatgpu_set_norm(gatgpu_ctx* ctx, int layer, const float* gamma, const float* beta, float eps);
+
 /* ---- misc ------------------------------------------------------------ */
 int gatgpu_set_option(gatgpu_ctx* ctx, int key, int64_t value);
 /* Blocks until all work on the context's stream is done. */
