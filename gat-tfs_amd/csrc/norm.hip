@@ -197,6 +197,24 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_any(const NormArgs a) {
     }
 }
 
+// Chunks of one row as they lie in memory: requested a row ahead.
+template <class T, int VEC>
+struct Raw {
+    uint4 w;
+};
+template <class T>
+struct Raw<T, 1> {
+    T w;
+};
+template <class T, int VEC>
+__device__ inline Raw<T, VEC> load_raw(const T* p) {
+    return *reinterpret_cast<const Raw<T, VEC>*>(p);
+}
+template <class T, int VEC>
+__device__ inline void unpack(const Raw<T, VEC>& r, float (&v)[VEC]) {
+    load_vec<T, VEC>(reinterpret_cast<const T*>(&r), v);
+}
+
 template <class T, int VEC, int TPR, int ITEMS>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormArgs a) {
     constexpr int BLOCK = TPR < 256 ? 256 : TPR, GROUPS = BLOCK / TPR;
@@ -204,47 +222,67 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormAr
     __shared__ float cols[GROUPS > 1 ? GROUPS * TPR * VEC : 1];
     const uint32_t t = threadIdx.x % TPR, group = threadIdx.x / TPR, W = a.width;
     const float inv = 1.0f / float(W);
-    float dg[ITEMS][VEC], db[ITEMS][VEC];
+    float dg[ITEMS][VEC], db[ITEMS][VEC], w[ITEMS][VEC];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t c = (i * TPR + t) * VEC;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) dg[i][e] = db[i][e] = 0.0f;
+        for (int e = 0; e < VEC; ++e) dg[i][e] = db[i][e] = w[i][e] = 0.0f;
+        if (c < W) load_weights<VEC>(a.gamma, c, 1.0f, w[i]);
+    }
+    Raw<T, VEC> hr[ITEMS], yr[ITEMS], sr[ITEMS];
+    float mean = 0.0f, rstd = 0.0f;
+    const auto request = [&](uint64_t row) {
+        if (row >= a.rows) return;
+        mean = a.mean[row];
+        rstd = a.rstd[row];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t c = (i * TPR + t) * VEC;
+            if (c >= W) continue;
+            hr[i] = load_raw<T, VEC>(static_cast<const T*>(a.h) + row * a.hs + c);
+            yr[i] = load_raw<T, VEC>(static_cast<const T*>(a.dy) + row * a.dys + c);
+            if (a.dsum) sr[i] = load_raw<T, VEC>(static_cast<const T*>(a.dsum) + row * a.dss + c);
+        }
+    };
     // (Rows beyond the last leave a row group's lanes idle, not its reductions: all threads make
     // the same rounds.)
     const uint64_t step = uint64_t(gridDim.x) * GROUPS, first = uint64_t(blockIdx.x) * GROUPS;
+    request(first + group);
     for (uint64_t r0 = first; r0 < a.rows; r0 += step) {
         const uint64_t row = r0 + group;
         const bool in = row < a.rows;
         float n[ITEMS][VEC], g[ITEMS][VEC];
+        Raw<T, VEC> ar[ITEMS];
         float2 s = make_float2(0.0f, 0.0f);
-        const float mean = in ? a.mean[row] : 0.0f, rstd = in ? a.rstd[row] : 0.0f;
+        const float scale = rstd, shift = mean;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const uint32_t c = (i * TPR + t) * VEC;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) n[i][e] = g[i][e] = 0.0f;
-            if (in && c < W) {
-                load_vec<T, VEC>(static_cast<const T*>(a.h) + row * a.hs + c, n[i]);
-                load_vec<T, VEC>(static_cast<const T*>(a.dy) + row * a.dys + c, g[i]);
-            }
+            if (!in || c >= W) continue;
+            unpack<T, VEC>(hr[i], n[i]);
+            unpack<T, VEC>(yr[i], g[i]);
+            ar[i] = sr[i];
         }
+        request(row + step);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const uint32_t c = (i * TPR + t) * VEC;
             if (!in || c >= W) continue;
-            float w[VEC], b[VEC];
-            load_weights<VEC>(a.gamma, c, 1.0f, w);
+            float b[VEC];
             if (a.elu) load_weights<VEC>(a.beta, c, 0.0f, b);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                n[i][e] = (n[i][e] - mean) * rstd;
+                n[i][e] = (n[i][e] - shift) * scale;
                 if (a.elu) {
-                    const float y = fmaf(n[i][e], w[e], b[e]);
-                    if (y < 0.0f) g[i][e] *= exp_w(y);
+                    const float y = fmaf(n[i][e], w[i][e], b[e]);
+                    g[i][e] *= y < 0.0f ? exp_w(y) : 1.0f;
                 }
                 dg[i][e] = fmaf(g[i][e], n[i][e], dg[i][e]);
                 db[i][e] += g[i][e];
-                g[i][e] *= w[e];
+                g[i][e] *= w[i][e];
                 s.x += g[i][e];
                 s.y = fmaf(g[i][e], n[i][e], s.y);
             }
@@ -259,9 +297,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormAr
             float add[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) add[e] = 0.0f;
-            if (a.dsum) load_vec<T, VEC>(static_cast<const T*>(a.dsum) + row * a.dss + c, add);
+            if (a.dsum) unpack<T, VEC>(ar[i], add);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) g[i][e] = fmaf(rstd, g[i][e] - s.x - n[i][e] * s.y, add[e]);
+            for (int e = 0; e < VEC; ++e) g[i][e] = fmaf(scale, g[i][e] - s.x - n[i][e] * s.y, add[e]);
             store_vec<T, VEC>(static_cast<T*>(a.dx) + row * a.dxs + c, g[i]);
         }
     }
@@ -353,21 +391,34 @@ __global__ __launch_bounds__(256) void k_norm_cols_any(const NormArgs a) {
     a.part[uint64_t(blockIdx.y) * 2 * W + W + c] = db;
 }
 
-// dgamma, dbeta: 64 columns a block, 4 waves over the partial rows, added in one fixed order.
-__global__ __launch_bounds__(256) void k_norm_sum(const float* __restrict__ part, uint32_t blocks, uint32_t W, float* dgamma,
-                                                  float* dbeta) {
-    const uint64_t c = uint64_t(blockIdx.x) * 64 + (threadIdx.x & 63);
-    __shared__ float lds[256];
+// dgamma, dbeta: 32 columns a block, 32 threads a column over the partial rows, added in one
+// fixed order.
+__global__ __launch_bounds__(1024) void k_norm_sum(const float* __restrict__ part, uint32_t blocks, uint32_t W, float* dgamma,
+                                                   float* dbeta) {
+    const uint64_t c = uint64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
+    const uint32_t g = threadIdx.x >> 5;
+    __shared__ float lds[32][33];
     float sum = 0.0f;
-    if (c < 2 * uint64_t(W))
-        for (uint32_t b = threadIdx.x >> 6; b < blocks; b += 4) sum += part[uint64_t(b) * 2 * W + c];
-    lds[threadIdx.x] = sum;
+    if (c < 2 * uint64_t(W)) {
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t b = g;
+        for (; b + 96 < blocks; b += 128)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += part[uint64_t(b + 32 * i) * 2 * W + c];
+        for (; b < blocks; b += 32) s[0] += part[uint64_t(b) * 2 * W + c];
+        sum = (s[0] + s[1]) + (s[2] + s[3]);
+    }
+    lds[g][threadIdx.x & 31] = sum;
     __syncthreads();
-    if (threadIdx.x >= 64 || c >= 2 * uint64_t(W)) return;
-    sum = lds[threadIdx.x] + lds[threadIdx.x + 64] + lds[threadIdx.x + 128] + lds[threadIdx.x + 192];
-    if (c < W) {
-        if (dgamma) dgamma[c] = sum;
-    } else if (dbeta) dbeta[c - W] = sum;
+    // Column g's sums in lanes 0 to 31 of a half wave
+    sum = lds[threadIdx.x & 31][g];
+#pragma unroll
+    for (int d = 16; d; d /= 2) sum += __shfl_xor(sum, d);
+    const uint64_t at = uint64_t(blockIdx.x) * 32 + g;
+    if ((threadIdx.x & 31) || at >= 2 * uint64_t(W)) return;
+    if (at < W) {
+        if (dgamma) dgamma[at] = sum;
+    } else if (dbeta) dbeta[at - W] = sum;
 }
 
 // Threads a row and chunks a thread for a row of `chunks` chunks: the fewest threads that keep
@@ -376,7 +427,7 @@ struct NormShape {
     int tpr, items;
 };
 NormShape norm_shape(uint64_t chunks) {
-    const NormShape all[] = {{16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}};
+    const NormShape all[] = {{16, 1}, {32, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}, {1024, 4}};
     for (const NormShape& s : all)
         if (chunks <= uint64_t(s.tpr) * s.items) return s;
     return {0, 0};
@@ -386,7 +437,7 @@ bool aligned(const void* p, uint64_t stride, int size) {
 }
 
 #define GATGPU_NORM_SHAPES(F) \
-    F(16, 1) F(16, 2) F(64, 1) F(64, 2) F(64, 4) F(256, 2) F(256, 4) F(1024, 2) F(1024, 4)
+    F(16, 1) F(32, 1) F(64, 1) F(64, 2) F(256, 1) F(256, 2) F(512, 2) F(1024, 2) F(1024, 4)
 
 template <class T, int VEC>
 hipError_t forward(const NormArgs& a, NormShape s, hipStream_t st) {
@@ -414,10 +465,13 @@ hipError_t backward(const NormArgs& a, NormShape s, uint32_t blocks, hipStream_t
 
 }  // namespace
 
+// Blocks are persistent, so no more than run at once: three of 256 threads a CU (131 registers a
+// thread).  169K x 256 bf16, residual and ELU: 768 blocks 80 us, 512 97, 1024 108, 2048 91.
+// Wider rows take blocks of 512 threads, one or two a CU (8190 x 8192: 106 us at 256 and 512).
+// A partial row costs 16 bytes a column, written and read, a row 6 to 16 a column.
 uint32_t norm_blocks(uint64_t rows, uint64_t width) {
-    // Two blocks a CU, fewer where rows are few; wide rows one a CU (a partial row costs 8 bytes a column).
-    const uint64_t most = width > 4096 ? 256 : 512;
-    return uint32_t(std::max<uint64_t>(1, std::min(most, (rows + 3) / 4)));
+    const uint64_t most = width > 1024 ? 512 : 768;
+    return uint32_t(std::max<uint64_t>(1, std::min({most, std::max<uint64_t>(256, rows / 32), (rows + 3) / 4})));
 }
 
 hipError_t launch_norm_forward(const NormArgs& a, bool bf16, hipStream_t s) {
@@ -438,7 +492,7 @@ hipError_t launch_norm_backward(const NormArgs& a, bool bf16, uint32_t blocks, f
     if (bf16) e = wide ? backward<uint16_t, 8>(a, shape, blocks, s) : backward<uint16_t, 1>(a, shape, blocks, s);
     else e = wide ? backward<float, 4>(a, shape, blocks, s) : backward<float, 1>(a, shape, blocks, s);
     if (e != hipSuccess || !a.part) return e;
-    k_norm_sum<<<uint32_t((2 * uint64_t(a.width) + 63) / 64), 256, 0, s>>>(a.part, blocks, a.width, dgamma, dbeta);
+    k_norm_sum<<<uint32_t((2 * uint64_t(a.width) + 31) / 32), 1024, 0, s>>>(a.part, blocks, a.width, dgamma, dbeta);
     return hipGetLastError();
 }
 
