@@ -18,6 +18,7 @@ struct gatgpu_attention {
     gatgpu::DevBuf dsegs, dfwd, dbwd_q, dbwd_kv, djoin;
     uint64_t nfwd = 0, nbwd_q = 0, nbwd_kv = 0, njoin = 0;
     int wfwd = 1, wbwd_q = 1, wbwd_kv = 1;  // waves a block
+    gatgpu::AttnCap capped;
     bool split = false;
     bool spread = false;
 };
@@ -102,6 +103,10 @@ int build(gatgpu_attention* P) {
     for (const AttnSeg& s : P->segs) rows += s.q_len * group, keys += s.k_len;
     P->wfwd = P->wbwd_q = full(rows, q4) ? 4 : 1;
     P->wbwd_kv = full(keys, k4) ? 4 : 1;
+    // Wide tables for many shared heads leave no room for four waves' tiles.
+    const auto lds = sh.precision == GATGPU_BF16 ? attention_backward_lds_bf16 : attention_backward_lds_fp32;
+    if (lds(kAttnBackwardQ, sh.dim, P->wbwd_q, sh.bias, int(group), sh.buckets) > kAttnLds) P->wbwd_q = 1;
+    if (lds(kAttnBackwardKv, sh.dim, P->wbwd_kv, sh.bias, int(group), sh.buckets) > kAttnLds) P->wbwd_kv = 1;
 
     std::vector<AttnTask> fwd, bq, bk, join;
     const auto q_tiles = [&](std::vector<AttnTask>& out, uint32_t tile) {
@@ -238,6 +243,7 @@ AttnArgs make_args(const gatgpu_attention* P, const gatgpu_attention_io* io) {
     a.spread = P->spread;
     a.scale = sh.scale;
     a.cap = sh.cap;
+    a.capped = P->capped;
     a.q = io->q;
     a.k = io->k;
     a.v = io->v;
@@ -274,6 +280,7 @@ int create(gatgpu_ctx* c, const gatgpu_attention_shape* sh, uint64_t n, const ui
     std::unique_ptr<gatgpu_attention> P(new gatgpu_attention);
     P->ctx = c;
     P->shape = *sh;
+    P->capped = attention_cap(sh->scale, sh->cap);
     if (sh->bias != GATGPU_BIAS_TABLE) P->shape.buckets = 0;
     P->segs.resize(n);
     for (uint64_t s = 0; s < n; ++s) {
@@ -360,7 +367,7 @@ int gatgpu_attention_forward(gatgpu_attention* P, const gatgpu_attention_io* io,
         a.part = static_cast<float*>(ws);
         a.stat = reinterpret_cast<float*>(static_cast<char*>(ws) + part_bytes(P));
     }
-    HIPCHECK(c, launch_attention_forward(a, bf16, P->wfwd, c->stream));
+    HIPCHECK(c, (bf16 ? launch_attention_forward_bf16 : launch_attention_forward_fp32)(a, P->wfwd, c->stream));
     if (P->split) HIPCHECK(c, launch_attention_join(a, bf16, P->djoin.as<AttnTask>(), P->njoin, c->stream));
     return GATGPU_OK;
 }
@@ -399,11 +406,11 @@ int gatgpu_attention_backward(gatgpu_attention* P, const gatgpu_attention_io* io
     a.dbias = io->dbias ? reinterpret_cast<float*>(static_cast<char*>(ws) + delta_bytes(P)) : nullptr;
     a.tasks = P->dbwd_q.as<AttnTask>();
     a.ntasks = P->nbwd_q;
-    if (a.ntasks) HIPCHECK(c, launch_attention_backward_q(a, bf16, P->wbwd_q, c->stream));
+    if (a.ntasks) HIPCHECK(c, (bf16 ? launch_attention_backward_q_bf16 : launch_attention_backward_q_fp32)(a, P->wbwd_q, c->stream));
     if (io->dbias) HIPCHECK(c, launch_attention_bias_sum(a, io->dbias, c->stream));
     a.tasks = P->dbwd_kv.as<AttnTask>();
     a.ntasks = P->nbwd_kv;
-    if (a.ntasks) HIPCHECK(c, launch_attention_backward_kv(a, bf16, P->wbwd_kv, c->stream));
+    if (a.ntasks) HIPCHECK(c, (bf16 ? launch_attention_backward_kv_bf16 : launch_attention_backward_kv_fp32)(a, P->wbwd_kv, c->stream));
     return GATGPU_OK;
 }
 

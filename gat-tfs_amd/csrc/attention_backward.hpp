@@ -1,0 +1,431 @@
+// Segment attention, backward, in two passes without atomics, so that results do
+// not depend on an order of arrival.
+//
+//   p_ij = 2^(s_ij - lse_i),  dp_ij = dout_i.v_j,  delta_i = dout_i.out_i,  ds_ij = p_ij (dp_ij - delta_i)
+//   dbias = sum of ds over the pairs of a distance,  dx_ij = ds_ij (1 - tanh^2)
+//   dq_i = scale sum_j dx_ij k_j,  dk_j = scale sum_i dx_ij q_i,  dv_j = sum_i p_ij dout_i
+//
+// The first pass (k_attn_bwd_q) holds 32 query rows a wave and walks the keys, as the
+// forward pass does; it forms delta on its way and sums the bias gradient in LDS, a
+// column a lane.  The second (k_attn_bwd_kv) holds 32 keys a wave and walks the packed
+// query rows of all heads that share them, which sums the shared heads' gradients; its
+// weights and score gradients pass through LDS, whose transpose read makes them operands
+// that contract over the rows.
+// Scores and dp are formed in both: 7 products a pair where 5 would do with atomic
+// sums of dq.
+//
+// As in the forward pass, no element is checked for NaN or infinity on the way: they show in
+// the sums, and the block then goes over its tiles again.  (A bad row of K in the first pass, of Q
+// in the second, counts as 0 in the product with the score gradients, which hold a NaN wherever
+// the row is seen; rows that give it no weight are left as they were.)
+#pragma once
+#include "attention_tile.hpp"
+
+namespace gatgpu {
+namespace {
+
+// Sum of products of 16 bytes of a and b (+ c).
+template <class T>
+__device__ inline float dot16(uint4 a, uint4 b, uint4 c) {
+    const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+            sum = fmaf(__uint_as_float(av[i] << 16), __uint_as_float(bv[i] << 16) + __uint_as_float(cv[i] << 16), sum);
+            sum = fmaf(__uint_as_float(av[i] & 0xffff0000u),
+                       __uint_as_float(bv[i] & 0xffff0000u) + __uint_as_float(cv[i] & 0xffff0000u), sum);
+        } else {
+            sum = fmaf(__uint_as_float(av[i]), __uint_as_float(bv[i]), sum);
+        }
+    }
+    return sum;
+}
+
+
+template <class T, int D, int NW, int BIAS, bool CAP>
+__global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_q(const AttnArgs a) {
+    constexpr int BK = attn_tile_rows<T, NW>(), NB = BK / 32, ROW = lds_row<T, D>(), NF = D * int(sizeof(T)) / 32,
+                  DB = D / 32, NBUF = attn_buffers<T, NW>(), COLS = NW * 64;
+    constexpr bool TABLE = BIAS == GATGPU_BIAS_TABLE;
+    __shared__ __align__(16) char lds_k[NBUF][BK * ROW];
+    __shared__ __align__(16) char lds_v[NBUF][BK * ROW];
+    extern __shared__ float table[];  // TABLE: [group][256], then the table's gradient [buckets][COLS]
+
+    uint64_t task_id;
+    int kv;
+    if (!attn_task(a, task_id, kv)) return;
+    const AttnTask task = a.tasks[task_id];
+    const AttnSeg seg = a.segs[task.seg];
+    const int lane = int(threadIdx.x) & 63, wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6),
+              l32 = lane & 31, half = lane >> 5;
+    const uint32_t rows = seg.q_len * uint32_t(a.group), row0 = task.at + uint32_t(wave) * 32;
+    const bool idle = row0 >= rows, live = row0 + uint32_t(l32) < rows;
+    const AttnRow w = attn_row(a, seg, min(row0 + uint32_t(l32), rows - 1), kv);
+    const int lim_first = __builtin_amdgcn_readlane(w.lim, 0), lim_last = __builtin_amdgcn_readlane(w.lim, 31);
+    const int dim = a.dim;
+    const bool binned = TABLE && a.dbias;
+    float* bins = table + a.group * 256;
+    const T* kbase = static_cast<const T*>(a.k) + seg.k_begin * a.ks + uint64_t(kv) * dim;
+    const T* vbase = static_cast<const T*>(a.v) + seg.k_begin * a.vs + uint64_t(kv) * dim;
+    const uint32_t end = task.hi;
+    AttnStage<T, D, NW, BK> sk, sv;
+    sk.load(kbase, a.ks, 0, end, dim);
+    sv.load(vbase, a.vs, 0, end, dim);
+
+    const uint64_t grow = seg.q_begin + uint64_t(w.query);
+    float lse2 = a.lse[grow * uint64_t(a.heads) + w.head];
+    const bool dead = !live || lse2 == -INFINITY;  // sees nothing: its weights are 0
+    lse2 = dead ? INFINITY : lse2 * kLog2e;
+    uint4 qf[NF], dof[NF];
+    float delta = 0.0f;
+    {
+        const T* q = static_cast<const T*>(a.q) + grow * a.qs + uint64_t(w.head) * dim;
+        const T* d = static_cast<const T*>(a.dout) + grow * a.dos + uint64_t(w.head) * dim;
+        const T* o = static_cast<const T*>(a.out) + grow * a.os + uint64_t(w.head) * dim;
+        const T* e = a.rest ? static_cast<const T*>(a.rest) + grow * a.os + uint64_t(w.head) * dim : nullptr;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int at = (2 * f + half) * AttnType<T>::kPer;
+            const bool in = at < dim && !dead;
+            qf[f] = in ? *reinterpret_cast<const uint4*>(q + at) : make_uint4(0, 0, 0, 0);
+            dof[f] = in ? *reinterpret_cast<const uint4*>(d + at) : make_uint4(0, 0, 0, 0);
+            if (in)
+                delta += dot16<T>(dof[f], *reinterpret_cast<const uint4*>(o + at),
+                                  sizeof(T) == 2 && e ? *reinterpret_cast<const uint4*>(e + at) : make_uint4(0, 0, 0, 0));
+        }
+    }
+    delta = xor32_add(delta);
+    if (live && half == 0) a.delta[(seg.base + uint64_t(w.query)) * uint64_t(a.heads) + w.head] = delta;
+
+    const uint8_t* drow = TABLE ? a.dist + seg.dist + uint64_t(w.query) * seg.dist_ld : nullptr;
+    AttnDist dist[NB], next_dist[NB];
+    if constexpr (TABLE) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, b * 32 + 4 * half, seg.dist_ld);
+        fill_table(a, kv, table);
+    }
+    const float cc = a.scale * kLog2e;
+    const float slope2 = BIAS == GATGPU_BIAS_LINEAR ? a.bias[w.head] * kLog2e : 0.0f;
+    const float uncap = CAP ? 1.0f / a.capped.out : 0.0f;
+    const float* trow = table + w.local * 256;
+
+    f32x16_t acc[DB];
+    const auto pass = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
+        if (binned)
+            for (int b = 0; b < a.buckets; ++b) bins[b * COLS + threadIdx.x] = 0.0f;
+        uint32_t tile = 0;
+        for (uint32_t k0 = 0; k0 < end; k0 += BK, ++tile) {
+            const int buf = NBUF == 2 ? int(tile & 1) : 0;
+            if (NBUF == 1) __syncthreads();
+            sk.store(lds_k[buf]);
+            sv.store(lds_v[buf]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) dist[b] = next_dist[b];
+            __syncthreads();
+            if (k0 + BK < end) {
+                sk.load(kbase, a.ks, k0 + BK, end, dim);
+                sv.load(vbase, a.vs, k0 + BK, end, dim);
+                if constexpr (TABLE) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, k0 + BK + b * 32 + 4 * half, seg.dist_ld);
+                }
+            }
+            if (idle || int(k0) >= lim_last) continue;
+            const bool masked = int(k0) + BK > lim_first;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                    const int at = (b * 32 + l32) * ROW + f * 32 + half * 16;
+                    s = mfma_rows<T>(s, *reinterpret_cast<const uint4*>(lds_k[buf] + at), qf[f]);
+                    dp = mfma_rows<T>(dp, *reinterpret_cast<const uint4*>(lds_v[buf] + at), dof[f]);
+                }
+                f32x16_t y;
+                score_gradients<BIAS, CAP, CAREFUL>(a, s, dp, y, cc, uncap, slope2, float(w.pos - int(k0) - b * 32 - 4 * half),
+                                                    dist[b], trow, masked ? w.lim - int(k0) - b * 32 - 4 * half : 32, lse2,
+                                                    delta, masked);
+                if constexpr (TABLE) {
+                    if (binned && live) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            bins[min(int(dist_of(dist[b], r)), a.buckets - 1) * COLS + threadIdx.x] += y[r];
+                    }
+                }
+                if constexpr (CAP) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) y[r] *= s[r];
+                }
+                const AttnCols<T> p = to_operand<T>(y);
+                const char* krows = lds_k[buf] + b * 32 * ROW;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+                    acc[d] = mfma_cols<T>(acc[d], load_cols<T, CAREFUL ? kClean : kRaw>(krows, ROW, d * 32, lane), p);
+            }
+        }
+    };
+    if constexpr (TABLE) __syncthreads();
+    pass(std::false_type{});
+    const bool bad = !idle && nonfinite(acc);
+    if (NW == 1 ? __any(bad) : __syncthreads_or(bad)) {
+        if (NW > 1) __syncthreads();
+        sk.load(kbase, a.ks, 0, end, dim);
+        sv.load(vbase, a.vs, 0, end, dim);
+        if constexpr (TABLE) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, b * 32 + 4 * half, seg.dist_ld);
+        }
+        pass(std::true_type{});
+    }
+    if (live) {
+        const uint64_t to = grow * a.dqs + uint64_t(w.head) * dim;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = d * 32 + 8 * i + 4 * half;
+                if (at < dim)
+                    store4<T>(a.dq, to + at, acc[d][4 * i] * a.scale, acc[d][4 * i + 1] * a.scale,
+                              acc[d][4 * i + 2] * a.scale, acc[d][4 * i + 3] * a.scale);
+            }
+    }
+    if (!binned) return;
+    // Each bucket's columns, by head of the group, in one fixed order.
+    __syncthreads();
+    float* to = a.dbias + (task_id * uint64_t(a.kv_heads) + uint64_t(kv)) * uint64_t(a.group * a.buckets);
+    for (int b = wave; b < a.buckets; b += NW)
+        for (int g = 0; g < a.group; ++g) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < NW; ++v) {
+                const float x = bins[b * COLS + v * 64 + lane];
+                sum += int((task.at + uint32_t(v) * 32 + uint32_t(l32)) % uint32_t(a.group)) == g ? x : 0.0f;
+            }
+#pragma unroll
+            for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+            if (lane == 0) to[g * a.buckets + b] = sum;
+        }
+}
+
+template <class T, int D, int NW, int BIAS, bool CAP>
+__global__ __launch_bounds__(NW * 64, (D < 128 ? attn_waves<T, D, NW>() : 1)) void k_attn_bwd_kv(const AttnArgs a) {
+    constexpr int BQ = attn_tile_rows<T, NW>(), NB = BQ / 32, ROW = lds_row<T, D>(), NF = D * int(sizeof(T)) / 32,
+                  DB = D / 32, NBUF = attn_buffers<T, NW>(), PROW = attn_turn_row<T>();
+    constexpr bool TABLE = BIAS == GATGPU_BIAS_TABLE;
+    __shared__ __align__(16) char lds_q[NBUF][BQ * ROW];
+    __shared__ __align__(16) char lds_o[NBUF][BQ * ROW];
+    __shared__ __align__(16) char lds_p[NW][2][32 * PROW];  // a wave's weights and score gradients, a row a query
+    // Per packed row of a tile: log-sum in units of log2 (+inf: weighs nothing), delta, keys seen,
+    // position, slope, first entry of its table, query
+    __shared__ float r_lse[NBUF][BQ], r_delta[NBUF][BQ], r_slope[NBUF][BQ];
+    __shared__ int r_lim[NBUF][BQ], r_pos[NBUF][BQ], r_tab[NBUF][BQ], r_query[NBUF][BQ];
+    extern __shared__ float table[];  // TABLE: [group][256]
+
+    uint64_t task_id;
+    int kv;
+    if (!attn_task(a, task_id, kv)) return;
+    const AttnTask task = a.tasks[task_id];
+    const AttnSeg seg = a.segs[task.seg];
+    const int tid = int(threadIdx.x), lane = tid & 63,
+              wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
+    const uint32_t key0 = task.at + uint32_t(wave) * 32, key = key0 + uint32_t(l32);
+    const bool idle = key0 >= seg.k_len;
+    const int dim = a.dim;
+    const uint64_t grow = seg.k_begin + min(key, seg.k_len - 1);
+    uint4 kf[NF], vf[NF];
+    {
+        const T* k = static_cast<const T*>(a.k) + grow * a.ks + uint64_t(kv) * dim;
+        const T* v = static_cast<const T*>(a.v) + grow * a.vs + uint64_t(kv) * dim;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int at = (2 * f + half) * AttnType<T>::kPer;
+            kf[f] = at < dim ? *reinterpret_cast<const uint4*>(k + at) : make_uint4(0, 0, 0, 0);
+            vf[f] = at < dim ? *reinterpret_cast<const uint4*>(v + at) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    const T* qbase = static_cast<const T*>(a.q) + seg.q_begin * a.qs + uint64_t(kv) * uint64_t(a.group * dim);
+    const T* obase = static_cast<const T*>(a.dout) + seg.q_begin * a.dos + uint64_t(kv) * uint64_t(a.group * dim);
+    const uint32_t rows = seg.q_len * uint32_t(a.group), end = min(task.hi, rows);
+    if constexpr (TABLE) fill_table(a, kv, table);
+    const float cc = a.scale * kLog2e, uncap = CAP ? 1.0f / a.capped.out : 0.0f;
+
+    f32x16_t acc_k[DB], acc_v[DB];
+    AttnStage<T, D, NW, BQ> sq, so;
+    float n_lse = 0.0f, n_delta = 0.0f;
+    const auto request = [&](uint32_t r0) {
+        sq.load_packed(qbase, a.qs, r0, end, dim, a.group);
+        so.load_packed(obase, a.dos, r0, end, dim, a.group);
+        if (tid < BQ) {
+            const uint32_t r = r0 + uint32_t(tid);
+            n_lse = INFINITY;
+            n_delta = 0.0f;
+            if (r < end) {
+                const uint32_t q = r / uint32_t(a.group);
+                const uint64_t h = uint64_t(kv) * uint64_t(a.group) + (r - q * uint32_t(a.group));
+                const float x = a.lse[(seg.q_begin + q) * uint64_t(a.heads) + h];
+                n_lse = x == -INFINITY ? INFINITY : x * kLog2e;
+                n_delta = a.delta[(seg.base + q) * uint64_t(a.heads) + h];
+            }
+        }
+    };
+    const auto pass = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc_k[d] = acc_v[d] = f32x16_t{};
+        if (task.lo < end) request(task.lo);
+        uint32_t tile = 0;
+        for (uint32_t r0 = task.lo; r0 < end; r0 += BQ, ++tile) {
+            const int buf = NBUF == 2 ? int(tile & 1) : 0;
+            if (NBUF == 1) __syncthreads();
+            sq.store(lds_q[buf]);
+            so.store(lds_o[buf]);
+            if (tid < BQ) {
+                const AttnRow w = attn_row(a, seg, min(r0 + uint32_t(tid), rows - 1), kv);
+                r_lse[buf][tid] = n_lse;
+                r_delta[buf][tid] = n_delta;
+                r_lim[buf][tid] = w.lim;
+                if (BIAS == GATGPU_BIAS_LINEAR) {
+                    r_pos[buf][tid] = w.pos;
+                    r_slope[buf][tid] = a.bias[w.head] * kLog2e;
+                }
+                if (TABLE) {
+                    r_tab[buf][tid] = w.local * 256;
+                    r_query[buf][tid] = w.query;
+                }
+            }
+            __syncthreads();
+            if (r0 + BQ < end) request(r0 + BQ);
+            if (idle) continue;
+            AttnDist dist[NB];
+            if constexpr (TABLE) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    dist[b] = load_dist(a.dist + seg.dist + uint64_t(r_query[buf][b * 32 + l32]) * seg.dist_ld, key0 + 4 * half,
+                                        seg.dist_ld);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int row = b * 32 + l32, lim = r_lim[buf][row];
+                const int lim_first = __builtin_amdgcn_readlane(lim, 0), lim_last = __builtin_amdgcn_readlane(lim, 31);
+                if (int(key0) >= lim_last) continue;
+                const bool masked = int(key0) + 32 > lim_first;
+                f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                    const int at = row * ROW + f * 32 + half * 16;
+                    s = mfma_rows<T>(s, kf[f], *reinterpret_cast<const uint4*>(lds_q[buf] + at));
+                    dp = mfma_rows<T>(dp, vf[f], *reinterpret_cast<const uint4*>(lds_o[buf] + at));
+                }
+                f32x16_t y, p;
+                score_gradients<BIAS, CAP, CAREFUL>(
+                    a, s, dp, y, cc, uncap, BIAS == GATGPU_BIAS_LINEAR ? r_slope[buf][row] : 0.0f,
+                    BIAS == GATGPU_BIAS_LINEAR ? float(r_pos[buf][row] - int(key0) - 4 * half) : 0.0f, dist[b],
+                    table + (TABLE ? r_tab[buf][row] : 0), masked ? lim - int(key0) - 4 * half : 32, r_lse[buf][row],
+                    r_delta[buf][row], masked, &p);
+                if constexpr (CAP) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) y[r] *= s[r];
+                }
+                char* turn = lds_p[wave][0];
+                turn_store<T>(turn, p, lane);
+                turn_store<T>(turn + 32 * PROW, y, lane);
+                wave_sync();
+                const AttnCols<T> pc = load_cols<T>(turn, PROW, 0, lane), yc = load_cols<T>(turn + 32 * PROW, PROW, 0, lane);
+                const char* orows = lds_o[buf] + b * 32 * ROW;
+                const char* qrows = lds_q[buf] + b * 32 * ROW;
+                if constexpr (CAREFUL) {
+                    f32x16_t one;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) one[r] = p[r] == 0.0f ? 0.0f : 1.0f;
+                    wave_sync();
+                    turn_store<T>(turn, one, lane);
+                    wave_sync();
+                    const AttnCols<T> seen = load_cols<T>(turn, PROW, 0, lane);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc_v[d] = mfma_cols_careful<T>(acc_v[d], orows, ROW, d * 32, lane, pc, seen);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc_v[d] = mfma_cols<T>(acc_v[d], load_cols<T>(orows, ROW, d * 32, lane), pc);
+                }
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+                    acc_k[d] = mfma_cols<T>(acc_k[d], load_cols<T, CAREFUL ? kClean : kRaw>(qrows, ROW, d * 32, lane), yc);
+                wave_sync();
+            }
+        }
+    };
+    __syncthreads();
+    pass(std::false_type{});
+    const bool bad = !idle && (nonfinite(acc_k) || nonfinite(acc_v));
+    if (NW == 1 ? __any(bad) : __syncthreads_or(bad)) {
+        if (NW > 1) __syncthreads();
+        pass(std::true_type{});
+    }
+    if (key >= seg.k_len) return;
+    const uint64_t tk = grow * a.dks + uint64_t(kv) * dim, tv = grow * a.dvs + uint64_t(kv) * dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = d * 32 + 8 * i + 4 * half;
+            if (at >= dim) continue;
+            store4<T>(a.dk, tk + at, acc_k[d][4 * i] * a.scale, acc_k[d][4 * i + 1] * a.scale, acc_k[d][4 * i + 2] * a.scale,
+                      acc_k[d][4 * i + 3] * a.scale);
+            store4<T>(a.dv, tv + at, acc_v[d][4 * i], acc_v[d][4 * i + 1], acc_v[d][4 * i + 2], acc_v[d][4 * i + 3]);
+        }
+}
+
+// LDS of a block, as the kernels declare it.
+template <class T, int D, int NW>
+constexpr size_t lds_q_pass() {
+    return size_t(attn_buffers<T, NW>()) * 2 * attn_tile_rows<T, NW>() * lds_row<T, D>();
+}
+template <class T, int D, int NW>
+constexpr size_t lds_kv_pass() {
+    return lds_q_pass<T, D, NW>() + size_t(NW) * 2 * 32 * attn_turn_row<T>() +
+           size_t(attn_buffers<T, NW>()) * attn_tile_rows<T, NW>() * 7 * 4;
+}
+template <class T>
+size_t backward_lds(int pass, int dim, int waves, int bias, int group, int buckets) {
+    AttnArgs a;
+    a.dim = dim;
+    size_t bytes = 0;
+    (void)attn_dispatch(a, waves, [&](auto d, auto nw, auto, auto) {
+        constexpr int D = decltype(d)::value, NW = decltype(nw)::value;
+        bytes = pass == kAttnBackwardKv ? lds_kv_pass<T, D, NW>() : lds_q_pass<T, D, NW>();
+        return hipSuccess;
+    });
+    if (bias == GATGPU_BIAS_TABLE) {
+        bytes += size_t(group) * 1024;
+        if (pass == kAttnBackwardQ) bytes += size_t(buckets) * size_t(waves) * 256;
+    }
+    return bytes;
+}
+
+template <class T>
+hipError_t backward_q(const AttnArgs& a, int waves, hipStream_t s) {
+    return attn_dispatch(a, waves, [&](auto d, auto nw, auto bias, auto cap) {
+        constexpr int NW = decltype(nw)::value, BIAS = decltype(bias)::value;
+        const size_t dyn = BIAS == GATGPU_BIAS_TABLE ? size_t(a.group) * 1024 + (a.dbias ? size_t(a.buckets) * NW * 256 : 0) : 0;
+        k_attn_bwd_q<T, decltype(d)::value, NW, BIAS, decltype(cap)::value>
+            <<<uint32_t(attn_blocks(a)), NW * 64, dyn, s>>>(a);
+        return hipGetLastError();
+    });
+}
+template <class T>
+hipError_t backward_kv(const AttnArgs& a, int waves, hipStream_t s) {
+    return attn_dispatch(a, waves, [&](auto d, auto nw, auto bias, auto cap) {
+        constexpr int NW = decltype(nw)::value, BIAS = decltype(bias)::value;
+        const size_t dyn = BIAS == GATGPU_BIAS_TABLE ? size_t(a.group) * 1024 : 0;
+        k_attn_bwd_kv<T, decltype(d)::value, NW, BIAS, decltype(cap)::value>
+            <<<uint32_t(attn_blocks(a)), NW * 64, dyn, s>>>(a);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace
+}  // namespace gatgpu

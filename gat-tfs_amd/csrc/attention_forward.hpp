@@ -1,0 +1,245 @@
+// Segment attention, forward: one pass over a row's keys with the running maximum
+// and sum of the softmax.
+//
+//   x_j = scale q.k_j,  y_j = cap tanh(x_j / cap),  s_j = y_j + bias(distance)
+//   m' = max(m, max s_j),  l' = l 2^(m - m') + sum 2^(s_j - m'),  O' = O 2^(m - m') + sum 2^(s_j - m') v_j
+// (in units of log2) and out = O / l, lse = ln 2 (m + log2 l).  Capped scores without a bias
+// stay within cap: they need no maximum, m is 0 throughout.
+//
+// A wave holds 32 packed query rows; scores are formed transposed (keys x rows), so
+// that a lane owns half a row's scores, its statistics are plain registers and the
+// weights are the operand of the second product as they stand.  Four waves share tiles
+// of 64 keys through LDS, requested a tile ahead; short segments and split key ranges run
+// one wave a block on tiles of 32.  m, l and O are FP32.
+//
+// The loop checks no element for NaN or infinity: a bad value in a tile shows in the sums of
+// every row that met it (0 x NaN), and then the block goes over its keys again, letting it
+// reach only the rows that see it.
+#pragma once
+#include "attention_tile.hpp"
+
+namespace gatgpu {
+namespace {
+
+template <class T, int D, int NW, int BIAS, bool CAP>
+__global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(const AttnArgs a) {
+    constexpr int BK = attn_tile_rows<T, NW>(), NB = BK / 32, ROW = lds_row<T, D>(), NF = D * int(sizeof(T)) / 32,
+                  DB = D / 32, NBUF = attn_buffers<T, NW>();
+    __shared__ __align__(16) char lds_k[NBUF][BK * ROW];
+    __shared__ __align__(16) char lds_v[NBUF][BK * ROW];
+    extern __shared__ float table[];  // TABLE: [group][256]
+
+    uint64_t task_id;
+    int kv;
+    if (!attn_task(a, task_id, kv)) return;
+    const AttnTask task = a.tasks[task_id];
+    const AttnSeg seg = a.segs[task.seg];
+    const int lane = int(threadIdx.x) & 63, wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6),
+              l32 = lane & 31, half = lane >> 5;
+    const uint32_t rows = seg.q_len * uint32_t(a.group), row0 = task.at + uint32_t(wave) * 32;
+    const bool idle = row0 >= rows;
+    const AttnRow w = attn_row(a, seg, min(row0 + uint32_t(l32), rows - 1), kv);
+    // Rows are in order of their queries, so the wave's limits are those of its first and last lane.
+    const int lim_first = __builtin_amdgcn_readlane(w.lim, 0), lim_last = __builtin_amdgcn_readlane(w.lim, 31);
+    const int dim = a.dim;
+    const T* kbase = static_cast<const T*>(a.k) + seg.k_begin * a.ks + uint64_t(kv) * dim;
+    const T* vbase = static_cast<const T*>(a.v) + seg.k_begin * a.vs + uint64_t(kv) * dim;
+    const uint32_t end = task.hi;
+    AttnStage<T, D, NW, BK> sk, sv;
+    sk.load(kbase, a.ks, task.lo, end, dim);
+    sv.load(vbase, a.vs, task.lo, end, dim);
+
+    uint4 qf[NF];
+    {
+        const T* q = static_cast<const T*>(a.q) + (seg.q_begin + uint64_t(w.query)) * a.qs + uint64_t(w.head) * dim;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int at = (2 * f + half) * AttnType<T>::kPer;
+            qf[f] = at < dim ? *reinterpret_cast<const uint4*>(q + at) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    const uint8_t* drow = BIAS == GATGPU_BIAS_TABLE ? a.dist + seg.dist + uint64_t(w.query) * seg.dist_ld : nullptr;
+    AttnDist dist[NB], next_dist[NB];
+    if constexpr (BIAS == GATGPU_BIAS_TABLE) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, task.lo + b * 32 + 4 * half, seg.dist_ld);
+        fill_table(a, kv, table);
+    }
+    const float cc = a.scale * kLog2e;
+    const float slope2 = BIAS == GATGPU_BIAS_LINEAR ? a.bias[w.head] * kLog2e : 0.0f;
+    const float* trow = table + w.local * 256;
+    const bool bounded = CAP && BIAS == GATGPU_BIAS_NONE && a.capped.bounded;
+    const bool exact = sizeof(T) == 2 && BIAS == GATGPU_BIAS_TABLE && a.rest;  // weights to 16 bits: delta's
+
+    f32x16_t acc[DB];
+    float m, l;
+    const auto pass = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
+        m = bounded ? 0.0f : -INFINITY;
+        l = 0.0f;
+        uint32_t tile = 0;
+        for (uint32_t k0 = task.lo; k0 < end; k0 += BK, ++tile) {
+            const int buf = NBUF == 2 ? int(tile & 1) : 0;
+            if (NBUF == 1) __syncthreads();
+            sk.store(lds_k[buf]);
+            sv.store(lds_v[buf]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) dist[b] = next_dist[b];
+            __syncthreads();
+            if (k0 + BK < end) {
+                sk.load(kbase, a.ks, k0 + BK, end, dim);
+                sv.load(vbase, a.vs, k0 + BK, end, dim);
+                if constexpr (BIAS == GATGPU_BIAS_TABLE) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, k0 + BK + b * 32 + 4 * half, seg.dist_ld);
+                }
+            }
+            if (idle || int(k0) >= lim_last) continue;  // (uniform over the wave; no barrier follows in the tile)
+            f32x16_t s[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                s[b] = f32x16_t{};
+#pragma unroll
+                for (int f = 0; f < NF; ++f)
+                    s[b] = mfma_rows<T>(
+                        s[b], *reinterpret_cast<const uint4*>(lds_k[buf] + (b * 32 + l32) * ROW + f * 32 + half * 16), qf[f]);
+                if constexpr (CAP) cap_scores(a.capped, s[b]);
+                bias_scores<BIAS, CAP, CAREFUL>(s[b], cc, slope2, float(w.pos - int(k0) - b * 32 - 4 * half), dist[b], trow);
+            }
+            if (int(k0) + BK > lim_first) {
+                const int left = w.lim - int(k0) - 4 * half;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (b * 32 + 8 * (r / 4) + r % 4 >= left) s[b][r] = -INFINITY;
+            }
+            constexpr bool RAW = BIAS == GATGPU_BIAS_NONE && !CAP;  // scores still to be scaled
+            float sum = 0.0f;
+            if (bounded) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        s[b][r] = exp2_hw(s[b][r]);
+                        sum += s[b][r];
+                    }
+            } else {
+                float top = s[0][0];
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+                top = xor32_max(top);
+                if (RAW) top *= cc;
+                const float next = fmaxf(m, top), ref = next == -INFINITY ? 0.0f : next;  // nothing seen yet: all weights 0
+                if (__any(next > m)) {
+                    const float fall = exp2_hw(m - ref);
+                    l *= fall;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[d][r] *= fall;
+                }
+                m = next;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        s[b][r] = exp2_hw(RAW ? fmaf(s[b][r], cc, -ref) : s[b][r] - ref);
+                        sum += s[b][r];
+                    }
+            }
+            l += sum;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const AttnCols<T> p = to_operand<T>(s[b]);
+                const char* vrows = lds_v[buf] + b * 32 * ROW;
+                if constexpr (CAREFUL) {
+                    const AttnCols<T> seen = seen_operand<T>(s[b]);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc[d] = mfma_cols_careful<T>(acc[d], vrows, ROW, d * 32, lane, p, seen);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc[d] = mfma_cols<T>(acc[d], load_cols<T>(vrows, ROW, d * 32, lane), p);
+                }
+                if constexpr (sizeof(T) == 2 && BIAS == GATGPU_BIAS_TABLE) {
+                    if (exact) {
+                        const AttnCols<T> lo = rest_operand(s[b], p);
+#pragma unroll
+                        for (int d = 0; d < DB; ++d)
+                            acc[d] = mfma_cols<T>(acc[d], load_cols<T, CAREFUL ? kClean : kRaw>(vrows, ROW, d * 32, lane), lo);
+                    }
+                }
+            }
+        }
+    };
+    if constexpr (BIAS == GATGPU_BIAS_TABLE) __syncthreads();
+    pass(std::false_type{});
+    const bool bad = !idle && nonfinite(acc);
+    if (NW == 1 ? __any(bad) : __syncthreads_or(bad)) {
+        if (NW > 1) __syncthreads();
+        sk.load(kbase, a.ks, task.lo, end, dim);
+        sv.load(vbase, a.vs, task.lo, end, dim);
+        if constexpr (BIAS == GATGPU_BIAS_TABLE) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, task.lo + b * 32 + 4 * half, seg.dist_ld);
+        }
+        if (NW == 1) __syncthreads();
+        pass(std::true_type{});
+    }
+    if (idle) return;
+    l = xor32_add(l);
+    if (a.part) {  // a range of the keys: joined by k_attn_join
+        const uint64_t at = (task_id * uint64_t(a.kv_heads) + uint64_t(kv)) * (NW * 32) + uint64_t(wave * 32 + l32);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                store4<float>(a.part, at * D + d * 32 + 8 * i + 4 * half, acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2],
+                              acc[d][4 * i + 3]);
+        if (half == 0) *reinterpret_cast<float2*>(a.stat + at * 2) = make_float2(m, l);
+        return;
+    }
+    if (row0 + uint32_t(l32) >= rows) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // nothing seen: 0
+    const uint64_t to = (seg.q_begin + uint64_t(w.query)) * a.os + uint64_t(w.head) * dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = d * 32 + 8 * i + 4 * half;
+            if (at >= dim) continue;
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = acc[d][4 * i + e] * inv;
+            store4<T>(a.out, to + at, o[0], o[1], o[2], o[3]);
+            if (sizeof(T) == 2 && a.rest) {  // what the rounding took
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] -= bf16_widen(bf16_hw(o[e]));
+                store4<T>(a.rest, to + at, o[0], o[1], o[2], o[3]);
+            }
+        }
+    if (a.lse && half == 0)
+        a.lse[(seg.q_begin + uint64_t(w.query)) * uint64_t(a.heads) + w.head] =
+            l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
+}
+
+template <class T, int D, int NW, int BIAS, bool CAP>
+hipError_t forward_as(const AttnArgs& a, hipStream_t s) {
+    const size_t dyn = BIAS == GATGPU_BIAS_TABLE ? size_t(a.group) * 1024 : 0;
+    k_attn_fwd<T, D, NW, BIAS, CAP><<<uint32_t(attn_blocks(a)), NW * 64, dyn, s>>>(a);
+    return hipGetLastError();
+}
+
+template <class T>
+hipError_t forward(const AttnArgs& a, int waves, hipStream_t s) {
+    return attn_dispatch(a, waves, [&](auto d, auto nw, auto bias, auto cap) {
+        return forward_as<T, decltype(d)::value, decltype(nw)::value, decltype(bias)::value, decltype(cap)::value>(a, s);
+    });
+}
+
+}  // namespace
+}  // namespace gatgpu

@@ -381,9 +381,11 @@ typedef struct gatgpu_attention_io {
     uint64_t out_stride;
     float* lse;           /* [row][heads], row as in out; forward: may be NULL   */
     void* rest;           /* bf16, may be NULL: what rounding took from out, as
-                             bf16, in rows like out's.  With it the backward
-                             pass forms dout.out to FP32 accuracy, which dbias
-                             needs: required when dbias is given              */
+                             bf16, in rows like out's, between a forward call
+                             and its backward call.  With a table bias the
+                             forward weights then enter as two bf16 each, and
+                             the backward pass has dout.out to 16 bits, which
+                             dbias needs: required when dbias is given        */
     const void* dout;
     uint64_t dout_stride;
     void *dq, *dk, *dv;

@@ -207,12 +207,16 @@ def test_same_bits_twice_and_without_training_arrays(ctx, precision):
         assert torch.equal(a[n], b[n]), n
     with p.plan(ctx) as plan:
         out, io = p.buffers(train=False)
+        rest = torch.empty_like(out["out"])  # (with it the weights keep 16 bits, so out may round otherwise without it)
         io.lse = None
+        if precision == BF:
+            io.rest = rest.data_ptr()
         ws = torch.empty(max(1, plan.workspace_bytes()), dtype=torch.uint8, device="cuda")
         torch.cuda.synchronize()
         plan.forward(io, ws.data_ptr(), ws.numel())
         ctx.synchronize()
     assert torch.equal(out["out"], a["out"]) and bool((out["lse"] == 7.0).all())
+    p.check(p.run(ctx, train=False), train=False)
 
 
 def test_shared_key_rows(ctx):
