@@ -15,8 +15,9 @@ struct gatgpu_attention {
     uint64_t rows = 0, dist_bytes = 0;
     bool shared_keys = false;  // key rows of two segments overlap
     // Tables on the device: segments; tiles of the forward, the query and the key pass; joined tiles.
-    gatgpu::DevBuf dsegs, dfwd, dbwd_q, dbwd_kv, djoin;
-    uint64_t nfwd = 0, nbwd_q = 0, nbwd_kv = 0, njoin = 0;
+    // Short segments: forward of one and two blocks of 32 keys, backward of 1, 2 and 4 waves.
+    gatgpu::DevBuf dsegs, dsmall[2], dsmall_bwd[3], dfwd, dbwd_q, dbwd_kv, djoin;
+    uint64_t nsmall[2] = {}, nsmall_bwd[3] = {}, small_parts = 0, nfwd = 0, nbwd_q = 0, nbwd_kv = 0, njoin = 0;
     int wfwd = 1, wbwd_q = 1, wbwd_kv = 1;  // waves a block
     gatgpu::AttnCap capped;
     bool split = false;
@@ -89,29 +90,75 @@ int build(gatgpu_attention* P) {
     gatgpu_ctx* c = P->ctx;
     const gatgpu_attention_shape& sh = P->shape;
     const uint64_t group = uint64_t(sh.heads / sh.kv_heads), kvh = uint64_t(sh.kv_heads), cus = uint64_t(c->cus);
-    uint64_t q4 = 0, k4 = 0, longest = 0;  // blocks of four waves, by rows and by keys
+    // Short segments go to the kernels that hold all their keys (their bias gradients are summed
+    // by lanes, so the query heads of a key/value head must divide 32).
+    const bool bf16 = sh.precision == GATGPU_BF16;
+    const int width = attention_width(sh.dim);
+    const bool holds = bf16 ? attention_small_width<uint16_t>(width) : attention_small_width<float>(width);
+    const auto small = [&](const AttnSeg& s) { return holds && s.k_len > 0 && s.k_len <= 64; };
+    uint32_t most = 0;  // keys of a short segment's backward pass
+    for (uint32_t w = 1; w <= 4 && 32 % group == 0; w *= 2)
+        if ((bf16 ? attention_small_backward_lds_bf16 : attention_small_backward_lds_fp32)(sh.dim, int(w), sh.bias, int(group),
+                                                                                           sh.buckets) <= kAttnLds)
+            most = 32 * w;
+    const auto small_bwd = [&](const AttnSeg& s) { return s.k_len > 0 && s.k_len <= most; };
+    std::vector<AttnTask> sf[2], sb[3];
+    const auto waves_of = [](const AttnSeg& s) { return s.k_len <= 32 ? 0 : s.k_len <= 64 ? 1 : 2; };  // log2
+    uint64_t count_f[2] = {}, count_b[3] = {};
     for (const AttnSeg& s : P->segs) {
-        q4 += (s.q_len * group + 127) / 128;
-        k4 += (uint64_t(s.k_len) + 127) / 128;
-        if (s.q_len) longest = std::max<uint64_t>(longest, s.k_len);
+        if (small(s)) ++count_f[s.k_len > 32];
+        if (small_bwd(s)) ++count_b[waves_of(s)];
+    }
+    // Heads a block: as many as leave 8 waves a SIMD, since each of them starts with a trip to memory.
+    const auto run = [&](uint64_t count, uint64_t waves) {
+        return std::max<uint64_t>(1, std::min(kvh, count * waves * kvh / (32 * cus)));
+    };
+    for (size_t s = 0; s < P->segs.size(); ++s) {
+        const AttnSeg& g = P->segs[s];
+        const auto add = [&](std::vector<AttnTask>& to, uint64_t heads) {
+            for (uint64_t h = 0; h < kvh; h += heads)
+                to.push_back({uint32_t(s), uint32_t(P->small_parts), uint32_t(h), uint32_t(std::min(kvh, h + heads))});
+        };
+        if (small(g) && g.q_len) add(sf[g.k_len > 32], run(count_f[g.k_len > 32], 1));
+        if (small_bwd(g)) {
+            const int w = waves_of(g);
+            add(sb[w], run(count_b[w], uint64_t(1) << w));
+            ++P->small_parts;
+        }
+    }
+    // What the general kernels take: blocks of four waves by rows and by keys, rows, keys.
+    uint64_t f4 = 0, q4 = 0, k4 = 0, frows = 0, brows = 0, keys = 0, longest = 0;
+    for (const AttnSeg& s : P->segs) {
+        const uint64_t rows = s.q_len * group;
+        if (!small(s)) {
+            f4 += (rows + 127) / 128;
+            frows += rows;
+            if (s.q_len) longest = std::max<uint64_t>(longest, s.k_len);
+        }
+        if (!small_bwd(s)) {
+            q4 += (rows + 127) / 128;
+            k4 += (uint64_t(s.k_len) + 127) / 128;
+            brows += rows;
+            keys += s.k_len;
+        }
     }
     const auto full = [&](uint64_t total, uint64_t tiles) {
         // Four waves a block where the chip is filled all the same and three of four waves have rows.
         return tiles * kvh >= 2 * cus && total >= tiles * 96;
     };
-    uint64_t rows = 0, keys = 0;
-    for (const AttnSeg& s : P->segs) rows += s.q_len * group, keys += s.k_len;
-    P->wfwd = P->wbwd_q = full(rows, q4) ? 4 : 1;
+    P->wfwd = full(frows, f4) ? 4 : 1;
+    P->wbwd_q = full(brows, q4) ? 4 : 1;
     P->wbwd_kv = full(keys, k4) ? 4 : 1;
     // Wide tables for many shared heads leave no room for four waves' tiles.
-    const auto lds = sh.precision == GATGPU_BF16 ? attention_backward_lds_bf16 : attention_backward_lds_fp32;
+    const auto lds = bf16 ? attention_backward_lds_bf16 : attention_backward_lds_fp32;
     if (lds(kAttnBackwardQ, sh.dim, P->wbwd_q, sh.bias, int(group), sh.buckets) > kAttnLds) P->wbwd_q = 1;
     if (lds(kAttnBackwardKv, sh.dim, P->wbwd_kv, sh.bias, int(group), sh.buckets) > kAttnLds) P->wbwd_kv = 1;
 
     std::vector<AttnTask> fwd, bq, bk, join;
-    const auto q_tiles = [&](std::vector<AttnTask>& out, uint32_t tile) {
+    const auto q_tiles = [&](std::vector<AttnTask>& out, uint32_t tile, const auto& skip) {
         for (size_t s = 0; s < P->segs.size(); ++s) {
             const AttnSeg& g = P->segs[s];
+            if (skip(g)) continue;
             const uint64_t n = g.q_len * group;
             for (uint64_t r = 0; r < n; r += tile) {
                 const uint64_t last = std::min<uint64_t>(n, r + tile) - 1;
@@ -119,8 +166,8 @@ int build(gatgpu_attention* P) {
             }
         }
     };
-    q_tiles(fwd, 32u * uint32_t(P->wfwd));
-    q_tiles(bq, 32u * uint32_t(P->wbwd_q));
+    q_tiles(fwd, 32u * uint32_t(P->wfwd), small);
+    q_tiles(bq, 32u * uint32_t(P->wbwd_q), small_bwd);
     // Few tiles over long rows of keys: each tile's keys are cut into ranges that fill the chip.
     uint64_t work = 0;
     for (const AttnTask& t : fwd) work += t.hi;
@@ -147,6 +194,7 @@ int build(gatgpu_attention* P) {
     }
     for (size_t s = 0; s < P->segs.size(); ++s) {
         const AttnSeg& g = P->segs[s];
+        if (small_bwd(g)) continue;
         const uint32_t n = uint32_t(g.q_len * group);
         for (uint64_t k = 0; k < g.k_len; k += 32u * uint32_t(P->wbwd_kv)) {
             uint32_t lo = 0;  // first row that sees key k
@@ -157,13 +205,21 @@ int build(gatgpu_attention* P) {
             bk.push_back({uint32_t(s), uint32_t(k), lo, n});
         }
     }
-    if (std::max({fwd.size(), bq.size(), bk.size(), join.size()}) * kvh >= kMaxTasks)
+    if (std::max({sf[0].size(), sf[1].size(), sb[0].size(), sb[1].size(), sb[2].size(), fwd.size(), bq.size(), bk.size(), join.size()}) * kvh >= kMaxTasks)
         return fail(c, GATGPU_EOVERFLOW, "too many tiles");
     if (!P->split) longest_first(fwd);
     longest_first(bq);
     longest_first(bk);
     // Rows of long segments: an XCD keeps few heads' keys in its L2; short segments: whole lines.
     P->spread = longest > 256;
+    for (int i = 0; i < 2; ++i) {
+        P->nsmall[i] = sf[i].size();
+        if (int r = upload(c, P->dsmall[i], sf[i].data(), sf[i].size() * sizeof(AttnTask))) return r;
+    }
+    for (int i = 0; i < 3; ++i) {
+        P->nsmall_bwd[i] = sb[i].size();
+        if (int r = upload(c, P->dsmall_bwd[i], sb[i].data(), sb[i].size() * sizeof(AttnTask))) return r;
+    }
     P->nfwd = fwd.size();
     P->nbwd_q = bq.size();
     P->nbwd_kv = bk.size();
@@ -187,7 +243,7 @@ uint64_t forward_bytes(const gatgpu_attention* P) {
 uint64_t delta_bytes(const gatgpu_attention* P) { return pad256(P->rows * uint64_t(P->shape.heads) * 4); }
 uint64_t backward_bytes(const gatgpu_attention* P) {
     const gatgpu_attention_shape& sh = P->shape;
-    return delta_bytes(P) + (sh.bias == GATGPU_BIAS_TABLE ? P->nbwd_q * uint64_t(sh.heads) * uint64_t(sh.buckets) * 4 : 0);
+    return delta_bytes(P) + (sh.bias == GATGPU_BIAS_TABLE ? (P->small_parts + P->nbwd_q) * uint64_t(sh.heads) * uint64_t(sh.buckets) * 4 : 0);
 }
 
 // A matrix of rows: there, aligned, wide enough, on the device.
@@ -360,6 +416,11 @@ int gatgpu_attention_forward(gatgpu_attention* P, const gatgpu_attention_io* io,
         if (int r = check_floats(c, "lse", io->lse)) return r;
     AttnArgs a = make_args(P, io);
     const bool bf16 = P->shape.precision == GATGPU_BF16;
+    for (int i = 1; i >= 0; --i) {
+        a.tasks = P->dsmall[i].as<AttnTask>();
+        a.ntasks = P->nsmall[i];
+        if (a.ntasks) HIPCHECK(c, (bf16 ? launch_attention_small_forward_bf16 : launch_attention_small_forward_fp32)(a, i + 1, c->stream));
+    }
     a.tasks = P->dfwd.as<AttnTask>();
     a.ntasks = P->nfwd;
     if (!a.ntasks) return GATGPU_OK;
@@ -404,10 +465,17 @@ int gatgpu_attention_backward(gatgpu_attention* P, const gatgpu_attention_io* io
     a.dvs = io->dv_stride;
     a.delta = static_cast<float*>(ws);
     a.dbias = io->dbias ? reinterpret_cast<float*>(static_cast<char*>(ws) + delta_bytes(P)) : nullptr;
+    for (int i = 2; i >= 0; --i) {
+        a.tasks = P->dsmall_bwd[i].as<AttnTask>();
+        a.ntasks = P->nsmall_bwd[i];
+        if (a.ntasks)
+            HIPCHECK(c, (bf16 ? launch_attention_small_backward_bf16 : launch_attention_small_backward_fp32)(a, 1 << i, c->stream));
+    }
+    a.first_part = P->small_parts;
     a.tasks = P->dbwd_q.as<AttnTask>();
     a.ntasks = P->nbwd_q;
     if (a.ntasks) HIPCHECK(c, (bf16 ? launch_attention_backward_q_bf16 : launch_attention_backward_q_fp32)(a, P->wbwd_q, c->stream));
-    if (io->dbias) HIPCHECK(c, launch_attention_bias_sum(a, io->dbias, c->stream));
+    if (io->dbias) HIPCHECK(c, launch_attention_bias_sum(a, P->small_parts + P->nbwd_q, io->dbias, c->stream));
     a.tasks = P->dbwd_kv.as<AttnTask>();
     a.ntasks = P->nbwd_kv;
     if (a.ntasks) HIPCHECK(c, (bf16 ? launch_attention_backward_kv_bf16 : launch_attention_backward_kv_fp32)(a, P->wbwd_kv, c->stream));

@@ -76,7 +76,8 @@ struct AttnArgs {
     void *dq = nullptr, *dk = nullptr, *dv = nullptr;
     uint64_t dqs = 0, dks = 0, dvs = 0;
     float* delta = nullptr;  // [rows][heads]
-    float* dbias = nullptr;  // [tasks][kv_heads][group][buckets] partial sums
+    float* dbias = nullptr;  // [parts][kv_heads][group][buckets] partial sums, those of ...
+    uint64_t first_part = 0; // ... this launch's tasks from here on
 };
 
 // Passes of the backward computation: over query rows, and over keys.
@@ -92,9 +93,17 @@ hipError_t launch_attention_backward_q_bf16(const AttnArgs& a, int waves, hipStr
 hipError_t launch_attention_backward_q_fp32(const AttnArgs& a, int waves, hipStream_t s);
 hipError_t launch_attention_backward_kv_bf16(const AttnArgs& a, int waves, hipStream_t s);
 hipError_t launch_attention_backward_kv_fp32(const AttnArgs& a, int waves, hipStream_t s);
+// Short segments (task: segment, row of dbias, heads [lo, hi)): forward of at most 32 x blocks keys
+// (1 or 2), backward of at most 32 x waves (1, 2 or 4), whose blocks take this much LDS.
+hipError_t launch_attention_small_forward_bf16(const AttnArgs& a, int blocks, hipStream_t s);
+hipError_t launch_attention_small_forward_fp32(const AttnArgs& a, int blocks, hipStream_t s);
+hipError_t launch_attention_small_backward_bf16(const AttnArgs& a, int waves, hipStream_t s);
+size_t attention_small_backward_lds_bf16(int dim, int waves, int bias, int group, int buckets);
+hipError_t launch_attention_small_backward_fp32(const AttnArgs& a, int waves, hipStream_t s);
+size_t attention_small_backward_lds_fp32(int dim, int waves, int bias, int group, int buckets);
 // tiles: per split tile its segment and first row, and in lo / hi its first task and how many it has.
 hipError_t launch_attention_join(const AttnArgs& a, bool bf16, const AttnTask* tiles, uint64_t ntiles, hipStream_t s);
-hipError_t launch_attention_bias_sum(const AttnArgs& a, float* dbias, hipStream_t s);
+hipError_t launch_attention_bias_sum(const AttnArgs& a, uint64_t parts, float* dbias, hipStream_t s);
 
 constexpr int kAttnMaxDim = 128, kAttnMaxBuckets = 64;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
@@ -102,6 +111,11 @@ constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 // Padded head width of the kernel that takes `dim`.
 inline int attention_width(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 
+// Widths of the forward kernel for short segments: a head's keys and values of 64 rows in registers.
+template <class T>
+constexpr bool attention_small_width(int width) {
+    return width * int(sizeof(T)) <= 128;
+}
 // f(width, waves, bias, cap) as compile-time values.
 template <class F>
 hipError_t attn_dispatch(const AttnArgs& a, int waves, F f) {

@@ -171,7 +171,7 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
     if constexpr (TABLE) __syncthreads();
     pass(std::false_type{});
     const bool bad = !idle && nonfinite(acc);
-    if (NW == 1 ? __any(bad) : __syncthreads_or(bad)) {
+    if (__builtin_expect(NW == 1 ? __any(bad) : __syncthreads_or(bad), 0)) {
         if (NW > 1) __syncthreads();
         sk.load(kbase, a.ks, 0, end, dim);
         sv.load(vbase, a.vs, 0, end, dim);
@@ -181,22 +181,11 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
         }
         pass(std::true_type{});
     }
-    if (live) {
-        const uint64_t to = grow * a.dqs + uint64_t(w.head) * dim;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = d * 32 + 8 * i + 4 * half;
-                if (at < dim)
-                    store4<T>(a.dq, to + at, acc[d][4 * i] * a.scale, acc[d][4 * i + 1] * a.scale,
-                              acc[d][4 * i + 2] * a.scale, acc[d][4 * i + 3] * a.scale);
-            }
-    }
+    store_rows<T, DB>(a.dq, grow * a.dqs + uint64_t(w.head) * dim, acc, a.scale, half, dim, live);
     if (!binned) return;
     // Each bucket's columns, by head of the group, in one fixed order.
     __syncthreads();
-    float* to = a.dbias + (task_id * uint64_t(a.kv_heads) + uint64_t(kv)) * uint64_t(a.group * a.buckets);
+    float* to = a.dbias + ((a.first_part + task_id) * uint64_t(a.kv_heads) + uint64_t(kv)) * uint64_t(a.group * a.buckets);
     for (int b = wave; b < a.buckets; b += NW)
         for (int g = 0; g < a.group; ++g) {
             float sum = 0.0f;
@@ -331,18 +320,15 @@ __global__ __launch_bounds__(NW * 64, (D < 128 ? attn_waves<T, D, NW>() : 1)) vo
                     for (int r = 0; r < 16; ++r) y[r] *= s[r];
                 }
                 char* turn = lds_p[wave][0];
-                turn_store<T>(turn, p, lane);
-                turn_store<T>(turn + 32 * PROW, y, lane);
+                turn_store<T>(turn, to_operand<T>(p), lane);
+                turn_store<T>(turn + 32 * PROW, to_operand<T>(y), lane);
                 wave_sync();
                 const AttnCols<T> pc = load_cols<T>(turn, PROW, 0, lane), yc = load_cols<T>(turn + 32 * PROW, PROW, 0, lane);
                 const char* orows = lds_o[buf] + b * 32 * ROW;
                 const char* qrows = lds_q[buf] + b * 32 * ROW;
                 if constexpr (CAREFUL) {
-                    f32x16_t one;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) one[r] = p[r] == 0.0f ? 0.0f : 1.0f;
                     wave_sync();
-                    turn_store<T>(turn, one, lane);
+                    turn_store<T>(turn, seen_operand<T>(p), lane);
                     wave_sync();
                     const AttnCols<T> seen = load_cols<T>(turn, PROW, 0, lane);
 #pragma unroll
@@ -361,22 +347,12 @@ __global__ __launch_bounds__(NW * 64, (D < 128 ? attn_waves<T, D, NW>() : 1)) vo
     __syncthreads();
     pass(std::false_type{});
     const bool bad = !idle && (nonfinite(acc_k) || nonfinite(acc_v));
-    if (NW == 1 ? __any(bad) : __syncthreads_or(bad)) {
+    if (__builtin_expect(NW == 1 ? __any(bad) : __syncthreads_or(bad), 0)) {
         if (NW > 1) __syncthreads();
         pass(std::true_type{});
     }
-    if (key >= seg.k_len) return;
-    const uint64_t tk = grow * a.dks + uint64_t(kv) * dim, tv = grow * a.dvs + uint64_t(kv) * dim;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = d * 32 + 8 * i + 4 * half;
-            if (at >= dim) continue;
-            store4<T>(a.dk, tk + at, acc_k[d][4 * i] * a.scale, acc_k[d][4 * i + 1] * a.scale, acc_k[d][4 * i + 2] * a.scale,
-                      acc_k[d][4 * i + 3] * a.scale);
-            store4<T>(a.dv, tv + at, acc_v[d][4 * i], acc_v[d][4 * i + 1], acc_v[d][4 * i + 2], acc_v[d][4 * i + 3]);
-        }
+    store_rows<T, DB>(a.dk, grow * a.dks + uint64_t(kv) * dim, acc_k, a.scale, half, dim, key < seg.k_len);
+    store_rows<T, DB>(a.dv, grow * a.dvs + uint64_t(kv) * dim, acc_v, 1.0f, half, dim, key < seg.k_len);
 }
 
 // LDS of a block, as the kernels declare it.

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(
     if constexpr (BIAS == GATGPU_BIAS_TABLE) __syncthreads();
     pass(std::false_type{});
     const bool bad = !idle && nonfinite(acc);
-    if (NW == 1 ? __any(bad) : __syncthreads_or(bad)) {
+    if (__builtin_expect(NW == 1 ? __any(bad) : __syncthreads_or(bad), 0)) {
         if (NW > 1) __syncthreads();
         sk.load(kbase, a.ks, task.lo, end, dim);
         sv.load(vbase, a.vs, task.lo, end, dim);
@@ -203,28 +203,7 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(
         if (half == 0) *reinterpret_cast<float2*>(a.stat + at * 2) = make_float2(m, l);
         return;
     }
-    if (row0 + uint32_t(l32) >= rows) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // nothing seen: 0
-    const uint64_t to = (seg.q_begin + uint64_t(w.query)) * a.os + uint64_t(w.head) * dim;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = d * 32 + 8 * i + 4 * half;
-            if (at >= dim) continue;
-            float o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = acc[d][4 * i + e] * inv;
-            store4<T>(a.out, to + at, o[0], o[1], o[2], o[3]);
-            if (sizeof(T) == 2 && a.rest) {  // what the rounding took
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] -= bf16_widen(bf16_hw(o[e]));
-                store4<T>(a.rest, to + at, o[0], o[1], o[2], o[3]);
-            }
-        }
-    if (a.lse && half == 0)
-        a.lse[(seg.q_begin + uint64_t(w.query)) * uint64_t(a.heads) + w.head] =
-            l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
+    store_out<T, DB>(a, seg, w, acc, m, l, half, row0 + uint32_t(l32) < rows);
 }
 
 template <class T, int D, int NW, int BIAS, bool CAP>

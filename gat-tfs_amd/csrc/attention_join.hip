@@ -59,22 +59,26 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const AttnT
             l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
-// dbias[head][bucket]: the first pass's partial sums of all tasks, in one fixed order; a block a
-// (head, bucket).
-__global__ __launch_bounds__(256) void k_attn_bias_sum(const AttnArgs a, float* __restrict__ dbias) {
-    const int cell = int(blockIdx.x), head = cell / a.buckets, kv = head / a.group;
-    const uint64_t step = uint64_t(a.heads) * a.buckets;
-    const uint64_t at = uint64_t(kv) * (a.group * a.buckets) + uint64_t(cell - kv * a.group * a.buckets);
-    float sum = 0.0f;
-    for (uint64_t t = threadIdx.x; t < a.ntasks; t += 256) sum += a.dbias[t * step + at];
-    __shared__ float part[256];
-    part[threadIdx.x] = sum;
-    __syncthreads();
-    for (int d = 128; d; d /= 2) {
-        if (int(threadIdx.x) < d) part[threadIdx.x] += part[threadIdx.x + d];
-        __syncthreads();
+// dbias[head][bucket]: partial sums of all parts, in one fixed order.  A block takes 32 cells, 32
+// threads a cell.
+__global__ __launch_bounds__(1024) void k_attn_bias_sum(const float* __restrict__ part, uint64_t parts, uint32_t cells,
+                                                        float* __restrict__ dbias) {
+    const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+    __shared__ float lds[32][33];
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < cells) {
+        uint64_t p = g;
+        for (; p + 96 < parts; p += 128)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += part[(p + 32 * i) * cells + c];
+        for (; p < parts; p += 32) s[0] += part[p * cells + c];
     }
-    if (threadIdx.x == 0) dbias[cell] = part[0];
+    lds[g][threadIdx.x & 31] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    float sum = lds[threadIdx.x & 31][g];
+#pragma unroll
+    for (int d = 16; d; d /= 2) sum += __shfl_xor(sum, d);
+    if ((threadIdx.x & 31) == 0 && blockIdx.x * 32 + g < cells) dbias[blockIdx.x * 32 + g] = sum;
 }
 
 template <class T, int D>
@@ -111,8 +115,9 @@ hipError_t launch_attention_join(const AttnArgs& a, bool bf16, const AttnTask* t
         default: return bf16 ? join<uint16_t, 128>(a, tiles, ntiles, s) : join<float, 128>(a, tiles, ntiles, s);
     }
 }
-hipError_t launch_attention_bias_sum(const AttnArgs& a, float* dbias, hipStream_t s) {
-    k_attn_bias_sum<<<uint32_t(a.heads * a.buckets), 256, 0, s>>>(a, dbias);
+hipError_t launch_attention_bias_sum(const AttnArgs& a, uint64_t parts, float* dbias, hipStream_t s) {
+    const uint32_t cells = uint32_t(a.heads) * uint32_t(a.buckets);
+    k_attn_bias_sum<<<(cells + 31) / 32, 1024, 0, s>>>(a.dbias, parts, cells, dbias);
     return hipGetLastError();
 }
 

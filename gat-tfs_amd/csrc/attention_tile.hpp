@@ -160,6 +160,16 @@ __device__ inline f32x16_t mfma_cols_careful(f32x16_t acc, const char* rows, int
     }
     return acc;
 }
+// Nonzero if a lane's part of a row operand holds a NaN or an infinity.
+template <class T, int NF>
+__device__ inline uint32_t nonfinite_row(const uint4 (&f)[NF]) {
+    constexpr uint32_t mask = sizeof(T) == 2 ? 0x7f807f80u : 0x7f800000u, one = sizeof(T) == 2 ? 0x00800080u : 0x00800000u;
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+        any |= ((f[i].x & mask) + one) | ((f[i].y & mask) + one) | ((f[i].z & mask) + one) | ((f[i].w & mask) + one);
+    return any & (sizeof(T) == 2 ? 0x80008000u : 0x80000000u);
+}
 // True if a lane's sums hold a NaN or an infinity.
 template <int N>
 __device__ inline bool nonfinite(const f32x16_t (&acc)[N]) {
@@ -278,22 +288,13 @@ constexpr int attn_turn_row() {
     return sizeof(T) == 2 ? 72 : 144;
 }
 template <class T>
-__device__ inline void turn_store(char* to, const f32x16_t& c, int lane) {
+__device__ inline void turn_store(char* to, const AttnCols<T>& c, int lane) {
     char* row = to + (lane & 31) * attn_turn_row<T>() + 4 * (lane >> 5) * int(sizeof(T));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 2)
-            *reinterpret_cast<uint2*>(row + 16 * i) = make_uint2(bf16x2(c[4 * i], c[4 * i + 1]), bf16x2(c[4 * i + 2], c[4 * i + 3]));
-        else *reinterpret_cast<float4*>(row + 32 * i) = make_float4(c[4 * i], c[4 * i + 1], c[4 * i + 2], c[4 * i + 3]);
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + 16 * i) = make_uint2(c.w[2 * i], c.w[2 * i + 1]);
+        else *reinterpret_cast<uint4*>(row + 32 * i) = make_uint4(c.w[4 * i], c.w[4 * i + 1], c.w[4 * i + 2], c.w[4 * i + 3]);
     }
-}
-
-// Four consecutive columns of an output row, rounded to the storage type.
-template <class T>
-__device__ inline void store4(void* base, uint64_t at, float a, float b, float c, float d) {
-    if constexpr (sizeof(T) == 2)
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) = make_uint2(bf16x2(a, b), bf16x2(c, d));
-    else *reinterpret_cast<float4*>(static_cast<float*>(base) + at) = make_float4(a, b, c, d);
 }
 
 // Rows of a tile in LDS.
@@ -361,6 +362,68 @@ __device__ inline AttnRow attn_row(const AttnArgs& a, const AttnSeg& s, uint32_t
     w.pos = w.query + int(s.k_len) - int(s.q_len);
     w.lim = a.causal ? min(int(s.k_len), max(w.pos + 1, int(s.prefix))) : int(s.k_len);
     return w;
+}
+
+// Rows of a C tile set (columns: rows of the output, registers: dim) times `factor`, rounded to
+// the storage type, to the lane's row at base + at.  bf16: the wave's halves swap 8 bytes, so that
+// each lane stores 16.  Every lane of the wave takes part; rows with `in` are stored.  REST: what
+// the rounding took instead.
+template <class T, int DB, bool REST = false>
+__device__ inline void store_rows(void* base, uint64_t at, const f32x16_t (&acc)[DB], float factor, int half, int dim, bool in) {
+    if constexpr (sizeof(T) == 2) {
+        uint16_t* to = static_cast<uint16_t*>(base) + at;
+        const auto pack = [&](float x, float y) {
+            x *= factor;
+            y *= factor;
+            uint32_t u = bf16x2(x, y);
+            if (REST) u = bf16x2(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xffff0000u));
+            return u;
+        };
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = pack(acc[d][8 * j + 2 * e], acc[d][8 * j + 2 * e + 1]);
+                const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+                const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+                const int c = d * 32 + 16 * j + 8 * half;
+                if (in && c < dim) *reinterpret_cast<uint4*>(to + c) = make_uint4(x[0], y[0], x[1], y[1]);
+            }
+    } else {
+        float* to = static_cast<float*>(base) + at;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = d * 32 + 8 * i + 4 * half;
+                if (in && c < dim)
+                    *reinterpret_cast<float4*>(to + c) = make_float4(acc[d][4 * i] * factor, acc[d][4 * i + 1] * factor,
+                                                                     acc[d][4 * i + 2] * factor, acc[d][4 * i + 3] * factor);
+            }
+    }
+}
+// A row's output, what its rounding took and its log-sum, from its sums.  l == 0: it saw nothing.
+template <class T, int DB>
+__device__ inline void store_out(const AttnArgs& a, const AttnSeg& seg, const AttnRow& w, const f32x16_t (&acc)[DB], float m,
+                                 float l, int half, bool in) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const uint64_t row = seg.q_begin + uint64_t(w.query), to = row * a.os + uint64_t(w.head) * a.dim;
+    store_rows<T, DB>(a.out, to, acc, inv, half, a.dim, in);
+    if constexpr (sizeof(T) == 2) {
+        if (a.rest) store_rows<T, DB, true>(a.rest, to, acc, inv, half, a.dim, in);
+    }
+    if (a.lse && half == 0 && in)
+        a.lse[row * uint64_t(a.heads) + w.head] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
+}
+
+// Four consecutive columns of an output row, rounded to the storage type.
+template <class T>
+__device__ inline void store4(void* base, uint64_t at, float a, float b, float c, float d) {
+    if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) = make_uint2(bf16x2(a, b), bf16x2(c, d));
+    else *reinterpret_cast<float4*>(static_cast<float*>(base) + at) = make_float4(a, b, c, d);
 }
 
 // Block b's (task, key/value head).  Blocks go to the 8 XCDs in turn.  spread:
