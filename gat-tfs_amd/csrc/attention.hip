@@ -137,18 +137,18 @@ int build(gatgpu_attention* P) {
         }
         if (!small_bwd(s)) {
             q4 += (rows + 127) / 128;
-            k4 += (uint64_t(s.k_len) + 127) / 128;
+            k4 += (uint64_t(s.k_len) + 63) / 64;
             brows += rows;
             keys += s.k_len;
         }
     }
-    const auto full = [&](uint64_t total, uint64_t tiles) {
+    const auto full = [&](uint64_t total, uint64_t tiles, uint64_t tile) {
         // Four waves a block where the chip is filled all the same and three of four waves have rows.
-        return tiles * kvh >= 2 * cus && total >= tiles * 96;
+        return tiles * kvh >= 2 * cus && total >= tiles * tile * 3 / 4;
     };
-    P->wfwd = full(frows, f4) ? 4 : 1;
-    P->wbwd_q = full(brows, q4) ? 4 : 1;
-    P->wbwd_kv = full(keys, k4) ? 4 : 1;
+    P->wfwd = full(frows, f4, 128) ? 4 : 1;
+    P->wbwd_q = full(brows, q4, 128) ? 4 : 1;
+    P->wbwd_kv = full(keys, k4, 64) ? 4 : 1;  // (two pairs of waves with 32 keys each, or one)
     // Wide tables for many shared heads leave no room for four waves' tiles.
     const auto lds = bf16 ? attention_backward_lds_bf16 : attention_backward_lds_fp32;
     if (lds(kAttnBackwardQ, sh.dim, P->wbwd_q, sh.bias, int(group), sh.buckets) > kAttnLds) P->wbwd_q = 1;
@@ -196,11 +196,11 @@ int build(gatgpu_attention* P) {
         const AttnSeg& g = P->segs[s];
         if (small_bwd(g)) continue;
         const uint32_t n = uint32_t(g.q_len * group);
-        for (uint64_t k = 0; k < g.k_len; k += 32u * uint32_t(P->wbwd_kv)) {
+        for (uint64_t k = 0; k < g.k_len; k += P->wbwd_kv == 1 ? 32 : 64) {
             uint32_t lo = 0;  // first row that sees key k
             if (sh.mask != GATGPU_MASK_FULL && k >= g.prefix) {
                 const int64_t first = int64_t(k) - (int64_t(g.k_len) - int64_t(g.q_len));
-                lo = uint32_t(std::min<int64_t>(g.q_len, std::max<int64_t>(0, first)) * int64_t(group));
+                lo = uint32_t(std::min<int64_t>(g.q_len, std::max<int64_t>(0, first)) * int64_t(group)) / 64 * 64;  // (of whole tiles)
             }
             bk.push_back({uint32_t(s), uint32_t(k), lo, n});
         }
@@ -291,7 +291,7 @@ AttnArgs make_args(const gatgpu_attention* P, const gatgpu_attention_io* io) {
     a.segs = P->dsegs.as<AttnSeg>();
     a.heads = sh.heads;
     a.kv_heads = sh.kv_heads;
-    a.group = sh.heads / sh.kv_heads;
+    set_group(a, sh.heads / sh.kv_heads);
     a.dim = sh.dim;
     a.causal = sh.mask == GATGPU_MASK_PREFIX;
     a.bias_kind = sh.bias;

@@ -41,14 +41,15 @@ struct AttnTask {
 };
 
 // The capped score in units of log2, y = cap log2(e) tanh(u), u = x scale / cap, from the raw
-// product x: up to |u| = 1/2 as x times a polynomial of degree 4 in x^2 (a Chebyshev fit of
-// tanh(u) / u there, 1.4e-8 off; 6 plain operations a score against 5 and two quarter-rate ones
-// of the exponential form), beyond by the exponential.
+// product x.  Where all of a tile is near 0 (scores of a few units under caps of 30 to 50) it is x
+// times a polynomial in x^2, a Chebyshev fit of tanh(u) / u: of degree 2 up to |u| = 0.18
+// (5.7e-8 off), of degree 4 up to 1/2 (1.4e-8); beyond by the exponential, which costs two
+// quarter-rate operations a score more.
 struct AttnCap {
-    float in = 0.0f, out = 0.0f;    // scale / cap, cap log2(e)
-    float near = -1.0f;             // largest |x| of the polynomial
-    float poly[5] = {};
-    int bounded = 0;                // scores are small enough for weights without a running maximum
+    float in = 0.0f, out = 0.0f;          // scale / cap, cap log2(e)
+    float near2 = -1.0f, near4 = -1.0f;   // largest |x| of the polynomials
+    float poly2[3] = {}, poly4[5] = {};
+    int bounded = 0;                      // scores are small enough for weights without a running maximum
 };
 AttnCap attention_cap(float scale, float cap);
 
@@ -57,6 +58,7 @@ struct AttnArgs {
     const AttnTask* tasks = nullptr;
     uint64_t ntasks = 0;
     int heads = 0, kv_heads = 0, group = 1, dim = 0;
+    uint32_t group_mul = 0, group_shift = 0;  // row / group by multiplication (group_of)
     int causal = 0, bias_kind = 0, buckets = 0;
     int spread = 0;  // blocks of one task go to different XCDs (else to the same)
     float scale = 1.0f, cap = 0.0f;
@@ -115,6 +117,12 @@ inline int attention_width(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 1
 template <class T>
 constexpr bool attention_small_width(int width) {
     return width * int(sizeof(T)) <= 128;
+}
+// a.group and what divides by it: (high half of n mul + n) >> shift for n < 2^31.
+inline void set_group(AttnArgs& a, int group) {
+    a.group = group;
+    while ((1u << a.group_shift) < uint32_t(group)) ++a.group_shift;
+    a.group_mul = uint32_t((uint64_t(1) << 32) * ((uint64_t(1) << a.group_shift) - uint64_t(group)) / uint64_t(group)) + 1;
 }
 // f(width, waves, bias, cap) as compile-time values.
 template <class F>

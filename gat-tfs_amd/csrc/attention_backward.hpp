@@ -7,7 +7,7 @@
 //
 // The first pass (k_attn_bwd_q) holds 32 query rows a wave and walks the keys, as the
 // forward pass does; it forms delta on its way and sums the bias gradient in LDS, a
-// column a lane.  The second (k_attn_bwd_kv) holds 32 keys a wave and walks the packed
+// column a lane.  The second (k_attn_bwd_kv) holds 32 keys a pair of waves and walks the packed
 // query rows of all heads that share them, which sums the shared heads' gradients; its
 // weights and score gradients pass through LDS, whose transpose read makes them operands
 // that contract over the rows.
@@ -70,8 +70,10 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
     const T* vbase = static_cast<const T*>(a.v) + seg.k_begin * a.vs + uint64_t(kv) * dim;
     const uint32_t end = task.hi;
     AttnStage<T, D, NW, BK> sk, sv;
-    sk.load(kbase, a.ks, 0, end, dim);
-    sv.load(vbase, a.vs, 0, end, dim);
+    sk.place(a, a.ks, 1);
+    sv.place(a, a.vs, 1);
+    sk.load(a, kbase, a.ks, 1, 0, end);
+    sv.load(a, vbase, a.vs, 1, 0, end);
 
     const uint64_t grow = seg.q_begin + uint64_t(w.query);
     float lse2 = a.lse[grow * uint64_t(a.heads) + w.head];
@@ -127,8 +129,8 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
             for (int b = 0; b < NB; ++b) dist[b] = next_dist[b];
             __syncthreads();
             if (k0 + BK < end) {
-                sk.load(kbase, a.ks, k0 + BK, end, dim);
-                sv.load(vbase, a.vs, k0 + BK, end, dim);
+                sk.load(a, kbase, a.ks, 1, k0 + BK, end);
+                sv.load(a, vbase, a.vs, 1, k0 + BK, end);
                 if constexpr (TABLE) {
 #pragma unroll
                     for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, k0 + BK + b * 32 + 4 * half, seg.dist_ld);
@@ -146,9 +148,9 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
                     dp = mfma_rows<T>(dp, *reinterpret_cast<const uint4*>(lds_v[buf] + at), dof[f]);
                 }
                 f32x16_t y;
-                score_gradients<BIAS, CAP, CAREFUL>(a, s, dp, y, cc, uncap, slope2, float(w.pos - int(k0) - b * 32 - 4 * half),
-                                                    dist[b], trow, masked ? w.lim - int(k0) - b * 32 - 4 * half : 32, lse2,
-                                                    delta, masked);
+                score_gradients<BIAS, CAP, CAREFUL>(a.capped, s, dp, y, nullptr, cc, uncap, slope2,
+                                                    float(w.pos - int(k0) - b * 32 - 4 * half), dist[b], trow, masked,
+                                                    w.lim - int(k0) - b * 32 - 4 * half, lse2, delta);
                 if constexpr (TABLE) {
                     if (binned && live) {
 #pragma unroll
@@ -173,8 +175,8 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
     const bool bad = !idle && nonfinite(acc);
     if (__builtin_expect(NW == 1 ? __any(bad) : __syncthreads_or(bad), 0)) {
         if (NW > 1) __syncthreads();
-        sk.load(kbase, a.ks, 0, end, dim);
-        sv.load(vbase, a.vs, 0, end, dim);
+        sk.load(a, kbase, a.ks, 1, 0, end);
+        sv.load(a, vbase, a.vs, 1, 0, end);
         if constexpr (TABLE) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, b * 32 + 4 * half, seg.dist_ld);
@@ -200,14 +202,28 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
         }
 }
 
-template <class T, int D, int NW, int BIAS, bool CAP>
-__global__ __launch_bounds__(NW * 64, (D < 128 ? attn_waves<T, D, NW>() : 1)) void k_attn_bwd_kv(const AttnArgs a) {
-    constexpr int BQ = attn_tile_rows<T, NW>(), NB = BQ / 32, ROW = lds_row<T, D>(), NF = D * int(sizeof(T)) / 32,
-                  DB = D / 32, NBUF = attn_buffers<T, NW>(), PROW = attn_turn_row<T>();
+// The pass over keys: a block of PAIRS pairs of waves, 32 keys a pair.  Of each tile of 64 packed query
+// rows the first wave of a pair forms the weights and score gradients of rows 0 to 31, the second
+// those of rows 32 to 63; both go through LDS, and then the first wave sums dv over the 64 rows, the second
+// dk.  So a wave holds one gradient's sums instead of two (64 registers at 128 columns), and two waves
+// a SIMD fit where one wave with both left only one (prefix sequences of 4K, 16 x 128: 1.38 ms).
+template <class T, int D, int PAIRS>
+struct KvLds {
+    static constexpr int kRows = 64, kThreads = PAIRS * 128, kTile = kRows * lds_row<T, D>();
+    static constexpr int kBuffers = 1;
+    static constexpr int kTurn = 32 * attn_turn_row<T>();
+    static constexpr int kBytes = kBuffers * (2 * kTile + kRows * 7 * 4) + PAIRS * 4 * kTurn;
+};
+
+template <class T, int D, int PAIRS, int BIAS, bool CAP>
+__global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS > 1) ? (D < 128 ? 3 : 2) : 1)) void k_attn_bwd_kv(const AttnArgs a) {
+    using L = KvLds<T, D, PAIRS>;
+    constexpr int BQ = L::kRows, ROW = lds_row<T, D>(), NF = D * int(sizeof(T)) / 32, DB = D / 32, NBUF = L::kBuffers,
+                  PROW = attn_turn_row<T>();
     constexpr bool TABLE = BIAS == GATGPU_BIAS_TABLE;
-    __shared__ __align__(16) char lds_q[NBUF][BQ * ROW];
-    __shared__ __align__(16) char lds_o[NBUF][BQ * ROW];
-    __shared__ __align__(16) char lds_p[NW][2][32 * PROW];  // a wave's weights and score gradients, a row a query
+    __shared__ __align__(16) char lds_q[NBUF][L::kTile];
+    __shared__ __align__(16) char lds_o[NBUF][L::kTile];
+    __shared__ __align__(16) char lds_p[PAIRS][2][2][L::kTurn];  // weights, score gradients; of the tile's halves
     // Per packed row of a tile: log-sum in units of log2 (+inf: weighs nothing), delta, keys seen,
     // position, slope, first entry of its table, query
     __shared__ float r_lse[NBUF][BQ], r_delta[NBUF][BQ], r_slope[NBUF][BQ];
@@ -219,9 +235,9 @@ __global__ __launch_bounds__(NW * 64, (D < 128 ? attn_waves<T, D, NW>() : 1)) vo
     if (!attn_task(a, task_id, kv)) return;
     const AttnTask task = a.tasks[task_id];
     const AttnSeg seg = a.segs[task.seg];
-    const int tid = int(threadIdx.x), lane = tid & 63,
-              wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
-    const uint32_t key0 = task.at + uint32_t(wave) * 32, key = key0 + uint32_t(l32);
+    const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31,
+              half = lane >> 5, pair = wave >> 1, role = wave & 1;
+    const uint32_t key0 = task.at + uint32_t(pair) * 32, key = key0 + uint32_t(l32);
     const bool idle = key0 >= seg.k_len;
     const int dim = a.dim;
     const uint64_t grow = seg.k_begin + min(key, seg.k_len - 1);
@@ -242,18 +258,20 @@ __global__ __launch_bounds__(NW * 64, (D < 128 ? attn_waves<T, D, NW>() : 1)) vo
     if constexpr (TABLE) fill_table(a, kv, table);
     const float cc = a.scale * kLog2e, uncap = CAP ? 1.0f / a.capped.out : 0.0f;
 
-    f32x16_t acc_k[DB], acc_v[DB];
-    AttnStage<T, D, NW, BQ> sq, so;
+    f32x16_t acc[DB];
+    AttnStage<T, D, PAIRS * 2, BQ> sq, so;
+    sq.place(a, a.qs, a.group);
+    so.place(a, a.dos, a.group);
     float n_lse = 0.0f, n_delta = 0.0f;
     const auto request = [&](uint32_t r0) {
-        sq.load_packed(qbase, a.qs, r0, end, dim, a.group);
-        so.load_packed(obase, a.dos, r0, end, dim, a.group);
+        sq.load(a, qbase, a.qs, a.group, r0, end);
+        so.load(a, obase, a.dos, a.group, r0, end);
         if (tid < BQ) {
             const uint32_t r = r0 + uint32_t(tid);
             n_lse = INFINITY;
             n_delta = 0.0f;
             if (r < end) {
-                const uint32_t q = r / uint32_t(a.group);
+                const uint32_t q = group_of(a, r);
                 const uint64_t h = uint64_t(kv) * uint64_t(a.group) + (r - q * uint32_t(a.group));
                 const float x = a.lse[(seg.q_begin + q) * uint64_t(a.heads) + h];
                 n_lse = x == -INFINITY ? INFINITY : x * kLog2e;
@@ -264,7 +282,7 @@ __global__ __launch_bounds__(NW * 64, (D < 128 ? attn_waves<T, D, NW>() : 1)) vo
     const auto pass = [&](auto careful) {
         constexpr bool CAREFUL = decltype(careful)::value;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) acc_k[d] = acc_v[d] = f32x16_t{};
+        for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
         if (task.lo < end) request(task.lo);
         uint32_t tile = 0;
         for (uint32_t r0 = task.lo; r0 < end; r0 += BQ, ++tile) {
@@ -288,20 +306,16 @@ __global__ __launch_bounds__(NW * 64, (D < 128 ? attn_waves<T, D, NW>() : 1)) vo
             }
             __syncthreads();
             if (r0 + BQ < end) request(r0 + BQ);
-            if (idle) continue;
-            AttnDist dist[NB];
-            if constexpr (TABLE) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    dist[b] = load_dist(a.dist + seg.dist + uint64_t(r_query[buf][b * 32 + l32]) * seg.dist_ld, key0 + 4 * half,
-                                        seg.dist_ld);
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const int row = b * 32 + l32, lim = r_lim[buf][row];
-                const int lim_first = __builtin_amdgcn_readlane(lim, 0), lim_last = __builtin_amdgcn_readlane(lim, 31);
-                if (int(key0) >= lim_last) continue;
-                const bool masked = int(key0) + 32 > lim_first;
+            const int row = role * 32 + l32, lim = r_lim[buf][row];
+            const int lim_last = __builtin_amdgcn_readlane(lim, 31);
+            // (Rows are in order of what they see: the tile's last row sees the most.)
+            const int lim_tile = __builtin_amdgcn_readfirstlane(r_lim[buf][63]);
+            const int lim_half = __builtin_amdgcn_readfirstlane(r_lim[buf][31]);
+            if (!idle && int(key0) < lim_last) {
+                const bool masked = int(key0) + 32 > __builtin_amdgcn_readlane(lim, 0);
+                AttnDist dist{};
+                if constexpr (TABLE)
+                    dist = load_dist(a.dist + seg.dist + uint64_t(r_query[buf][row]) * seg.dist_ld, key0 + 4 * half, seg.dist_ld);
                 f32x16_t s = f32x16_t{}, dp = f32x16_t{};
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
@@ -311,59 +325,56 @@ __global__ __launch_bounds__(NW * 64, (D < 128 ? attn_waves<T, D, NW>() : 1)) vo
                 }
                 f32x16_t y, p;
                 score_gradients<BIAS, CAP, CAREFUL>(
-                    a, s, dp, y, cc, uncap, BIAS == GATGPU_BIAS_LINEAR ? r_slope[buf][row] : 0.0f,
-                    BIAS == GATGPU_BIAS_LINEAR ? float(r_pos[buf][row] - int(key0) - 4 * half) : 0.0f, dist[b],
-                    table + (TABLE ? r_tab[buf][row] : 0), masked ? lim - int(key0) - 4 * half : 32, r_lse[buf][row],
-                    r_delta[buf][row], masked, &p);
+                    a.capped, s, dp, y, &p, cc, uncap, BIAS == GATGPU_BIAS_LINEAR ? r_slope[buf][row] : 0.0f,
+                    BIAS == GATGPU_BIAS_LINEAR ? float(r_pos[buf][row] - int(key0) - 4 * half) : 0.0f, dist,
+                    table + (TABLE ? r_tab[buf][row] : 0), masked, lim - int(key0) - 4 * half, r_lse[buf][row],
+                    r_delta[buf][row]);
                 if constexpr (CAP) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) y[r] *= s[r];
                 }
-                char* turn = lds_p[wave][0];
-                turn_store<T>(turn, to_operand<T>(p), lane);
-                turn_store<T>(turn + 32 * PROW, to_operand<T>(y), lane);
-                wave_sync();
-                const AttnCols<T> pc = load_cols<T>(turn, PROW, 0, lane), yc = load_cols<T>(turn + 32 * PROW, PROW, 0, lane);
-                const char* orows = lds_o[buf] + b * 32 * ROW;
-                const char* qrows = lds_q[buf] + b * 32 * ROW;
-                if constexpr (CAREFUL) {
-                    wave_sync();
-                    turn_store<T>(turn, seen_operand<T>(p), lane);
-                    wave_sync();
-                    const AttnCols<T> seen = load_cols<T>(turn, PROW, 0, lane);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc_v[d] = mfma_cols_careful<T>(acc_v[d], orows, ROW, d * 32, lane, pc, seen);
-                } else {
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc_v[d] = mfma_cols<T>(acc_v[d], load_cols<T>(orows, ROW, d * 32, lane), pc);
-                }
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-                    acc_k[d] = mfma_cols<T>(acc_k[d], load_cols<T, CAREFUL ? kClean : kRaw>(qrows, ROW, d * 32, lane), yc);
-                wave_sync();
+                turn_store<T>(lds_p[pair][0][role], to_operand<T>(p), lane);
+                turn_store<T>(lds_p[pair][1][role], to_operand<T>(y), lane);
             }
+            __syncthreads();
+            if (idle || int(key0) >= lim_tile) continue;
+            // dv: dout and the weights; dk: Q and the score gradients.
+            const char* cols = role ? lds_q[buf] : lds_o[buf];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (b == 0 && int(key0) >= lim_half) continue;
+                const AttnCols<T> w = load_cols<T>(lds_p[pair][role][b], PROW, 0, lane);
+                const char* c = cols + b * 32 * ROW;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    if constexpr (CAREFUL) {
+                        if (role) acc[d] = mfma_cols<T>(acc[d], load_cols<T, kClean>(c, ROW, d * 32, lane), w);
+                        else acc[d] = mfma_cols_careful<T>(acc[d], c, ROW, d * 32, lane, w, nonzero_operand<T>(w));
+                    } else {
+                        acc[d] = mfma_cols<T>(acc[d], load_cols<T>(c, ROW, d * 32, lane), w);
+                    }
+                }
+            }
+            // (With one buffer the barrier ahead of the next tile's stores, with two the one behind
+            // them, keeps the turned tiles until every wave has read them: they are written after it.)
         }
     };
     __syncthreads();
     pass(std::false_type{});
-    const bool bad = !idle && (nonfinite(acc_k) || nonfinite(acc_v));
-    if (__builtin_expect(NW == 1 ? __any(bad) : __syncthreads_or(bad), 0)) {
-        if (NW > 1) __syncthreads();
+    const bool bad = !idle && nonfinite(acc);
+    if (__builtin_expect(__syncthreads_or(bad), 0)) {
+        __syncthreads();
         pass(std::true_type{});
     }
-    store_rows<T, DB>(a.dk, grow * a.dks + uint64_t(kv) * dim, acc_k, a.scale, half, dim, key < seg.k_len);
-    store_rows<T, DB>(a.dv, grow * a.dvs + uint64_t(kv) * dim, acc_v, 1.0f, half, dim, key < seg.k_len);
+    const bool in = key < seg.k_len;
+    if (role) store_rows<T, DB>(a.dk, grow * a.dks + uint64_t(kv) * dim, acc, a.scale, half, dim, in);
+    else store_rows<T, DB>(a.dv, grow * a.dvs + uint64_t(kv) * dim, acc, 1.0f, half, dim, in);
 }
 
 // LDS of a block, as the kernels declare it.
 template <class T, int D, int NW>
 constexpr size_t lds_q_pass() {
     return size_t(attn_buffers<T, NW>()) * 2 * attn_tile_rows<T, NW>() * lds_row<T, D>();
-}
-template <class T, int D, int NW>
-constexpr size_t lds_kv_pass() {
-    return lds_q_pass<T, D, NW>() + size_t(NW) * 2 * 32 * attn_turn_row<T>() +
-           size_t(attn_buffers<T, NW>()) * attn_tile_rows<T, NW>() * 7 * 4;
 }
 template <class T>
 size_t backward_lds(int pass, int dim, int waves, int bias, int group, int buckets) {
@@ -372,7 +383,7 @@ size_t backward_lds(int pass, int dim, int waves, int bias, int group, int bucke
     size_t bytes = 0;
     (void)attn_dispatch(a, waves, [&](auto d, auto nw, auto, auto) {
         constexpr int D = decltype(d)::value, NW = decltype(nw)::value;
-        bytes = pass == kAttnBackwardKv ? lds_kv_pass<T, D, NW>() : lds_q_pass<T, D, NW>();
+        bytes = pass == kAttnBackwardKv ? size_t(KvLds<T, D, NW == 1 ? 1 : 2>::kBytes) : lds_q_pass<T, D, NW>();
         return hipSuccess;
     });
     if (bias == GATGPU_BIAS_TABLE) {
@@ -395,10 +406,10 @@ hipError_t backward_q(const AttnArgs& a, int waves, hipStream_t s) {
 template <class T>
 hipError_t backward_kv(const AttnArgs& a, int waves, hipStream_t s) {
     return attn_dispatch(a, waves, [&](auto d, auto nw, auto bias, auto cap) {
-        constexpr int NW = decltype(nw)::value, BIAS = decltype(bias)::value;
+        constexpr int PAIRS = decltype(nw)::value == 1 ? 1 : 2, BIAS = decltype(bias)::value;
         const size_t dyn = BIAS == GATGPU_BIAS_TABLE ? size_t(a.group) * 1024 : 0;
-        k_attn_bwd_kv<T, decltype(d)::value, NW, BIAS, decltype(cap)::value>
-            <<<uint32_t(attn_blocks(a)), NW * 64, dyn, s>>>(a);
+        k_attn_bwd_kv<T, decltype(d)::value, PAIRS, BIAS, decltype(cap)::value>
+            <<<uint32_t(attn_blocks(a)), PAIRS * 128, dyn, s>>>(a);
         return hipGetLastError();
     });
 }

@@ -2,7 +2,7 @@
 // and sum of the softmax.
 //
 //   x_j = scale q.k_j,  y_j = cap tanh(x_j / cap),  s_j = y_j + bias(distance)
-//   m' = max(m, max s_j),  l' = l 2^(m - m') + sum 2^(s_j - m'),  O' = O 2^(m - m') + sum 2^(s_j - m') v_j
+//   l' = l 2^(m - m') + sum 2^(s_j - m'),  O' = O 2^(m - m') + sum 2^(s_j - m') v_j,  m' a score near the maximum
 // (in units of log2) and out = O / l, lse = ln 2 (m + log2 l).  Capped scores without a bias
 // stay within cap: they need no maximum, m is 0 throughout.
 //
@@ -46,8 +46,10 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(
     const T* vbase = static_cast<const T*>(a.v) + seg.k_begin * a.vs + uint64_t(kv) * dim;
     const uint32_t end = task.hi;
     AttnStage<T, D, NW, BK> sk, sv;
-    sk.load(kbase, a.ks, task.lo, end, dim);
-    sv.load(vbase, a.vs, task.lo, end, dim);
+    sk.place(a, a.ks, 1);
+    sv.place(a, a.vs, 1);
+    sk.load(a, kbase, a.ks, 1, task.lo, end);
+    sv.load(a, vbase, a.vs, 1, task.lo, end);
 
     uint4 qf[NF];
     {
@@ -89,14 +91,15 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(
             for (int b = 0; b < NB; ++b) dist[b] = next_dist[b];
             __syncthreads();
             if (k0 + BK < end) {
-                sk.load(kbase, a.ks, k0 + BK, end, dim);
-                sv.load(vbase, a.vs, k0 + BK, end, dim);
+                sk.load(a, kbase, a.ks, 1, k0 + BK, end);
+                sv.load(a, vbase, a.vs, 1, k0 + BK, end);
                 if constexpr (BIAS == GATGPU_BIAS_TABLE) {
 #pragma unroll
                     for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, k0 + BK + b * 32 + 4 * half, seg.dist_ld);
                 }
             }
             if (idle || int(k0) >= lim_last) continue;  // (uniform over the wave; no barrier follows in the tile)
+            const float ref = m == -INFINITY ? 0.0f : m;
             f32x16_t s[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -105,8 +108,8 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(
                 for (int f = 0; f < NF; ++f)
                     s[b] = mfma_rows<T>(
                         s[b], *reinterpret_cast<const uint4*>(lds_k[buf] + (b * 32 + l32) * ROW + f * 32 + half * 16), qf[f]);
-                if constexpr (CAP) cap_scores(a.capped, s[b]);
-                bias_scores<BIAS, CAP, CAREFUL>(s[b], cc, slope2, float(w.pos - int(k0) - b * 32 - 4 * half), dist[b], trow);
+                tile_scores<BIAS, CAP, CAREFUL>(a.capped, s[b], cc, ref, slope2, float(w.pos - int(k0) - b * 32 - 4 * half),
+                                                dist[b], trow);
             }
             if (int(k0) + BK > lim_first) {
                 const int left = w.lim - int(k0) - 4 * half;
@@ -116,42 +119,39 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(
                     for (int r = 0; r < 16; ++r)
                         if (b * 32 + 8 * (r / 4) + r % 4 >= left) s[b][r] = -INFINITY;
             }
-            constexpr bool RAW = BIAS == GATGPU_BIAS_NONE && !CAP;  // scores still to be scaled
-            float sum = 0.0f;
-            if (bounded) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        s[b][r] = exp2_hw(s[b][r]);
-                        sum += s[b][r];
-                    }
-            } else {
+            if (!bounded) {
+                // The reference m is the maximum of an earlier tile.  It is raised, and the sums with it,
+                // only when a score passes it by 2^8: weights of up to 2^8 are as exact as those up to 1.
                 float top = s[0][0];
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+                    for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(top, s[b][r]), s[b][r + 1]);
                 top = xor32_max(top);
-                if (RAW) top *= cc;
-                const float next = fmaxf(m, top), ref = next == -INFINITY ? 0.0f : next;  // nothing seen yet: all weights 0
-                if (__any(next > m)) {
-                    const float fall = exp2_hw(m - ref);
+                const bool fresh = m == -INFINITY;  // the row has seen nothing yet
+                if (__any(fresh || top > 8.0f)) {
+                    const float up = fresh ? top : fmaxf(top, 0.0f), down = up == -INFINITY ? 0.0f : up;
+                    const float fall = fresh ? 0.0f : exp2_hw(-up);
+                    m = fresh ? top : m + up;
                     l *= fall;
 #pragma unroll
                     for (int d = 0; d < DB; ++d)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) acc[d][r] *= fall;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[b][r] -= down;
                 }
-                m = next;
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        s[b][r] = exp2_hw(RAW ? fmaf(s[b][r], cc, -ref) : s[b][r] - ref);
-                        sum += s[b][r];
-                    }
             }
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[b][r] = exp2_hw(s[b][r]);
+                    sum += s[b][r];
+                }
             l += sum;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -181,8 +181,8 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(
     const bool bad = !idle && nonfinite(acc);
     if (__builtin_expect(NW == 1 ? __any(bad) : __syncthreads_or(bad), 0)) {
         if (NW > 1) __syncthreads();
-        sk.load(kbase, a.ks, task.lo, end, dim);
-        sv.load(vbase, a.vs, task.lo, end, dim);
+        sk.load(a, kbase, a.ks, 1, task.lo, end);
+        sv.load(a, vbase, a.vs, 1, task.lo, end);
         if constexpr (BIAS == GATGPU_BIAS_TABLE) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, task.lo + b * 32 + 4 * half, seg.dist_ld);

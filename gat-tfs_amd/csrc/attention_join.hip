@@ -92,17 +92,22 @@ hipError_t join(const AttnArgs& a, const AttnTask* tiles, uint64_t ntiles, hipSt
 AttnCap attention_cap(float scale, float cap) {
     AttnCap c;
     if (!(cap > 0.0f)) return c;
-    const double fit[5] = {0.9999999871, -0.3333307189, 0.13324829, -0.05298924118, 0.01714131905};
+    const double fit2[3] = {0.9999999439, -0.3333021063, 0.1307500945};
+    const double fit4[5] = {0.9999999871, -0.3333307189, 0.13324829, -0.05298924118, 0.01714131905};
     const double in = double(scale) / double(cap), out = double(cap) * 1.4426950408889634;
     c.in = float(in);
     c.out = float(out);
     bool fits = true;
     double f = out * in;
     for (int k = 0; k < 5; ++k, f *= in * in) {
-        c.poly[k] = float(fit[k] * f);
-        fits = fits && std::isfinite(c.poly[k]);
+        if (k < 3) c.poly2[k] = float(fit2[k] * f);
+        c.poly4[k] = float(fit4[k] * f);
+        fits = fits && std::isfinite(c.poly4[k]);
     }
-    c.near = fits ? float(0.5 / in) : -1.0f;
+    if (fits) {
+        c.near2 = float(0.18 / in);
+        c.near4 = float(0.5 / in);
+    }
     // 2^y and sums of 2^30 of them stay inside FP32, and 2^-y far above its smallest values.
     c.bounded = out <= 90.0;
     return c;

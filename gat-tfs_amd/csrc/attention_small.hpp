@@ -119,6 +119,7 @@ __global__ __launch_bounds__(64, (D * int(sizeof(T)) * KB <= 128 ? 2 : 1)) void 
             const AttnRow w = attn_row(a, seg, min(r, rows - 1), kv);
             const float slope2 = BIAS == GATGPU_BIAS_LINEAR ? a.bias[w.head] * kLog2e : 0.0f;
             const float* trow = table + w.local * 256;
+            const int lim_first = __builtin_amdgcn_readlane(w.lim, 0);
             f32x16_t acc[DB];
             float m, l;
             const auto pass = [&](auto careful) {
@@ -130,18 +131,16 @@ __global__ __launch_bounds__(64, (D * int(sizeof(T)) * KB <= 128 ? 2 : 1)) void 
                     s[b] = f32x16_t{};
 #pragma unroll
                     for (int f = 0; f < NF; ++f) s[b] = mfma_rows<T>(s[b], kf[b][f], qf[f]);
-                    if constexpr (CAP) cap_scores(a.capped, s[b]);
-                    if constexpr (BIAS == GATGPU_BIAS_NONE && !CAP) {
+                    tile_scores<BIAS, CAP, CAREFUL>(a.capped, s[b], cc, 0.0f, slope2, float(w.pos - b * 32 - 4 * half), dist[b],
+                                                    trow);
+                    if (lim_first < 32 * b + 32) {
+                        const int left = w.lim - 32 * b - 4 * half;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) s[b][e] *= cc;
+                        for (int e = 0; e < 16; ++e)
+                            if (8 * (e / 4) + e % 4 >= left) s[b][e] = -INFINITY;
                     }
-                    bias_scores<BIAS, CAP, CAREFUL>(s[b], cc, slope2, float(w.pos - b * 32 - 4 * half), dist[b], trow);
-                    const int left = w.lim - 32 * b - 4 * half;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        if (8 * (e / 4) + e % 4 >= left) s[b][e] = -INFINITY;
-                        top = fmaxf(top, s[b][e]);
-                    }
+                    for (int e = 0; e < 16; e += 2) top = fmaxf(fmaxf(top, s[b][e]), s[b][e + 1]);
                 }
                 m = xor32_max(top);
                 const float ref = m == -INFINITY ? 0.0f : m;
@@ -239,7 +238,7 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int chunk = tid + i * NW * 64, c = chunk % CPR * AttnType<T>::kPer;
-            const uint32_t r = tile * 32 + uint32_t(chunk / CPR), query = a.group == 1 ? r : r / uint32_t(a.group);
+            const uint32_t r = tile * 32 + uint32_t(chunk / CPR), query = group_of(a, r);
             // (Rows behind the last are 0 and weigh nothing.)
             const bool in = r < rows && c < dim && (CHUNKS >= NW * 64 || chunk < CHUNKS);
             const uint32_t at = (r - query * uint32_t(a.group)) * uint32_t(dim) + uint32_t(c);
@@ -297,7 +296,8 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
             const AttnRow w = attn_row(a, seg, min(r, rows - 1), kv);
             const float slope2 = BIAS == GATGPU_BIAS_LINEAR ? a.bias[w.head] * kLog2e : 0.0f;
             const float* trow = table + w.local * 256;
-            const int left = w.lim - int(key0) - 4 * half;
+            const int left = w.lim - int(key0) - 4 * half, lim_first = __builtin_amdgcn_readlane(w.lim, 0);
+            const float gap = float(w.pos - int(key0) - 4 * half);
             f32x16_t acc_q[DB];
             // Adds the tile to the gradients, and returns whether all of its rows' deltas were finite: if
             // not, nothing was added and the careful form follows (a NaN or an infinity in any
@@ -313,18 +313,25 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
                         y = mfma_rows<T>(y, vf[f], from_lds(lds_o, f));
                     }
                 }
-                if constexpr (CAP) cap_scores(a.capped, s);
-                f32x16_t p = s;
-                if constexpr (BIAS == GATGPU_BIAS_NONE && !CAP) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) p[e] *= cc;
+                // (s keeps the capped scores for their slope)
+                f32x16_t p;
+                if constexpr (CAP) {
+                    cap_scores(a.capped, s, 0.0f);
+                    p = s;
+                    tile_scores<BIAS, false, CAREFUL>(a.capped, p, 1.0f, lse2, slope2, gap, dist, trow);
+                } else {
+                    p = s;
+                    tile_scores<BIAS, false, CAREFUL>(a.capped, p, cc, lse2, slope2, gap, dist, trow);
                 }
-                bias_scores<BIAS, CAP, CAREFUL>(p, cc, slope2, float(w.pos - int(key0) - 4 * half), dist, trow);
+                if (lim_first < int(key0) + 32) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (8 * (e / 4) + e % 4 >= left) p[e] = -INFINITY;
+                }
                 float delta = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    if (8 * (e / 4) + e % 4 >= left) p[e] = -INFINITY;
-                    p[e] = exp2_hw(p[e] - lse2);
+                    p[e] = exp2_hw(p[e]);
                     if (CAREFUL && p[e] == 0.0f) y[e] = 0.0f;
                     delta = fmaf(p[e], y[e], delta);
                 }
@@ -410,7 +417,7 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
 #pragma unroll
                         for (int e = 0; e < 8; ++e) v[e] += x[e];
                     }
-                    const uint32_t query = row / uint32_t(a.group);
+                    const uint32_t query = group_of(a, row);
                     const uint64_t to = (seg.q_begin + query) * a.dqs + uint64_t(kv * a.group) * uint64_t(dim) +
                                         (row - query * uint32_t(a.group)) * uint32_t(dim) + uint32_t(col);
 #pragma unroll

@@ -145,6 +145,17 @@ __device__ inline AttnCols<T> seen_operand(const f32x16_t& c) {
     for (int i = 0; i < 16; ++i) one[i] = c[i] == 0.0f ? 0.0f : 1.0f;
     return to_operand<T>(one);
 }
+// An operand of weights: 1 for each that is not 0.
+template <class T>
+__device__ inline AttnCols<T> nonzero_operand(const AttnCols<T>& w) {
+    AttnCols<T> one;
+#pragma unroll
+    for (int i = 0; i < int(8 * sizeof(T) / 2); ++i) {
+        if constexpr (sizeof(T) == 2) one.w[i] = (w.w[i] & 0xffffu ? 0x3f80u : 0u) | (w.w[i] >> 16 ? 0x3f800000u : 0u);
+        else one.w[i] = w.w[i] ? 0x3f800000u : 0u;
+    }
+    return one;
+}
 // acc += weights p (as operand w) x columns of a tile that may hold NaN and infinities: one reaches
 // the rows that give its own row of the tile some weight, and no other.
 template <class T>
@@ -183,22 +194,29 @@ __device__ inline bool nonfinite(const f32x16_t (&acc)[N]) {
 
 __device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Capped scores of a tile from its raw products (AttnCap).
-__device__ inline void cap_scores(const AttnCap& c, f32x16_t& s) {
+// Capped scores of a tile from its raw products (AttnCap), less `less`.
+__device__ inline void cap_scores(const AttnCap& c, f32x16_t& s, float less) {
     float top = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[r]));
-    if (__all(top <= c.near)) {
+    for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(top, fabsf(s[r])), fabsf(s[r + 1]));
+    if (__all(top <= c.near2)) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float t = s[r] * s[r];
-            s[r] *= fmaf(fmaf(fmaf(fmaf(c.poly[4], t, c.poly[3]), t, c.poly[2]), t, c.poly[1]), t, c.poly[0]);
+            s[r] = fmaf(s[r], fmaf(fmaf(c.poly2[2], t, c.poly2[1]), t, c.poly2[0]), -less);
+        }
+    } else if (__all(top <= c.near4)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float t = s[r] * s[r];
+            const float p = fmaf(fmaf(fmaf(fmaf(c.poly4[4], t, c.poly4[3]), t, c.poly4[2]), t, c.poly4[1]), t, c.poly4[0]);
+            s[r] = fmaf(s[r], p, -less);
         }
     } else {  // tanh(u) = 1 - 2 / (1 + e^2u), exact at both ends
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float e = __builtin_amdgcn_exp2f(s[r] * c.in * (2.0f * kLog2e));
-            s[r] = c.out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e));
+            s[r] = fmaf(c.out, 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + e), -less);
         }
     }
 }
@@ -231,25 +249,23 @@ __device__ inline AttnDist load_dist(const uint8_t* row, uint32_t first, uint32_
 }
 __device__ inline uint32_t dist_of(const AttnDist& d, int r) { return d.w[r / 4] >> (8 * (r % 4)) & 255u; }
 
-// Biased scores of a block, in units of log2.  s: raw products (capped ones with CAP), cc: their
-// factor.  gap: the row's position less the block's first key of the lane; table: the row's entries.
+// Scores of a block in units of log2, less `less`, from its raw products.  cc: their factor without
+// a cap; gap: the row's position less the block's first key of the lane; table: the row's entries.
 // A hidden pair's score is -inf; only CAREFUL keeps it so where its product is a NaN or +inf.
 template <int BIAS, bool CAP, bool CAREFUL>
-__device__ inline void bias_scores(f32x16_t& s, float cc, float slope2, float gap, const AttnDist& d, const float* table) {
-    if constexpr (BIAS == GATGPU_BIAS_LINEAR) {
+__device__ inline void tile_scores(const AttnCap& cap, f32x16_t& s, float cc, float less, float slope2, float gap,
+                                   const AttnDist& d, const float* table) {
+    if constexpr (CAP) cap_scores(cap, s, less);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float far = slope2 * fabsf(gap - float(8 * (r / 4) + r % 4));
-            s[r] = CAP ? s[r] - far : fmaf(s[r], cc, -far);
-        }
-    }
-    if constexpr (BIAS == GATGPU_BIAS_TABLE) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
+    for (int r = 0; r < 16; ++r) {
+        float x = CAP ? s[r] : fmaf(s[r], cc, -less);
+        if constexpr (BIAS == GATGPU_BIAS_LINEAR) x = fmaf(-slope2, fabsf(gap - float(8 * (r / 4) + r % 4)), x);
+        if constexpr (BIAS == GATGPU_BIAS_TABLE) {
             const float t = table[dist_of(d, r)];
-            s[r] = CAP ? s[r] + t : fmaf(s[r], cc, t);
-            if (CAREFUL && t == -INFINITY) s[r] = t;
+            x += t;
+            if (CAREFUL && t == -INFINITY) x = t;
         }
+        s[r] = x;
     }
 }
 
@@ -257,12 +273,31 @@ __device__ inline void bias_scores(f32x16_t& s, float cc, float slope2, float ga
 // with CAP, s becomes 1 - tanh^2, the capped score's slope.  left: keys of the lane from its first
 // on that the row sees (where masked).  CAREFUL: a weight of 0 has no gradient, whatever dp is.
 template <int BIAS, bool CAP, bool CAREFUL>
-__device__ inline void score_gradients(const AttnArgs& a, f32x16_t& s, const f32x16_t& dp, f32x16_t& y, float cc, float uncap,
-                                       float slope2, float gap, const AttnDist& dist, const float* table, int left, float lse2,
-                                       float delta, bool masked, f32x16_t* weights = nullptr) {
-    if constexpr (CAP) cap_scores(a.capped, s);
-    y = s;
-    bias_scores<BIAS, CAP, CAREFUL>(y, cc, slope2, gap, dist, table);
+__device__ inline void score_gradients(const AttnCap& cap, f32x16_t& s, const f32x16_t& dp, f32x16_t& y, f32x16_t* weights,
+                                       float cc, float uncap, float slope2, float gap, const AttnDist& dist,
+                                       const float* table, bool masked, int left, float lse2, float delta) {
+    if constexpr (CAP) {
+        cap_scores(cap, s, 0.0f);
+        y = s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float t = s[r] * uncap;
+            s[r] = fmaf(-t, t, 1.0f);
+            y[r] -= lse2;
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y[r] = fmaf(s[r], cc, -lse2);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        if constexpr (BIAS == GATGPU_BIAS_LINEAR) y[r] = fmaf(-slope2, fabsf(gap - float(8 * (r / 4) + r % 4)), y[r]);
+        if constexpr (BIAS == GATGPU_BIAS_TABLE) {
+            const float t = table[dist_of(dist, r)];
+            y[r] += t;
+            if (CAREFUL && t == -INFINITY) y[r] = t;
+        }
+    }
     if (masked) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -270,13 +305,9 @@ __device__ inline void score_gradients(const AttnArgs& a, f32x16_t& s, const f32
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const float p = exp2_hw(BIAS == GATGPU_BIAS_NONE && !CAP ? fmaf(y[r], cc, -lse2) : y[r] - lse2);
+        const float p = exp2_hw(y[r]);
         if (weights) (*weights)[r] = p;
         y[r] = CAREFUL && p == 0.0f ? 0.0f : p * (dp[r] - delta);
-        if (CAP) {
-            const float t = s[r] * uncap;
-            s[r] = fmaf(-t, t, 1.0f);
-        }
     }
 }
 
@@ -295,6 +326,11 @@ __device__ inline void turn_store(char* to, const AttnCols<T>& c, int lane) {
         if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + 16 * i) = make_uint2(c.w[2 * i], c.w[2 * i + 1]);
         else *reinterpret_cast<uint4*>(row + 32 * i) = make_uint4(c.w[4 * i], c.w[4 * i + 1], c.w[4 * i + 2], c.w[4 * i + 3]);
     }
+}
+
+// Query of a packed row.
+__device__ inline uint32_t group_of(const AttnArgs& a, uint32_t row) {
+    return (__umulhi(row, a.group_mul) + row) >> a.group_shift;
 }
 
 // Rows of a tile in LDS.
@@ -316,28 +352,49 @@ constexpr int attn_waves() {
 
 // Tile of BK rows (keys, or packed query rows) of one head on its way from memory to LDS: loads
 // of 16 bytes a thread, requested a tile ahead.  Rows from `end` on and columns from `dim` on are 0.
+// A thread's first place in a tile is the same in every tile, its others lie a fixed number of rows
+// further, and a tile's address is the block's own; where these do not fit 31 bits, or those rows
+// are no whole number of queries, addresses are formed anew.
 template <class T, int D, int NW, int BK>
 struct AttnStage {
-    static constexpr int kCpr = D * int(sizeof(T)) / 16, kPerThread = BK * kCpr / (NW * 64);
+    static constexpr int kCpr = D * int(sizeof(T)) / 16, kPerThread = BK * kCpr / (NW * 64), kRowStep = NW * 64 / kCpr;
     uint4 r[kPerThread];
-    __device__ void load(const T* base, uint64_t stride, uint32_t first, uint32_t end, int dim) {
-#pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            const int chunk = int(threadIdx.x) + i * NW * 64, c = chunk % kCpr * AttnType<T>::kPer;
-            const uint32_t row = first + uint32_t(chunk / kCpr);
-            r[i] = row < end && c < dim ? *reinterpret_cast<const uint4*>(base + row * stride + c) : make_uint4(0, 0, 0, 0);
-        }
+    uint32_t at;    // byte offset of the first place in a tile
+    uint32_t step;  // bytes from place to place, 0: addresses are formed anew
+    __device__ void place(const AttnArgs& a, uint64_t stride, int group) {
+        const uint64_t bytes = stride * sizeof(T) * uint64_t(BK);
+        step = kRowStep % group == 0 && bytes < (uint64_t(1) << 31)
+                   ? uint32_t(stride * sizeof(T)) * uint32_t(kRowStep / group)
+                   : 0u;
+        const uint32_t row = threadIdx.x / uint32_t(kCpr), q = group == 1 ? row : group_of(a, row);
+        at = uint32_t((q * stride + (row - q * uint32_t(group)) * uint32_t(a.dim)) * sizeof(T)) +
+             threadIdx.x % uint32_t(kCpr) * 16u;
     }
-    // The same of packed rows: `group` vectors of `dim` side by side in each row of the array.
-    __device__ void load_packed(const T* base, uint64_t stride, uint32_t first, uint32_t end, int dim, int group) {
-        if (group == 1) return load(base, stride, first, end, dim);
+    // Rows first .. first + BK of `base`; first is a multiple of BK.
+    __device__ void load(const AttnArgs& a, const T* base, uint64_t stride, int group, uint32_t first, uint32_t end) {
+        const bool wide = a.dim == D;
+        if (__builtin_expect(step != 0, 1)) {
+            const char* tile = reinterpret_cast<const char*>(base) + uint64_t(first / uint32_t(kRowStep)) * step;
+            if (wide && first + BK <= end) {
+#pragma unroll
+                for (int i = 0; i < kPerThread; ++i) r[i] = *reinterpret_cast<const uint4*>(tile + uint64_t(i) * step + at);
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                const int chunk = int(threadIdx.x) + i * NW * 64;
+                const bool in = first + uint32_t(chunk / kCpr) < end && chunk % kCpr * AttnType<T>::kPer < a.dim;
+                r[i] = in ? *reinterpret_cast<const uint4*>(tile + uint64_t(i) * step + at) : make_uint4(0, 0, 0, 0);
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
             const int chunk = int(threadIdx.x) + i * NW * 64, c = chunk % kCpr * AttnType<T>::kPer;
-            const uint32_t row = first + uint32_t(chunk / kCpr), q = row / uint32_t(group);
-            r[i] = row < end && c < dim
-                       ? *reinterpret_cast<const uint4*>(base + q * stride + (row - q * uint32_t(group)) * uint32_t(dim) + c)
-                       : make_uint4(0, 0, 0, 0);
+            const uint32_t row = first + uint32_t(chunk / kCpr), q = group == 1 ? row : group_of(a, row);
+            r[i] = row < end && c < a.dim ? *reinterpret_cast<const uint4*>(base + q * stride +
+                                                                           (row - q * uint32_t(group)) * uint32_t(a.dim) + c)
+                                          : make_uint4(0, 0, 0, 0);
         }
     }
     __device__ void store(char* lds) const {
@@ -356,8 +413,8 @@ struct AttnRow {
 };
 __device__ inline AttnRow attn_row(const AttnArgs& a, const AttnSeg& s, uint32_t row, int kv) {
     AttnRow w;
-    w.query = int(row / uint32_t(a.group));
-    w.local = int(row % uint32_t(a.group));
+    w.query = int(group_of(a, row));
+    w.local = int(row) - w.query * a.group;
     w.head = kv * a.group + w.local;
     w.pos = w.query + int(s.k_len) - int(s.q_len);
     w.lim = a.causal ? min(int(s.k_len), max(w.pos + 1, int(s.prefix))) : int(s.k_len);
