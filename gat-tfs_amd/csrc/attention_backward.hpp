@@ -122,12 +122,12 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
         uint32_t tile = 0;
         for (uint32_t k0 = 0; k0 < end; k0 += BK, ++tile) {
             const int buf = NBUF == 2 ? int(tile & 1) : 0;
-            if (NBUF == 1) __syncthreads();
+            if (NBUF == 1) lds_barrier();
             sk.store(lds_k[buf]);
             sv.store(lds_v[buf]);
 #pragma unroll
             for (int b = 0; b < NB; ++b) dist[b] = next_dist[b];
-            __syncthreads();
+            lds_barrier();
             if (k0 + BK < end) {
                 sk.load(a, kbase, a.ks, 1, k0 + BK, end);
                 sv.load(a, vbase, a.vs, 1, k0 + BK, end);
@@ -152,11 +152,7 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
                                                     float(w.pos - int(k0) - b * 32 - 4 * half), dist[b], trow, masked,
                                                     w.lim - int(k0) - b * 32 - 4 * half, lse2, delta);
                 if constexpr (TABLE) {
-                    if (binned && live) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            bins[min(int(dist_of(dist[b], r)), a.buckets - 1) * COLS + threadIdx.x] += y[r];
-                    }
+                    if (binned && live) add_bins(bins + threadIdx.x, COLS, a.buckets, dist[b], y);
                 }
                 if constexpr (CAP) {
 #pragma unroll
@@ -170,11 +166,11 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
             }
         }
     };
-    if constexpr (TABLE) __syncthreads();
+    if constexpr (TABLE) lds_barrier();
     pass(std::false_type{});
     const bool bad = !idle && nonfinite(acc);
     if (__builtin_expect(NW == 1 ? __any(bad) : __syncthreads_or(bad), 0)) {
-        if (NW > 1) __syncthreads();
+        if (NW > 1) lds_barrier();
         sk.load(a, kbase, a.ks, 1, 0, end);
         sv.load(a, vbase, a.vs, 1, 0, end);
         if constexpr (TABLE) {
@@ -186,7 +182,7 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
     store_rows<T, DB>(a.dq, grow * a.dqs + uint64_t(w.head) * dim, acc, a.scale, half, dim, live);
     if (!binned) return;
     // Each bucket's columns, by head of the group, in one fixed order.
-    __syncthreads();
+    lds_barrier();
     float* to = a.dbias + ((a.first_part + task_id) * uint64_t(a.kv_heads) + uint64_t(kv)) * uint64_t(a.group * a.buckets);
     for (int b = wave; b < a.buckets; b += NW)
         for (int g = 0; g < a.group; ++g) {
@@ -287,7 +283,7 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
         uint32_t tile = 0;
         for (uint32_t r0 = task.lo; r0 < end; r0 += BQ, ++tile) {
             const int buf = NBUF == 2 ? int(tile & 1) : 0;
-            if (NBUF == 1) __syncthreads();
+            if (NBUF == 1) lds_barrier();
             sq.store(lds_q[buf]);
             so.store(lds_o[buf]);
             if (tid < BQ) {
@@ -304,7 +300,7 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
                     r_query[buf][tid] = w.query;
                 }
             }
-            __syncthreads();
+            lds_barrier();
             if (r0 + BQ < end) request(r0 + BQ);
             const int row = role * 32 + l32, lim = r_lim[buf][row];
             const int lim_last = __builtin_amdgcn_readlane(lim, 31);
@@ -336,7 +332,7 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
                 turn_store<T>(lds_p[pair][0][role], to_operand<T>(p), lane);
                 turn_store<T>(lds_p[pair][1][role], to_operand<T>(y), lane);
             }
-            __syncthreads();
+            lds_barrier();
             if (idle || int(key0) >= lim_tile) continue;
             // dv: dout and the weights; dk: Q and the score gradients.
             const char* cols = role ? lds_q[buf] : lds_o[buf];
@@ -359,11 +355,11 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
             // them, keeps the turned tiles until every wave has read them: they are written after it.)
         }
     };
-    __syncthreads();
+    lds_barrier();
     pass(std::false_type{});
     const bool bad = !idle && nonfinite(acc);
     if (__builtin_expect(__syncthreads_or(bad), 0)) {
-        __syncthreads();
+        lds_barrier();
         pass(std::true_type{});
     }
     const bool in = key < seg.k_len;

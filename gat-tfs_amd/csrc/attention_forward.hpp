@@ -84,12 +84,12 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(
         uint32_t tile = 0;
         for (uint32_t k0 = task.lo; k0 < end; k0 += BK, ++tile) {
             const int buf = NBUF == 2 ? int(tile & 1) : 0;
-            if (NBUF == 1) __syncthreads();
+            if (NBUF == 1) lds_barrier();
             sk.store(lds_k[buf]);
             sv.store(lds_v[buf]);
 #pragma unroll
             for (int b = 0; b < NB; ++b) dist[b] = next_dist[b];
-            __syncthreads();
+            lds_barrier();
             if (k0 + BK < end) {
                 sk.load(a, kbase, a.ks, 1, k0 + BK, end);
                 sv.load(a, vbase, a.vs, 1, k0 + BK, end);
@@ -176,18 +176,18 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(
             }
         }
     };
-    if constexpr (BIAS == GATGPU_BIAS_TABLE) __syncthreads();
+    if constexpr (BIAS == GATGPU_BIAS_TABLE) lds_barrier();
     pass(std::false_type{});
     const bool bad = !idle && nonfinite(acc);
     if (__builtin_expect(NW == 1 ? __any(bad) : __syncthreads_or(bad), 0)) {
-        if (NW > 1) __syncthreads();
+        if (NW > 1) lds_barrier();
         sk.load(a, kbase, a.ks, 1, task.lo, end);
         sv.load(a, vbase, a.vs, 1, task.lo, end);
         if constexpr (BIAS == GATGPU_BIAS_TABLE) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, task.lo + b * 32 + 4 * half, seg.dist_ld);
         }
-        if (NW == 1) __syncthreads();
+        if (NW == 1) lds_barrier();
         pass(std::true_type{});
     }
     if (idle) return;

@@ -21,10 +21,16 @@ namespace {
 // Row operand of 32 rows: lane's row at p (null columns behind dim).
 template <class T, int NF>
 __device__ inline void load_row(uint4 (&f)[NF], const T* p, int half, int dim) {
+    p += half * AttnType<T>::kPer;
+    if (dim == 2 * NF * AttnType<T>::kPer) {
 #pragma unroll
-    for (int i = 0; i < NF; ++i) {
-        const int at = (2 * i + half) * AttnType<T>::kPer;
-        f[i] = at < dim ? *reinterpret_cast<const uint4*>(p + at) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < NF; ++i) f[i] = *reinterpret_cast<const uint4*>(p + 2 * i * AttnType<T>::kPer);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+            const bool in = (2 * i + half) * AttnType<T>::kPer < dim;
+            f[i] = in ? *reinterpret_cast<const uint4*>(p + 2 * i * AttnType<T>::kPer) : make_uint4(0, 0, 0, 0);
+        }
     }
 }
 // The same to LDS, as rows.
@@ -188,23 +194,33 @@ struct SmallLds {
     static constexpr int kSum = (D + 4) * 4;  // a row of a wave's share of dq
     static constexpr int kKeys = NW * 32 * kRow, kTile = 32 * kRow, kTurn = NW * 32 * attn_turn_row<T>(),
                          kDelta = 2 * NW * 32 * 4, kShare = NW == 1 ? 0 : NW * 32 * kSum;
-    static constexpr int kBytes = kKeys + 2 * kTile + kTurn + kDelta + kShare;
+    static constexpr int kBytes = 2 * kKeys + 2 * kTile + kTurn + kDelta + kShare;
     static constexpr int kCols = NW * 64 + 1;  // bias gradient: [buckets][kCols], a column a lane
     static size_t bytes(int bias, int group, int buckets, bool binned) {
         return size_t(kBytes) + (bias == GATGPU_BIAS_TABLE ? size_t(group) * 1024 + (binned ? size_t(buckets) * kCols * 4 : 0) : 0);
     }
 };
 
+// Orders the LDS traffic of a block; of one wave without a barrier.
+template <int NW>
+__device__ inline void block_sync() {
+    if constexpr (NW == 1) wave_sync();
+    else lds_barrier();
+}
+
 template <class T, int D, int NW, int BIAS, bool CAP>
 __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void k_attn_small_bwd(const AttnArgs a) {
     using L = SmallLds<T, D, NW>;
     constexpr int ROW = L::kRow, NF = D * int(sizeof(T)) / 32, DB = D / 32, PROW = attn_turn_row<T>(), COLS = L::kCols;
-    constexpr int CPR = D * int(sizeof(T)) / 16, CHUNKS = 32 * CPR, PER = (CHUNKS + NW * 64 - 1) / (NW * 64);
+    // Of a tile's rows one wave loads Q and dout; of two or four the even ones load Q, the odd ones dout,
+    // PART of the row's NF parts of 32 bytes each.
+    constexpr int PART = NW <= 2 ? NF : (NF + 1) / 2, LOADS = NW == 1 ? 2 * NF : PART;
     constexpr bool TABLE = BIAS == GATGPU_BIAS_TABLE;
     constexpr bool AHEAD = D * int(sizeof(T)) <= 128;  // the next head's keys are requested ahead
     extern __shared__ __align__(16) char lds[];
     char* const lds_k = lds;
-    char* const lds_q = lds_k + L::kKeys;
+    char* const lds_v = lds_k + L::kKeys;
+    char* const lds_q = lds_v + L::kKeys;
     char* const lds_o = lds_q + L::kTile;
     char* const turns = lds_o + L::kTile;
     float* const lds_delta = reinterpret_cast<float*>(turns + L::kTurn);  // [2][NW][32]
@@ -223,8 +239,10 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
     const uint64_t krow = seg.k_begin + min(key, seg.k_len - 1);
     char* const turn = turns + wave * 32 * PROW;
     char* const own_k = lds_k + wave * 32 * ROW;
+    char* const own_v = lds_v + wave * 32 * ROW;
 
-    uint4 nk[NF], nv[NF], nq[PER], no[PER];
+    uint4 nk[NF], nv[NF], nr[LOADS];
+    const int first_part = NW == 4 ? wave / 2 * PART : 0;
     float nlse = 0.0f, nt = 0.0f;
     AttnDist nd{};
     const auto request_keys = [&](int kv) {
@@ -233,21 +251,20 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
         load_row<T, NF>(nv, static_cast<const T*>(a.v) + krow * a.vs + uint64_t(kv) * dim, half, dim);
     };
     const auto request_rows = [&](int kv, uint32_t tile) {
-        const T* q = static_cast<const T*>(a.q) + seg.q_begin * a.qs + uint64_t(kv) * uint64_t(a.group * dim);
-        const T* o = static_cast<const T*>(a.dout) + seg.q_begin * a.dos + uint64_t(kv) * uint64_t(a.group * dim);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int chunk = tid + i * NW * 64, c = chunk % CPR * AttnType<T>::kPer;
-            const uint32_t r = tile * 32 + uint32_t(chunk / CPR), query = group_of(a, r);
-            // (Rows behind the last are 0 and weigh nothing.)
-            const bool in = r < rows && c < dim && (CHUNKS >= NW * 64 || chunk < CHUNKS);
-            const uint32_t at = (r - query * uint32_t(a.group)) * uint32_t(dim) + uint32_t(c);
-            nq[i] = in ? *reinterpret_cast<const uint4*>(q + query * a.qs + at) : make_uint4(0, 0, 0, 0);
-            no[i] = in ? *reinterpret_cast<const uint4*>(o + query * a.dos + at) : make_uint4(0, 0, 0, 0);
-        }
         const uint32_t r = tile * 32 + uint32_t(l32);
         const AttnRow w = attn_row(a, seg, min(r, rows - 1), kv);
-        nlse = r < rows ? a.lse[(seg.q_begin + uint64_t(w.query)) * uint64_t(a.heads) + w.head] : -INFINITY;
+        const uint64_t g = seg.q_begin + uint64_t(w.query);
+        const T* q = static_cast<const T*>(a.q) + g * a.qs + uint64_t(w.head) * dim + half * AttnType<T>::kPer;
+        const T* o = static_cast<const T*>(a.dout) + g * a.dos + uint64_t(w.head) * dim + half * AttnType<T>::kPer;
+        const T* p = wave & 1 ? o : q;
+        // (Rows behind the last are 0 and weigh nothing.)
+        const int there = r < rows ? dim - half * AttnType<T>::kPer : 0;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int f = NW == 1 ? i % NF : first_part + i, c = 2 * f * AttnType<T>::kPer;
+            nr[i] = c < there ? *reinterpret_cast<const uint4*>((NW > 1 ? p : i < NF ? q : o) + c) : make_uint4(0, 0, 0, 0);
+        }
+        nlse = r < rows ? a.lse[g * uint64_t(a.heads) + w.head] : -INFINITY;
         if constexpr (TABLE)
             nd = load_dist(a.dist + seg.dist + uint64_t(w.query) * seg.dist_ld, key0 + 4 * half, seg.dist_ld);
     };
@@ -257,17 +274,15 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
     request_keys(int(task.lo));
     if (tiles) request_rows(int(task.lo), 0);
     for (int kv = int(task.lo); kv < int(task.hi); ++kv) {
-        uint4 kf[NF], vf[NF];
         f32x16_t acc_k[DB], acc_v[DB];
         if (!AHEAD && kv > int(task.lo)) request_keys(kv);
-        __syncthreads();
+        block_sync<NW>();
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc_k[d] = acc_v[d] = f32x16_t{};
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
-            kf[f] = nk[f];
-            vf[f] = nv[f];
             *reinterpret_cast<uint4*>(own_k + l32 * ROW + half * 16 + 32 * f) = nk[f];
+            *reinterpret_cast<uint4*>(own_v + l32 * ROW + half * 16 + 32 * f) = nv[f];
         }
         if constexpr (TABLE) {
             if (wave == 0 || a.group > 1) spread_table(a, kv, lane, nt, table);
@@ -276,16 +291,14 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
             for (int b = 0; b < a.buckets; ++b) bins[b * COLS + tid] = 0.0f;
         for (uint32_t tile = 0; tile < tiles; ++tile) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int chunk = tid + i * NW * 64;
-                if (CHUNKS >= NW * 64 || chunk < CHUNKS) {
-                    *reinterpret_cast<uint4*>(lds_q + chunk / CPR * ROW + chunk % CPR * 16) = nq[i];
-                    *reinterpret_cast<uint4*>(lds_o + chunk / CPR * ROW + chunk % CPR * 16) = no[i];
-                }
+            for (int i = 0; i < LOADS; ++i) {
+                const int f = NW == 1 ? i % NF : first_part + i;
+                char* to = NW == 1 ? (i < NF ? lds_q : lds_o) : wave & 1 ? lds_o : lds_q;
+                if (NF % PART == 0 || f < NF) *reinterpret_cast<uint4*>(to + l32 * ROW + half * 16 + 32 * f) = nr[i];
             }
             const float lse2 = nlse == -INFINITY ? INFINITY : nlse * kLog2e;
             const AttnDist dist = nd;
-            __syncthreads();
+            block_sync<NW>();
             if (tile + 1 < tiles) {
                 request_rows(kv, tile + 1);
             } else if (kv + 1 < int(task.hi)) {
@@ -298,37 +311,29 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
             const float* trow = table + w.local * 256;
             const int left = w.lim - int(key0) - 4 * half, lim_first = __builtin_amdgcn_readlane(w.lim, 0);
             const float gap = float(w.pos - int(key0) - 4 * half);
-            f32x16_t acc_q[DB];
-            // Adds the tile to the gradients, and returns whether all of its rows' deltas were finite: if
-            // not, nothing was added and the careful form follows (a NaN or an infinity in any
-            // operand, or in a product, makes its row's delta one).  All waves have the same deltas.
-            const auto pass = [&](auto careful) {
+            f32x16_t s, y, p, acc_q[DB];
+            float delta;
+            // Weights p, dp (in y) and the rows' deltas, the same in every wave.  (s keeps the capped
+            // scores for their slope.)
+            const auto weights = [&](auto careful) {
                 constexpr bool CAREFUL = decltype(careful)::value;
-                constexpr int CLEAN = CAREFUL ? kClean : kRaw;
-                f32x16_t s = f32x16_t{}, y = f32x16_t{};
+                s = y = f32x16_t{};
                 if (!idle) {
 #pragma unroll
                     for (int f = 0; f < NF; ++f) {
-                        s = mfma_rows<T>(s, kf[f], from_lds(lds_q, f));
-                        y = mfma_rows<T>(y, vf[f], from_lds(lds_o, f));
+                        s = mfma_rows<T>(s, from_lds(own_k, f), from_lds(lds_q, f));
+                        y = mfma_rows<T>(y, from_lds(own_v, f), from_lds(lds_o, f));
                     }
                 }
-                // (s keeps the capped scores for their slope)
-                f32x16_t p;
-                if constexpr (CAP) {
-                    cap_scores(a.capped, s, 0.0f);
-                    p = s;
-                    tile_scores<BIAS, false, CAREFUL>(a.capped, p, 1.0f, lse2, slope2, gap, dist, trow);
-                } else {
-                    p = s;
-                    tile_scores<BIAS, false, CAREFUL>(a.capped, p, cc, lse2, slope2, gap, dist, trow);
-                }
+                if constexpr (CAP) cap_scores(a.capped, s, 0.0f);
+                p = s;
+                tile_scores<BIAS, false, CAREFUL>(a.capped, p, CAP ? 1.0f : cc, lse2, slope2, gap, dist, trow);
                 if (lim_first < int(key0) + 32) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         if (8 * (e / 4) + e % 4 >= left) p[e] = -INFINITY;
                 }
-                float delta = 0.0f;
+                delta = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     p[e] = exp2_hw(p[e]);
@@ -339,24 +344,29 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
                 if (NW > 1) {
                     float* all = lds_delta + (CAREFUL ? NW * 32 : 0);
                     if (half == 0) all[wave * 32 + l32] = delta;
-                    __syncthreads();
+                    block_sync<NW>();
                     delta = 0.0f;
 #pragma unroll
                     for (int v = 0; v < NW; ++v) delta += all[v * 32 + l32];
                 }
-                if (!CAREFUL && __any(delta * 0.0f != 0.0f)) return false;
+            };
+            weights(std::false_type{});
+            // A NaN or an infinity in any operand, or in a product, makes its row's delta one: then weights
+            // of 0 are kept out of everything.
+            const bool careful = __any(delta * 0.0f != 0.0f);
+            if (__builtin_expect(careful, 0)) weights(std::true_type{});
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc_q[d] = f32x16_t{};
-                if (idle) return true;
-                wave_sync();
+            for (int d = 0; d < DB; ++d) acc_q[d] = f32x16_t{};
+            if (!idle) {
                 turn_store<T>(turn, to_operand<T>(p), lane);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) y[e] = CAREFUL && p[e] == 0.0f ? 0.0f : p[e] * (y[e] - delta);
-                if constexpr (TABLE) {
-                    if (binned && r < rows) {
+                for (int e = 0; e < 16; ++e) y[e] = p[e] * (y[e] - delta);
+                if (__builtin_expect(careful, 0)) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) bins[min(int(dist_of(dist, e)), a.buckets - 1) * COLS + tid] += y[e];
-                    }
+                    for (int e = 0; e < 16; ++e) y[e] = p[e] == 0.0f ? 0.0f : y[e];
+                }
+                if constexpr (TABLE) {
+                    if (binned && r < rows) add_bins(bins + tid, COLS, a.buckets, dist, y);
                 }
                 if constexpr (CAP) {
 #pragma unroll
@@ -366,32 +376,29 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
                     }
                 }
                 wave_sync();
-                const AttnCols<T> pc = load_cols<T>(turn, PROW, 0, lane);
-                const AttnCols<T> yo = to_operand<T>(y);
-                if constexpr (CAREFUL) {
-                    wave_sync();
-                    turn_store<T>(turn, seen_operand<T>(p), lane);
-                    wave_sync();
-                    const AttnCols<T> seen = load_cols<T>(turn, PROW, 0, lane);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc_v[d] = mfma_cols_careful<T>(acc_v[d], lds_o, ROW, d * 32, lane, pc, seen);
-                } else {
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc_v[d] = mfma_cols<T>(acc_v[d], load_cols<T>(lds_o, ROW, d * 32, lane), pc);
-                }
+                const AttnCols<T> pc = load_cols<T>(turn, PROW, 0, lane), yo = to_operand<T>(y);
                 wave_sync();
                 turn_store<T>(turn, yo, lane);
                 wave_sync();
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-                    acc_q[d] = mfma_cols<T>(acc_q[d], load_cols<T, CLEAN>(own_k, ROW, d * 32, lane), yo);
                 const AttnCols<T> yc = load_cols<T>(turn, PROW, 0, lane);
+                if (__builtin_expect(!careful, 1)) {
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
-                    acc_k[d] = mfma_cols<T>(acc_k[d], load_cols<T, CLEAN>(lds_q, ROW, d * 32, lane), yc);
-                return true;
-            };
-            if (__builtin_expect(!pass(std::false_type{}), 0)) (void)pass(std::true_type{});
+                    for (int d = 0; d < DB; ++d) {
+                        acc_v[d] = mfma_cols<T>(acc_v[d], load_cols<T>(lds_o, ROW, d * 32, lane), pc);
+                        acc_q[d] = mfma_cols<T>(acc_q[d], load_cols<T>(own_k, ROW, d * 32, lane), yo);
+                        acc_k[d] = mfma_cols<T>(acc_k[d], load_cols<T>(lds_q, ROW, d * 32, lane), yc);
+                        if (DB > 1) __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else {
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        acc_v[d] = mfma_cols_careful<T>(acc_v[d], lds_o, ROW, d * 32, lane, pc, nonzero_operand<T>(pc));
+                        acc_q[d] = mfma_cols<T>(acc_q[d], load_cols<T, kClean>(own_k, ROW, d * 32, lane), yo);
+                        acc_k[d] = mfma_cols<T>(acc_k[d], load_cols<T, kClean>(lds_q, ROW, d * 32, lane), yc);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            }
             if constexpr (NW == 1) {
                 store_rows<T, DB>(a.dq, (seg.q_begin + uint64_t(w.query)) * a.dqs + uint64_t(w.head) * dim, acc_q, a.scale, half,
                                   dim, r < rows);
@@ -405,7 +412,7 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
                     for (int i = 0; i < 4; ++i)
                         *reinterpret_cast<float4*>(mine + d * 32 + 8 * i) =
                             make_float4(acc_q[d][4 * i], acc_q[d][4 * i + 1], acc_q[d][4 * i + 2], acc_q[d][4 * i + 3]);
-                __syncthreads();
+                block_sync<NW>();
                 for (int c = tid; c < 32 * D / 8; c += NW * 64) {
                     const uint32_t row = tile * 32 + uint32_t(c / (D / 8));
                     const int col = c % (D / 8) * 8;
@@ -436,19 +443,28 @@ __global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void 
         store_rows<T, DB>(a.dk, krow * a.dks + uint64_t(kv) * dim, acc_k, a.scale, half, dim, key < seg.k_len);
         store_rows<T, DB>(a.dv, krow * a.dvs + uint64_t(kv) * dim, acc_v, 1.0f, half, dim, key < seg.k_len);
         if (binned) {
-            // Two lanes a bucket, which add half of each wave's columns, those of one head of the group at a time.
-            __syncthreads();
+            // Two lanes a bucket, which add half of each wave's columns, those of one head of the group at a
+            // time.  (With one head the reads are independent of each other and go out together.)
+            block_sync<NW>();
             float* to = a.dbias + (uint64_t(task.at) * uint64_t(a.kv_heads) + uint64_t(kv)) * uint64_t(a.group * a.buckets);
-            for (int b = wave * 32 + l32; b < (a.buckets + 31) / 32 * 32; b += NW * 32)
+            for (int b = wave * 32 + l32; b < (a.buckets + 31) / 32 * 32; b += NW * 32) {
+                const float* row = bins + min(b, a.buckets - 1) * COLS + 32 * half;
                 for (int g = 0; g < a.group; ++g) {
                     float sum = 0.0f;
-                    if (b < a.buckets)
+                    if (a.group == 1) {
 #pragma unroll
                         for (int v = 0; v < NW; ++v)
-                            for (int i = g; i < 32; i += a.group) sum += bins[b * COLS + v * 64 + 32 * half + i];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sum += row[v * 64 + i];
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < NW; ++v)
+                            for (int i = g; i < 32; i += a.group) sum += row[v * 64 + i];
+                    }
                     sum = xor32_add(sum);
                     if (half == 0 && b < a.buckets) to[g * a.buckets + b] = sum;
                 }
+            }
         }
     }
 }

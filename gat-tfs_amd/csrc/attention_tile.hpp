@@ -163,12 +163,14 @@ __device__ inline f32x16_t mfma_cols_careful(f32x16_t acc, const char* rows, int
                                              const AttnCols<T>& w, const AttnCols<T>& seen) {
     acc = mfma_cols<T>(acc, load_cols<T, kClean>(rows, row, col, lane), w);
     const f32x16_t up = mfma_cols<T>(f32x16_t{}, load_cols<T, kUp>(rows, row, col, lane), seen);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if (up[r] > 0.0f) acc[r] += INFINITY;
+    __builtin_amdgcn_sched_barrier(0);  // (one at a time: no registers for both)
     const f32x16_t down = mfma_cols<T>(f32x16_t{}, load_cols<T, kDown>(rows, row, col, lane), seen);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        if (up[r] > 0.0f) acc[r] += INFINITY;
+    for (int r = 0; r < 16; ++r)
         if (down[r] > 0.0f) acc[r] -= INFINITY;
-    }
     return acc;
 }
 // Nonzero if a lane's part of a row operand holds a NaN or an infinity.
@@ -236,19 +238,30 @@ __device__ inline void fill_table(const AttnArgs& a, int kv, float* table) {
                        : table_log2(a.bias[(kv * a.group + (i >> 8)) * a.buckets + min(d, a.buckets - 1)]);
     }
 }
-// A lane's distance bytes of one 32-key block: keys first + 8 i + (0 .. 3), none behind the row's end.
+// A lane's distance bytes of one 32-key block: keys first + 8 i + (0 .. 3).  Behind the row's ld
+// bytes they are some others of the row: no query sees those keys.  (A segment without keys has no
+// distances at all.)
 struct AttnDist {
     uint32_t w[4];
 };
 __device__ inline AttnDist load_dist(const uint8_t* row, uint32_t first, uint32_t ld) {
-    AttnDist d;
+    AttnDist d{};
+    if (ld == 0) return d;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        d.w[i] = first + 8 * i < ld ? *reinterpret_cast<const uint32_t*>(row + first + 8 * i) : ~0u;
+    for (int i = 0; i < 4; ++i) d.w[i] = *reinterpret_cast<const uint32_t*>(row + min(first + 8 * i, ld - 4));
     return d;
 }
 __device__ inline uint32_t dist_of(const AttnDist& d, int r) { return d.w[r / 4] >> (8 * (r % 4)) & 255u; }
 
+// Adds a block's score gradients to the lane's column of the bias gradient, [buckets][cols].  (Graphs of
+// 130 to 1300 rows, the pass over query rows: 109 us so; 129 four at a time with equal buckets joined in
+// registers; 490 with LDS additions without a return.)
+__device__ inline void add_bins(float* column, int cols, int buckets, AttnDist d, const f32x16_t& y) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("" : "+v"(d.w[i]));  // (the bytes are taken apart anew, not kept since the scores)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) column[min(int(dist_of(d, r)), buckets - 1) * cols] += y[r];
+}
 // Scores of a block in units of log2, less `less`, from its raw products.  cc: their factor without
 // a cap; gap: the row's position less the block's first key of the lane; table: the row's entries.
 // A hidden pair's score is -inf; only CAREFUL keeps it so where its product is a NaN or +inf.
@@ -333,6 +346,13 @@ __device__ inline uint32_t group_of(const AttnArgs& a, uint32_t row) {
     return (__umulhi(row, a.group_mul) + row) >> a.group_shift;
 }
 
+// A barrier of the block for what its waves have in LDS.  Unlike __syncthreads it does not wait for
+// requests to memory: the next tile's loads and the last one's stores stay in flight across it.
+__device__ inline void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 // Rows of a tile in LDS.
 template <class T, int NW>
 constexpr int attn_tile_rows() {
