@@ -18,6 +18,7 @@ struct gatgpu_attention {
     // Short segments: forward of one and two blocks of 32 keys, backward of 1, 2 and 4 waves.
     gatgpu::DevBuf dsegs, dsmall[2], dsmall_bwd[3], dfwd, dbwd_q, dbwd_kv, djoin;
     uint64_t nsmall[2] = {}, nsmall_bwd[3] = {}, small_parts = 0, nfwd = 0, nbwd_q = 0, nbwd_kv = 0, njoin = 0;
+    uint32_t join_rows = 0;  // rows of the fullest joined tile
     int wfwd = 1, wbwd_q = 1, wbwd_kv = 1;  // waves a block
     gatgpu::AttnCap capped;
     bool split = false;
@@ -169,14 +170,17 @@ int build(gatgpu_attention* P) {
     q_tiles(fwd, 32u * uint32_t(P->wfwd), small);
     q_tiles(bq, 32u * uint32_t(P->wbwd_q), small_bwd);
     // Few tiles over long rows of keys: each tile's keys are cut into ranges that fill the chip.
+    // 4, 6, 8 and 12 ranges a unit and head took 200, 197, 197 and 210 us over 48 sequences of up to
+    // 24K keys, the join included: more ranges even out the last ones and cost more sums to join.
     uint64_t work = 0;
     for (const AttnTask& t : fwd) work += t.hi;
     if (P->wfwd == 1 && !fwd.empty() && fwd.size() * kvh < 4 * cus && longest > 256) {
-        const uint64_t want = std::max<uint64_t>(1, 8 * cus / kvh);  // tasks
+        const uint64_t want = std::max<uint64_t>(1, 6 * cus / kvh);  // tasks
         const uint64_t chunk = std::max<uint64_t>(128, (work / want + 31) / 32 * 32);
         std::vector<AttnTask> cut;
         for (const AttnTask& t : fwd) {
             join.push_back({t.seg, t.at, uint32_t(cut.size()), 0});
+            P->join_rows = std::max<uint32_t>(P->join_rows, std::min<uint32_t>(32, uint32_t(P->segs[t.seg].q_len * group) - t.at));
             uint64_t lo = 0;
             do {
                 const uint64_t hi = std::min<uint64_t>(t.hi, lo + chunk);
@@ -429,7 +433,8 @@ int gatgpu_attention_forward(gatgpu_attention* P, const gatgpu_attention_io* io,
         a.stat = reinterpret_cast<float*>(static_cast<char*>(ws) + part_bytes(P));
     }
     HIPCHECK(c, (bf16 ? launch_attention_forward_bf16 : launch_attention_forward_fp32)(a, P->wfwd, c->stream));
-    if (P->split) HIPCHECK(c, launch_attention_join(a, bf16, P->djoin.as<AttnTask>(), P->njoin, c->stream));
+    if (P->split) HIPCHECK(c, launch_attention_join(a, bf16, P->djoin.as<AttnTask>(), P->njoin, P->join_rows,
+                                                c->stream));
     return GATGPU_OK;
 }
 

@@ -103,8 +103,10 @@ hipError_t launch_attention_small_backward_bf16(const AttnArgs& a, int waves, hi
 size_t attention_small_backward_lds_bf16(int dim, int waves, int bias, int group, int buckets);
 hipError_t launch_attention_small_backward_fp32(const AttnArgs& a, int waves, hipStream_t s);
 size_t attention_small_backward_lds_fp32(int dim, int waves, int bias, int group, int buckets);
-// tiles: per split tile its segment and first row, and in lo / hi its first task and how many it has.
-hipError_t launch_attention_join(const AttnArgs& a, bool bf16, const AttnTask* tiles, uint64_t ntiles, hipStream_t s);
+// tiles: per split tile its segment and first row, and in lo / hi its first task and how many it has;
+// rows: the most that one of them has.
+hipError_t launch_attention_join(const AttnArgs& a, bool bf16, const AttnTask* tiles, uint64_t ntiles, uint32_t rows,
+                                 hipStream_t s);
 hipError_t launch_attention_bias_sum(const AttnArgs& a, uint64_t parts, float* dbias, hipStream_t s);
 
 constexpr int kAttnMaxDim = 128, kAttnMaxBuckets = 64;

@@ -208,17 +208,20 @@ struct KvLds {
     static constexpr int kRows = 64, kThreads = PAIRS * 128, kTile = kRows * lds_row<T, D>();
     static constexpr int kBuffers = 1;
     static constexpr int kTurn = 32 * attn_turn_row<T>();
-    static constexpr int kBytes = kBuffers * (2 * kTile + kRows * 7 * 4) + PAIRS * 4 * kTurn;
+    static constexpr bool kKeep = sizeof(T) == 2 && D == 128;  // V in LDS, for its 32 registers
+    static constexpr int kValues = kKeep ? PAIRS * 32 * lds_row<T, D>() : 16;
+    static constexpr int kBytes = kBuffers * (2 * kTile + kRows * 7 * 4) + PAIRS * 4 * kTurn + kValues;
 };
 
 template <class T, int D, int PAIRS, int BIAS, bool CAP>
-__global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS > 1) ? (D < 128 ? 3 : 2) : 1)) void k_attn_bwd_kv(const AttnArgs a) {
+__global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS > 1) ? (D < 64 ? 3 : 2) : 1)) void k_attn_bwd_kv(const AttnArgs a) {
     using L = KvLds<T, D, PAIRS>;
     constexpr int BQ = L::kRows, ROW = lds_row<T, D>(), NF = D * int(sizeof(T)) / 32, DB = D / 32, NBUF = L::kBuffers,
                   PROW = attn_turn_row<T>();
     constexpr bool TABLE = BIAS == GATGPU_BIAS_TABLE;
     __shared__ __align__(16) char lds_q[NBUF][L::kTile];
     __shared__ __align__(16) char lds_o[NBUF][L::kTile];
+    __shared__ __align__(16) char lds_v[L::kValues];
     __shared__ __align__(16) char lds_p[PAIRS][2][2][L::kTurn];  // weights, score gradients; of the tile's halves
     // Per packed row of a tile: log-sum in units of log2 (+inf: weighs nothing), delta, keys seen,
     // position, slope, first entry of its table, query
@@ -237,7 +240,8 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
     const bool idle = key0 >= seg.k_len;
     const int dim = a.dim;
     const uint64_t grow = seg.k_begin + min(key, seg.k_len - 1);
-    uint4 kf[NF], vf[NF];
+    uint4 kf[NF], vf[L::kKeep ? 1 : NF];
+    char* const own_v = lds_v + (L::kKeep ? (pair * 32 + l32) * ROW + half * 16 : 0);
     {
         const T* k = static_cast<const T*>(a.k) + grow * a.ks + uint64_t(kv) * dim;
         const T* v = static_cast<const T*>(a.v) + grow * a.vs + uint64_t(kv) * dim;
@@ -245,7 +249,9 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
         for (int f = 0; f < NF; ++f) {
             const int at = (2 * f + half) * AttnType<T>::kPer;
             kf[f] = at < dim ? *reinterpret_cast<const uint4*>(k + at) : make_uint4(0, 0, 0, 0);
-            vf[f] = at < dim ? *reinterpret_cast<const uint4*>(v + at) : make_uint4(0, 0, 0, 0);
+            const uint4 x = at < dim ? *reinterpret_cast<const uint4*>(v + at) : make_uint4(0, 0, 0, 0);
+            if constexpr (L::kKeep) *reinterpret_cast<uint4*>(own_v + 32 * f) = x;  // (both waves of the pair: the same)
+            else vf[f] = x;
         }
     }
     const T* qbase = static_cast<const T*>(a.q) + seg.q_begin * a.qs + uint64_t(kv) * uint64_t(a.group * dim);
@@ -317,7 +323,10 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
                 for (int f = 0; f < NF; ++f) {
                     const int at = row * ROW + f * 32 + half * 16;
                     s = mfma_rows<T>(s, kf[f], *reinterpret_cast<const uint4*>(lds_q[buf] + at));
-                    dp = mfma_rows<T>(dp, vf[f], *reinterpret_cast<const uint4*>(lds_o[buf] + at));
+                    uint4 value;
+                    if constexpr (L::kKeep) value = *reinterpret_cast<const uint4*>(own_v + 32 * f);
+                    else value = vf[f];
+                    dp = mfma_rows<T>(dp, value, *reinterpret_cast<const uint4*>(lds_o[buf] + at));
                 }
                 f32x16_t y, p;
                 score_gradients<BIAS, CAP, CAREFUL>(

@@ -194,6 +194,7 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_fwd(
     l = xor32_add(l);
     if (a.part) {  // a range of the keys: joined by k_attn_join
         const uint64_t at = (task_id * uint64_t(a.kv_heads) + uint64_t(kv)) * (NW * 32) + uint64_t(wave * 32 + l32);
+        if (row0 + uint32_t(l32) >= rows) return;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll

@@ -6,84 +6,101 @@
 namespace gatgpu {
 namespace {
 
-// Joins the key ranges of a split tile: 32 rows, 8 threads each.
+// Joins the key ranges of a split tile's rows: a wave a row and key/value head, a lane a range's
+// weight and D / 64 columns of the sums.  Ranges are added in order.
 template <class T, int D>
-__global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a, const AttnTask* __restrict__ tiles) {
-    const AttnTask tile = tiles[blockIdx.x / uint32_t(a.kv_heads)];
-    const int kv = int(blockIdx.x % uint32_t(a.kv_heads));
+__global__ __launch_bounds__(64) void k_attn_join(const AttnArgs a, const AttnTask* __restrict__ tiles, uint32_t per_tile) {
+    const uint32_t cell = blockIdx.x / per_tile;  // (tile, head)
+    const AttnTask tile = tiles[cell / uint32_t(a.kv_heads)];
+    const int kv = int(cell % uint32_t(a.kv_heads)), lane = int(threadIdx.x);
     const AttnSeg seg = a.segs[tile.seg];
-    const uint32_t rows = seg.q_len * uint32_t(a.group), row = tile.at + threadIdx.x / 8;
+    const uint32_t rows = seg.q_len * uint32_t(a.group), local = blockIdx.x % per_tile, row = tile.at + local;
     if (row >= rows) return;
     const AttnRow w = attn_row(a, seg, row, kv);
-    constexpr int N = D / 32;  // float4 a thread: columns 4 (8 i + threadIdx.x % 8)
-    const uint64_t step = uint64_t(a.kv_heads) * 32;
-    const uint64_t first = (uint64_t(tile.lo) * uint64_t(a.kv_heads) + uint64_t(kv)) * 32 + threadIdx.x / 8;
+    constexpr int N = D > 64 ? D / 64 : 1;
+    const uint64_t step = uint64_t(a.kv_heads) * 32, first = (uint64_t(tile.lo) * uint64_t(a.kv_heads) + uint64_t(kv)) * 32 + local;
     float m = -INFINITY;
-    for (uint32_t t = 0; t < tile.hi; ++t) m = fmaxf(m, a.stat[(first + t * step) * 2]);
+    for (uint32_t t = uint32_t(lane); t < tile.hi; t += 64) m = fmaxf(m, a.stat[(first + t * step) * 2]);
+#pragma unroll
+    for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
     const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    float4 o[N];
+    float l = 0.0f, o[N] = {};
+    const bool mine = D >= 64 || lane < D;
+    const int col = lane * N;
+    for (uint32_t t0 = 0; t0 < tile.hi; t0 += 64) {
+        const uint32_t t = t0 + uint32_t(lane), n = min(64u, tile.hi - t0);
+        float f = 0.0f, part_l = 0.0f;
+        if (t < tile.hi) {
+            const float2 st = *reinterpret_cast<const float2*>(a.stat + (first + t * step) * 2);
+            f = st.y == 0.0f ? 0.0f : exp2_hw(st.x - ref);  // (a range of which nothing is seen)
+            part_l = st.y * f;
+        }
+        for (uint32_t i = 0; i < n; i += 16) {  // 16 ranges' columns in flight
+            float v[16][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = make_float4(0, 0, 0, 0);
-    for (uint32_t t = 0; t < tile.hi; ++t) {
-        const float2 st = *reinterpret_cast<const float2*>(a.stat + (first + t * step) * 2);
-        const float f = exp2_hw(st.x - ref);
-        if (st.y == 0.0f) continue;  // a range of which nothing is seen
-        l += st.y * f;
+            for (int u = 0; u < 16; ++u)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float4 p = *reinterpret_cast<const float4*>(a.part + (first + t * step) * D + 4 * (8 * i + threadIdx.x % 8));
-            o[i].x += p.x * f;
-            o[i].y += p.y * f;
-            o[i].z += p.z * f;
-            o[i].w += p.w * f;
+                for (int e = 0; e < N; ++e)
+                    v[u][e] = mine ? a.part[(first + (t0 + min(i + u, n - 1)) * step) * D + uint64_t(col + e)] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                if (i + u >= n) break;
+                const float fi = __shfl(f, int(i) + u);
+                l += __shfl(part_l, int(i) + u);
+#pragma unroll
+                for (int e = 0; e < N; ++e) o[e] = fmaf(v[u][e], fi, o[e]);
+            }
         }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const uint64_t to = (seg.q_begin + uint64_t(w.query)) * a.os + uint64_t(w.head) * a.dim;
+    const uint64_t at = (seg.q_begin + uint64_t(w.query)) * a.os + uint64_t(w.head) * a.dim + uint64_t(col);
+    if (mine && col < a.dim) {  // (dim is a multiple of 8)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int at = 4 * (8 * i + int(threadIdx.x) % 8);
-        if (at >= a.dim) continue;
-        const float v[4] = {o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv};
-        store4<T>(a.out, to + at, v[0], v[1], v[2], v[3]);
-        if (sizeof(T) == 2 && a.rest) {
-            float d[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) d[e] = v[e] - bf16_widen(bf16_hw(v[e]));
-            store4<T>(a.rest, to + at, d[0], d[1], d[2], d[3]);
+        for (int e = 0; e < N; ++e) {
+            const float v = o[e] * inv;
+            if constexpr (sizeof(T) == 2) {
+                const uint16_t b = bf16_hw(v);
+                static_cast<uint16_t*>(a.out)[at + e] = b;
+                if (a.rest) static_cast<uint16_t*>(a.rest)[at + e] = bf16_hw(v - bf16_widen(b));
+            } else {
+                static_cast<float*>(a.out)[at + e] = v;
+            }
         }
     }
-    if (a.lse && threadIdx.x % 8 == 0)
+    if (a.lse && lane == 0)
         a.lse[(seg.q_begin + uint64_t(w.query)) * uint64_t(a.heads) + w.head] =
             l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
-// dbias[head][bucket]: partial sums of all parts, in one fixed order.  A block takes 32 cells, 32
+// dbias[head][bucket]: partial sums of all parts, in one fixed order.  A block takes 8 cells, 128
 // threads a cell.
 __global__ __launch_bounds__(1024) void k_attn_bias_sum(const float* __restrict__ part, uint64_t parts, uint32_t cells,
                                                         float* __restrict__ dbias) {
-    const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
-    __shared__ float lds[32][33];
+    const uint32_t c = blockIdx.x * 8 + (threadIdx.x & 7), g = threadIdx.x >> 3;
+    __shared__ float lds[128][9];
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (c < cells) {
         uint64_t p = g;
-        for (; p + 96 < parts; p += 128)
+        for (; p + 384 < parts; p += 512)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] += part[(p + 32 * i) * cells + c];
-        for (; p < parts; p += 32) s[0] += part[p * cells + c];
+            for (int i = 0; i < 4; ++i) s[i] += part[(p + 128 * i) * cells + c];
+        for (; p < parts; p += 128) s[0] += part[p * cells + c];
     }
-    lds[g][threadIdx.x & 31] = (s[0] + s[1]) + (s[2] + s[3]);
+    lds[g][threadIdx.x & 7] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
-    float sum = lds[threadIdx.x & 31][g];
+    const uint32_t cell = threadIdx.x >> 7, lane = threadIdx.x & 127;  // two waves a cell
+    float sum = lds[lane][cell];
 #pragma unroll
-    for (int d = 16; d; d /= 2) sum += __shfl_xor(sum, d);
-    if ((threadIdx.x & 31) == 0 && blockIdx.x * 32 + g < cells) dbias[blockIdx.x * 32 + g] = sum;
+    for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6][0] = sum;
+    __syncthreads();
+    if (lane == 0 && blockIdx.x * 8 + cell < cells) dbias[blockIdx.x * 8 + cell] = lds[2 * cell][0] + lds[2 * cell + 1][0];
 }
 
 template <class T, int D>
-hipError_t join(const AttnArgs& a, const AttnTask* tiles, uint64_t ntiles, hipStream_t s) {
-    k_attn_join<T, D><<<uint32_t(ntiles * uint64_t(a.kv_heads)), 256, 0, s>>>(a, tiles);
+hipError_t join(const AttnArgs& a, const AttnTask* tiles, uint64_t ntiles, uint32_t rows, hipStream_t s) {
+    k_attn_join<T, D><<<uint32_t(ntiles * uint64_t(a.kv_heads) * rows), 64, 0, s>>>(a, tiles, rows);
     return hipGetLastError();
 }
 
@@ -113,16 +130,17 @@ AttnCap attention_cap(float scale, float cap) {
     return c;
 }
 
-hipError_t launch_attention_join(const AttnArgs& a, bool bf16, const AttnTask* tiles, uint64_t ntiles, hipStream_t s) {
+hipError_t launch_attention_join(const AttnArgs& a, bool bf16, const AttnTask* tiles, uint64_t ntiles, uint32_t rows,
+                                 hipStream_t s) {
     switch (attention_width(a.dim)) {
-        case 32: return bf16 ? join<uint16_t, 32>(a, tiles, ntiles, s) : join<float, 32>(a, tiles, ntiles, s);
-        case 64: return bf16 ? join<uint16_t, 64>(a, tiles, ntiles, s) : join<float, 64>(a, tiles, ntiles, s);
-        default: return bf16 ? join<uint16_t, 128>(a, tiles, ntiles, s) : join<float, 128>(a, tiles, ntiles, s);
+        case 32: return bf16 ? join<uint16_t, 32>(a, tiles, ntiles, rows, s) : join<float, 32>(a, tiles, ntiles, rows, s);
+        case 64: return bf16 ? join<uint16_t, 64>(a, tiles, ntiles, rows, s) : join<float, 64>(a, tiles, ntiles, rows, s);
+        default: return bf16 ? join<uint16_t, 128>(a, tiles, ntiles, rows, s) : join<float, 128>(a, tiles, ntiles, rows, s);
     }
 }
 hipError_t launch_attention_bias_sum(const AttnArgs& a, uint64_t parts, float* dbias, hipStream_t s) {
     const uint32_t cells = uint32_t(a.heads) * uint32_t(a.buckets);
-    k_attn_bias_sum<<<(cells + 31) / 32, 1024, 0, s>>>(a.dbias, parts, cells, dbias);
+    k_attn_bias_sum<<<(cells + 7) / 8, 1024, 0, s>>>(a.dbias, parts, cells, dbias);
     return hipGetLastError();
 }
 
