@@ -17,11 +17,13 @@ struct gatgpu_attention {
     // Tables on the device: segments; tiles of the forward, the query and the key pass; joined tiles.
     // Short segments: forward of one and two blocks of 32 keys, backward of 1, 2 and 4 waves.
     gatgpu::DevBuf dsegs, dsmall[2], dsmall_bwd[3], dfwd, dbwd_q, dbwd_kv, djoin;
+    uint32_t own_delta = 0;  // segments of so many keys need no rest: their backward pass forms delta from its weights
     uint64_t nsmall[2] = {}, nsmall_bwd[3] = {}, small_parts = 0, nfwd = 0, nbwd_q = 0, nbwd_kv = 0, njoin = 0;
     uint32_t join_rows = 0;  // rows of the fullest joined tile
     int wfwd = 1, wbwd_q = 1, wbwd_kv = 1;  // waves a block
     gatgpu::AttnCap capped;
-    bool split = false;
+    bool split = false;  // the forward pass leaves ranges of keys to be joined
+    bool cut = false;    // its blocks cut the keys among their waves
     bool spread = false;
 };
 
@@ -54,7 +56,8 @@ namespace {
 
 using namespace gatgpu;
 
-constexpr uint64_t kMaxLen = uint64_t(1) << 30, kMaxRow = uint64_t(1) << 44, kMaxTasks = uint64_t(1) << 30;
+constexpr uint64_t kMaxLen = uint64_t(1) << 30, kMaxRow = uint64_t(1) << 44;
+constexpr uint64_t kMaxThreads = (uint64_t(1) << 32) - (1 << 16);  // of a launch
 
 // Keys that query i of a segment sees by position.
 uint32_t seen(const gatgpu_attention_shape& sh, const AttnSeg& s, int64_t i) {
@@ -96,12 +99,21 @@ int build(gatgpu_attention* P) {
     const bool bf16 = sh.precision == GATGPU_BF16;
     const int width = attention_width(sh.dim);
     const bool holds = bf16 ? attention_small_width<uint16_t>(width) : attention_small_width<float>(width);
-    const auto small = [&](const AttnSeg& s) { return holds && s.k_len > 0 && s.k_len <= 64; };
-    uint32_t most = 0;  // keys of a short segment's backward pass
+    // Forward, us with and without that kernel, 8 heads, table: 23 / 28 (1500 segments of up to 30 keys, 8 x 32 in
+    // bf16), 37 / 46 (in FP32); of 33 to 64 keys 94 / 129 (1500 segments, 8 x 64 in bf16), but 29 / 23 where a
+    // head's two tiles in turn leave the chip few waves (300 segments), and 126 / 110 in FP32.
+    uint64_t half = 0;  // segments of 33 to 64 keys
+    for (const AttnSeg& s : P->segs) half += s.k_len > 32 && s.k_len <= 64;
+    const uint32_t held = !holds ? 0 : bf16 && half * kvh >= 12 * cus ? 64 : 32;
+    const auto small = [&](const AttnSeg& s) { return s.k_len > 0 && s.k_len <= held; };
+    // Backward, the same: 53 / 122 (1500 of up to 30 keys, 8 x 32 in bf16), 167 / 249 (60), 533 / 558 (120); 8 x 64:
+    // 113 / 229, 303 / 472, but 1152 / 952 (120): four waves with a table, but one block a CU.
+    uint32_t most = 0;  // keys
     for (uint32_t w = 1; w <= 4 && 32 % group == 0; w *= 2)
-        if ((bf16 ? attention_small_backward_lds_bf16 : attention_small_backward_lds_fp32)(sh.dim, int(w), sh.bias, int(group),
-                                                                                           sh.buckets) <= kAttnLds)
+        if ((bf16 ? attention_small_backward_lds_bf16 : attention_small_backward_lds_fp32)(sh.dim, int(w), sh.bias, int(group), sh.buckets) <=
+            (w == 4 && sh.bias == GATGPU_BIAS_TABLE ? kAttnLds / 2 : kAttnLds))
             most = 32 * w;
+    P->own_delta = most;
     const auto small_bwd = [&](const AttnSeg& s) { return s.k_len > 0 && s.k_len <= most; };
     std::vector<AttnTask> sf[2], sb[3];
     const auto waves_of = [](const AttnSeg& s) { return s.k_len <= 32 ? 0 : s.k_len <= 64 ? 1 : 2; };  // log2
@@ -143,11 +155,12 @@ int build(gatgpu_attention* P) {
             keys += s.k_len;
         }
     }
-    const auto full = [&](uint64_t total, uint64_t tiles, uint64_t tile) {
-        // Four waves a block where the chip is filled all the same and three of four waves have rows.
-        return tiles * kvh >= 2 * cus && total >= tiles * tile * 3 / 4;
-    };
-    P->wfwd = full(frows, f4, 128) ? 4 : 1;
+    // Four waves a block share their tiles' keys (rows) where three of four have rows (keys).  Backward, us by
+    // four waves and by one: 35 / 37 (one segment of 600, 8 x 64), 100 / 133 (two of 2000), 22 / 23 (one of 300).
+    // Forward only where that leaves no units idle, since single waves can be cut further: 16 / 20 (four of 600,
+    // 160 blocks), 39 / 28 (one of 2000, 128 blocks); 32 columns 36 / 30 (256 blocks), 18.7 / 19.6 (320).
+    const auto full = [&](uint64_t total, uint64_t tiles, uint64_t tile) { return tiles && total >= tiles * tile * 3 / 4; };
+    P->wfwd = full(frows, f4, 128) && f4 * kvh * 2 > (width < 64 ? 2 * cus : cus) ? 4 : 1;
     P->wbwd_q = full(brows, q4, 128) ? 4 : 1;
     P->wbwd_kv = full(keys, k4, 64) ? 4 : 1;  // (two pairs of waves with 32 keys each, or one)
     // Wide tables for many shared heads leave no room for four waves' tiles.
@@ -169,16 +182,26 @@ int build(gatgpu_attention* P) {
     };
     q_tiles(fwd, 32u * uint32_t(P->wfwd), small);
     q_tiles(bq, 32u * uint32_t(P->wbwd_q), small_bwd);
-    // Few tiles over long rows of keys: each tile's keys are cut into ranges that fill the chip.
-    // 4, 6, 8 and 12 ranges a unit and head took 200, 197, 197 and 210 us over 48 sequences of up to
-    // 24K keys, the join included: more ranges even out the last ones and cost more sums to join.
-    uint64_t work = 0;
-    for (const AttnTask& t : fwd) work += t.hi;
-    if (P->wfwd == 1 && !fwd.empty() && fwd.size() * kvh < 4 * cus && longest > 256) {
+    // Few tiles: the keys of each are cut into ranges, so that more waves take part.  Those of at most
+    // `chunk` keys are tasks of their own, which another launch joins; 4, 6, 8 and 12 of them a unit and head
+    // took 200, 197, 197 and 210 us over 48 sequences of up to 24K keys: more ranges even out the last
+    // ones and cost more sums to join.  The waves of one block cut the keys instead (and join them in LDS)
+    // where that leaves each of them not much more.  One token over n keys, 8 x 64, bf16, us by
+    // blocks and by tasks: 5.5 / 8.1 (n = 400), 7.5 / 8.5 (900), 11.4 / 9.4 (1800); 16 of them: 13.4 / 19.5
+    // (1800); FP32 products take 8 times as long: 8.4 / 11.8 (400), 13.5 / 12.0 (900; 8 x 32).  Where blocks of
+    // one wave fill the chip, short rows stay with them: 64 tokens over 200 keys 9.2 by blocks, 8.6 so.
+    const uint64_t blocks = fwd.size() * kvh;
+    if (P->wfwd == 1 && blocks && blocks < 4 * cus && (longest > 256 || blocks <= cus)) {
+        uint64_t work = 0;
+        for (const AttnTask& t : fwd) work += t.hi;
         const uint64_t want = std::max<uint64_t>(1, 6 * cus / kvh);  // tasks
         const uint64_t chunk = std::max<uint64_t>(128, (work / want + 31) / 32 * 32);
+        const uint64_t cuts = uint64_t(bf16 ? attention_cuts<uint16_t>(width) : attention_cuts<float>(width));
+        P->cut = longest * 4 <= cuts * chunk * (bf16 ? 6 : 3) &&
+                 (bf16 ? attention_forward_cut_lds_bf16 : attention_forward_cut_lds_fp32)(sh.dim, sh.bias, int(group)) <= kAttnLds;
         std::vector<AttnTask> cut;
         for (const AttnTask& t : fwd) {
+            if (P->cut) break;
             join.push_back({t.seg, t.at, uint32_t(cut.size()), 0});
             P->join_rows = std::max<uint32_t>(P->join_rows, std::min<uint32_t>(32, uint32_t(P->segs[t.seg].q_len * group) - t.at));
             uint64_t lo = 0;
@@ -209,13 +232,14 @@ int build(gatgpu_attention* P) {
             bk.push_back({uint32_t(s), uint32_t(k), lo, n});
         }
     }
-    if (std::max({sf[0].size(), sf[1].size(), sb[0].size(), sb[1].size(), sb[2].size(), fwd.size(), bq.size(), bk.size(), join.size()}) * kvh >= kMaxTasks)
-        return fail(c, GATGPU_EOVERFLOW, "too many tiles");
     if (!P->split) longest_first(fwd);
     longest_first(bq);
     longest_first(bk);
-    // Rows of long segments: an XCD keeps few heads' keys in its L2; short segments: whole lines.
-    P->spread = longest > 256;
+    // A task's heads go to different XCDs, whose L2s then keep few heads' keys each, or to the same one, which
+    // then has whole lines of narrow rows.  Forward and backward in bf16, us: 24 graphs of 650 to 1300 rows, 8 x 64
+    // 139 + 413 spread, 164 + 500 not; 500 of 60 to 120 69 + 310, 71 + 314; 8 x 32: 100 of 250 29 + 80, 27 + 65;
+    // 24 of 1300 84 + 210, 92 + 218.
+    P->spread = longest > 512 || sh.dim * (bf16 ? 2 : 4) >= 128;
     for (int i = 0; i < 2; ++i) {
         P->nsmall[i] = sf[i].size();
         if (int r = upload(c, P->dsmall[i], sf[i].data(), sf[i].size() * sizeof(AttnTask))) return r;
@@ -335,7 +359,7 @@ int create(gatgpu_ctx* c, const gatgpu_attention_shape* sh, uint64_t n, const ui
     if (!(sh->scale > 0.0f) || !std::isfinite(sh->scale)) return fail(c, GATGPU_EINVAL, "scale must be positive and finite");
     if (!(sh->cap >= 0.0f) || !std::isfinite(sh->cap)) return fail(c, GATGPU_EINVAL, "cap must be 0 or positive and finite");
     if (n && (!q_begin || !q_len || !k_begin || !k_len)) return fail(c, GATGPU_EINVAL, "null segment array");
-    if (n > kMaxTasks) return fail(c, GATGPU_EOVERFLOW, "too many segments");
+    if (n > kMaxThreads / 64) return fail(c, GATGPU_EOVERFLOW, "too many segments");
     const uint64_t group = uint64_t(sh->heads / sh->kv_heads);
     std::unique_ptr<gatgpu_attention> P(new gatgpu_attention);
     P->ctx = c;
@@ -343,6 +367,7 @@ int create(gatgpu_ctx* c, const gatgpu_attention_shape* sh, uint64_t n, const ui
     P->capped = attention_cap(sh->scale, sh->cap);
     if (sh->bias != GATGPU_BIAS_TABLE) P->shape.buckets = 0;
     P->segs.resize(n);
+    uint64_t threads = 0;
     for (uint64_t s = 0; s < n; ++s) {
         AttnSeg& g = P->segs[s];
         g.q_begin = q_begin[s];
@@ -355,6 +380,9 @@ int create(gatgpu_ctx* c, const gatgpu_attention_shape* sh, uint64_t n, const ui
             return fail(c, GATGPU_EOVERFLOW, "segment " + std::to_string(s) + " is longer than 2^30 rows");
         if (g.q_begin > kMaxRow || g.k_begin > kMaxRow)
             return fail(c, GATGPU_EOVERFLOW, "segment " + std::to_string(s) + " begins beyond 2^44 rows");
+        // A wave 32 packed rows, two waves 32 keys, of each key/value head.
+        threads += std::max((g.q_len * group + 31) / 32, (uint64_t(g.k_len) + 31) / 32 * 2) * 64 * uint64_t(sh->kv_heads);
+        if (threads > kMaxThreads) return fail(c, GATGPU_EOVERFLOW, "more tiles than a launch takes");
         g.base = P->rows;
         g.dist = P->dist_bytes;
         P->rows += g.q_len;
@@ -423,8 +451,10 @@ int gatgpu_attention_forward(gatgpu_attention* P, const gatgpu_attention_io* io,
     for (int i = 1; i >= 0; --i) {
         a.tasks = P->dsmall[i].as<AttnTask>();
         a.ntasks = P->nsmall[i];
+        a.rest = P->own_delta >= uint32_t(32 * (i + 1)) ? nullptr : io->rest;
         if (a.ntasks) HIPCHECK(c, (bf16 ? launch_attention_small_forward_bf16 : launch_attention_small_forward_fp32)(a, i + 1, c->stream));
     }
+    a.rest = io->rest;
     a.tasks = P->dfwd.as<AttnTask>();
     a.ntasks = P->nfwd;
     if (!a.ntasks) return GATGPU_OK;
@@ -432,9 +462,12 @@ int gatgpu_attention_forward(gatgpu_attention* P, const gatgpu_attention_io* io,
         a.part = static_cast<float*>(ws);
         a.stat = reinterpret_cast<float*>(static_cast<char*>(ws) + part_bytes(P));
     }
+    if (P->cut) {
+        HIPCHECK(c, (bf16 ? launch_attention_forward_cut_bf16 : launch_attention_forward_cut_fp32)(a, c->stream));
+        return GATGPU_OK;
+    }
     HIPCHECK(c, (bf16 ? launch_attention_forward_bf16 : launch_attention_forward_fp32)(a, P->wfwd, c->stream));
-    if (P->split) HIPCHECK(c, launch_attention_join(a, bf16, P->djoin.as<AttnTask>(), P->njoin, P->join_rows,
-                                                c->stream));
+    if (P->split) HIPCHECK(c, launch_attention_join(a, bf16, P->djoin.as<AttnTask>(), P->njoin, P->join_rows, c->stream));
     return GATGPU_OK;
 }
 

@@ -91,6 +91,11 @@ constexpr size_t kAttnLds = 160 * 1024;
 // waves: 1 or 4 waves a block, 32 packed rows (keys) each.
 hipError_t launch_attention_forward_bf16(const AttnArgs& a, int waves, hipStream_t s);
 hipError_t launch_attention_forward_fp32(const AttnArgs& a, int waves, hipStream_t s);
+// Blocks that cut the keys of 32 packed rows among their waves; the LDS of such a block.
+hipError_t launch_attention_forward_cut_bf16(const AttnArgs& a, hipStream_t s);
+hipError_t launch_attention_forward_cut_fp32(const AttnArgs& a, hipStream_t s);
+size_t attention_forward_cut_lds_bf16(int dim, int bias, int group);
+size_t attention_forward_cut_lds_fp32(int dim, int bias, int group);
 hipError_t launch_attention_backward_q_bf16(const AttnArgs& a, int waves, hipStream_t s);
 hipError_t launch_attention_backward_q_fp32(const AttnArgs& a, int waves, hipStream_t s);
 hipError_t launch_attention_backward_kv_bf16(const AttnArgs& a, int waves, hipStream_t s);
@@ -119,6 +124,11 @@ inline int attention_width(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 1
 template <class T>
 constexpr bool attention_small_width(int width) {
     return width * int(sizeof(T)) <= 128;
+}
+// Waves of a block that cut its rows' keys among themselves: as many as the LDS of a CU holds tiles of.
+template <class T>
+constexpr int attention_cuts(int width) {
+    return width * int(sizeof(T)) > 256 ? 4 : 8;
 }
 // a.group and what divides by it: (high half of n mul + n) >> shift for n < 2^31.
 inline void set_group(AttnArgs& a, int group) {

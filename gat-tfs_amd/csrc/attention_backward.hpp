@@ -42,7 +42,6 @@ __device__ inline float dot16(uint4 a, uint4 b, uint4 c) {
     return sum;
 }
 
-
 template <class T, int D, int NW, int BIAS, bool CAP>
 __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_q(const AttnArgs a) {
     constexpr int BK = attn_tile_rows<T, NW>(), NB = BK / 32, ROW = lds_row<T, D>(), NF = D * int(sizeof(T)) / 32,
@@ -113,7 +112,7 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
     const float* trow = table + w.local * 256;
 
     f32x16_t acc[DB];
-    const auto pass = [&](auto careful) {
+    const auto pass = [&](auto careful) __attribute__((always_inline)) {
         constexpr bool CAREFUL = decltype(careful)::value;
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
@@ -206,27 +205,26 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
 template <class T, int D, int PAIRS>
 struct KvLds {
     static constexpr int kRows = 64, kThreads = PAIRS * 128, kTile = kRows * lds_row<T, D>();
-    static constexpr int kBuffers = 1;
     static constexpr int kTurn = 32 * attn_turn_row<T>();
     static constexpr bool kKeep = sizeof(T) == 2 && D == 128;  // V in LDS, for its 32 registers
     static constexpr int kValues = kKeep ? PAIRS * 32 * lds_row<T, D>() : 16;
-    static constexpr int kBytes = kBuffers * (2 * kTile + kRows * 7 * 4) + PAIRS * 4 * kTurn + kValues;
+    static constexpr int kBytes = 2 * kTile + kRows * 7 * 4 + PAIRS * 4 * kTurn + kValues;
 };
 
 template <class T, int D, int PAIRS, int BIAS, bool CAP>
 __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS > 1) ? (D < 64 ? 3 : 2) : 1)) void k_attn_bwd_kv(const AttnArgs a) {
     using L = KvLds<T, D, PAIRS>;
-    constexpr int BQ = L::kRows, ROW = lds_row<T, D>(), NF = D * int(sizeof(T)) / 32, DB = D / 32, NBUF = L::kBuffers,
+    constexpr int BQ = L::kRows, ROW = lds_row<T, D>(), NF = D * int(sizeof(T)) / 32, DB = D / 32,
                   PROW = attn_turn_row<T>();
     constexpr bool TABLE = BIAS == GATGPU_BIAS_TABLE;
-    __shared__ __align__(16) char lds_q[NBUF][L::kTile];
-    __shared__ __align__(16) char lds_o[NBUF][L::kTile];
+    __shared__ __align__(16) char lds_q[L::kTile];
+    __shared__ __align__(16) char lds_o[L::kTile];
     __shared__ __align__(16) char lds_v[L::kValues];
     __shared__ __align__(16) char lds_p[PAIRS][2][2][L::kTurn];  // weights, score gradients; of the tile's halves
     // Per packed row of a tile: log-sum in units of log2 (+inf: weighs nothing), delta, keys seen,
     // position, slope, first entry of its table, query
-    __shared__ float r_lse[NBUF][BQ], r_delta[NBUF][BQ], r_slope[NBUF][BQ];
-    __shared__ int r_lim[NBUF][BQ], r_pos[NBUF][BQ], r_tab[NBUF][BQ], r_query[NBUF][BQ];
+    __shared__ float r_lse[BQ], r_delta[BQ], r_slope[BQ];
+    __shared__ int r_lim[BQ], r_pos[BQ], r_tab[BQ], r_query[BQ];
     extern __shared__ float table[];  // TABLE: [group][256]
 
     uint64_t task_id;
@@ -265,7 +263,7 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
     sq.place(a, a.qs, a.group);
     so.place(a, a.dos, a.group);
     float n_lse = 0.0f, n_delta = 0.0f;
-    const auto request = [&](uint32_t r0) {
+    const auto request = [&](uint32_t r0) __attribute__((always_inline)) {
         sq.load(a, qbase, a.qs, a.group, r0, end);
         so.load(a, obase, a.dos, a.group, r0, end);
         if (tid < BQ) {
@@ -281,59 +279,57 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
             }
         }
     };
-    const auto pass = [&](auto careful) {
+    const auto pass = [&](auto careful) __attribute__((always_inline)) {
         constexpr bool CAREFUL = decltype(careful)::value;
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
         if (task.lo < end) request(task.lo);
-        uint32_t tile = 0;
-        for (uint32_t r0 = task.lo; r0 < end; r0 += BQ, ++tile) {
-            const int buf = NBUF == 2 ? int(tile & 1) : 0;
-            if (NBUF == 1) lds_barrier();
-            sq.store(lds_q[buf]);
-            so.store(lds_o[buf]);
+        for (uint32_t r0 = task.lo; r0 < end; r0 += BQ) {
+            lds_barrier();
+            sq.store(lds_q);
+            so.store(lds_o);
             if (tid < BQ) {
                 const AttnRow w = attn_row(a, seg, min(r0 + uint32_t(tid), rows - 1), kv);
-                r_lse[buf][tid] = n_lse;
-                r_delta[buf][tid] = n_delta;
-                r_lim[buf][tid] = w.lim;
+                r_lse[tid] = n_lse;
+                r_delta[tid] = n_delta;
+                r_lim[tid] = w.lim;
                 if (BIAS == GATGPU_BIAS_LINEAR) {
-                    r_pos[buf][tid] = w.pos;
-                    r_slope[buf][tid] = a.bias[w.head] * kLog2e;
+                    r_pos[tid] = w.pos;
+                    r_slope[tid] = a.bias[w.head] * kLog2e;
                 }
                 if (TABLE) {
-                    r_tab[buf][tid] = w.local * 256;
-                    r_query[buf][tid] = w.query;
+                    r_tab[tid] = w.local * 256;
+                    r_query[tid] = w.query;
                 }
             }
             lds_barrier();
             if (r0 + BQ < end) request(r0 + BQ);
-            const int row = role * 32 + l32, lim = r_lim[buf][row];
+            const int row = role * 32 + l32, lim = r_lim[row];
             const int lim_last = __builtin_amdgcn_readlane(lim, 31);
             // (Rows are in order of what they see: the tile's last row sees the most.)
-            const int lim_tile = __builtin_amdgcn_readfirstlane(r_lim[buf][63]);
-            const int lim_half = __builtin_amdgcn_readfirstlane(r_lim[buf][31]);
+            const int lim_tile = __builtin_amdgcn_readfirstlane(r_lim[63]);
+            const int lim_half = __builtin_amdgcn_readfirstlane(r_lim[31]);
             if (!idle && int(key0) < lim_last) {
                 const bool masked = int(key0) + 32 > __builtin_amdgcn_readlane(lim, 0);
                 AttnDist dist{};
                 if constexpr (TABLE)
-                    dist = load_dist(a.dist + seg.dist + uint64_t(r_query[buf][row]) * seg.dist_ld, key0 + 4 * half, seg.dist_ld);
+                    dist = load_dist(a.dist + seg.dist + uint64_t(r_query[row]) * seg.dist_ld, key0 + 4 * half, seg.dist_ld);
                 f32x16_t s = f32x16_t{}, dp = f32x16_t{};
 #pragma unroll
                 for (int f = 0; f < NF; ++f) {
                     const int at = row * ROW + f * 32 + half * 16;
-                    s = mfma_rows<T>(s, kf[f], *reinterpret_cast<const uint4*>(lds_q[buf] + at));
+                    s = mfma_rows<T>(s, kf[f], *reinterpret_cast<const uint4*>(lds_q + at));
                     uint4 value;
                     if constexpr (L::kKeep) value = *reinterpret_cast<const uint4*>(own_v + 32 * f);
                     else value = vf[f];
-                    dp = mfma_rows<T>(dp, value, *reinterpret_cast<const uint4*>(lds_o[buf] + at));
+                    dp = mfma_rows<T>(dp, value, *reinterpret_cast<const uint4*>(lds_o + at));
                 }
                 f32x16_t y, p;
                 score_gradients<BIAS, CAP, CAREFUL>(
-                    a.capped, s, dp, y, &p, cc, uncap, BIAS == GATGPU_BIAS_LINEAR ? r_slope[buf][row] : 0.0f,
-                    BIAS == GATGPU_BIAS_LINEAR ? float(r_pos[buf][row] - int(key0) - 4 * half) : 0.0f, dist,
-                    table + (TABLE ? r_tab[buf][row] : 0), masked, lim - int(key0) - 4 * half, r_lse[buf][row],
-                    r_delta[buf][row]);
+                    a.capped, s, dp, y, &p, cc, uncap, BIAS == GATGPU_BIAS_LINEAR ? r_slope[row] : 0.0f,
+                    BIAS == GATGPU_BIAS_LINEAR ? float(r_pos[row] - int(key0) - 4 * half) : 0.0f, dist,
+                    table + (TABLE ? r_tab[row] : 0), masked, lim - int(key0) - 4 * half, r_lse[row],
+                    r_delta[row]);
                 if constexpr (CAP) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) y[r] *= s[r];
@@ -344,7 +340,7 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
             lds_barrier();
             if (idle || int(key0) >= lim_tile) continue;
             // dv: dout and the weights; dk: Q and the score gradients.
-            const char* cols = role ? lds_q[buf] : lds_o[buf];
+            const char* cols = role ? lds_q : lds_o;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 if (b == 0 && int(key0) >= lim_half) continue;
@@ -360,8 +356,7 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
                     }
                 }
             }
-            // (With one buffer the barrier ahead of the next tile's stores, with two the one behind
-            // them, keeps the turned tiles until every wave has read them: they are written after it.)
+            // (The barriers of the next tile keep the turned tiles until every wave has read them.)
         }
     };
     lds_barrier();

@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64, (D * int(sizeof(T)) * KB <= 128 ? 2 : 1)) void 
     const int lane = int(threadIdx.x), l32 = lane & 31, half = lane >> 5, dim = a.dim;
     const uint32_t rows = seg.q_len * uint32_t(a.group), tiles = (rows + 31) / 32;
     const float cc = a.scale * kLog2e;
-    const bool exact = sizeof(T) == 2 && TABLE && a.rest;
+    const bool exact = sizeof(T) == 2 && a.rest;
 
     uint4 nk[KB][NF], nv[KB][NF], nq[NF];
     AttnDist nd[KB];
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(64, (D * int(sizeof(T)) * KB <= 128 ? 2 : 1)) void 
             const int lim_first = __builtin_amdgcn_readlane(w.lim, 0);
             f32x16_t acc[DB];
             float m, l;
-            const auto pass = [&](auto careful) {
+            const auto pass = [&](auto careful) __attribute__((always_inline)) {
                 constexpr bool CAREFUL = decltype(careful)::value;
                 f32x16_t s[KB];
                 float top = -INFINITY;
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(64, (D * int(sizeof(T)) * KB <= 128 ? 2 : 1)) void 
                             acc[d] = mfma_cols_careful<T>(acc[d], vrows, ROW, d * 32, lane, p, seen_operand<T>(s[b]));
                         else acc[d] = mfma_cols<T>(acc[d], load_cols<T>(vrows, ROW, d * 32, lane), p);
                     }
-                    if constexpr (sizeof(T) == 2 && TABLE) {
+                    if constexpr (sizeof(T) == 2) {
                         if (exact) {
                             const AttnCols<T> lo = rest_operand(s[b], p);
 #pragma unroll
@@ -208,8 +208,16 @@ __device__ inline void block_sync() {
     else lds_barrier();
 }
 
+// Waves a SIMD that its registers are held to: those of 64 bf16 columns, or of 32 FP32 ones and several
+// waves, do not fit half a SIMD's registers (1500 segments of up to 60 keys, 8 x 64 in bf16 with a
+// table: 461 us with what did not fit in memory, 303 us so; 8 x 32 in FP32: 426, 362).
+template <class T, int D, int NW>
+constexpr int small_bwd_waves() {
+    return D * int(sizeof(T)) <= 64 || (sizeof(T) == 4 && D == 32 && NW == 1) ? 2 : 1;
+}
+
 template <class T, int D, int NW, int BIAS, bool CAP>
-__global__ __launch_bounds__(NW * 64, (D * int(sizeof(T)) <= 128 ? 2 : 1)) void k_attn_small_bwd(const AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, (small_bwd_waves<T, D, NW>())) void k_attn_small_bwd(const AttnArgs a) {
     using L = SmallLds<T, D, NW>;
     constexpr int ROW = L::kRow, NF = D * int(sizeof(T)) / 32, DB = D / 32, PROW = attn_turn_row<T>(), COLS = L::kCols;
     // Of a tile's rows one wave loads Q and dout; of two or four the even ones load Q, the odd ones dout,
@@ -477,9 +485,15 @@ hipError_t small_forward(const AttnArgs& a, int blocks, hipStream_t s) {
         constexpr bool CAP = decltype(cap)::value;
         if constexpr (attention_small_width<T>(D)) {
             const size_t dyn = BIAS == GATGPU_BIAS_TABLE ? size_t(a.group) * 1024 : 0;
-            if (blocks == 1) k_attn_small_fwd<T, D, 1, BIAS, CAP><<<uint32_t(a.ntasks), 64, dyn, s>>>(a);
-            else k_attn_small_fwd<T, D, 2, BIAS, CAP><<<uint32_t(a.ntasks), 64, dyn, s>>>(a);
-            return hipGetLastError();
+            if (blocks == 1) {
+                k_attn_small_fwd<T, D, 1, BIAS, CAP><<<uint32_t(a.ntasks), 64, dyn, s>>>(a);
+                return hipGetLastError();
+            }
+            if constexpr (sizeof(T) == 2) {
+                k_attn_small_fwd<T, D, 2, BIAS, CAP><<<uint32_t(a.ntasks), 64, dyn, s>>>(a);
+                return hipGetLastError();
+            }
+            return hipErrorInvalidValue;
         } else {
             return hipErrorInvalidValue;
         }

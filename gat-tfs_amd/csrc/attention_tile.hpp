@@ -173,16 +173,6 @@ __device__ inline f32x16_t mfma_cols_careful(f32x16_t acc, const char* rows, int
         if (down[r] > 0.0f) acc[r] -= INFINITY;
     return acc;
 }
-// Nonzero if a lane's part of a row operand holds a NaN or an infinity.
-template <class T, int NF>
-__device__ inline uint32_t nonfinite_row(const uint4 (&f)[NF]) {
-    constexpr uint32_t mask = sizeof(T) == 2 ? 0x7f807f80u : 0x7f800000u, one = sizeof(T) == 2 ? 0x00800080u : 0x00800000u;
-    uint32_t any = 0;
-#pragma unroll
-    for (int i = 0; i < NF; ++i)
-        any |= ((f[i].x & mask) + one) | ((f[i].y & mask) + one) | ((f[i].z & mask) + one) | ((f[i].w & mask) + one);
-    return any & (sizeof(T) == 2 ? 0x80008000u : 0x80000000u);
-}
 // True if a lane's sums hold a NaN or an infinity.
 template <int N>
 __device__ inline bool nonfinite(const f32x16_t (&acc)[N]) {
@@ -378,20 +368,21 @@ constexpr int attn_waves() {
 template <class T, int D, int NW, int BK>
 struct AttnStage {
     static constexpr int kCpr = D * int(sizeof(T)) / 16, kPerThread = BK * kCpr / (NW * 64), kRowStep = NW * 64 / kCpr;
+    static __device__ uint32_t thread() { return NW == 1 ? threadIdx.x & 63u : threadIdx.x; }
     uint4 r[kPerThread];
     uint32_t at;    // byte offset of the first place in a tile
     uint32_t step;  // bytes from place to place, 0: addresses are formed anew
-    __device__ void place(const AttnArgs& a, uint64_t stride, int group) {
+    __device__ __forceinline__ void place(const AttnArgs& a, uint64_t stride, int group) {
         const uint64_t bytes = stride * sizeof(T) * uint64_t(BK);
         step = kRowStep % group == 0 && bytes < (uint64_t(1) << 31)
                    ? uint32_t(stride * sizeof(T)) * uint32_t(kRowStep / group)
                    : 0u;
-        const uint32_t row = threadIdx.x / uint32_t(kCpr), q = group == 1 ? row : group_of(a, row);
+        const uint32_t row = thread() / uint32_t(kCpr), q = group == 1 ? row : group_of(a, row);
         at = uint32_t((q * stride + (row - q * uint32_t(group)) * uint32_t(a.dim)) * sizeof(T)) +
-             threadIdx.x % uint32_t(kCpr) * 16u;
+             thread() % uint32_t(kCpr) * 16u;
     }
     // Rows first .. first + BK of `base`; first is a multiple of BK.
-    __device__ void load(const AttnArgs& a, const T* base, uint64_t stride, int group, uint32_t first, uint32_t end) {
+    __device__ __forceinline__ void load(const AttnArgs& a, const T* base, uint64_t stride, int group, uint32_t first, uint32_t end) {
         const bool wide = a.dim == D;
         if (__builtin_expect(step != 0, 1)) {
             const char* tile = reinterpret_cast<const char*>(base) + uint64_t(first / uint32_t(kRowStep)) * step;
@@ -402,7 +393,7 @@ struct AttnStage {
             }
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
-                const int chunk = int(threadIdx.x) + i * NW * 64;
+                const int chunk = int(thread()) + i * NW * 64;
                 const bool in = first + uint32_t(chunk / kCpr) < end && chunk % kCpr * AttnType<T>::kPer < a.dim;
                 r[i] = in ? *reinterpret_cast<const uint4*>(tile + uint64_t(i) * step + at) : make_uint4(0, 0, 0, 0);
             }
@@ -410,17 +401,17 @@ struct AttnStage {
         }
 #pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
-            const int chunk = int(threadIdx.x) + i * NW * 64, c = chunk % kCpr * AttnType<T>::kPer;
+            const int chunk = int(thread()) + i * NW * 64, c = chunk % kCpr * AttnType<T>::kPer;
             const uint32_t row = first + uint32_t(chunk / kCpr), q = group == 1 ? row : group_of(a, row);
             r[i] = row < end && c < a.dim ? *reinterpret_cast<const uint4*>(base + q * stride +
                                                                            (row - q * uint32_t(group)) * uint32_t(a.dim) + c)
                                           : make_uint4(0, 0, 0, 0);
         }
     }
-    __device__ void store(char* lds) const {
+    __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
-            const int chunk = int(threadIdx.x) + i * NW * 64;
+            const int chunk = int(thread()) + i * NW * 64;
             *reinterpret_cast<uint4*>(lds + chunk / kCpr * lds_row<T, D>() + chunk % kCpr * 16) = r[i];
         }
     }

@@ -356,12 +356,21 @@ def test_refusals(ctx):
                 refused(call, **{n: width - 8})
                 refused(call, **{n: width + 4})
             refused(call, k_stride=64)
-            refused(call, size=0)
-            refused(call, at=host.data_ptr() // 16 * 16 + 16)
+        refused(made.backward, size=0)
+        refused(made.backward, at=host.data_ptr() // 16 * 16 + 16)
         for n in ("dout", "dq", "dk", "dv", "lse"):
             refused(made.backward, **{n: None})
         refused(made.backward, rest=None)
         refused(made.backward, dbias=base + 2)
+    q = Problem([1], [20000], 4, 2, 64, BF, seed=26)  # its keys are cut into ranges that need a workspace
+    with q.plan(ctx) as made:
+        _, io = q.buffers(train=False)
+        need = made.workspace_bytes()
+        assert need > 0
+        for at, size in ((ws.data_ptr(), need - 1), (None, need), (host.data_ptr() // 16 * 16 + 16, need), (ws.data_ptr() + 8, need)):
+            with pytest.raises(gatgpu.GatGpuError) as err:
+                made.forward(io, at, size)
+            assert err.value.code == gatgpu.EINVAL
     q = Problem([4], [4], 2, 2, 32, FP, seed=24)
     with q.plan(ctx) as made, pytest.raises(gatgpu.GatGpuError):
         _, io = q.buffers()
