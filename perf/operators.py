@@ -194,9 +194,9 @@ def _own_attention(state):
         if case["bias"] == "table":
             out["dbias"] = torch.empty_like(state["bias"])
             io.dbias = out["dbias"].data_ptr()
-            if case["precision"] == "bf16":  # what rounding took from out: the table's gradient keeps FP32
-                state["rest"] = torch.empty_like(out["out"])
-                io.rest = state["rest"].data_ptr()
+        if case["precision"] == "bf16":  # what rounding took from out: the gradients keep their precision
+            state["rest"] = torch.empty_like(out["out"])
+            io.rest = state["rest"].data_ptr()
     need = max(plan.workspace_bytes(), plan.workspace_bytes(backward=True) if case["train"] else 0)
     state["work"] = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
     state.update(plan=plan, io=io, outputs=out)
