@@ -387,3 +387,54 @@ def test_the_current_device_stays(ctx):
     p = Problem([4], [4], 2, 2, 32, FP, seed=26)
     p.run(ctx)
     assert torch.cuda.current_device() == before
+
+
+@pytest.mark.parametrize("precision", [FP, BF])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("heads,kv_heads,q_len,bias,buckets", [(8, 8, 1, LINEAR, 0), (32, 2, 1, NONE, 0), (6, 2, 3, TABLE, 9), (40, 1, 2, TABLE, 64)])
+def test_waves_cut_the_keys(ctx, precision, dim, heads, kv_heads, q_len, bias, buckets):
+    """Few rows over some hundred keys: the waves of a block take a range each, some of them none."""
+    keys = [300, 33, 1, 0, 380, 97]
+    p = Problem([q_len] * 6, keys, heads, kv_heads, dim, precision, mask=PREFIX, bias=bias, buckets=buckets, cap=4.0, seed=31, gap=2)
+    if heads < 40:  # (a table for 40 heads leaves the widest tiles no room: tasks, joined by a launch)
+        assert p.plan(ctx).workspace_bytes() == 0
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("precision", [FP, BF])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_bad_values_where_waves_cut_the_keys(ctx, precision, value):
+    """The first query sees no bad key, the second one of them."""
+    p = Problem([2, 1], [290, 310], 4, 2, 64, precision, mask=PREFIX, seed=32)
+    p.v[289, 1, 5] = value
+    p.k[290 + 100, 0, 3] = math.nan
+    p.check(p.run(ctx, train=False), train=False)
+
+
+@pytest.mark.parametrize("precision", [FP, BF])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("heads,kv_heads,bias,buckets,cap", [(3, 1, LINEAR, 0, 3.0), (8, 1, TABLE, 5, 0.0), (2, 2, TABLE, 64, 0.0), (4, 2, NONE, 0, 2.0)])
+def test_segments_of_up_to_128_keys(ctx, precision, dim, heads, kv_heads, bias, buckets, cap):
+    """Every number of waves of the short segments' backward pass, and lengths at its edges."""
+    lens = [32, 33, 64, 65, 96, 97, 128, 129]
+    p = Problem([32, 5, 70, 65, 1, 97, 40, 20], lens, heads, kv_heads, dim, precision, mask=PREFIX, prefix=[10] * 8, bias=bias,
+                buckets=buckets, cap=cap, seed=33)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("dim", [32, 64])
+@pytest.mark.parametrize("bias,buckets", [(TABLE, 6), (LINEAR, 0)])
+def test_many_short_segments(ctx, dim, bias, buckets):
+    """So many that a wave takes several heads of a segment, and two blocks of keys."""
+    keys = [34 + i % 31 for i in range(56)] + [1 + i % 32 for i in range(140)]
+    p = Problem([n if i % 3 else 2 for i, n in enumerate(keys)], keys, 64, 64, dim, BF, bias=bias, buckets=buckets, seed=34)
+    p.check(p.run(ctx, train=False), train=False)
+
+
+def test_too_many_tiles_are_refused(ctx):
+    """Before anything is laid out for them."""
+    n = 1 << 30
+    with pytest.raises(gatgpu.GatGpuError) as err:
+        gatgpu.Attention(ctx, [n] * 5, [n] * 5, heads=1, kv_heads=1, dim=32, precision=BF, q_begin=[i * n for i in range(5)],
+                         k_begin=[i * n for i in range(5)])
+    assert err.value.code == gatgpu.EOVERFLOW
