@@ -101,12 +101,20 @@ __device__ inline float elu_to(float t) {
     else return elu(t);
 }
 
+// Blocks of a launch of n: a dimension has at most 2^32 - 1 threads.  Blocks behind the last have no row.
+constexpr uint64_t kNormGridX = uint64_t(1) << 20;
+dim3 norm_grid(uint64_t n) {
+    const uint64_t y = (n + kNormGridX - 1) / kNormGridX;
+    return dim3(uint32_t((n + y - 1) / y), uint32_t(y));
+}
+__device__ inline uint64_t norm_block() { return uint64_t(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 template <class T, int VEC, int TPR, int ITEMS>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const NormArgs a) {
     constexpr int BLOCK = TPR < 256 ? 256 : TPR;
     __shared__ float lds[BLOCK / 64];
-    const uint64_t row = uint64_t(blockIdx.x) * (BLOCK / TPR) + threadIdx.x / TPR;
-    if (TPR <= 64 && row >= a.rows) return;  // (whole row groups; wider rows are whole blocks)
+    const uint64_t row = norm_block() * (BLOCK / TPR) + threadIdx.x / TPR;
+    if (row >= a.rows) return;  // (whole row groups; of rows wider than a wave whole blocks)
     const uint32_t t = threadIdx.x % TPR, W = a.width;
     const T* x = static_cast<const T*>(a.x) + row * a.xs;
     float v[ITEMS][VEC];
@@ -168,7 +176,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const NormAr
 template <class T>
 __global__ __launch_bounds__(1024) void k_norm_fwd_any(const NormArgs a) {
     __shared__ float lds[16];
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = norm_block();
+    if (row >= a.rows) return;
     const uint32_t W = a.width;
     const T* x = static_cast<const T*>(a.x) + row * a.xs;
     const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.rs : nullptr;
@@ -333,7 +342,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormAr
 template <class T>
 __global__ __launch_bounds__(1024) void k_norm_bwd_any(const NormArgs a) {
     __shared__ float2 lds[16];
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = norm_block();
+    if (row >= a.rows) return;
     const uint32_t W = a.width;
     const float mean = a.mean[row], rstd = a.rstd[row];
     const T* h = static_cast<const T*>(a.h) + row * a.hs;
@@ -441,13 +451,16 @@ bool aligned(const void* p, uint64_t stride, int size) {
 
 template <class T, int VEC>
 hipError_t forward(const NormArgs& a, NormShape s, hipStream_t st) {
-    const uint64_t per = s.tpr < 256 ? 256 / s.tpr : 1;
-    const dim3 grid{uint32_t((a.rows + per - 1) / per)};
+    if (!s.tpr) {
+        k_norm_fwd_any<T><<<norm_grid(a.rows), 1024, 0, st>>>(a);
+        return hipGetLastError();
+    }
+    const uint64_t per = s.tpr < 256 ? 256 / uint64_t(s.tpr) : 1;
+    const dim3 grid = norm_grid((a.rows + per - 1) / per);
 #define F(TPR, ITEMS) \
     if (s.tpr == TPR && s.items == ITEMS) k_norm_fwd<T, VEC, TPR, ITEMS><<<grid, TPR < 256 ? 256 : TPR, 0, st>>>(a);
     GATGPU_NORM_SHAPES(F)
 #undef F
-    if (!s.tpr) k_norm_fwd_any<T><<<uint32_t(a.rows), 1024, 0, st>>>(a);
     return hipGetLastError();
 }
 template <class T, int VEC>
@@ -458,7 +471,7 @@ hipError_t backward(const NormArgs& a, NormShape s, uint32_t blocks, hipStream_t
 #undef F
     if (!s.tpr) {
         if (a.part) k_norm_cols_any<T><<<dim3((a.width + 255) / 256, blocks), 256, 0, st>>>(a);
-        if (a.rows) k_norm_bwd_any<T><<<uint32_t(a.rows), 1024, 0, st>>>(a);
+        if (a.rows) k_norm_bwd_any<T><<<norm_grid(a.rows), 1024, 0, st>>>(a);
     }
     return hipGetLastError();
 }

@@ -225,6 +225,25 @@ def test_no_rows(ctx):
     assert bool((got["y"] == 7.0).all()) and bool((got["dgamma"] == 0).all()) and bool((got["dbeta"] == 0).all())
 
 
+@pytest.mark.parametrize("width,rows", [(2, (1 << 28) + 5), (1040, (1 << 20) + 3), (4097, (1 << 20) + 3)])
+def test_more_rows_than_one_grid_dimension_takes(ctx, width, rows):
+    """In place; more than 2^32 threads, and more than 2^20 blocks of a row each."""
+    x = torch.empty(rows, width, dtype=torch.bfloat16, device="cuda").fill_(3.0)
+    at = torch.tensor([0, 1, (1 << 20) - 1, rows // 2, rows - 2, rows - 1], device="cuda")
+    x[at] = torch.randn(at.numel(), width, generator=torch.Generator(device="cuda").manual_seed(8), device="cuda").to(torch.bfloat16)
+    h = x[at].double()
+    io = gatgpu.NormIO(precision=gatgpu.BF16, rows=rows, width=width, eps=1e-5, x=x.data_ptr(), x_stride=width,
+                       y=x.data_ptr(), y_stride=width)
+    torch.cuda.synchronize()
+    ctx.norm_forward(io)
+    ctx.synchronize()
+    want = (h - h.mean(1, keepdim=True)) / torch.sqrt(h.var(1, unbiased=False, keepdim=True) + 1e-5)
+    # FP32 sums of at most 4097 columns by 16 threads or more, values of at most 6, beside the stored rounding
+    assert float(((x[at].double() - want).abs() - UB * want.abs()).max()) <= 600 * U * 36
+    # (a constant row's norm is 0 up to its mean's rounding, 3 u, over sqrt(eps))
+    assert sum(int((part.abs() > 1e-2).any(1).sum()) for part in x.split(1 << 24)) == at.numel()
+
+
 def test_gradients_against_differences(ctx):
     p = Norm(20, 48, gatgpu.FP32, residual=False, elu=True, seed=6)
     got = p.run(ctx)
