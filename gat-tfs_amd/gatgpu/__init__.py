@@ -380,6 +380,11 @@ class Attention:
                                                     _ptr(begins[1]), _ptr(lens[1]), _ptr(prefix), ctypes.byref(h)))
         self.h = h
 
+    def _plan(self):
+        if not self.h or not self.ctx.h:
+            raise ValueError("the plan or its context is closed")
+        return self.h
+
     def close(self):
         if self.h and self.ctx.h:  # (a context that is gone has taken its stream with it)
             self.lib.gatgpu_attention_destroy(self.h)
@@ -399,18 +404,18 @@ class Attention:
 
     def workspace_bytes(self, backward=False):
         f, b = ctypes.c_uint64(), ctypes.c_uint64()
-        self.ctx._check(self.lib.gatgpu_attention_workspace(self.h, ctypes.byref(f), ctypes.byref(b)))
+        self.ctx._check(self.lib.gatgpu_attention_workspace(self._plan(), ctypes.byref(f), ctypes.byref(b)))
         return b.value if backward else f.value
 
     def distance_layout(self):
         """(bytes, offsets, row strides) of the pair distances, per segment."""
         n = ctypes.c_uint64()
         off, ld = np.empty(self.segments, np.uint64), np.empty(self.segments, np.uint32)
-        self.ctx._check(self.lib.gatgpu_attention_distances(self.h, ctypes.byref(n), _ptr(off), _ptr(ld)))
+        self.ctx._check(self.lib.gatgpu_attention_distances(self._plan(), ctypes.byref(n), _ptr(off), _ptr(ld)))
         return n.value, off, ld
 
     def forward(self, io, workspace=None, workspace_bytes=0):
-        self.ctx._check(self.lib.gatgpu_attention_forward(self.h, io, workspace, workspace_bytes))
+        self.ctx._check(self.lib.gatgpu_attention_forward(self._plan(), io, workspace, workspace_bytes))
 
     def backward(self, io, workspace=None, workspace_bytes=0):
-        self.ctx._check(self.lib.gatgpu_attention_backward(self.h, io, workspace, workspace_bytes))
+        self.ctx._check(self.lib.gatgpu_attention_backward(self._plan(), io, workspace, workspace_bytes))
