@@ -12,7 +12,11 @@
 // weights and score gradients pass through LDS, whose transpose read makes them operands
 // that contract over the rows.
 // Scores and dp are formed in both: 7 products a pair where 5 would do with atomic
-// sums of dq.
+// sums of dq.  (24 graphs of 130 to 1300 rows, 8 x 64, table: 110 us and 107; four sequences of 4K, 16 x 128,
+// capped: 600 and 960.)
+//
+// Weights and score gradients enter the products with Q, K and dout rounded to bf16 (2^-9 of each; the
+// gradients' own stored rounding is as large), the bias gradient unrounded.
 //
 // As in the forward pass, no element is checked for NaN or infinity on the way: they show in
 // the sums, and the block then goes over its tiles again.  (A bad row of K in the first pass, of Q
@@ -200,8 +204,10 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
 // The pass over keys: a block of PAIRS pairs of waves, 32 keys a pair.  Of each tile of 64 packed query
 // rows the first wave of a pair forms the weights and score gradients of rows 0 to 31, the second
 // those of rows 32 to 63; both go through LDS, and then the first wave sums dv over the 64 rows, the second
-// dk.  So a wave holds one gradient's sums instead of two (64 registers at 128 columns), and two waves
-// a SIMD fit where one wave with both left only one (prefix sequences of 4K, 16 x 128: 1.38 ms).
+// dk.  So a wave holds one gradient's sums instead of two (64 registers at 128 columns), and with V in LDS at
+// bf16's 128 columns two waves a SIMD fit.  Four sequences of 4K, 16 x 128, capped: 960 us so, 1105 with V in
+// registers and one wave a SIMD, 1380 with both gradients in a wave.  Vector instructions issue in 44 % of the
+// cycles, matrix ones in 25 %, LDS in 38 %: the waits between a tile's phases bound it.
 template <class T, int D, int PAIRS>
 struct KvLds {
     static constexpr int kRows = 64, kThreads = PAIRS * 128, kTile = kRows * lds_row<T, D>();

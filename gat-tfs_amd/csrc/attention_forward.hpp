@@ -9,8 +9,12 @@
 // A wave holds 32 packed query rows; scores are formed transposed (keys x rows), so
 // that a lane owns half a row's scores, its statistics are plain registers and the
 // weights are the operand of the second product as they stand.  Four waves share tiles
-// of 64 keys through LDS, requested a tile ahead; short segments and split key ranges run
-// one wave a block on tiles of 32.  m, l and O are FP32.
+// of 64 keys through LDS, requested a tile ahead; few rows run one wave a block, or eight with a range
+// of the keys each, on tiles of 32.  m, l and O are FP32.
+//
+// Bound by the vector instructions of the scores (four or more and a quarter-rate exponential each) beside the
+// products: one graph of 16K nodes, 8 x 64, capped, takes 800 us, 686 TFLOP/s where a large product reaches 1086;
+// 48 single tokens over up to 24K keys 182 us, the keys' and values' bytes at 5 TB/s.
 //
 // The loop checks no element for NaN or infinity: a bad value in a tile shows in the sums of
 // every row that met it (0 x NaN), and then the block goes over its keys again, letting it

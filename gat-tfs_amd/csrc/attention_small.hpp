@@ -10,6 +10,9 @@
 // current one is computed: a step is about as long as a trip to memory, and the bytes of few
 // waves a SIMD keep the memory busy.
 //
+// 1500 segments of 9 to 60 rows, 8 x 32, bf16, table: forward 22 + 16 us (33 to 64 keys, up to 32), backward
+// 66 + 32, of which the bias gradient's LDS sums take a third; the rows' bytes would take 35 in all.
+//
 // Row operands of the forward pass come straight from memory; what is contracted over its rows
 // (V; backward K, Q, dout and the turned weights) passes through LDS.
 #pragma once
