@@ -16,9 +16,9 @@ struct gatgpu_attention {
     bool shared_keys = false;  // key rows of two segments overlap
     // Tables on the device: segments; tiles of the forward, the query and the key pass; joined tiles.
     // Short segments: forward of one and two blocks of 32 keys, backward of 1, 2 and 4 waves.
-    gatgpu::DevBuf dsegs, dsmall[2], dsmall_bwd[3], dfwd, dbwd_q, dbwd_kv, djoin;
+    gatgpu::DevBuf dsegs, dsmall[2], dsmall_bwd[3], dfwd, dbwd_q, dbwd_kv, djoin, djoin_q, djoin_kv;
     uint32_t own_delta = 0;  // segments of so many keys need no rest: their backward pass forms delta from its weights
-    uint64_t nsmall[2] = {}, nsmall_bwd[3] = {}, small_parts = 0, nfwd = 0, nbwd_q = 0, nbwd_kv = 0, njoin = 0;
+    uint64_t nsmall[2] = {}, nsmall_bwd[3] = {}, small_parts = 0, nfwd = 0, nbwd_q = 0, nbwd_kv = 0, njoin = 0, njoin_q = 0, njoin_kv = 0;
     uint32_t join_rows = 0;  // rows of the fullest joined tile
     int wfwd = 1, wbwd_q = 1, wbwd_kv = 1;  // waves a block
     gatgpu::AttnCap capped;
@@ -88,6 +88,29 @@ int upload(gatgpu_ctx* c, DevBuf& b, const void* p, size_t bytes) {
 // Long tiles first: the last blocks to start are then short ones.
 void longest_first(std::vector<AttnTask>& t) {
     std::stable_sort(t.begin(), t.end(), [](const AttnTask& x, const AttnTask& y) { return x.hi - x.lo > y.hi - y.lo; });
+}
+
+// Cuts tasks into equal ranges (multiples of 64) of `chunk` and less, or (whole) of `chunk` and more; tiles: what
+// launch_attention_join takes.  False where none was longer.
+bool split_tasks(std::vector<AttnTask>& tasks, std::vector<AttnTask>& tiles, uint64_t chunk, bool whole) {
+    std::vector<AttnTask> cut;
+    for (const AttnTask& t : tasks) {
+        const uint32_t first = uint32_t(cut.size());
+        const uint64_t len = t.hi - std::min(t.lo, t.hi), n = std::max<uint64_t>(1, whole ? len / chunk : (len + chunk - 1) / chunk), size = ((len + n - 1) / n + 63) / 64 * 64;
+        uint64_t lo = t.lo;
+        do {
+            const uint64_t hi = n == 1 ? t.hi : std::min<uint64_t>(t.hi, lo + size);
+            cut.push_back({t.seg, t.at, uint32_t(lo), uint32_t(hi)});
+            lo = hi;
+        } while (lo < t.hi);
+        tiles.push_back({t.seg, t.at, first, uint32_t(cut.size()) - first});
+    }
+    if (cut.size() == tasks.size()) {
+        tiles.clear();
+        return false;
+    }
+    tasks.swap(cut);
+    return true;
 }
 
 int build(gatgpu_attention* P) {
@@ -199,25 +222,9 @@ int build(gatgpu_attention* P) {
         const uint64_t cuts = uint64_t(bf16 ? attention_cuts<uint16_t>(width) : attention_cuts<float>(width));
         P->cut = longest * 4 <= cuts * chunk * (bf16 ? 6 : 3) &&
                  (bf16 ? attention_forward_cut_lds_bf16 : attention_forward_cut_lds_fp32)(sh.dim, sh.bias, int(group)) <= kAttnLds;
-        std::vector<AttnTask> cut;
-        for (const AttnTask& t : fwd) {
-            if (P->cut) break;
-            join.push_back({t.seg, t.at, uint32_t(cut.size()), 0});
+        if (!P->cut) P->split = split_tasks(fwd, join, chunk, false);
+        for (const AttnTask& t : join)
             P->join_rows = std::max<uint32_t>(P->join_rows, std::min<uint32_t>(32, uint32_t(P->segs[t.seg].q_len * group) - t.at));
-            uint64_t lo = 0;
-            do {
-                const uint64_t hi = std::min<uint64_t>(t.hi, lo + chunk);
-                cut.push_back({t.seg, t.at, uint32_t(lo), uint32_t(hi)});
-                lo = hi;
-            } while (lo < t.hi);
-            join.back().hi = uint32_t(cut.size()) - join.back().lo;
-        }
-        if (cut.size() > fwd.size()) {
-            fwd.swap(cut);
-            P->split = true;
-        } else {
-            join.clear();
-        }
     }
     for (size_t s = 0; s < P->segs.size(); ++s) {
         const AttnSeg& g = P->segs[s];
@@ -232,9 +239,24 @@ int build(gatgpu_attention* P) {
             bk.push_back({uint32_t(s), uint32_t(k), lo, n});
         }
     }
+    // Backward passes with few blocks: the same, keys of query tiles and rows of key tiles, into about two ranges a
+    // unit.  The joined sums are as large as several outputs, so ranges are long, and none are cut from as many
+    // blocks as units (two segments of 2000, 8 x 64: 101 us so, 107 cut).  us without and with: one segment of
+    // 2000 91 / 85 (8 x 64, bf16), 398 / 297 (FP32), of 1000 108 / 44 (8 heads on 2), of 3000 579 / 106 (8 on 1).
+    std::vector<AttnTask> join_q, join_kv;
+    const auto spread_out = [&](std::vector<AttnTask>& tasks, std::vector<AttnTask>& tiles) {
+        const uint64_t blocks = tasks.size() * kvh, want = std::max<uint64_t>(1, 2 * cus / kvh);
+        uint64_t work = 0;
+        for (const AttnTask& t : tasks) work += t.hi - std::min(t.lo, t.hi);
+        if (blocks == 0 || blocks >= cus) return;
+        const uint64_t least = bf16 ? (blocks * 4 <= cus ? 256 : 512) : (blocks * 2 <= cus ? 96 : 512);
+        (void)split_tasks(tasks, tiles, std::max(least, work / want), true);
+    };
+    spread_out(bq, join_q);
+    spread_out(bk, join_kv);
     if (!P->split) longest_first(fwd);
-    longest_first(bq);
-    longest_first(bk);
+    if (join_q.empty()) longest_first(bq);
+    if (join_kv.empty()) longest_first(bk);
     // A task's heads go to different XCDs, whose L2s then keep few heads' keys each, or to the same one, which
     // then has whole lines of narrow rows.  Forward and backward in bf16, us: 24 graphs of 650 to 1300 rows, 8 x 64
     // 139 + 413 spread, 164 + 500 not; 500 of 60 to 120 69 + 310, 71 + 314; 8 x 32: 100 of 250 29 + 80, 27 + 65;
@@ -252,11 +274,15 @@ int build(gatgpu_attention* P) {
     P->nbwd_q = bq.size();
     P->nbwd_kv = bk.size();
     P->njoin = join.size();
+    P->njoin_q = join_q.size();
+    P->njoin_kv = join_kv.size();
     if (int r = upload(c, P->dsegs, P->segs.data(), P->segs.size() * sizeof(AttnSeg))) return r;
     if (int r = upload(c, P->dfwd, fwd.data(), fwd.size() * sizeof(AttnTask))) return r;
     if (int r = upload(c, P->dbwd_q, bq.data(), bq.size() * sizeof(AttnTask))) return r;
     if (int r = upload(c, P->dbwd_kv, bk.data(), bk.size() * sizeof(AttnTask))) return r;
     if (int r = upload(c, P->djoin, join.data(), join.size() * sizeof(AttnTask))) return r;
+    if (int r = upload(c, P->djoin_q, join_q.data(), join_q.size() * sizeof(AttnTask))) return r;
+    if (int r = upload(c, P->djoin_kv, join_kv.data(), join_kv.size() * sizeof(AttnTask))) return r;
     HIPCHECK(c, hipStreamSynchronize(c->stream));
     return GATGPU_OK;
 }
@@ -269,9 +295,17 @@ uint64_t forward_bytes(const gatgpu_attention* P) {
     return P->split ? part_bytes(P) + P->nfwd * uint64_t(P->shape.kv_heads) * 32 * 8 : 0;
 }
 uint64_t delta_bytes(const gatgpu_attention* P) { return pad256(P->rows * uint64_t(P->shape.heads) * 4); }
-uint64_t backward_bytes(const gatgpu_attention* P) {
+uint64_t bias_bytes(const gatgpu_attention* P) {
     const gatgpu_attention_shape& sh = P->shape;
-    return delta_bytes(P) + (sh.bias == GATGPU_BIAS_TABLE ? (P->small_parts + P->nbwd_q) * uint64_t(sh.heads) * uint64_t(sh.buckets) * 4 : 0);
+    return sh.bias == GATGPU_BIAS_TABLE ? pad256((P->small_parts + P->nbwd_q) * uint64_t(sh.heads) * uint64_t(sh.buckets) * 4) : 0;
+}
+// Rows of a task's tile in the backward passes.
+uint32_t height_q(const gatgpu_attention* P) { return 32 * uint32_t(P->wbwd_q); }
+uint32_t height_kv(const gatgpu_attention* P) { return P->wbwd_kv == 1 ? 32 : 64; }
+uint64_t backward_bytes(const gatgpu_attention* P) {
+    const uint64_t row = uint64_t(P->shape.kv_heads) * uint64_t(attention_width(P->shape.dim)) * 4;
+    const uint64_t part = std::max(P->njoin_q ? P->nbwd_q * height_q(P) * row : 0, P->njoin_kv ? P->nbwd_kv * height_kv(P) * 2 * row : 0);
+    return delta_bytes(P) + bias_bytes(P) + part;
 }
 
 // A matrix of rows: there, aligned, wide enough, on the device.
@@ -512,11 +546,18 @@ int gatgpu_attention_backward(gatgpu_attention* P, const gatgpu_attention_io* io
     a.first_part = P->small_parts;
     a.tasks = P->dbwd_q.as<AttnTask>();
     a.ntasks = P->nbwd_q;
+    float* const part = reinterpret_cast<float*>(static_cast<char*>(ws) + delta_bytes(P) + bias_bytes(P));
+    a.part = P->njoin_q ? part : nullptr;
     if (a.ntasks) HIPCHECK(c, (bf16 ? launch_attention_backward_q_bf16 : launch_attention_backward_q_fp32)(a, P->wbwd_q, c->stream));
+    if (P->njoin_q)
+        HIPCHECK(c, launch_attention_grad_join(a, bf16, false, P->djoin_q.as<AttnTask>(), P->njoin_q, height_q(P), c->stream));
     if (io->dbias) HIPCHECK(c, launch_attention_bias_sum(a, P->small_parts + P->nbwd_q, io->dbias, c->stream));
     a.tasks = P->dbwd_kv.as<AttnTask>();
     a.ntasks = P->nbwd_kv;
+    a.part = P->njoin_kv ? part : nullptr;
     if (a.ntasks) HIPCHECK(c, (bf16 ? launch_attention_backward_kv_bf16 : launch_attention_backward_kv_fp32)(a, P->wbwd_kv, c->stream));
+    if (P->njoin_kv)
+        HIPCHECK(c, launch_attention_grad_join(a, bf16, true, P->djoin_kv.as<AttnTask>(), P->njoin_kv, height_kv(P), c->stream));
     return GATGPU_OK;
 }
 

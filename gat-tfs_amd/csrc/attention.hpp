@@ -70,7 +70,7 @@ struct AttnArgs {
     void *out = nullptr, *rest = nullptr;
     uint64_t os = 0;
     float* lse = nullptr;
-    // split over keys: unnormalised partial sums and (max, sum) per task row
+    // tasks of a part of a tile's keys (or rows): their unfinished sums, and forward (max, sum) per task row
     float *part = nullptr, *stat = nullptr;
     // backward
     const void* dout = nullptr;
@@ -112,6 +112,9 @@ size_t attention_small_backward_lds_fp32(int dim, int waves, int bias, int group
 // rows: the most that one of them has.
 hipError_t launch_attention_join(const AttnArgs& a, bool bf16, const AttnTask* tiles, uint64_t ntiles, uint32_t rows,
                                  hipStream_t s);
+// Backward: the same tables for tiles of `height` rows (dq) or keys (dk, dv).
+hipError_t launch_attention_grad_join(const AttnArgs& a, bool bf16, bool keys, const AttnTask* tiles, uint64_t ntiles, uint32_t height,
+                                      hipStream_t s);
 hipError_t launch_attention_bias_sum(const AttnArgs& a, uint64_t parts, float* dbias, hipStream_t s);
 
 constexpr int kAttnMaxDim = 128, kAttnMaxBuckets = 64;

@@ -12,11 +12,14 @@
 // weights and score gradients pass through LDS, whose transpose read makes them operands
 // that contract over the rows.
 // Scores and dp are formed in both: 7 products a pair where 5 would do with atomic
-// sums of dq.  (24 graphs of 130 to 1300 rows, 8 x 64, table: 110 us and 107; four sequences of 4K, 16 x 128,
+// sums of dq.  (24 graphs of 130 to 1300 rows, 8 x 64, table: 110 us and 115; four sequences of 4K, 16 x 128,
 // capped: 600 and 960.)
 //
 // Weights and score gradients enter the products with Q, K and dout rounded to bf16 (2^-9 of each; the
 // gradients' own stored rounding is as large), the bias gradient unrounded.
+//
+// Where a pass has few blocks, each takes a range of its tile's keys (rows) and leaves FP32 sums, which
+// k_attn_grad_join adds in order.
 //
 // As in the forward pass, no element is checked for NaN or infinity on the way: they show in
 // the sums, and the block then goes over its tiles again.  (A bad row of K in the first pass, of Q
@@ -71,12 +74,12 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
     float* bins = table + a.group * 256;
     const T* kbase = static_cast<const T*>(a.k) + seg.k_begin * a.ks + uint64_t(kv) * dim;
     const T* vbase = static_cast<const T*>(a.v) + seg.k_begin * a.vs + uint64_t(kv) * dim;
-    const uint32_t end = task.hi;
+    const uint32_t begin = task.lo, end = task.hi;
     AttnStage<T, D, NW, BK> sk, sv;
     sk.place(a, a.ks, 1);
     sv.place(a, a.vs, 1);
-    sk.load(a, kbase, a.ks, 1, 0, end);
-    sv.load(a, vbase, a.vs, 1, 0, end);
+    sk.load(a, kbase, a.ks, 1, begin, end);
+    sv.load(a, vbase, a.vs, 1, begin, end);
 
     const uint64_t grow = seg.q_begin + uint64_t(w.query);
     float lse2 = a.lse[grow * uint64_t(a.heads) + w.head];
@@ -101,13 +104,13 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
         }
     }
     delta = xor32_add(delta);
-    if (live && half == 0) a.delta[(seg.base + uint64_t(w.query)) * uint64_t(a.heads) + w.head] = delta;
+    if (live && half == 0 && begin == 0) a.delta[(seg.base + uint64_t(w.query)) * uint64_t(a.heads) + w.head] = delta;
 
     const uint8_t* drow = TABLE ? a.dist + seg.dist + uint64_t(w.query) * seg.dist_ld : nullptr;
     AttnDist dist[NB], next_dist[NB];
     if constexpr (TABLE) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, b * 32 + 4 * half, seg.dist_ld);
+        for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, begin + b * 32 + 4 * half, seg.dist_ld);
         fill_table(a, kv, table);
     }
     const float cc = a.scale * kLog2e;
@@ -123,7 +126,7 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
         if (binned)
             for (int b = 0; b < a.buckets; ++b) bins[b * COLS + threadIdx.x] = 0.0f;
         uint32_t tile = 0;
-        for (uint32_t k0 = 0; k0 < end; k0 += BK, ++tile) {
+        for (uint32_t k0 = begin; k0 < end; k0 += BK, ++tile) {
             const int buf = NBUF == 2 ? int(tile & 1) : 0;
             if (NBUF == 1) lds_barrier();
             sk.store(lds_k[buf]);
@@ -174,15 +177,18 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
     const bool bad = !idle && nonfinite(acc);
     if (__builtin_expect(NW == 1 ? __any(bad) : __syncthreads_or(bad), 0)) {
         if (NW > 1) lds_barrier();
-        sk.load(a, kbase, a.ks, 1, 0, end);
-        sv.load(a, vbase, a.vs, 1, 0, end);
+        sk.load(a, kbase, a.ks, 1, begin, end);
+        sv.load(a, vbase, a.vs, 1, begin, end);
         if constexpr (TABLE) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, b * 32 + 4 * half, seg.dist_ld);
+            for (int b = 0; b < NB; ++b) next_dist[b] = load_dist(drow, begin + b * 32 + 4 * half, seg.dist_ld);
         }
         pass(std::true_type{});
     }
-    store_rows<T, DB>(a.dq, grow * a.dqs + uint64_t(w.head) * dim, acc, a.scale, half, dim, live);
+    if (__builtin_expect(a.part != nullptr, 0))  // a range of the keys: joined by k_attn_grad_join
+        store_part<DB>(a.part, (task_id * uint64_t(a.kv_heads) + uint64_t(kv)) * (NW * 32) + uint64_t(wave * 32 + l32), acc, half, live);
+    else
+        store_rows<T, DB>(a.dq, grow * a.dqs + uint64_t(w.head) * dim, acc, a.scale, half, dim, live);
     if (!binned) return;
     // Each bucket's columns, by head of the group, in one fixed order.
     lds_barrier();
@@ -373,7 +379,10 @@ __global__ __launch_bounds__(PAIRS * 128, (sizeof(T) == 2 && (D < 128 || PAIRS >
         pass(std::true_type{});
     }
     const bool in = key < seg.k_len;
-    if (role) store_rows<T, DB>(a.dk, grow * a.dks + uint64_t(kv) * dim, acc, a.scale, half, dim, in);
+    if (__builtin_expect(a.part != nullptr, 0)) {  // a range of the rows: joined by k_attn_grad_join
+        const uint64_t plane = (task_id * uint64_t(a.kv_heads) + uint64_t(kv)) * 2 + (role ? 0 : 1);
+        store_part<DB>(a.part, plane * (PAIRS * 32) + uint64_t(pair * 32 + l32), acc, half, in);
+    } else if (role) store_rows<T, DB>(a.dk, grow * a.dks + uint64_t(kv) * dim, acc, a.scale, half, dim, in);
     else store_rows<T, DB>(a.dv, grow * a.dvs + uint64_t(kv) * dim, acc, 1.0f, half, dim, in);
 }
 

@@ -261,14 +261,9 @@ __global__ __launch_bounds__(NW * CUTS * 64, (attn_waves<T, D, NW>())) void k_at
     }
     if (a.part) {  // a range of the keys: joined by k_attn_join
         const uint64_t at = (task_id * uint64_t(a.kv_heads) + uint64_t(kv)) * (NW * 32) + uint64_t(wave * 32 + l32);
-        if (row0 + uint32_t(l32) >= rows) return;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                store4<float>(a.part, at * D + d * 32 + 8 * i + 4 * half, acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2],
-                              acc[d][4 * i + 3]);
-        if (half == 0) *reinterpret_cast<float2*>(a.stat + at * 2) = make_float2(m, l);
+        const bool in = row0 + uint32_t(l32) < rows;
+        store_part<DB>(a.part, at, acc, half, in);
+        if (half == 0 && in) *reinterpret_cast<float2*>(a.stat + at * 2) = make_float2(m, l);
         return;
     }
     store_out<T, DB>(a, seg, w, acc, m, l, half, row0 + uint32_t(l32) < rows);

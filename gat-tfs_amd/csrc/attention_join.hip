@@ -72,6 +72,52 @@ __global__ __launch_bounds__(64) void k_attn_join(const AttnArgs a, const AttnTa
             l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
+// Adds the partial gradients of a split tile, in order: a wave a row and key/value head.  KEYS: dk and dv
+// of `height` keys a tile, else dq of `height` packed query rows.
+template <class T, int D, bool KEYS>
+__global__ __launch_bounds__(64) void k_attn_grad_join(const AttnArgs a, const AttnTask* __restrict__ tiles, uint32_t height) {
+    constexpr int N = D > 64 ? D / 64 : 1, PLANES = KEYS ? 2 : 1;
+    const uint32_t local = blockIdx.x % height, cell = blockIdx.x / height;
+    const AttnTask tile = tiles[cell / uint32_t(a.kv_heads)];
+    const int kv = int(cell % uint32_t(a.kv_heads)), col = int(threadIdx.x) * N;
+    const AttnSeg seg = a.segs[tile.seg];
+    const uint32_t row = tile.at + local;
+    if (row >= (KEYS ? seg.k_len : seg.q_len * uint32_t(a.group)) || col >= a.dim) return;
+    const uint64_t step = uint64_t(a.kv_heads) * PLANES * height * D;
+#pragma unroll
+    for (int plane = 0; plane < PLANES; ++plane) {
+        const float* p = a.part + (((uint64_t(tile.lo) * uint64_t(a.kv_heads) + uint64_t(kv)) * PLANES + plane) * height + local) * D + col;
+        float sum[N] = {};
+        for (uint32_t t = 0; t < tile.hi; t += 8) {  // 8 ranges in flight
+            float x[8][N];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[i][e] = t + i < tile.hi ? p[(t + i) * step + e] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum[e] += x[i][e];
+        }
+        void* base;
+        uint64_t at;
+        if (KEYS) {
+            base = plane ? a.dv : a.dk;
+            at = (seg.k_begin + row) * (plane ? a.dvs : a.dks) + uint64_t(kv) * uint64_t(a.dim);
+        } else {
+            const AttnRow w = attn_row(a, seg, row, kv);
+            base = a.dq;
+            at = (seg.q_begin + uint64_t(w.query)) * a.dqs + uint64_t(w.head) * uint64_t(a.dim);
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float v = sum[e] * (plane ? 1.0f : a.scale);
+            if constexpr (sizeof(T) == 2) static_cast<uint16_t*>(base)[at + uint64_t(col + e)] = bf16_hw(v);
+            else static_cast<float*>(base)[at + uint64_t(col + e)] = v;
+        }
+    }
+}
+
 // dbias[head][bucket]: partial sums of all parts, in one fixed order.  A block takes 8 cells, 128
 // threads a cell.
 __global__ __launch_bounds__(1024) void k_attn_bias_sum(const float* __restrict__ part, uint64_t parts, uint32_t cells,
@@ -98,6 +144,13 @@ __global__ __launch_bounds__(1024) void k_attn_bias_sum(const float* __restrict_
     if (lane == 0 && blockIdx.x * 8 + cell < cells) dbias[blockIdx.x * 8 + cell] = lds[2 * cell][0] + lds[2 * cell + 1][0];
 }
 
+template <class T, int D>
+hipError_t grad_join(const AttnArgs& a, bool keys, const AttnTask* tiles, uint64_t ntiles, uint32_t height, hipStream_t s) {
+    const uint32_t blocks = uint32_t(ntiles * uint64_t(a.kv_heads) * height);
+    if (keys) k_attn_grad_join<T, D, true><<<blocks, 64, 0, s>>>(a, tiles, height);
+    else k_attn_grad_join<T, D, false><<<blocks, 64, 0, s>>>(a, tiles, height);
+    return hipGetLastError();
+}
 template <class T, int D>
 hipError_t join(const AttnArgs& a, const AttnTask* tiles, uint64_t ntiles, uint32_t rows, hipStream_t s) {
     k_attn_join<T, D><<<uint32_t(ntiles * uint64_t(a.kv_heads) * rows), 64, 0, s>>>(a, tiles, rows);
@@ -136,6 +189,17 @@ hipError_t launch_attention_join(const AttnArgs& a, bool bf16, const AttnTask* t
         case 32: return bf16 ? join<uint16_t, 32>(a, tiles, ntiles, rows, s) : join<float, 32>(a, tiles, ntiles, rows, s);
         case 64: return bf16 ? join<uint16_t, 64>(a, tiles, ntiles, rows, s) : join<float, 64>(a, tiles, ntiles, rows, s);
         default: return bf16 ? join<uint16_t, 128>(a, tiles, ntiles, rows, s) : join<float, 128>(a, tiles, ntiles, rows, s);
+    }
+}
+hipError_t launch_attention_grad_join(const AttnArgs& a, bool bf16, bool keys, const AttnTask* tiles, uint64_t ntiles, uint32_t height,
+                                      hipStream_t s) {
+    switch (attention_width(a.dim)) {
+        case 32:
+            return bf16 ? grad_join<uint16_t, 32>(a, keys, tiles, ntiles, height, s) : grad_join<float, 32>(a, keys, tiles, ntiles, height, s);
+        case 64:
+            return bf16 ? grad_join<uint16_t, 64>(a, keys, tiles, ntiles, height, s) : grad_join<float, 64>(a, keys, tiles, ntiles, height, s);
+        default:
+            return bf16 ? grad_join<uint16_t, 128>(a, keys, tiles, ntiles, height, s) : grad_join<float, 128>(a, keys, tiles, ntiles, height, s);
     }
 }
 hipError_t launch_attention_bias_sum(const AttnArgs& a, uint64_t parts, float* dbias, hipStream_t s) {

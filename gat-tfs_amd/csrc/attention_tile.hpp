@@ -494,6 +494,18 @@ __device__ inline void store4(void* base, uint64_t at, float a, float b, float c
     else *reinterpret_cast<float4*>(static_cast<float*>(base) + at) = make_float4(a, b, c, d);
 }
 
+// A row's FP32 sums to row `at` of a workspace of rows of 32 DB columns, where a launch joins them.
+template <int DB>
+__device__ inline void store_part(float* part, uint64_t at, const f32x16_t (&acc)[DB], int half, bool in) {
+    if (!in) return;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            store4<float>(part, at * (32 * DB) + uint64_t(d * 32 + 8 * i + 4 * half), acc[d][4 * i], acc[d][4 * i + 1],
+                          acc[d][4 * i + 2], acc[d][4 * i + 3]);
+}
+
 // Block b's (task, key/value head).  Blocks go to the 8 XCDs in turn.  spread:
 // heads of a task side by side, so an XCD sees few heads (of 8: one) of all tasks
 // and keeps that head's keys in its L2; else each XCD takes a run of tasks with

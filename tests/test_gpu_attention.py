@@ -431,6 +431,31 @@ def test_many_short_segments(ctx, dim, bias, buckets):
     p.check(p.run(ctx, train=False), train=False)
 
 
+@pytest.mark.parametrize("precision", [FP, BF])
+@pytest.mark.parametrize("dim", [24, 64, 128])
+@pytest.mark.parametrize("heads,kv_heads,bias,buckets,cap", [(8, 1, LINEAR, 0, 3.0), (3, 1, TABLE, 9, 0.0), (2, 2, NONE, 0, 0.0)])
+def test_few_long_segments(ctx, precision, dim, heads, kv_heads, bias, buckets, cap):
+    """Few blocks: the backward passes take ranges of a tile's keys and of its rows, which are joined."""
+    p = Problem([700, 1, 1100], [1090, 900, 1100], heads, kv_heads, dim, precision, mask=PREFIX, prefix=[0, 0, 1000], bias=bias,
+                buckets=buckets, cap=cap, seed=35, gap=1)
+    assert p.plan(ctx).workspace_bytes(backward=True) > 4 * heads * 1801 + 100 * heads * buckets * 4 + 512
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("precision", [FP, BF])
+def test_bad_values_in_ranges_of_the_backward_passes(ctx, precision):
+    """A bad key, value and gradient reach the rows that see them, through every range's sum."""
+    p = Problem([1100], [1100], 2, 1, 32, precision, mask=PREFIX, seed=36)
+    p.k[900, 0, 3] = math.nan
+    p.v[1000, 0, 1] = math.inf
+    p.dout[800, 1, 2] = math.nan
+    out = p.run(ctx)
+    for n, rows in (("dq", 800), ("out", 900)):
+        assert bool(torch.isfinite(out[n][:rows]).all()), n
+    assert not bool(torch.isfinite(out["dq"][900:, 0]).any()) and not bool(torch.isfinite(out["dq"][800, 1]).any())
+    assert bool(torch.isfinite(out["dq"][801:900]).all())
+
+
 def test_too_many_tiles_are_refused(ctx):
     """Before anything is laid out for them."""
     n = 1 << 30
