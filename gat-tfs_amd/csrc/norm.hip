@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "context.hpp"
 #include "norm.hpp"
@@ -20,34 +21,88 @@
 namespace gatgpu {
 namespace {
 
+// Chunks of 16 bytes; FREE: at any element's address, for rows of no whole chunks or off 16 bytes (29817 x 566 bf16,
+// forward: 30 us, 71 an element at a time; 169K x 255, training: 192, x 256 in whole chunks: 143).
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef u32x4_t u32x4_at2 __attribute__((aligned(2)));
+typedef u32x4_t u32x4_at4 __attribute__((aligned(4)));
+template <class T, bool FREE>
+__device__ inline u32x4_t load16(const T* p) {
+    if constexpr (!FREE) return *reinterpret_cast<const u32x4_t*>(p);
+    else if constexpr (sizeof(T) == 2) return *reinterpret_cast<const u32x4_at2*>(p);
+    else return *reinterpret_cast<const u32x4_at4*>(p);
+}
+template <class T, bool FREE>
+__device__ inline void store16(T* p, u32x4_t v) {
+    if constexpr (!FREE) *reinterpret_cast<u32x4_t*>(p) = v;
+    else if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x4_at2*>(p) = v;
+    else *reinterpret_cast<u32x4_at4*>(p) = v;
+}
+template <class T>
+__device__ inline float widen(T x) {
+    if constexpr (sizeof(T) == 2) return bf16_widen(x);
+    else return x;
+}
+template <class T>
+__device__ inline void store_one(T* p, float v) {
+    if constexpr (sizeof(T) == 2) *p = bf16_rne(v);
+    else *p = v;
+}
+// Chunks of one row as they lie in memory: requested a row ahead.
 template <class T, int VEC>
-__device__ inline void load_vec(const T* p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        if constexpr (sizeof(T) == 2) v[0] = bf16_widen(p[0]);
-        else v[0] = p[0];
-    } else if constexpr (sizeof(T) == 2) {  // 8
-        const uint4 w = *reinterpret_cast<const uint4*>(p);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(u[i] << 16);
-            v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-        }
-    } else {  // 4
-        const float4 w = *reinterpret_cast<const float4*>(p);
-        v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
-    }
+struct Raw {
+    u32x4_t w;
+};
+template <class T>
+struct Raw<T, 1> {
+    T w;
+};
+template <class T, int VEC, bool FREE>
+__device__ inline Raw<T, VEC> load_raw(const T* p) {
+    if constexpr (VEC == 1) return {p[0]};
+    else return {load16<T, FREE>(p)};
 }
 template <class T, int VEC>
-__device__ inline void store_vec(T* p, const float (&v)[VEC]) {
+__device__ inline void unpack(const Raw<T, VEC>& r, float (&v)[VEC]) {
     if constexpr (VEC == 1) {
-        if constexpr (sizeof(T) == 2) p[0] = bf16_rne(v[0]);
-        else p[0] = v[0];
-    } else if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7]));
-    } else {
-        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        v[0] = widen(r.w);
+    } else if constexpr (sizeof(T) == 2) {  // 8
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(r.w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+        }
+    } else {  // 4
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r.w[i]);
     }
+}
+// Elements `skip` on of a chunk (the others belong to the chunk before).
+template <class T, int VEC, bool FREE>
+__device__ inline void store_vec(T* p, const float (&v)[VEC], uint32_t skip) {
+    if constexpr (VEC == 1) {
+        store_one(p, v[0]);
+    } else {
+        if (FREE && skip) {
+#pragma unroll
+            for (uint32_t e = 0; e < VEC; ++e)
+                if (e >= skip) store_one(p + e, v[e]);
+            return;
+        }
+        u32x4_t w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 2) w[i] = bf16x2(v[2 * i], v[2 * i + 1]);
+            else w[i] = __float_as_uint(v[i]);
+        }
+        store16<T, FREE>(p, w);
+    }
+}
+// First column of a chunk at column c: a row of no whole number of chunks ends with one that begins
+// before its place and shares its first columns (skip) with the chunk ahead of it.
+template <int VEC, bool FREE>
+__device__ inline uint32_t chunk_begin(uint32_t c, uint32_t W) {
+    return FREE ? min(c, W - uint32_t(VEC)) : c;
 }
 // FP32 weights of VEC columns.
 template <int VEC>
@@ -109,7 +164,7 @@ dim3 norm_grid(uint64_t n) {
 }
 __device__ inline uint64_t norm_block() { return uint64_t(blockIdx.y) * gridDim.x + blockIdx.x; }
 
-template <class T, int VEC, int TPR, int ITEMS>
+template <class T, int VEC, int TPR, int ITEMS, bool FREE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const NormArgs a) {
     constexpr int BLOCK = TPR < 256 ? 256 : TPR;
     __shared__ float lds[BLOCK / 64];
@@ -124,7 +179,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const NormAr
         const uint32_t c = (i * TPR + t) * VEC;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[i][e] = 0.0f;
-        if (c < W) load_vec<T, VEC>(x + c, v[i]);
+        if (c < W) unpack<T, VEC>(load_raw<T, VEC, FREE>(x + chunk_begin<VEC, FREE>(c, W)), v[i]);
     }
     if (a.residual) {
         const T* res = static_cast<const T*>(a.residual) + row * a.rs;
@@ -132,39 +187,49 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const NormAr
         for (int i = 0; i < ITEMS; ++i) {
             const uint32_t c = (i * TPR + t) * VEC;
             if (c < W) {
+                const uint32_t s = chunk_begin<VEC, FREE>(c, W);
                 float r[VEC];
-                load_vec<T, VEC>(res + c, r);
+                unpack<T, VEC>(load_raw<T, VEC, FREE>(res + s), r);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[i][e] = round_to<T>(v[i][e] + r[e]);
-                if (a.sum) store_vec<T, VEC>(static_cast<T*>(a.sum) + row * a.ss + c, v[i]);
+                if (a.sum) store_vec<T, VEC, FREE>(static_cast<T*>(a.sum) + row * a.ss + s, v[i], c - s);
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t c = (i * TPR + t) * VEC, skip = c < W ? c - chunk_begin<VEC, FREE>(c, W) : 0;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sum += v[i][e];
+        for (int e = 0; e < VEC; ++e) sum += FREE && uint32_t(e) < skip ? 0.0f : v[i][e];
+    }
     const float inv = 1.0f / float(W), mean = row_sum<TPR>(sum, lds) * inv;
     sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-        if ((i * TPR + t) * VEC < W)
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t c = (i * TPR + t) * VEC;
+        if (c >= W) continue;
+        const uint32_t skip = c - chunk_begin<VEC, FREE>(c, W);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) sum = fmaf(v[i][e] - mean, v[i][e] - mean, sum);
+        for (int e = 0; e < VEC; ++e) {
+            const float d = FREE && uint32_t(e) < skip ? 0.0f : v[i][e] - mean;
+            sum = fmaf(d, d, sum);
+        }
+    }
     const float rstd = 1.0f / sqrtf(row_sum<TPR>(sum, lds) * inv + a.eps);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const uint32_t c = (i * TPR + t) * VEC;
         if (c >= W) continue;
+        const uint32_t s = chunk_begin<VEC, FREE>(c, W);
         float g[VEC], b[VEC];
-        load_weights<VEC>(a.gamma, c, 1.0f, g);
-        load_weights<VEC>(a.beta, c, 0.0f, b);
+        load_weights<VEC>(a.gamma, s, 1.0f, g);
+        load_weights<VEC>(a.beta, s, 0.0f, b);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const float y = fmaf((v[i][e] - mean) * rstd, g[e], b[e]);
             v[i][e] = a.elu ? elu_to<T>(y) : y;
         }
-        store_vec<T, VEC>(static_cast<T*>(a.y) + row * a.ys + c, v[i]);
+        store_vec<T, VEC, FREE>(static_cast<T*>(a.y) + row * a.ys + s, v[i], c - s);
     }
     if (t == 0) {
         if (a.mean) a.mean[row] = mean;
@@ -182,11 +247,8 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_any(const NormArgs a) {
     const T* x = static_cast<const T*>(a.x) + row * a.xs;
     const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.rs : nullptr;
     const auto h = [&](uint32_t c) {
-        float v[1], r[1] = {0.0f};
-        load_vec<T, 1>(x + c, v);
-        if (!res) return v[0];
-        load_vec<T, 1>(res + c, r);
-        return round_to<T>(v[0] + r[0]);
+        const float v = widen(x[c]);
+        return res ? round_to<T>(v + widen(res[c])) : v;
     };
     float sum = 0.0f;
     for (uint32_t c = threadIdx.x; c < W; c += 1024) sum += h(c);
@@ -195,10 +257,10 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_any(const NormArgs a) {
     for (uint32_t c = threadIdx.x; c < W; c += 1024) sum = fmaf(h(c) - mean, h(c) - mean, sum);
     const float rstd = 1.0f / sqrtf(row_sum<1024>(sum, lds) / float(W) + a.eps);
     for (uint32_t c = threadIdx.x; c < W; c += 1024) {
-        const float v[1] = {h(c)}, g = a.gamma ? a.gamma[c] : 1.0f, b = a.beta ? a.beta[c] : 0.0f;
-        if (a.sum) store_vec<T, 1>(static_cast<T*>(a.sum) + row * a.ss + c, v);
-        const float y = fmaf((v[0] - mean) * rstd, g, b), o[1] = {a.elu ? elu_to<T>(y) : y};
-        store_vec<T, 1>(static_cast<T*>(a.y) + row * a.ys + c, o);
+        const float v = h(c), g = a.gamma ? a.gamma[c] : 1.0f, b = a.beta ? a.beta[c] : 0.0f;
+        if (a.sum) store_one(static_cast<T*>(a.sum) + row * a.ss + c, v);
+        const float y = fmaf((v - mean) * rstd, g, b);
+        store_one(static_cast<T*>(a.y) + row * a.ys + c, a.elu ? elu_to<T>(y) : y);
     }
     if (threadIdx.x == 0) {
         if (a.mean) a.mean[row] = mean;
@@ -206,25 +268,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_any(const NormArgs a) {
     }
 }
 
-// Chunks of one row as they lie in memory: requested a row ahead.
-template <class T, int VEC>
-struct Raw {
-    uint4 w;
-};
-template <class T>
-struct Raw<T, 1> {
-    T w;
-};
-template <class T, int VEC>
-__device__ inline Raw<T, VEC> load_raw(const T* p) {
-    return *reinterpret_cast<const Raw<T, VEC>*>(p);
-}
-template <class T, int VEC>
-__device__ inline void unpack(const Raw<T, VEC>& r, float (&v)[VEC]) {
-    load_vec<T, VEC>(reinterpret_cast<const T*>(&r), v);
-}
-
-template <class T, int VEC, int TPR, int ITEMS>
+template <class T, int VEC, int TPR, int ITEMS, bool FREE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormArgs a) {
     constexpr int BLOCK = TPR < 256 ? 256 : TPR, GROUPS = BLOCK / TPR;
     __shared__ float2 lds[BLOCK / 64];
@@ -237,7 +281,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormAr
         const uint32_t c = (i * TPR + t) * VEC;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) dg[i][e] = db[i][e] = w[i][e] = 0.0f;
-        if (c < W) load_weights<VEC>(a.gamma, c, 1.0f, w[i]);
+        if (c < W) load_weights<VEC>(a.gamma, chunk_begin<VEC, FREE>(c, W), 1.0f, w[i]);
     }
     Raw<T, VEC> hr[ITEMS], yr[ITEMS], sr[ITEMS];
     float mean = 0.0f, rstd = 0.0f;
@@ -249,9 +293,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormAr
         for (int i = 0; i < ITEMS; ++i) {
             const uint32_t c = (i * TPR + t) * VEC;
             if (c >= W) continue;
-            hr[i] = load_raw<T, VEC>(static_cast<const T*>(a.h) + row * a.hs + c);
-            yr[i] = load_raw<T, VEC>(static_cast<const T*>(a.dy) + row * a.dys + c);
-            if (a.dsum) sr[i] = load_raw<T, VEC>(static_cast<const T*>(a.dsum) + row * a.dss + c);
+            const uint32_t s = chunk_begin<VEC, FREE>(c, W);
+            hr[i] = load_raw<T, VEC, FREE>(static_cast<const T*>(a.h) + row * a.hs + s);
+            yr[i] = load_raw<T, VEC, FREE>(static_cast<const T*>(a.dy) + row * a.dys + s);
+            if (a.dsum) sr[i] = load_raw<T, VEC, FREE>(static_cast<const T*>(a.dsum) + row * a.dss + s);
         }
     };
     // (Rows beyond the last leave a row group's lanes idle, not its reductions: all threads make
@@ -280,11 +325,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormAr
         for (int i = 0; i < ITEMS; ++i) {
             const uint32_t c = (i * TPR + t) * VEC;
             if (!in || c >= W) continue;
+            const uint32_t begin = chunk_begin<VEC, FREE>(c, W), skip = c - begin;
             float b[VEC];
-            if (a.elu) load_weights<VEC>(a.beta, c, 0.0f, b);
+            if (a.elu) load_weights<VEC>(a.beta, begin, 0.0f, b);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 n[i][e] = (n[i][e] - shift) * scale;
+                if (FREE && uint32_t(e) < skip) n[i][e] = g[i][e] = 0.0f;
                 if (a.elu) {
                     const float y = fmaf(n[i][e], w[i][e], b[e]);
                     g[i][e] *= y < 0.0f ? exp_w(y) : 1.0f;
@@ -309,7 +356,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormAr
             if (a.dsum) unpack<T, VEC>(ar[i], add);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) g[i][e] = fmaf(scale, g[i][e] - s.x - n[i][e] * s.y, add[e]);
-            store_vec<T, VEC>(static_cast<T*>(a.dx) + row * a.dxs + c, g[i]);
+            const uint32_t begin = chunk_begin<VEC, FREE>(c, W);
+            store_vec<T, VEC, FREE>(static_cast<T*>(a.dx) + row * a.dxs + begin, g[i], c - begin);
         }
     }
     if (!a.part) return;
@@ -333,9 +381,17 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormAr
                     for (int e = 0; e < VEC; ++e)
                         for (int q = 1; q < GROUPS; ++q) v[e] += cols[(q * VEC + e) * TPR + t];
             }
-            if (group == 0 && c < W)
+            if (group == 0 && c < W) {
+                const uint32_t begin = chunk_begin<VEC, FREE>(c, W);
+                if (!FREE || begin == c) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) to[uint64_t(which) * W + c + e] = v[e];
+                    for (int e = 0; e < VEC; ++e) to[uint64_t(which) * W + c + e] = v[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (uint32_t(e) >= c - begin) to[uint64_t(which) * W + begin + e] = v[e];
+                }
+            }
         }
 }
 
@@ -349,11 +405,8 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_any(const NormArgs a) {
     const T* h = static_cast<const T*>(a.h) + row * a.hs;
     const T* dy = static_cast<const T*>(a.dy) + row * a.dys;
     const auto terms = [&](uint32_t c, float& n, float& dt) {
-        float v[1], d[1];
-        load_vec<T, 1>(h + c, v);
-        load_vec<T, 1>(dy + c, d);
-        n = (v[0] - mean) * rstd;
-        dt = d[0];
+        n = (widen(h[c]) - mean) * rstd;
+        dt = widen(dy[c]);
         if (a.elu) {
             const float y = fmaf(n, a.gamma ? a.gamma[c] : 1.0f, a.beta ? a.beta[c] : 0.0f);
             if (y < 0.0f) dt *= exp_w(y);
@@ -369,12 +422,11 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_any(const NormArgs a) {
     }
     s = row_sum2<1024>(s, lds);
     for (uint32_t c = threadIdx.x; c < W; c += 1024) {
-        float n, dt, add[1] = {0.0f};
+        float n, dt;
         terms(c, n, dt);
-        if (a.dsum) load_vec<T, 1>(static_cast<const T*>(a.dsum) + row * a.dss + c, add);
+        const float add = a.dsum ? widen(static_cast<const T*>(a.dsum)[row * a.dss + c]) : 0.0f;
         dt *= a.gamma ? a.gamma[c] : 1.0f;
-        const float o[1] = {fmaf(rstd, dt - s.x / float(W) - n * (s.y / float(W)), add[0])};
-        store_vec<T, 1>(static_cast<T*>(a.dx) + row * a.dxs + c, o);
+        store_one(static_cast<T*>(a.dx) + row * a.dxs + c, fmaf(rstd, dt - s.x / float(W) - n * (s.y / float(W)), add));
     }
 }
 // Column sums of rows of any width: block (columns, row strip), a thread a column.  It runs
@@ -386,16 +438,14 @@ __global__ __launch_bounds__(256) void k_norm_cols_any(const NormArgs a) {
     const float w = a.gamma ? a.gamma[c] : 1.0f, b = a.beta ? a.beta[c] : 0.0f;
     float dg = 0.0f, db = 0.0f;
     for (uint64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        float v[1], d[1];
-        load_vec<T, 1>(static_cast<const T*>(a.h) + row * a.hs + c, v);
-        load_vec<T, 1>(static_cast<const T*>(a.dy) + row * a.dys + c, d);
-        const float n = (v[0] - a.mean[row]) * a.rstd[row];
+        const float n = (widen(static_cast<const T*>(a.h)[row * a.hs + c]) - a.mean[row]) * a.rstd[row];
+        float d = widen(static_cast<const T*>(a.dy)[row * a.dys + c]);
         if (a.elu) {
             const float y = fmaf(n, w, b);
-            if (y < 0.0f) d[0] *= exp_w(y);
+            if (y < 0.0f) d *= exp_w(y);
         }
-        dg = fmaf(d[0], n, dg);
-        db += d[0];
+        dg = fmaf(d, n, dg);
+        db += d;
     }
     a.part[uint64_t(blockIdx.y) * 2 * W + c] = dg;
     a.part[uint64_t(blockIdx.y) * 2 * W + W + c] = db;
@@ -446,64 +496,91 @@ bool aligned(const void* p, uint64_t stride, int size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * uint64_t(size) % 16 == 0;
 }
 
-#define GATGPU_NORM_SHAPES(F) \
-    F(16, 1) F(32, 1) F(64, 1) F(64, 2) F(256, 1) F(256, 2) F(512, 2) F(1024, 2) F(1024, 4)
-
-template <class T, int VEC>
-hipError_t forward(const NormArgs& a, NormShape s, hipStream_t st) {
-    if (!s.tpr) {
-        k_norm_fwd_any<T><<<norm_grid(a.rows), 1024, 0, st>>>(a);
-        return hipGetLastError();
+// f(tpr, items) of a shape as compile-time values.
+template <int VEC, class F>
+void with_shape(NormShape s, F f) {
+    const auto as = [&](auto tpr, auto items) {
+        if (s.tpr == tpr && s.items == items) f(tpr, items);
+    };
+    as(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+    if constexpr (VEC > 1) {  // (narrower rows than a chunk have at most 7 columns)
+        as(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+        as(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+        as(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+        as(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
+        as(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+        as(std::integral_constant<int, 512>{}, std::integral_constant<int, 2>{});
+        as(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
+        as(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
     }
-    const uint64_t per = s.tpr < 256 ? 256 / uint64_t(s.tpr) : 1;
-    const dim3 grid = norm_grid((a.rows + per - 1) / per);
-#define F(TPR, ITEMS) \
-    if (s.tpr == TPR && s.items == ITEMS) k_norm_fwd<T, VEC, TPR, ITEMS><<<grid, TPR < 256 ? 256 : TPR, 0, st>>>(a);
-    GATGPU_NORM_SHAPES(F)
-#undef F
-    return hipGetLastError();
 }
-template <class T, int VEC>
-hipError_t backward(const NormArgs& a, NormShape s, uint32_t blocks, hipStream_t st) {
-#define F(TPR, ITEMS) \
-    if (s.tpr == TPR && s.items == ITEMS) k_norm_bwd<T, VEC, TPR, ITEMS><<<blocks, TPR < 256 ? 256 : TPR, 0, st>>>(a);
-    GATGPU_NORM_SHAPES(F)
-#undef F
-    if (!s.tpr) {
-        if (a.part) k_norm_cols_any<T><<<dim3((a.width + 255) / 256, blocks), 256, 0, st>>>(a);
-        if (a.rows) k_norm_bwd_any<T><<<norm_grid(a.rows), 1024, 0, st>>>(a);
-    }
-    return hipGetLastError();
+// f(elements a load, whether loads are free of alignment) for rows of W columns.
+template <class T, class F>
+hipError_t with_chunks(uint32_t W, bool wide, F f) {
+    constexpr int VEC = 16 / int(sizeof(T));
+    if (W < uint32_t(VEC)) return f(std::integral_constant<int, 1>{}, std::false_type{}, norm_shape(W));
+    const NormShape s = norm_shape((uint64_t(W) + VEC - 1) / VEC);
+    return wide ? f(std::integral_constant<int, VEC>{}, std::false_type{}, s) : f(std::integral_constant<int, VEC>{}, std::true_type{}, s);
+}
+
+template <class T>
+hipError_t forward(const NormArgs& a, bool wide, hipStream_t st) {
+    return with_chunks<T>(a.width, wide, [&](auto vec, auto free, NormShape s) {
+        constexpr int VEC = decltype(vec)::value;
+        if (!s.tpr) {
+            k_norm_fwd_any<T><<<norm_grid(a.rows), 1024, 0, st>>>(a);
+            return hipGetLastError();
+        }
+        with_shape<VEC>(s, [&](auto tpr, auto items) {
+            constexpr int TPR = decltype(tpr)::value, BLOCK = TPR < 256 ? 256 : TPR;
+            k_norm_fwd<T, VEC, TPR, decltype(items)::value, decltype(free)::value>
+                <<<norm_grid((a.rows + BLOCK / TPR - 1) / (BLOCK / TPR)), BLOCK, 0, st>>>(a);
+        });
+        return hipGetLastError();
+    });
+}
+template <class T>
+hipError_t backward(const NormArgs& a, bool wide, uint32_t blocks, hipStream_t st) {
+    return with_chunks<T>(a.width, wide, [&](auto vec, auto free, NormShape s) {
+        constexpr int VEC = decltype(vec)::value;
+        if (!s.tpr) {
+            if (a.part) k_norm_cols_any<T><<<dim3((a.width + 255) / 256, blocks), 256, 0, st>>>(a);
+            if (a.rows) k_norm_bwd_any<T><<<norm_grid(a.rows), 1024, 0, st>>>(a);
+            return hipGetLastError();
+        }
+        with_shape<VEC>(s, [&](auto tpr, auto items) {
+            constexpr int TPR = decltype(tpr)::value;
+            k_norm_bwd<T, VEC, TPR, decltype(items)::value, decltype(free)::value><<<blocks, TPR < 256 ? 256 : TPR, 0, st>>>(a);
+        });
+        return hipGetLastError();
+    });
 }
 
 }  // namespace
 
 // Blocks are persistent, so no more than run at once: three of 256 threads a CU (131 registers a
 // thread).  169K x 256 bf16, residual and ELU: 768 blocks 80 us, 512 97, 1024 108, 2048 91.
-// Wider rows take blocks of 512 threads, one or two a CU (8190 x 8192: 106 us at 256 and 512).
+// Wider rows take blocks of 512 threads, one or two a CU (8190 x 8192: 106 us at 256 and 512).  Few rows: a block
+// a row where a block holds one at a time (100 x 2000, forward and backward: 10.7 us; 13.7 with four rows a block).
 // A partial row costs 16 bytes a column, written and read, a row 6 to 16 a column.
 uint32_t norm_blocks(uint64_t rows, uint64_t width) {
     const uint64_t most = width > 1024 ? 512 : 768;
-    return uint32_t(std::max<uint64_t>(1, std::min({most, std::max<uint64_t>(256, rows / 32), (rows + 3) / 4})));
+    const uint64_t least = width > 1024 ? 1 : 4;  // rows a block
+    return uint32_t(std::max<uint64_t>(1, std::min({most, std::max<uint64_t>(256, rows / 32), (rows + least - 1) / least})));
 }
 
 hipError_t launch_norm_forward(const NormArgs& a, bool bf16, hipStream_t s) {
     const int size = bf16 ? 2 : 4, vec = 16 / size;
     const bool wide = a.width % uint32_t(vec) == 0 && aligned(a.x, a.xs, size) && aligned(a.y, a.ys, size) &&
                       (!a.residual || aligned(a.residual, a.rs, size)) && (!a.sum || aligned(a.sum, a.ss, size));
-    const NormShape shape = norm_shape(wide ? a.width / uint32_t(vec) : a.width);
-    if (bf16) return wide ? forward<uint16_t, 8>(a, shape, s) : forward<uint16_t, 1>(a, shape, s);
-    return wide ? forward<float, 4>(a, shape, s) : forward<float, 1>(a, shape, s);
+    return bf16 ? forward<uint16_t>(a, wide, s) : forward<float>(a, wide, s);
 }
 
 hipError_t launch_norm_backward(const NormArgs& a, bool bf16, uint32_t blocks, float* dgamma, float* dbeta, hipStream_t s) {
     const int size = bf16 ? 2 : 4, vec = 16 / size;
     const bool wide = a.width % uint32_t(vec) == 0 && aligned(a.h, a.hs, size) && aligned(a.dy, a.dys, size) &&
                       aligned(a.dx, a.dxs, size) && (!a.dsum || aligned(a.dsum, a.dss, size));
-    const NormShape shape = norm_shape(wide ? a.width / uint32_t(vec) : a.width);
-    hipError_t e;
-    if (bf16) e = wide ? backward<uint16_t, 8>(a, shape, blocks, s) : backward<uint16_t, 1>(a, shape, blocks, s);
-    else e = wide ? backward<float, 4>(a, shape, blocks, s) : backward<float, 1>(a, shape, blocks, s);
+    const hipError_t e = bf16 ? backward<uint16_t>(a, wide, blocks, s) : backward<float>(a, wide, blocks, s);
     if (e != hipSuccess || !a.part) return e;
     k_norm_sum<<<uint32_t((2 * uint64_t(a.width) + 31) / 32), 1024, 0, s>>>(a.part, blocks, a.width, dgamma, dbeta);
     return hipGetLastError();

@@ -201,6 +201,31 @@ def test_in_place(ctx, width):
     assert torch.equal(out["dgamma"], want["dgamma"]) and torch.equal(out["dbeta"], want["dbeta"])
 
 
+@pytest.mark.parametrize("precision", [gatgpu.FP32, gatgpu.BF16])
+@pytest.mark.parametrize("width", [3, 9, 131, 4099, 16001])
+def test_in_place_at_widths_of_no_whole_loads(ctx, precision, width):
+    """The row's last load begins before its place: its first columns are another thread's to write."""
+    p = Norm(37, width, precision, residual=True, elu=True, seed=9)
+    p.x[5, -2], p.dy[7, 0] = math.nan, math.inf
+    want = p.run(ctx)
+    bad = torch.zeros(37, dtype=torch.bool, device="cuda")
+    bad[5] = True
+    assert bool((torch.isfinite(want["y"]).all(1) == ~bad).all())
+    bad[7] = True
+    assert bool((torch.isfinite(want["dx"]).all(1) == ~bad).all())
+    x, res, dsum, dy = p.x.clone(), p.residual.clone(), p.dsum.clone(), p.dy.clone()
+    out, io = p.arrays()
+    io.x, io.residual, io.sum, io.y = x.data_ptr(), res.data_ptr(), x.data_ptr(), res.data_ptr()
+    io.dsum, io.dx, io.dy = dsum.data_ptr(), dsum.data_ptr(), dy.data_ptr()
+    ws = torch.empty(ctx.norm_workspace(37, width), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    ctx.norm_forward(io)
+    ctx.norm_backward(io, ws.data_ptr(), ws.numel())
+    ctx.synchronize()
+    for have, name in ((res, "y"), (x, "sum"), (dsum, "dx"), (out["dgamma"], "dgamma"), (out["dbeta"], "dbeta")):
+        assert torch.equal(torch.nan_to_num(have, 5.0), torch.nan_to_num(want[name], 5.0)), name
+
+
 def test_optional_arrays(ctx):
     p = Norm(50, 256, gatgpu.FP32, residual=True, seed=5)
     want = p.run(ctx)
