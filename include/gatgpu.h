@@ -409,7 +409,7 @@ int gatgpu_attention_backward(gatgpu_attention* plan, const gatgpu_attention_io*
  *   1 / sqrt(variance + eps);  y = n gamma + beta, through ELU if elu != 0
  * and the gradients of x (= residual), gamma and beta.  Device arrays; rows of
  * `width` elements at strides in elements, any alignment (16-byte aligned rows of
- * whole 16 bytes are faster); gamma, beta, mean, rstd and their gradients are
+ * whole 16 bytes are somewhat faster); gamma, beta, mean, rstd and their gradients are
  * FP32.  Stream, capture, device and workspace: as gatgpu_attention_forward.
  * y may be x or residual, sum x or residual, dx dy or dsum (same stride). */
 typedef struct gatgpu_norm_io {
