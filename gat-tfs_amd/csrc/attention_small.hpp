@@ -336,6 +336,11 @@ __global__ __launch_bounds__(NW * 64, (small_bwd_waves<T, D, NW>())) void k_attn
                         y = mfma_rows<T>(y, from_lds(own_v, f), from_lds(lds_o, f));
                     }
                 }
+                delta = 0.0f;
+                if constexpr (!CAREFUL) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) delta = fmaf(s[e], 0.0f, delta);
+                }
                 if constexpr (CAP) cap_scores(a.capped, s, 0.0f);
                 p = s;
                 tile_scores<BIAS, false, CAREFUL>(a.capped, p, CAP ? 1.0f : cc, lse2, slope2, gap, dist, trow);
@@ -344,7 +349,6 @@ __global__ __launch_bounds__(NW * 64, (small_bwd_waves<T, D, NW>())) void k_attn
                     for (int e = 0; e < 16; ++e)
                         if (8 * (e / 4) + e % 4 >= left) p[e] = -INFINITY;
                 }
-                delta = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     p[e] = exp2_hw(p[e]);
@@ -362,8 +366,9 @@ __global__ __launch_bounds__(NW * 64, (small_bwd_waves<T, D, NW>())) void k_attn
                 }
             };
             weights(std::false_type{});
-            // A NaN or an infinity in any operand, or in a product, makes its row's delta one: then weights
-            // of 0 are kept out of everything.
+            // A NaN or an infinity in V or dout makes dp one and so the row's delta, whatever its weight.  One in K
+            // or Q shows in the raw products only, since a mask puts -inf in a score's place: they are added to
+            // delta, as 0 or NaN.  Then weights of 0 are kept out of everything.
             const bool careful = __any(delta * 0.0f != 0.0f);
             if (__builtin_expect(careful, 0)) weights(std::true_type{});
 #pragma unroll
