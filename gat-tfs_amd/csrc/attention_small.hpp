@@ -379,7 +379,10 @@ __global__ __launch_bounds__(NW * 64, (small_bwd_waves<T, D, NW>())) void k_attn
                 for (int e = 0; e < 16; ++e) y[e] = p[e] * (y[e] - delta);
                 if (__builtin_expect(careful, 0)) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) y[e] = p[e] == 0.0f ? 0.0f : y[e];
+                    for (int e = 0; e < 16; ++e) {
+                        y[e] = p[e] == 0.0f ? 0.0f : y[e];
+                        if (CAP) s[e] = p[e] == 0.0f ? 0.0f : s[e];  // (its slope)
+                    }
                 }
                 if constexpr (TABLE) {
                     if (binned && r < rows) add_bins(bins + tid, COLS, a.buckets, dist, y);

@@ -274,7 +274,7 @@ __device__ inline void tile_scores(const AttnCap& cap, f32x16_t& s, float cc, fl
 
 // Weights p and score gradients y = p (dp - delta) of a block from its raw products s and dp;
 // with CAP, s becomes 1 - tanh^2, the capped score's slope.  left: keys of the lane from its first
-// on that the row sees (where masked).  CAREFUL: a weight of 0 has no gradient, whatever dp is.
+// on that the row sees (where masked).  CAREFUL: a weight of 0 has no gradient, whatever dp and the slope are.
 template <int BIAS, bool CAP, bool CAREFUL>
 __device__ inline void score_gradients(const AttnCap& cap, f32x16_t& s, const f32x16_t& dp, f32x16_t& y, f32x16_t* weights,
                                        float cc, float uncap, float slope2, float gap, const AttnDist& dist,
@@ -311,6 +311,7 @@ __device__ inline void score_gradients(const AttnCap& cap, f32x16_t& s, const f3
         const float p = exp2_hw(y[r]);
         if (weights) (*weights)[r] = p;
         y[r] = CAREFUL && p == 0.0f ? 0.0f : p * (dp[r] - delta);
+        if (CAP && CAREFUL && p == 0.0f) s[r] = 0.0f;
     }
 }
 

@@ -18,7 +18,7 @@ BF, FP = gatgpu.BF16, gatgpu.FP32
 VALUES = [math.nan, math.inf, -math.inf]
 # Backward kernels of one, two and four waves that hold all keys; of one and of four waves a block; of ranges
 LENGTHS = [(20, 32), (50, 64), (100, 32), (132, 64), (384, 32), (1100, 32)]
-CAPS = [0.0]
+CAPS = [0.0, 3.0]
 
 
 @pytest.fixture(scope="module")
