@@ -4,7 +4,8 @@
 //   x_j = scale q.k_j,  y_j = cap tanh(x_j / cap),  s_j = y_j + bias(distance)
 //   l' = l 2^(m - m') + sum 2^(s_j - m'),  O' = O 2^(m - m') + sum 2^(s_j - m') v_j,  m' a score near the maximum
 // (in units of log2) and out = O / l, lse = ln 2 (m + log2 l).  Capped scores without a bias
-// stay within cap: they need no maximum, m is 0 throughout.
+// stay within cap: they need no maximum, m is 0 throughout.  (Their weights of 2^-90 to 2^90 fit FP32, but not always
+// their products with the values: rows whose sums overflow, or lie low, are taken again with the maximum.)
 //
 // A wave holds 32 packed query rows; scores are formed transposed (keys x rows), so
 // that a lane owns half a row's scores, its statistics are plain registers and the
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(NW * CUTS * 64, (attn_waves<T, D, NW>())) void k_at
         constexpr bool CAREFUL = decltype(careful)::value;
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
-        m = bounded ? 0.0f : -INFINITY;
+        m = bounded && !CAREFUL ? 0.0f : -INFINITY;
         l = 0.0f;
         uint32_t tile = 0;
         for (uint32_t k0 = begin; k0 < end; k0 += BK, ++tile) {
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(NW * CUTS * 64, (attn_waves<T, D, NW>())) void k_at
                     for (int r = 0; r < 16; ++r)
                         if (b * 32 + 8 * (r / 4) + r % 4 >= left) s[b][r] = -INFINITY;
             }
-            if (!bounded) {
+            if (CAREFUL || !bounded) {
                 // The reference m is the maximum of an earlier tile.  It is raised, and the sums with it,
                 // only when a score passes it by 2^8: weights of up to 2^8 are as exact as those up to 1.
                 float top = s[0][0];
@@ -198,7 +199,11 @@ __global__ __launch_bounds__(NW * CUTS * 64, (attn_waves<T, D, NW>())) void k_at
     };
     if constexpr (BIAS == GATGPU_BIAS_TABLE) lds_barrier();
     pass(std::false_type{});
-    const bool bad = !idle && nonfinite(acc);
+    bool bad = !idle && nonfinite(acc);
+    if (bounded) {  // a row of low scores only: values below 2^-86 would leave FP32
+        const float sum = xor32_add(l);
+        bad = bad || (sum > 0.0f && sum < 0x1p-40f);
+    }
     if (__builtin_expect(NW == 1 ? __any(bad) : __syncthreads_or(bad), 0)) {
         sync();
         sk.load(a, kbase, a.ks, 1, begin, end);

@@ -178,7 +178,8 @@ AttnCap attention_cap(float scale, float cap) {
         c.near2 = float(0.18 / in);
         c.near4 = float(0.5 / in);
     }
-    // 2^y and sums of 2^30 of them stay inside FP32, and 2^-y far above its smallest values.
+    // 2^y and sums of 2^30 of them stay inside FP32, and 2^-y far above its smallest values.  (The forward kernel sees to
+    // their products with large and small values.)
     c.bounded = out <= 90.0;
     return c;
 }
