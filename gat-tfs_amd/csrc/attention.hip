@@ -12,7 +12,7 @@ struct gatgpu_attention {
     gatgpu_ctx* ctx = nullptr;
     gatgpu_attention_shape shape{};
     std::vector<gatgpu::AttnSeg> segs;
-    uint64_t rows = 0, dist_bytes = 0;
+    uint64_t rows = 0, keys = 0, dist_bytes = 0;
     bool shared_keys = false;  // key rows of two segments overlap
     // Tables on the device: segments; tiles of the forward, the query and the key pass; joined tiles.
     // Short segments: forward of one and two blocks of 32 keys, backward of 1, 2 and 4 waves.
@@ -308,8 +308,10 @@ uint64_t backward_bytes(const gatgpu_attention* P) {
     return delta_bytes(P) + bias_bytes(P) + part;
 }
 
-// A matrix of rows: there, aligned, wide enough, on the device.
-int check_rows(gatgpu_ctx* c, const char* name, const void* p, uint64_t stride, uint64_t width, int size) {
+// A matrix of rows: there, aligned, wide enough, on the device.  Of no rows: anything, since nothing reads or writes it
+// (and an empty array may have no address).
+int check_rows(gatgpu_ctx* c, const char* name, const void* p, uint64_t stride, uint64_t width, int size, uint64_t rows = 1) {
+    if (!rows) return GATGPU_OK;
     if (!p) return fail(c, GATGPU_EINVAL, std::string("null ") + name);
     if (reinterpret_cast<uintptr_t>(p) % 16 || stride * uint64_t(size) % 16)
         return fail(c, GATGPU_EINVAL, std::string(name) + " and its stride must be 16-byte aligned");
@@ -328,17 +330,17 @@ int check_call(gatgpu_attention* P, const gatgpu_attention_io* io, void* ws, uin
     const gatgpu_attention_shape& sh = P->shape;
     const int size = sh.precision == GATGPU_BF16 ? 2 : 4;
     const uint64_t qw = uint64_t(sh.heads) * uint64_t(sh.dim), kw = uint64_t(sh.kv_heads) * uint64_t(sh.dim);
-    if (int r = check_rows(c, "q", io->q, io->q_stride, qw, size)) return r;
-    if (int r = check_rows(c, "k", io->k, io->k_stride, kw, size)) return r;
-    if (int r = check_rows(c, "v", io->v, io->v_stride, kw, size)) return r;
-    if (int r = check_rows(c, "out", io->out, io->out_stride, qw, size)) return r;
+    if (int r = check_rows(c, "q", io->q, io->q_stride, qw, size, P->rows)) return r;
+    if (int r = check_rows(c, "k", io->k, io->k_stride, kw, size, P->keys)) return r;
+    if (int r = check_rows(c, "v", io->v, io->v_stride, kw, size, P->keys)) return r;
+    if (int r = check_rows(c, "out", io->out, io->out_stride, qw, size, P->rows)) return r;
     if (sh.bias != GATGPU_BIAS_NONE)
         if (int r = check_floats(c, "bias", io->bias)) return r;
     if (sh.bias == GATGPU_BIAS_TABLE && P->dist_bytes)
         if (int r = check_rows(c, "dist", io->dist, 16, 16, 1)) return r;
     if (io->rest) {
         if (sh.precision != GATGPU_BF16) return fail(c, GATGPU_EINVAL, "rest belongs to bf16 outputs");
-        if (int r = check_rows(c, "rest", io->rest, io->out_stride, qw, size)) return r;
+        if (int r = check_rows(c, "rest", io->rest, io->out_stride, qw, size, P->rows)) return r;
     }
     if (need) {
         if (bytes < need) return fail(c, GATGPU_EINVAL, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
@@ -420,6 +422,7 @@ int create(gatgpu_ctx* c, const gatgpu_attention_shape* sh, uint64_t n, const ui
         g.base = P->rows;
         g.dist = P->dist_bytes;
         P->rows += g.q_len;
+        P->keys += g.k_len;
         if (sh->bias == GATGPU_BIAS_TABLE) P->dist_bytes += uint64_t(g.q_len) * g.dist_ld;
     }
     if (overlap(P->segs, false)) return fail(c, GATGPU_EINVAL, "query rows of two segments overlap");
@@ -478,7 +481,7 @@ int gatgpu_attention_forward(gatgpu_attention* P, const gatgpu_attention_io* io,
     DeviceGuard on(c->device);
     if (!on.ok) return fail(c, GATGPU_EDEVICE, "cannot select the context's device");
     if (int r = check_call(P, io, ws, bytes, forward_bytes(P))) return r;
-    if (io->lse)
+    if (io->lse && P->rows)
         if (int r = check_floats(c, "lse", io->lse)) return r;
     AttnArgs a = make_args(P, io);
     const bool bf16 = P->shape.precision == GATGPU_BF16;
@@ -516,14 +519,15 @@ int gatgpu_attention_backward(gatgpu_attention* P, const gatgpu_attention_io* io
     const bool bf16 = sh.precision == GATGPU_BF16;
     const int size = bf16 ? 2 : 4;
     const uint64_t qw = uint64_t(sh.heads) * uint64_t(sh.dim), kw = uint64_t(sh.kv_heads) * uint64_t(sh.dim);
-    if (int r = check_floats(c, "lse", io->lse)) return r;
-    if (int r = check_rows(c, "dout", io->dout, io->dout_stride, qw, size)) return r;
-    if (int r = check_rows(c, "dq", io->dq, io->dq_stride, qw, size)) return r;
-    if (int r = check_rows(c, "dk", io->dk, io->dk_stride, kw, size)) return r;
-    if (int r = check_rows(c, "dv", io->dv, io->dv_stride, kw, size)) return r;
+    if (P->rows)
+        if (int r = check_floats(c, "lse", io->lse)) return r;
+    if (int r = check_rows(c, "dout", io->dout, io->dout_stride, qw, size, P->rows)) return r;
+    if (int r = check_rows(c, "dq", io->dq, io->dq_stride, qw, size, P->rows)) return r;
+    if (int r = check_rows(c, "dk", io->dk, io->dk_stride, kw, size, P->keys)) return r;
+    if (int r = check_rows(c, "dv", io->dv, io->dv_stride, kw, size, P->keys)) return r;
     if (io->dbias) {
         if (sh.bias != GATGPU_BIAS_TABLE) return fail(c, GATGPU_EINVAL, "dbias without a bias table");
-        if (bf16 && !io->rest) return fail(c, GATGPU_EINVAL, "dbias of bf16 rows needs rest");
+        if (bf16 && !io->rest && P->rows) return fail(c, GATGPU_EINVAL, "dbias of bf16 rows needs rest");
         if (int r = check_floats(c, "dbias", io->dbias)) return r;
     }
     AttnArgs a = make_args(P, io);

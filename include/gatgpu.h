@@ -371,7 +371,9 @@ int gatgpu_attention_distances(const gatgpu_attention* plan, uint64_t* bytes, ui
 
 /* Device arrays of one call.  Rows of `heads` (or kv_heads) vectors of dim
  * elements side by side; strides in elements, 16-byte aligned like the bases,
- * at least the row's width (so q, k and v may be parts of one array's rows). */
+ * at least the row's width (so q, k and v may be parts of one array's rows).
+ * Arrays of query rows may be NULL where every q_len is 0, arrays of key rows
+ * where every k_len is. */
 typedef struct gatgpu_attention_io {
     const void *q, *k, *v;
     uint64_t q_stride, k_stride, v_stride;
