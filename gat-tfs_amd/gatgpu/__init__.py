@@ -160,6 +160,21 @@ def _ptr(a):
     return None if a is None else a.ctypes.data
 
 
+def _counts(values, dtype):
+    """`values` as an array of the unsigned `dtype`, which numpy's own conversion would wrap them into."""
+    a = np.asarray(values)
+    end = int(np.iinfo(dtype).max) + 1
+    if a.dtype.kind == "O":
+        fine = all(isinstance(x, (int, np.integer)) and 0 <= x < end for x in a.flat)
+    elif a.dtype.kind == "f":
+        fine = bool(((a >= 0) & (a < float(end)) & (a == np.trunc(a))).all())
+    else:
+        fine = a.dtype.kind in "biu" and (a.size == 0 or (int(a.min()) >= 0 and int(a.max()) < end))
+    if not fine:
+        raise ValueError(f"lengths, begins and prefixes are whole numbers from 0 to 2^{8 * np.dtype(dtype).itemsize} - 1")
+    return np.ascontiguousarray(a, dtype)
+
+
 def validate_graph(row, col, n=None, e=None):
     """gatgpu_validate_graph: raises GatGpuError for a CSR set_graph would
     reject (no device needed).  n and e default to the arrays' sizes."""
@@ -363,13 +378,13 @@ class Attention:
         self.h = None
         self.ctx = ctx
         self.lib = ctx.lib
-        lens = [np.ascontiguousarray(a, np.uint32) for a in (q_len, k_len)]
+        lens = [_counts(a, np.uint32) for a in (q_len, k_len)]
         begins = []
         for begin, length in zip((q_begin, k_begin), lens):
             if begin is None:
                 begin = np.cumsum(length, dtype=np.uint64) - length
-            begins.append(np.ascontiguousarray(begin, np.uint64))
-        prefix = None if prefix is None else np.ascontiguousarray(prefix, np.uint32)
+            begins.append(_counts(begin, np.uint64))
+        prefix = None if prefix is None else _counts(prefix, np.uint32)
         self.segments = lens[0].size
         if any(a.shape != (self.segments,) for a in (*lens, *begins)) or (prefix is not None and prefix.shape != (self.segments,)):
             raise ValueError("one length, begin and prefix per segment")
