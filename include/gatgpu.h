@@ -319,7 +319,10 @@ int gatgpu_static_scratch_need(gatgpu_ctx* ctx, int layer, int precision, int hi
  * GATGPU_BIAS_LINEAR: bias = -slope[h] |pos - j|, slope constant.
  * GATGPU_BIAS_TABLE: bias = table[h][min(d, buckets - 1)] with one byte d of
  * distance per pair (a shortest path, say); d = GATGPU_HIDDEN: not seen.  A
- * table entry of -infinity hides its pairs as well.
+ * table entry of -infinity hides its pairs as well, and so does any of -1e6 or
+ * below (beside a key of an ordinary score it weighs 0 anyway; the log-sum of a
+ * row of nothing else has FP32 steps of 1/16 and more, too wide to form weights
+ * from again).
  * A row that sees no key of finite score gets out = 0, lse = -infinity, and no
  * gradient.  Keys that are not seen add nothing, whatever they hold (NaN
  * included); a NaN or infinity in a seen value reaches that row's output.
