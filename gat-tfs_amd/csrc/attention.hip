@@ -182,7 +182,10 @@ int build(gatgpu_attention* P) {
     // four waves and by one: 35 / 37 (one segment of 600, 8 x 64), 100 / 133 (two of 2000), 22 / 23 (one of 300).
     // Forward only where that leaves no units idle, since single waves can be cut further: 16 / 20 (four of 600,
     // 160 blocks), 39 / 28 (one of 2000, 128 blocks); 32 columns 36 / 30 (256 blocks), 18.7 / 19.6 (320).
-    const auto full = [&](uint64_t total, uint64_t tiles, uint64_t tile) { return tiles && total >= tiles * tile * 3 / 4; };
+    // (A launch must take their threads too: blocks that are not full have more than the single waves have.)
+    const auto full = [&](uint64_t total, uint64_t tiles, uint64_t tile) {
+        return tiles && total >= tiles * tile * 3 / 4 && tiles * kvh * 256 <= kMaxThreads;
+    };
     P->wfwd = full(frows, f4, 128) && f4 * kvh * 2 > (width < 64 ? 2 * cus : cus) ? 4 : 1;
     P->wbwd_q = full(brows, q4, 128) ? 4 : 1;
     P->wbwd_kv = full(keys, k4, 64) ? 4 : 1;  // (two pairs of waves with 32 keys each, or one)
