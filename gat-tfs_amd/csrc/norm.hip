@@ -455,7 +455,7 @@ __global__ __launch_bounds__(256) void k_norm_cols_any(const NormArgs a) {
 // fixed order.
 __global__ __launch_bounds__(1024) void k_norm_sum(const float* __restrict__ part, uint32_t blocks, uint32_t W, float* dgamma,
                                                    float* dbeta) {
-    const uint64_t c = uint64_t(blockIdx.x) * 32 + (threadIdx.x & 31);
+    const uint64_t first = norm_block() * 32, c = first + (threadIdx.x & 31);
     const uint32_t g = threadIdx.x >> 5;
     __shared__ float lds[32][33];
     float sum = 0.0f;
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(1024) void k_norm_sum(const float* __restrict__ par
     sum = lds[threadIdx.x & 31][g];
 #pragma unroll
     for (int d = 16; d; d /= 2) sum += __shfl_xor(sum, d);
-    const uint64_t at = uint64_t(blockIdx.x) * 32 + g;
+    const uint64_t at = first + g;
     if ((threadIdx.x & 31) || at >= 2 * uint64_t(W)) return;
     if (at < W) {
         if (dgamma) dgamma[at] = sum;
@@ -582,7 +582,7 @@ hipError_t launch_norm_backward(const NormArgs& a, bool bf16, uint32_t blocks, f
                       aligned(a.dx, a.dxs, size) && (!a.dsum || aligned(a.dsum, a.dss, size));
     const hipError_t e = bf16 ? backward<uint16_t>(a, wide, blocks, s) : backward<float>(a, wide, blocks, s);
     if (e != hipSuccess || !a.part) return e;
-    k_norm_sum<<<uint32_t((2 * uint64_t(a.width) + 31) / 32), 1024, 0, s>>>(a.part, blocks, a.width, dgamma, dbeta);
+    k_norm_sum<<<norm_grid((2 * uint64_t(a.width) + 31) / 32), 1024, 0, s>>>(a.part, blocks, a.width, dgamma, dbeta);
     return hipGetLastError();
 }
 
