@@ -15,7 +15,7 @@
 // sums of dq.  (24 graphs of 130 to 1300 rows, 8 x 64, table: 110 us and 115; four sequences of 4K, 16 x 128,
 // capped: 600 and 960.)
 //
-// Weights and score gradients enter the products with Q, K and dout rounded to bf16 (2^-9 of each; the
+// Weights and score gradients enter the products with Q, K and dout rounded to bf16 (2^-8 of each; the
 // gradients' own stored rounding is as large), the bias gradient unrounded.
 //
 // Where a pass has few blocks, each takes a range of its tile's keys (rows) and leaves FP32 sums, which
@@ -31,17 +31,18 @@
 namespace gatgpu {
 namespace {
 
-// Sum of products of 16 bytes of a and b (+ c).
+// Sum of products of 16 bytes of a and b; bf16 and `rested`: of b with its rest c.
 template <class T>
-__device__ inline float dot16(uint4 a, uint4 b, uint4 c) {
+__device__ inline float dot16(uint4 a, uint4 b, uint4 c, bool rested) {
     const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (sizeof(T) == 2) {
-            sum = fmaf(__uint_as_float(av[i] << 16), __uint_as_float(bv[i] << 16) + __uint_as_float(cv[i] << 16), sum);
-            sum = fmaf(__uint_as_float(av[i] & 0xffff0000u),
-                       __uint_as_float(bv[i] & 0xffff0000u) + __uint_as_float(cv[i] & 0xffff0000u), sum);
+            const float lo = rested ? with_rest(bv[i] & 0xffffu, cv[i] & 0xffffu) : __uint_as_float(bv[i] << 16);
+            const float hi = rested ? with_rest(bv[i] >> 16, cv[i] >> 16) : __uint_as_float(bv[i] & 0xffff0000u);
+            sum = fmaf(__uint_as_float(av[i] << 16), lo, sum);
+            sum = fmaf(__uint_as_float(av[i] & 0xffff0000u), hi, sum);
         } else {
             sum = fmaf(__uint_as_float(av[i]), __uint_as_float(bv[i]), sum);
         }
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
             dof[f] = in ? *reinterpret_cast<const uint4*>(d + at) : make_uint4(0, 0, 0, 0);
             if (in)
                 delta += dot16<T>(dof[f], *reinterpret_cast<const uint4*>(o + at),
-                                  sizeof(T) == 2 && e ? *reinterpret_cast<const uint4*>(e + at) : make_uint4(0, 0, 0, 0));
+                                  sizeof(T) == 2 && e ? *reinterpret_cast<const uint4*>(e + at) : make_uint4(0, 0, 0, 0), e != nullptr);
         }
     }
     delta = xor32_add(delta);

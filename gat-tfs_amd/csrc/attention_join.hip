@@ -61,7 +61,7 @@ __global__ __launch_bounds__(64) void k_attn_join(const AttnArgs a, const AttnTa
             if constexpr (sizeof(T) == 2) {
                 const uint16_t b = bf16_hw(v);
                 static_cast<uint16_t*>(a.out)[at + e] = b;
-                if (a.rest) static_cast<uint16_t*>(a.rest)[at + e] = bf16_hw(v - bf16_widen(b));
+                if (a.rest) static_cast<uint16_t*>(a.rest)[at + e] = uint16_t(rest_bits(v, b));
             } else {
                 static_cast<float*>(a.out)[at + e] = v;
             }

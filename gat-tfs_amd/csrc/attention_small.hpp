@@ -61,7 +61,8 @@ __device__ inline void spread_table(const AttnArgs& a, int kv, int lane, float e
     *reinterpret_cast<float4*>(table + 4 * lane) = v;
 }
 
-template <class T, int D, int KB, int BIAS, bool CAP>
+// REST: as of k_attn_fwd.
+template <class T, int D, int KB, int BIAS, bool CAP, bool REST>
 __global__ __launch_bounds__(64, (D * int(sizeof(T)) * KB <= 128 ? 2 : 1)) void k_attn_small_fwd(const AttnArgs a) {
     constexpr int ROW = lds_row<T, D>(), NF = D * int(sizeof(T)) / 32, DB = D / 32;
     constexpr bool TABLE = BIAS == GATGPU_BIAS_TABLE;
@@ -73,7 +74,6 @@ __global__ __launch_bounds__(64, (D * int(sizeof(T)) * KB <= 128 ? 2 : 1)) void 
     const int lane = int(threadIdx.x), l32 = lane & 31, half = lane >> 5, dim = a.dim;
     const uint32_t rows = seg.q_len * uint32_t(a.group), tiles = (rows + 31) / 32;
     const float cc = a.scale * kLog2e;
-    const bool exact = sizeof(T) == 2 && a.rest;
 
     uint4 nk[KB][NF], nv[KB][NF], nq[NF];
     AttnDist nd[KB];
@@ -171,12 +171,14 @@ __global__ __launch_bounds__(64, (D * int(sizeof(T)) * KB <= 128 ? 2 : 1)) void 
                             acc[d] = mfma_cols_careful<T>(acc[d], vrows, ROW, d * 32, lane, p, seen_operand<T>(s[b]));
                         else acc[d] = mfma_cols<T>(acc[d], load_cols<T>(vrows, ROW, d * 32, lane), p);
                     }
-                    if constexpr (sizeof(T) == 2) {
-                        if (exact) {
-                            const AttnCols<T> lo = rest_operand(s[b], p);
+                    if constexpr (REST) {
+                        AttnCols<T> lo, last;
+                        rest_operands(s[b], p, lo, TABLE ? &last : nullptr);
 #pragma unroll
-                            for (int d = 0; d < DB; ++d)
-                                acc[d] = mfma_cols<T>(acc[d], load_cols<T, CAREFUL ? kClean : kRaw>(vrows, ROW, d * 32, lane), lo);
+                        for (int d = 0; d < DB; ++d) {
+                            const AttnCols<T> v = load_cols<T, CAREFUL ? kClean : kRaw>(vrows, ROW, d * 32, lane);
+                            acc[d] = mfma_cols<T>(acc[d], v, lo);
+                            if constexpr (TABLE) acc[d] = mfma_cols<T>(acc[d], v, last);
                         }
                     }
                 }
@@ -496,14 +498,17 @@ hipError_t small_forward(const AttnArgs& a, int blocks, hipStream_t s) {
         constexpr bool CAP = decltype(cap)::value;
         if constexpr (attention_small_width<T>(D)) {
             const size_t dyn = BIAS == GATGPU_BIAS_TABLE ? size_t(a.group) * 1024 : 0;
-            if (blocks == 1) {
-                k_attn_small_fwd<T, D, 1, BIAS, CAP><<<uint32_t(a.ntasks), 64, dyn, s>>>(a);
+            const auto launch = [&](auto kb, auto rest) {
+                k_attn_small_fwd<T, D, decltype(kb)::value, BIAS, CAP, decltype(rest)::value><<<uint32_t(a.ntasks), 64, dyn, s>>>(a);
                 return hipGetLastError();
-            }
+            };
+            constexpr std::integral_constant<int, 1> one{};
             if constexpr (sizeof(T) == 2) {
-                k_attn_small_fwd<T, D, 2, BIAS, CAP><<<uint32_t(a.ntasks), 64, dyn, s>>>(a);
-                return hipGetLastError();
+                constexpr std::integral_constant<int, 2> two{};
+                if (blocks == 2) return a.rest ? launch(two, std::true_type{}) : launch(two, std::false_type{});
+                if (a.rest) return launch(one, std::true_type{});
             }
+            if (blocks == 1) return launch(one, std::false_type{});
             return hipErrorInvalidValue;
         } else {
             return hipErrorInvalidValue;

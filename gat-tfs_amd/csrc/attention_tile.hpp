@@ -128,13 +128,14 @@ __device__ inline AttnCols<T> to_operand(const f32x16_t& c) {
     }
     return p;
 }
-// What the rounding to bf16 took, as a second operand.
-__device__ inline AttnCols<uint16_t> rest_operand(const f32x16_t& c, const AttnCols<uint16_t>& p) {
-    AttnCols<uint16_t> r;
+// What the rounding to bf16 took, as a second operand; and what that one's rounding took, which is exactly a third's.
+__device__ inline void rest_operands(const f32x16_t& c, const AttnCols<uint16_t>& p, AttnCols<uint16_t>& r, AttnCols<uint16_t>* last) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        r.w[i] = bf16x2(c[2 * i] - __uint_as_float(p.w[i] << 16), c[2 * i + 1] - __uint_as_float(p.w[i] & 0xffff0000u));
-    return r;
+    for (int i = 0; i < 8; ++i) {
+        const float x = c[2 * i] - __uint_as_float(p.w[i] << 16), y = c[2 * i + 1] - __uint_as_float(p.w[i] & 0xffff0000u);
+        r.w[i] = bf16x2(x, y);
+        if (last) last->w[i] = bf16x2(x - __uint_as_float(r.w[i] << 16), y - __uint_as_float(r.w[i] & 0xffff0000u));
+    }
 }
 
 // Weight tile of which every element that is not 0 counts as 1.
@@ -433,6 +434,17 @@ __device__ inline AttnRow attn_row(const AttnArgs& a, const AttnSeg& s, uint32_t
     return w;
 }
 
+// What rounding to the bf16 `b` took from x: the difference of their FP32 patterns, -2^15 to 2^15, halved to 15 bits, so that
+// both give x to 23 bits (a bf16 rest would give 17).  Bit 14 stays 0: as a bf16 a rest is never a NaN.
+__device__ inline uint32_t rest_bits(float x, uint32_t b) {
+    const int t = max(-32768, min(32767, int(__float_as_uint(x) - (b << 16))));
+    const uint32_t u = uint32_t(t + 32768) >> 1;
+    return (u & 0x4000u) << 1 | (u & 0x3fffu);
+}
+__device__ inline float with_rest(uint32_t b, uint32_t rest) {
+    return __uint_as_float((b << 16) + 2 * ((rest >> 1 & 0x4000u) | (rest & 0x3fffu)) - 32768u);
+}
+
 // Rows of a C tile set (columns: rows of the output, registers: dim) times `factor`, rounded to
 // the storage type, to the lane's row at base + at.  bf16: the wave's halves swap 8 bytes, so that
 // each lane stores 16.  Every lane of the wave takes part; rows with `in` are stored.  REST: what
@@ -445,7 +457,7 @@ __device__ inline void store_rows(void* base, uint64_t at, const f32x16_t (&acc)
             x *= factor;
             y *= factor;
             uint32_t u = bf16x2(x, y);
-            if (REST) u = bf16x2(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xffff0000u));
+            if (REST) u = rest_bits(x, u & 0xffffu) | rest_bits(y, u >> 16) << 16;
             return u;
         };
 #pragma unroll

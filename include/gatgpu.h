@@ -385,13 +385,14 @@ typedef struct gatgpu_attention_io {
     void* out;
     uint64_t out_stride;
     float* lse;           /* [row][heads], row as in out; forward: may be NULL   */
-    void* rest;           /* bf16, may be NULL: an array like out (of its stride),
+    void* rest;           /* bf16, may be NULL: an array of out's size and stride,
                              which a forward call leaves for its backward call
-                             (rows for which it needs nothing stay as they
-                             were).  It holds what rounding took from out,
-                             whose weights then enter as two bf16 each, so that
-                             dout.out has 16 bits: without it an error of out's
-                             rounding, 2^-9 of dout.out, stays in the score
+                             (rows for which it needs nothing may stay as they
+                             were).  It holds the next 16 bits of out, encoded.
+                             With it the weights enter out as two bf16 each, so
+                             that dout.out has 16 bits, and as three with a
+                             table: FP32's.  Without it an error of out's
+                             rounding, 2^-8 of dout.out, stays in the score
                              gradients.  Required when dbias is given         */
     const void* dout;
     uint64_t dout_stride;
