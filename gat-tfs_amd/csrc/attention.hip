@@ -245,7 +245,7 @@ int build(gatgpu_attention* P) {
     // Backward passes with few blocks: the same, keys of query tiles and rows of key tiles, into about two ranges a
     // unit.  The joined sums are as large as several outputs, so ranges are long, and none are cut from as many
     // blocks as units (two segments of 2000, 8 x 64: 101 us so, 107 cut).  us without and with: one segment of
-    // 2000 91 / 85 (8 x 64, bf16), 398 / 297 (FP32), of 1000 108 / 44 (8 heads on 2), of 3000 579 / 106 (8 on 1).
+    // 2000 91 / 85 (8 x 64, bf16), 398 / 297 (FP32), of 1000 108 / 43 (8 heads on 2), of 3000 579 / 109 (8 on 1, causal).
     std::vector<AttnTask> join_q, join_kv;
     const auto spread_out = [&](std::vector<AttnTask>& tasks, std::vector<AttnTask>& tiles) {
         const uint64_t blocks = tasks.size() * kvh, want = std::max<uint64_t>(1, 2 * cus / kvh);

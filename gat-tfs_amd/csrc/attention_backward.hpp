@@ -213,8 +213,8 @@ __global__ __launch_bounds__(NW * 64, (attn_waves<T, D, NW>())) void k_attn_bwd_
 // those of rows 32 to 63; both go through LDS, and then the first wave sums dv over the 64 rows, the second
 // dk.  So a wave holds one gradient's sums instead of two (64 registers at 128 columns), and with V in LDS at
 // bf16's 128 columns two waves a SIMD fit.  Four sequences of 4K, 16 x 128, capped: 960 us so, 1105 with V in
-// registers and one wave a SIMD, 1380 with both gradients in a wave.  Vector instructions issue in 44 % of the
-// cycles, matrix ones in 25 %, LDS in 38 %: the waits between a tile's phases bound it.
+// registers and one wave a SIMD, 1380 with both gradients in a wave.  Vector instructions issue in 39 % of the
+// cycles, matrix ones in 30 %, LDS works in 54 %: the waits between a tile's phases bound it.
 template <class T, int D, int PAIRS>
 struct KvLds {
     static constexpr int kRows = 64, kThreads = PAIRS * 128, kTile = kRows * lds_row<T, D>();

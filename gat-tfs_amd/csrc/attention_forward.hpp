@@ -14,7 +14,7 @@
 // of the keys each, on tiles of 32.  m, l and O are FP32.
 //
 // Bound by the vector instructions of the scores (four or more and a quarter-rate exponential each) beside the
-// products: one graph of 16K nodes, 8 x 64, capped, takes 800 us, 686 TFLOP/s where a large product reaches 1086;
+// products: one graph of 16K nodes, 8 x 64, capped, takes 800 to 830 us, 660 to 690 TFLOP/s where a large product reaches 1086;
 // 48 single tokens over up to 24K keys 182 us, the keys' and values' bytes at 5 TB/s.
 //
 // The loop checks no element for NaN or infinity: a bad value in a tile shows in the sums of

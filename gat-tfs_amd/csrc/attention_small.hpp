@@ -10,8 +10,8 @@
 // current one is computed: a step is about as long as a trip to memory, and the bytes of few
 // waves a SIMD keep the memory busy.
 //
-// 1500 segments of 9 to 60 rows, 8 x 32, bf16, table: forward 22 + 16 us (33 to 64 keys, up to 32), backward
-// 66 + 32, of which the bias gradient's LDS sums take a third; the rows' bytes would take 35 in all.
+// 1500 segments of 9 to 60 rows, 8 x 32, bf16, table: forward 22 + 15 us (33 to 64 keys, up to 32), backward
+// 63 + 33, of which the bias gradient's LDS sums take a third; the rows' bytes would take 35 in all.
 //
 // Row operands of the forward pass come straight from memory; what is contracted over its rows
 // (V; backward K, Q, dout and the turned weights) passes through LDS.
@@ -213,9 +213,9 @@ __device__ inline void block_sync() {
     else lds_barrier();
 }
 
-// Waves a SIMD that its registers are held to: those of 64 bf16 columns, or of 32 FP32 ones and several
-// waves, do not fit half a SIMD's registers (1500 segments of up to 60 keys, 8 x 64 in bf16 with a
-// table: 461 us with what did not fit in memory, 303 us so; 8 x 32 in FP32: 426, 362).
+// Waves a SIMD that its registers are held to: those of 64 bf16 columns, or of 32 FP32 ones and several waves, do not fit
+// half a SIMD's registers (1500 segments of up to 60 keys, 8 x 64 in bf16 with a table: 461 us with what did not fit in
+// memory, 303 us so; 8 x 32 in FP32: 426, 362).  Those of 32 FP32 columns and one wave do, but for 26 with a table.
 template <class T, int D, int NW>
 constexpr int small_bwd_waves() {
     return D * int(sizeof(T)) <= 64 || (sizeof(T) == 4 && D == 32 && NW == 1) ? 2 : 1;

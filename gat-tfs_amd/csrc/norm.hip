@@ -560,7 +560,7 @@ hipError_t backward(const NormArgs& a, bool wide, uint32_t blocks, hipStream_t s
 
 // Blocks are persistent, so no more than run at once: three of 256 threads a CU (131 registers a
 // thread).  169K x 256 bf16, residual and ELU: 768 blocks 80 us, 512 97, 1024 108, 2048 91.
-// Wider rows take blocks of 512 threads, one or two a CU (8190 x 8192: 106 us at 256 and 512).  Few rows: a block
+// Wider rows take blocks of 256 to 1024 threads, one or two a CU (8190 x 8192: 106 us at 256 blocks and at 512).  Few rows: a block
 // a row where a block holds one at a time (100 x 2000, forward and backward: 10.7 us; 13.7 with four rows a block).
 // A partial row costs 16 bytes a column, written and read, a row 6 to 16 a column.
 uint32_t norm_blocks(uint64_t rows, uint64_t width) {

@@ -326,6 +326,8 @@ int gatgpu_static_scratch_need(gatgpu_ctx* ctx, int layer, int precision, int hi
  * A row that sees no key of finite score gets out = 0, lse = -infinity, and no
  * gradient.  Keys that are not seen add nothing, whatever they hold (NaN
  * included); a NaN or infinity in a seen value reaches that row's output.
+ * Sums of weights times values are formed in FP32 before they are divided by
+ * the weights' sum, with weights of up to 2^8: values beyond 1e30 may overflow.
  *
  * Storage: GATGPU_FP32 (products in FP32) or GATGPU_BF16 (bf16 rows, FP32
  * scores, softmax state and sums; the weights and, backward, the score
@@ -376,7 +378,8 @@ int gatgpu_attention_distances(const gatgpu_attention* plan, uint64_t* bytes, ui
  * elements side by side; strides in elements, 16-byte aligned like the bases,
  * at least the row's width (so q, k and v may be parts of one array's rows).
  * Arrays of query rows may be NULL where every q_len is 0, arrays of key rows
- * where every k_len is. */
+ * where every k_len is.  What a call writes must share no memory with what it
+ * reads or else writes. */
 typedef struct gatgpu_attention_io {
     const void *q, *k, *v;
     uint64_t q_stride, k_stride, v_stride;
