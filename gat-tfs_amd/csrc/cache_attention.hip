@@ -1,0 +1,565 @@
+// Attention over a paged 8-bit cache (cache_attention.hpp says how operands lie).
+//
+// Few rows a request: bound by the cache's bytes.  The calls' keys, in tiles of 64 and over all requests, are cut into
+// equal ranges for a fixed number of blocks a key/value head, since lengths are known on the device only: each block
+// sums the requests' tiles to find its own range, its four waves take its tiles in turn and join their sums in LDS.
+// What is cut between blocks leaves partial sums, which a second launch joins in the order of the keys.
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "cache_attention.hpp"
+
+namespace gatgpu {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+
+// The queries of a wave's 16 rows as operands: PARTS bf16 of each value.
+template <class T, int NB>
+struct Queries {
+    static constexpr int PARTS = sizeof(T) == 2 ? 1 : 3;
+    uint4 w[PARTS][NB][2];
+};
+template <class T, int NB>
+__device__ inline Queries<T, NB> load_queries(const CacheAttnArgs& a, const CacheRequest& rq, uint32_t packed, uint32_t head, int g) {
+    Queries<T, NB> q;
+    const bool there = packed < rq.rows * a.c.group;
+    const uint32_t i = packed / a.c.group, h = head * a.c.group + packed % a.c.group;
+    const T* const row = static_cast<const T*>(a.q) + uint64_t(rq.begin + (there ? i : 0)) * a.qs + uint64_t(h) * uint64_t(a.c.dim);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int col = 64 * b + 16 * g + 8 * s;
+            uint4 zero = make_uint4(0, 0, 0, 0);
+            if constexpr (sizeof(T) == 2) {
+                q.w[0][b][s] = there && uint32_t(col) < a.c.dim ? *reinterpret_cast<const uint4*>(row + col) : zero;
+            } else {
+                float x[8] = {};
+                if (there && uint32_t(col) < a.c.dim) {
+                    const float4 lo = *reinterpret_cast<const float4*>(row + col), hi = *reinterpret_cast<const float4*>(row + col + 4);
+                    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+                }
+                uint32_t p[3][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) {
+                        p[k][j] = bf16x2(x[2 * j], x[2 * j + 1]);
+                        x[2 * j] -= __uint_as_float(p[k][j] << 16);
+                        x[2 * j + 1] -= __uint_as_float(p[k][j] & 0xffff0000u);
+                    }
+#pragma unroll
+                for (int k = 0; k < 3; ++k) q.w[k][b][s] = make_uint4(p[k][0], p[k][1], p[k][2], p[k][3]);
+            }
+        }
+    return q;
+}
+
+// A tile's bytes as they come: keys [operand][64 columns], values [16 columns], and the scales of the lane's 16 keys.
+template <int NB>
+struct Tile {
+    uint4 k[4][NB], v[4 * NB];
+    float ks, vs;
+    bool page;  // the lane's keys have one
+};
+
+// Pages of a tile's keys: of the lane's scores and values, and of the keys whose bytes it loads.
+struct TilePages {
+    uint32_t own, load;
+};
+__device__ inline uint32_t own_key(uint32_t tile, int lane) { return tile * kCacheTile + 16u * uint32_t(lane / 16); }
+__device__ inline uint32_t loaded_key(uint32_t tile, int lane) { return tile * kCacheTile + 16u * uint32_t(lane % 16 / 4) + uint32_t(lane % 4); }
+__device__ inline TilePages tile_pages(const CacheAttnArgs& a, const uint32_t* row, uint32_t keys, uint32_t tile, int lane) {
+    const uint32_t own = block_of(a.c, keys, own_key(tile, lane)), load = block_of(a.c, keys, loaded_key(tile, lane) & ~15u);
+    return {own == kNoPage ? own : row[own], load == kNoPage ? load : row[load]};
+}
+template <int NB>
+__device__ inline Tile<NB> load_tile(const CacheAttnArgs& a, TilePages p, uint32_t tile, uint32_t head, int lane) {
+    Tile<NB> t;
+    const uint32_t m = uint32_t(lane % 16), g = uint32_t(lane / 16);
+    t.page = p.own < a.c.pages;
+    const uint32_t own = some_page(a.c, p.own);
+    const uint8_t* const k = a.k + key_byte(a.c, some_page(a.c, p.load), head, loaded_key(tile, lane)) + 16 * g;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b)
+            t.k[i][b] = 64 * b + 16 * g < a.c.dim ? *reinterpret_cast<const uint4*>(k + i * 4 * a.c.dim + 64 * b) : make_uint4(0, 0, 0, 0);
+    const uint8_t* const v = a.v + value_byte(a.c, own, head, own_key(tile, lane), m);
+#pragma unroll
+    for (uint32_t d = 0; d < 4 * NB; ++d)
+        t.v[d] = 16 * d < a.c.dim ? *reinterpret_cast<const uint4*>(v + (uint64_t(16 * d) << a.c.page_log)) : make_uint4(0, 0, 0, 0);
+    t.ks = a.k_scale[uint64_t(own) * a.c.kv_heads + head];
+    t.vs = a.v_scale[uint64_t(own) * a.c.kv_heads + head];
+    return t;
+}
+
+// A wave's running softmax: lane (n, g) has row n's reference, the weights' sum of its own keys, and its columns' sums.
+template <int NB>
+struct Running {
+    f32x4_t o[4 * NB];
+    float ref, sum;
+};
+
+// One step: 64 keys.  seen: keys that the lane's row sees; least, most: of the wave's rows; keys: of the request.
+template <class T, int NB>
+__device__ inline void step(const CacheAttnArgs& a, Running<NB>& run, const Queries<T, NB>& q, Tile<NB>& t, uint32_t tile, uint32_t keys, uint32_t seen,
+                            uint32_t least, int lane) {
+    constexpr int PARTS = Queries<T, NB>::PARTS;
+    const uint32_t first = tile * kCacheTile + 16u * uint32_t(lane / 16);
+    f32x4_t s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        s[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const uint4 lo = keys_operand(t.k[i][b].x, t.k[i][b].y), hi = keys_operand(t.k[i][b].z, t.k[i][b].w);
+#pragma unroll
+            for (int p = PARTS - 1; p >= 0; --p) {
+                s[i] = mfma_bf16(lo, q.w[p][b][0], s[i]);
+                s[i] = mfma_bf16(hi, q.w[p][b][1], s[i]);
+            }
+        }
+    }
+    const int ev = scale_exponent(t.vs);
+    const float by = a.scale * power_of_two(scale_exponent(t.ks));
+    const bool whole = tile * kCacheTile + kCacheTile <= least && __all(t.page);  // every row sees every key
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (!whole && !(t.page && first + uint32_t(4 * i + r) < seen)) s[i][r] = -INFINITY;
+            top = fmaxf(top, s[i][r]);
+        }
+    top = fmaf(top, by, float(ev));
+    if (__any(top > run.ref + kCacheRoom)) {
+        const float all = xor32_max(xor16_max(top));
+        const bool up = all > run.ref + kCacheRoom;
+        const float ref = up ? ceilf(all) - kCacheSet : run.ref, less = up ? __builtin_amdgcn_exp2f(run.ref - ref) : 1.0f;
+        run.ref = ref;
+        run.sum *= less;
+#pragma unroll
+        for (int d = 0; d < 4 * NB; ++d) run.o[d] *= less;
+    }
+    const float shift = float(ev) - run.ref;  // (whole numbers: exact)
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], by, shift));
+            sum += s[i][r];
+        }
+    run.sum = fmaf(sum, power_of_two(-ev), run.sum);
+    uint4 w[2], rest[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t u[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float x = s[2 * h + j / 2][j % 2 * 2], y = s[2 * h + j / 2][j % 2 * 2 + 1];
+            u[j] = f16x2(x, y);
+            if constexpr (PARTS > 1) {
+                const f16x2_t up = __builtin_bit_cast(f16x2_t, u[j]);
+                l[j] = f16x2(x - float(up[0]), y - float(up[1]));
+            }
+        }
+        w[h] = make_uint4(u[0], u[1], u[2], u[3]);
+        if constexpr (PARTS > 1) rest[h] = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+    bool bad = false;
+    if (!whole) {
+        // Values of no token count as 0; a NaN that some rows see and others do not needs care.
+        const int valid = t.page ? int(min(keys > first ? keys - first : 0u, 16u)) : 0;
+        uint32_t nan = 0;
+#pragma unroll
+        for (int d = 0; d < 4 * NB; ++d) {
+            t.v[d].x &= low_bytes(valid);
+            t.v[d].y &= low_bytes(valid - 4);
+            t.v[d].z &= low_bytes(valid - 8);
+            t.v[d].w &= low_bytes(valid - 12);
+            nan |= nan_bytes(t.v[d].x) | nan_bytes(t.v[d].y) | nan_bytes(t.v[d].z) | nan_bytes(t.v[d].w);
+        }
+        bad = __any(nan != 0);
+    }
+    if (bad) {
+        uint32_t u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t at = first + uint32_t(2 * j);
+            u[j] = (t.page && at < seen ? 0x3c00u : 0u) | (t.page && at + 1 < seen ? 0x3c000000u : 0u);
+        }
+        const uint4 one[2] = {make_uint4(u[0], u[1], u[2], u[3]), make_uint4(u[4], u[5], u[6], u[7])};
+#pragma unroll
+        for (int d = 0; d < 4 * NB; ++d) {
+            uint32_t* const c[4] = {&t.v[d].x, &t.v[d].y, &t.v[d].z, &t.v[d].w};
+            uint32_t mark[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t n = nan_bytes(*c[j]) >> 7;  // 1 at each NaN
+                *c[j] &= ~(n * 0xffu);
+                mark[j] = n * 0x38u;  // 1.0 in e4m3
+            }
+            f32x4_t count = {0.0f, 0.0f, 0.0f, 0.0f};
+            count = mfma_f16(values_operand(mark[0], mark[1]), one[0], count);
+            count = mfma_f16(values_operand(mark[2], mark[3]), one[1], count);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (count[r] > 0.0f) run.o[d][r] = NAN;
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < 4 * NB; ++d) {
+        const uint4 lo = values_operand(t.v[d].x, t.v[d].y), hi = values_operand(t.v[d].z, t.v[d].w);
+        if constexpr (PARTS > 1) {
+            run.o[d] = mfma_f16(lo, rest[0], run.o[d]);
+            run.o[d] = mfma_f16(hi, rest[1], run.o[d]);
+        }
+        run.o[d] = mfma_f16(lo, w[0], run.o[d]);
+        run.o[d] = mfma_f16(hi, w[1], run.o[d]);
+    }
+}
+
+// Row n's output: columns 16 d + 4 g ... + 3 from o[d], and its lse (lanes of g = 0).
+template <class T, int NB>
+__device__ inline void store_columns(const CacheAttnArgs& a, const CacheRequest& rq, uint32_t packed, uint32_t head, int d, int g, f32x4_t o, float sum) {
+    if (packed >= rq.rows * a.c.group || uint32_t(16 * d) >= a.c.dim) return;
+    const uint32_t i = packed / a.c.group, h = head * a.c.group + packed % a.c.group;
+    T* const to = static_cast<T*>(a.out) + uint64_t(rq.begin + i) * a.os + uint64_t(h) * uint64_t(a.c.dim) + 16 * d + 4 * g;
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (sum == 0.0f) o = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(to) = make_uint2(bf16x2(o[0] * by, o[1] * by), bf16x2(o[2] * by, o[3] * by));
+    else *reinterpret_cast<float4*>(to) = make_float4(o[0] * by, o[1] * by, o[2] * by, o[3] * by);
+}
+__device__ inline void store_lse(const CacheAttnArgs& a, const CacheRequest& rq, uint32_t packed, uint32_t head, float ref, float sum) {
+    if (!a.lse || packed >= rq.rows * a.c.group) return;
+    const uint32_t i = packed / a.c.group, h = head * a.c.group + packed % a.c.group;
+    a.lse[uint64_t(rq.begin + i) * uint64_t(a.c.heads) + h] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Sums of the four waves: [wave][columns / 16][lane] columns, [wave][row] references and weights.
+template <int NB>
+struct JoinLds {
+    f32x4_t o[kWaves][4 * NB][kWave];
+    float ref[kWaves][kCacheRows], sum[kWaves][kCacheRows];
+};
+
+// 8 waves a unit hide their requests behind each other; a wave has a tile's 16 KB (128 columns) in flight while it works
+// on the one before.
+template <class T, int NB>
+__global__ __launch_bounds__(kThreads, 2) void k_cache_attention(const CacheAttnArgs a) {
+    __shared__ JoinLds<NB> join;
+    __shared__ uint64_t s_sum[kWaves], s_start;
+    __shared__ uint32_t s_request;
+    const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
+    const uint32_t head = blockIdx.x % a.c.kv_heads;
+    const uint32_t worker = blockIdx.x / a.c.kv_heads;
+    uint64_t at = 0, end = 0, base = 0, share = 1;  // the worker's tiles, and those before its request
+    uint32_t request = worker;
+    if (a.workers) {
+        const uint32_t per = (a.c.requests + kThreads - 1) / kThreads, from = min(a.c.requests, uint32_t(tid) * per), to = min(a.c.requests, from + per);
+        uint64_t own = 0;
+        for (uint32_t r = from; r < to; ++r) {
+            const CacheRequest q = request_of(a, r);
+            own += uint64_t(row_tiles(a.c, q)) * key_tiles(q);
+        }
+        uint64_t upto = own;
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) {
+            const uint64_t p = __shfl_up(upto, d);
+            if (lane >= d) upto += p;
+        }
+        if (lane == kWave - 1) s_sum[wave] = upto;
+        __syncthreads();
+        uint64_t total = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) upto += s_sum[w];
+            total += s_sum[w];
+        }
+        share = max(uint64_t(a.least), (total + a.workers - 1) / a.workers);
+        at = min(total, uint64_t(worker) * share);
+        end = min(total, at + share);
+        if (at < end && at >= upto - own && at < upto) {  // one thread's requests hold the first tile
+            uint64_t sum = upto - own;
+            for (uint32_t r = from; r < to; ++r) {
+                const CacheRequest q = request_of(a, r);
+                const uint64_t cost = uint64_t(row_tiles(a.c, q)) * key_tiles(q);
+                if (at < sum + cost) {
+                    s_request = r;
+                    s_start = sum;
+                    break;
+                }
+                sum += cost;
+            }
+        }
+        __syncthreads();
+        if (at >= end) {
+            if (tid == 0) a.meta[blockIdx.x] = make_uint4(0, 0, 0, 0);
+            return;
+        }
+        request = s_request;
+        base = s_start;
+    }
+    uint4 meta = make_uint4(0, 0, 0, 0);
+    while (request < a.c.requests) {
+        const CacheRequest rq = request_of(a, request);
+        const uint32_t tiles = key_tiles(rq), rows = row_tiles(a.c, rq);
+        if (!a.workers) end = uint64_t(rows) * tiles;  // (a block a request)
+        if (at >= end) break;
+        const uint64_t in = at - base;
+        if (in >= uint64_t(rows) * tiles) {  // the next request
+            base += uint64_t(rows) * tiles;
+            ++request;
+            continue;
+        }
+        const uint32_t row_tile = uint32_t(in / tiles), lo = uint32_t(in % tiles);
+        const uint32_t hi = index_min(tiles, lo + (end - at));
+        const uint32_t packed = row_tile * kCacheRows + uint32_t(n);
+        const bool there = packed < rq.rows * a.c.group;
+        const uint32_t seen = there ? cache_seen(rq, packed / a.c.group) : 0;
+        // Rows of a tile stand in the order of their positions.
+        const uint32_t last = min(rq.rows * a.c.group, (row_tile + 1) * kCacheRows) - 1;
+        const uint32_t least = cache_seen(rq, row_tile * kCacheRows / a.c.group), most = cache_seen(rq, last / a.c.group);
+        const uint32_t* const row = a.table + uint64_t(request) * a.ld;
+        const Queries<T, NB> q = load_queries<T, NB>(a, rq, packed, head, g);
+        Running<NB> run;
+#pragma unroll
+        for (int d = 0; d < 4 * NB; ++d) run.o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        run.ref = kCacheNoRef;
+        run.sum = 0.0f;
+        const uint32_t stop = min(hi, (most + kCacheTile - 1) / kCacheTile);
+        uint32_t tile = lo + uint32_t(wave);
+        if (tile < stop) {
+            Tile<NB> now = load_tile<NB>(a, tile_pages(a, row, rq.keys, tile, lane), tile, head, lane);
+            TilePages ahead = tile_pages(a, row, rq.keys, tile + kWaves, lane);
+            for (; tile < stop; tile += kWaves) {
+                Tile<NB> next = now;
+                if (tile + kWaves < stop) {
+                    next = load_tile<NB>(a, ahead, tile + kWaves, head, lane);
+                    ahead = tile_pages(a, row, rq.keys, tile + 2 * kWaves, lane);
+                }
+                step<T, NB>(a, run, q, now, tile, rq.keys, seen, least, lane);
+                now = next;
+            }
+        }
+        run.sum = xor32_add(xor16_add(run.sum));
+        // The waves' sums to those of the block: each wave joins its share of the columns.
+        if (lane < 16) {
+            join.ref[wave][n] = run.ref;
+            join.sum[wave][n] = run.sum;
+        }
+#pragma unroll
+        for (int d = 0; d < 4 * NB; ++d) join.o[wave][d][lane] = run.o[d];
+        __syncthreads();
+        float ref = join.ref[0][n], sum = 0.0f, less[kWaves];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) ref = fmaxf(ref, join.ref[w][n]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            less[w] = __builtin_amdgcn_exp2f(join.ref[w][n] - ref);
+            sum = fmaf(join.sum[w][n], less[w], sum);
+        }
+        const bool cut = lo > 0 || hi < tiles;
+        const uint64_t piece = (uint64_t(blockIdx.x) * 2 + (lo > 0 ? 0 : 1));
+#pragma unroll
+        for (int d = 0; d < NB; ++d) {
+            const int db = wave * NB + d;
+            f32x4_t o = join.o[0][db][lane] * less[0];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) o += join.o[w][db][lane] * less[w];
+            if (cut) *reinterpret_cast<f32x4_t*>(a.part + ((piece * (4 * NB) + uint64_t(db)) * kWave + uint64_t(lane)) * 4) = o;
+            else store_columns<T, NB>(a, rq, packed, head, db, g, o, sum);
+        }
+        if (wave == 0 && lane < 16) {
+            if (cut) {
+                a.stat[piece * 32 + uint64_t(n)] = ref;
+                a.stat[piece * 32 + 16 + uint64_t(n)] = sum;
+            } else {
+                store_lse(a, rq, packed, head, ref, sum);
+            }
+        }
+        if (lo == 0 && hi < tiles) {
+            const uint64_t task_end = base + uint64_t(row_tile + 1) * tiles;
+            meta = make_uint4(request, row_tile, uint32_t((task_end - 1) / share) - worker + 1, 0);
+        }
+        at += hi - lo;
+        __syncthreads();
+    }
+    if (a.workers && tid == 0) a.meta[blockIdx.x] = meta;
+}
+
+// The pieces of the task that begins in a worker and ends in another: 16 columns a block, its waves a quarter of the pieces each.
+template <class T, int NB>
+__global__ __launch_bounds__(kThreads) void k_cache_join(const CacheAttnArgs a) {
+    __shared__ f32x4_t s_o[kWaves][kWave];
+    __shared__ float s_ref[kWaves][kCacheRows], s_sum[kWaves][kCacheRows];
+    const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
+    const uint32_t block = blockIdx.x, db = blockIdx.y;
+    const uint4 meta = a.meta[block];
+    if (!meta.z) return;
+    const uint32_t head = block % a.c.kv_heads;
+    const auto piece_of = [&](uint32_t p) { return (uint64_t(block) + uint64_t(p) * uint64_t(a.c.kv_heads)) * 2 + (p ? 0 : 1); };
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float ref = kCacheNoRef, sum = 0.0f;
+    for (uint32_t p = uint32_t(wave); p < meta.z; p += kWaves) {
+        const uint64_t piece = piece_of(p);
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part + ((piece * (4 * NB) + db) * kWave + uint64_t(lane)) * 4);
+        const float r = a.stat[piece * 32 + uint64_t(n)], s = a.stat[piece * 32 + 16 + uint64_t(n)];
+        const float top = fmaxf(ref, r), less = __builtin_amdgcn_exp2f(ref - top), more = __builtin_amdgcn_exp2f(r - top);
+        o = o * less + x * more;
+        sum = sum * less + s * more;
+        ref = top;
+    }
+    s_o[wave][lane] = o;
+    if (lane < 16) {
+        s_ref[wave][n] = ref;
+        s_sum[wave][n] = sum;
+    }
+    __syncthreads();
+    if (wave) return;
+    float top = s_ref[0][n];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_ref[w][n]);
+    o = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const float less = __builtin_amdgcn_exp2f(s_ref[w][n] - top);
+        o += s_o[w][lane] * less;
+        sum = fmaf(s_sum[w][n], less, sum);
+    }
+    const CacheRequest rq = request_of(a, meta.x);
+    const uint32_t packed = meta.y * kCacheRows + uint32_t(n);
+    store_columns<T, NB>(a, rq, packed, head, int(db), g, o, sum);
+    if (db == 0 && lane < 16) store_lse(a, rq, packed, head, top, sum);
+}
+
+// Blocks a key/value head: two a unit in all.
+uint32_t cache_workers(const gatgpu_ctx* c, int kv_heads) { return uint32_t(std::max(1, 2 * c->cus / kv_heads)); }
+
+template <class T, int NB>
+hipError_t launch(const CacheAttnArgs& a, hipStream_t s) {
+    const uint32_t blocks = (a.workers ? a.workers : a.c.requests) * a.c.kv_heads;
+    k_cache_attention<T, NB><<<blocks, kThreads, 0, s>>>(a);
+    if (!a.workers) return hipGetLastError();
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    k_cache_join<T, NB><<<dim3(blocks, uint32_t(a.c.dim / 16)), kThreads, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+uint64_t pad256(uint64_t b) { return (b + 255) / 256 * 256; }
+struct Workspace {
+    uint64_t part, stat, meta;
+};
+Workspace workspace_of(const gatgpu_ctx* c, const gatgpu_cache* cache) {
+    const uint64_t blocks = uint64_t(cache_workers(c, cache->kv_heads)) * uint64_t(cache->kv_heads), nb = cache->dim > 64 ? 2 : 1;
+    return {pad256(blocks * 2 * 4 * nb * kWave * 16), pad256(blocks * 2 * 32 * 4), pad256(blocks * 16)};
+}
+
+}  // namespace
+}  // namespace gatgpu
+
+namespace {
+
+using namespace gatgpu;
+
+int check_sizes(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgpu_cache_attention_io* io) {
+    if (!io) return fail(c, GATGPU_EINVAL, "null arrays");
+    if (io->precision != GATGPU_FP32 && io->precision != GATGPU_BF16) return fail(c, GATGPU_EINVAL, "bad precision");
+    if (io->heads < 1 || io->heads > 64 || io->heads % cache->kv_heads) return fail(c, GATGPU_EINVAL, "heads must be 1 to 64 and a multiple of kv_heads");
+    if (io->rows >= (uint64_t(1) << 31) / uint64_t(io->heads)) return fail(c, GATGPU_EOVERFLOW, "rows * heads must be below 2^31");
+    if (io->requests > (1u << 20)) return fail(c, GATGPU_EOVERFLOW, "more than 2^20 requests");
+    if (uint64_t(io->blocks) * cache->page >= (uint64_t(1) << 32)) return fail(c, GATGPU_EOVERFLOW, "blocks * page must be below 2^32");
+    if (io->table_stride < io->blocks || io->table_stride > (uint64_t(1) << 40)) return fail(c, GATGPU_EINVAL, "table has a bad row stride");
+    return GATGPU_OK;
+}
+int check_rows(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgpu_cache_attention_io* io, const char* name, const void* p, uint64_t stride) {
+    if (!p) return fail(c, GATGPU_EINVAL, std::string("null ") + name);
+    const uint64_t size = io->precision == GATGPU_BF16 ? 2 : 4;
+    if (stride < uint64_t(io->heads) * uint64_t(cache->dim) || stride > (uint64_t(1) << 44))
+        return fail(c, GATGPU_EINVAL, std::string(name) + " has a bad row stride");
+    if (reinterpret_cast<uintptr_t>(p) % 16 || stride * size % 16) return fail(c, GATGPU_EINVAL, std::string(name) + " and its stride must be 16-byte aligned");
+    return check_device_array(c, p, name);
+}
+int check_words(gatgpu_ctx* c, const char* name, const void* p) {
+    if (!p) return fail(c, GATGPU_EINVAL, std::string("null ") + name);
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(c, GATGPU_EINVAL, std::string(name) + " must be 4-byte aligned");
+    return check_device_array(c, p, name);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gatgpu_cache_attention_workspace(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgpu_cache_attention_io* io, uint64_t* bytes) {
+    if (!c) return fail(nullptr, GATGPU_EINVAL, "null context");
+    if (!bytes) return fail(c, GATGPU_EINVAL, "null output");
+    if (int r = check_cache(c, cache, false)) return r;
+    if (int r = check_sizes(c, cache, io)) return r;
+    const Workspace w = workspace_of(c, cache);
+    *bytes = w.part + w.stat + w.meta;
+    return GATGPU_OK;
+}
+
+int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgpu_cache_attention_io* io, void* ws, uint64_t bytes) {
+    if (!c) return fail(nullptr, GATGPU_EINVAL, "null context");
+    DeviceGuard on(c->device);
+    if (!on.ok) return fail(c, GATGPU_EDEVICE, "cannot select the context's device");
+    if (int r = check_cache(c, cache, true)) return r;
+    if (int r = check_sizes(c, cache, io)) return r;
+    if (!(io->scale > 0.0f) || !std::isfinite(io->scale)) return fail(c, GATGPU_EINVAL, "scale must be positive and finite");
+    if (!io->rows || !io->requests || !io->most) return GATGPU_OK;
+    if (int r = check_rows(c, cache, io, "q", io->q, io->q_stride)) return r;
+    if (int r = check_rows(c, cache, io, "out", io->out, io->out_stride)) return r;
+    if (int r = check_words(c, "q_begin", io->q_begin)) return r;
+    if (int r = check_words(c, "k_len", io->k_len)) return r;
+    if (io->blocks)
+        if (int r = check_words(c, "table", io->table)) return r;
+    if (io->lse)
+        if (int r = check_words(c, "lse", io->lse)) return r;
+    const Workspace w = workspace_of(c, cache);
+    const uint64_t need = w.part + w.stat + w.meta;
+    if (bytes < need) return fail(c, GATGPU_EINVAL, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
+    if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return fail(c, GATGPU_EINVAL, "workspace must be 16-byte aligned device memory");
+    if (int r = check_device_array(c, ws, "workspace")) return r;
+    CacheAttnArgs a;
+    a.c.rows = io->rows;
+    a.c.requests = io->requests;
+    a.c.most = io->most;
+    a.c.blocks = io->blocks;
+    a.c.pages = cache->pages;
+    while ((1u << a.c.page_log) < cache->page) ++a.c.page_log;
+    a.c.heads = uint32_t(io->heads);
+    a.c.kv_heads = uint32_t(cache->kv_heads);
+    a.c.group = uint32_t(io->heads / cache->kv_heads);
+    a.c.dim = uint32_t(cache->dim);
+    a.workers = cache_workers(c, cache->kv_heads);
+    a.least = 4;
+    a.scale = io->scale * 1.44269504088896341f;
+    a.ld = io->table_stride;
+    a.qs = io->q_stride;
+    a.os = io->out_stride;
+    a.q = io->q;
+    a.out = io->out;
+    a.lse = io->lse;
+    a.q_begin = io->q_begin;
+    a.k_len = io->k_len;
+    a.table = io->table;
+    a.k = cache->k;
+    a.v = cache->v;
+    a.k_scale = cache->k_scale;
+    a.v_scale = cache->v_scale;
+    a.part = static_cast<float*>(ws);
+    a.stat = reinterpret_cast<float*>(static_cast<char*>(ws) + w.part);
+    a.meta = reinterpret_cast<uint4*>(static_cast<char*>(ws) + w.part + w.stat);
+    const bool bf16 = io->precision == GATGPU_BF16, wide = cache->dim > 64;
+    HIPCHECK(c, bf16 ? (wide ? launch<uint16_t, 2>(a, c->stream) : launch<uint16_t, 1>(a, c->stream))
+                     : (wide ? launch<float, 2>(a, c->stream) : launch<float, 1>(a, c->stream)));
+    return GATGPU_OK;
+}
+
+}  // extern "C"

@@ -582,7 +582,11 @@ hipError_t launch_norm_backward(const NormArgs& a, bool bf16, uint32_t blocks, f
                       aligned(a.dx, a.dxs, size) && (!a.dsum || aligned(a.dsum, a.dss, size));
     const hipError_t e = bf16 ? backward<uint16_t>(a, wide, blocks, s) : backward<float>(a, wide, blocks, s);
     if (e != hipSuccess || !a.part) return e;
-    k_norm_sum<<<norm_grid((2 * uint64_t(a.width) + 31) / 32), 1024, 0, s>>>(a.part, blocks, a.width, dgamma, dbeta);
+    return launch_column_sums(a.part, blocks, a.width, dgamma, dbeta, s);
+}
+
+hipError_t launch_column_sums(const float* part, uint32_t blocks, uint32_t width, float* a, float* b, hipStream_t s) {
+    k_norm_sum<<<norm_grid((2 * uint64_t(width) + 31) / 32), 1024, 0, s>>>(part, blocks, width, a, b);
     return hipGetLastError();
 }
 

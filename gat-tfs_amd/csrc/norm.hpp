@@ -26,5 +26,7 @@ struct NormArgs {
 uint32_t norm_blocks(uint64_t rows, uint64_t width);
 hipError_t launch_norm_forward(const NormArgs& a, bool bf16, hipStream_t s);
 hipError_t launch_norm_backward(const NormArgs& a, bool bf16, uint32_t blocks, float* dgamma, float* dbeta, hipStream_t s);
+// a[c], b[c] (either may be null): sums over the blocks of part[block][2][width], in one fixed order.
+hipError_t launch_column_sums(const float* part, uint32_t blocks, uint32_t width, float* a, float* b, hipStream_t s);
 
 }  // namespace gatgpu

@@ -24,6 +24,8 @@ OPT_BLOCK_ROW_MIN_DEGREE, OPT_SPLIT_ROW_MIN_DEGREE, OPT_SPLIT_CHUNK_EDGES, OPT_K
 OPT_FUSE_NEXT_PROJECTION = 6
 MASK_FULL, MASK_PREFIX = 0, 1
 BIAS_NONE, BIAS_LINEAR, BIAS_TABLE = 0, 1, 2
+PAIRS_HALVES, PAIRS_NEIGHBOURS = 0, 1
+NO_PAGE = 0xFFFFFFFF  # GATGPU_NO_PAGE: in a block table no page, as a slot no token
 HIDDEN = 255  # GATGPU_HIDDEN: the distance of a pair that does not see each other
 
 STATIC_SCRATCH_BYTES = 64 << 20  # GATGPU_STATIC_SCRATCH_BYTES
@@ -41,7 +43,9 @@ EXPORTS = (
     "gatgpu_static_scratch_need", "gatgpu_attention_create", "gatgpu_attention_destroy",
     "gatgpu_attention_workspace", "gatgpu_attention_distances", "gatgpu_attention_forward",
     "gatgpu_attention_backward", "gatgpu_norm_forward", "gatgpu_norm_backward", "gatgpu_norm_workspace",
-    "gatgpu_set_norm",
+    "gatgpu_set_norm", "gatgpu_rotate_forward", "gatgpu_rotate_backward", "gatgpu_rotate_workspace",
+    "gatgpu_blocks_assign", "gatgpu_blocks_release", "gatgpu_blocks_workspace", "gatgpu_cache_append",
+    "gatgpu_cache_attention", "gatgpu_cache_attention_workspace",
 )
 
 
@@ -93,6 +97,45 @@ class NormIO(ctypes.Structure):
                 ("rstd", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_uint64),
                 ("dsum", ctypes.c_void_p), ("dsum_stride", ctypes.c_uint64), ("dx", ctypes.c_void_p),
                 ("dx_stride", ctypes.c_uint64), ("dgamma", ctypes.c_void_p), ("dbeta", ctypes.c_void_p)]
+
+
+def _fields(*groups):
+    return [(name, t) for t, names in groups for name in names.split()]
+
+
+class RotateIO(ctypes.Structure):
+    """gatgpu_rotate_io: shape and device arrays of norms and rotation of queries and keys."""
+    _fields_ = _fields((ctypes.c_int, "precision heads kv_heads dim norm rot pairs"), (ctypes.c_float, "eps"),
+                       (ctypes.c_uint64, "rows"), (ctypes.c_void_p, "q k"), (ctypes.c_uint64, "q_stride k_stride"),
+                       (ctypes.c_void_p, "gamma_q gamma_k position freq q_out k_out"),
+                       (ctypes.c_uint64, "q_out_stride k_out_stride"), (ctypes.c_void_p, "dq_out dk_out"),
+                       (ctypes.c_uint64, "dq_out_stride dk_out_stride"), (ctypes.c_void_p, "dq dk"),
+                       (ctypes.c_uint64, "dq_stride dk_stride"), (ctypes.c_void_p, "dgamma_q dgamma_k"))
+
+
+class BlocksIO(ctypes.Structure):
+    """gatgpu_blocks_io: block tables and slots of a step."""
+    _fields_ = _fields((ctypes.c_uint32, "requests page pages rows blocks"), (ctypes.c_uint64, "table_stride"),
+                       (ctypes.c_void_p, "cached fresh table free free_count free_left stored k_len q_begin slot position unserved"))
+
+
+class Cache(ctypes.Structure):
+    """gatgpu_cache: a paged 8-bit cache of keys and values."""
+    _fields_ = _fields((ctypes.c_uint32, "pages page"), (ctypes.c_int, "kv_heads dim"), (ctypes.c_void_p, "k v k_scale v_scale"))
+
+
+class AppendIO(ctypes.Structure):
+    """gatgpu_append_io: rows of new tokens and their slots."""
+    _fields_ = _fields((ctypes.c_int, "precision"), (ctypes.c_uint64, "rows"), (ctypes.c_void_p, "k v"),
+                       (ctypes.c_uint64, "k_stride v_stride"), (ctypes.c_void_p, "slot"))
+
+
+class CacheAttentionIO(ctypes.Structure):
+    """gatgpu_cache_attention_io: attention of a packed batch's rows over its requests' pages."""
+    _fields_ = _fields((ctypes.c_int, "precision heads"), (ctypes.c_float, "scale"), (ctypes.c_uint64, "rows"),
+                       (ctypes.c_uint32, "requests most blocks"), (ctypes.c_uint64, "table_stride"), (ctypes.c_void_p, "q"),
+                       (ctypes.c_uint64, "q_stride"), (ctypes.c_void_p, "q_begin k_len table out"),
+                       (ctypes.c_uint64, "out_stride"), (ctypes.c_void_p, "lse"))
 
 
 class GatGpuError(RuntimeError):
@@ -148,6 +191,16 @@ def load_library(path: os.PathLike | None = None):
     L.gatgpu_norm_backward.argtypes = [P, ctypes.POINTER(NormIO), P, u64]
     L.gatgpu_norm_workspace.argtypes = [P, u64, ctypes.c_uint32, ctypes.POINTER(u64)]
     L.gatgpu_set_norm.argtypes = [P, i32, P, P, ctypes.c_float]
+    ref = ctypes.POINTER
+    L.gatgpu_rotate_forward.argtypes = [P, ref(RotateIO)]
+    L.gatgpu_rotate_backward.argtypes = [P, ref(RotateIO), P, u64]
+    L.gatgpu_rotate_workspace.argtypes = [P, ref(RotateIO), ref(u64)]
+    L.gatgpu_blocks_assign.argtypes = [P, ref(BlocksIO), P, u64]
+    L.gatgpu_blocks_release.argtypes = [P, ref(BlocksIO), P, u64]
+    L.gatgpu_blocks_workspace.argtypes = [P, ref(BlocksIO), ref(u64)]
+    L.gatgpu_cache_append.argtypes = [P, ref(Cache), ref(AppendIO)]
+    L.gatgpu_cache_attention.argtypes = [P, ref(Cache), ref(CacheAttentionIO), P, u64]
+    L.gatgpu_cache_attention_workspace.argtypes = [P, ref(Cache), ref(CacheAttentionIO), ref(u64)]
     for name in EXPORTS:
         if name not in ("gatgpu_last_error", "gatgpu_stream"):
             getattr(L, name).restype = i32
@@ -350,6 +403,45 @@ class Context:
     def norm_workspace(self, rows, width):
         b = ctypes.c_uint64()
         self._check(self.lib.gatgpu_norm_workspace(self.h, rows, width, ctypes.byref(b)))
+        return b.value
+
+    # -- norms and rotation of queries and keys
+    def rotate_forward(self, io):
+        """gatgpu_rotate_forward of a RotateIO.  Enqueued on the context's stream."""
+        self._check(self.lib.gatgpu_rotate_forward(self.h, io))
+
+    def rotate_backward(self, io, workspace=None, workspace_bytes=0):
+        self._check(self.lib.gatgpu_rotate_backward(self.h, io, workspace, workspace_bytes))
+
+    def rotate_workspace(self, io):
+        b = ctypes.c_uint64()
+        self._check(self.lib.gatgpu_rotate_workspace(self.h, io, ctypes.byref(b)))
+        return b.value
+
+    # -- paged 8-bit cache
+    def blocks_assign(self, io, workspace=None, workspace_bytes=0):
+        """gatgpu_blocks_assign of a BlocksIO: tables, slots, positions and lengths of a step."""
+        self._check(self.lib.gatgpu_blocks_assign(self.h, io, workspace, workspace_bytes))
+
+    def blocks_release(self, io, workspace=None, workspace_bytes=0):
+        self._check(self.lib.gatgpu_blocks_release(self.h, io, workspace, workspace_bytes))
+
+    def blocks_workspace(self, io):
+        b = ctypes.c_uint64()
+        self._check(self.lib.gatgpu_blocks_workspace(self.h, io, ctypes.byref(b)))
+        return b.value
+
+    def cache_append(self, cache, io):
+        """gatgpu_cache_append of a Cache and an AppendIO."""
+        self._check(self.lib.gatgpu_cache_append(self.h, cache, io))
+
+    def cache_attention(self, cache, io, workspace=None, workspace_bytes=0):
+        """gatgpu_cache_attention of a Cache and a CacheAttentionIO."""
+        self._check(self.lib.gatgpu_cache_attention(self.h, cache, io, workspace, workspace_bytes))
+
+    def cache_attention_workspace(self, cache, io):
+        b = ctypes.c_uint64()
+        self._check(self.lib.gatgpu_cache_attention_workspace(self.h, cache, io, ctypes.byref(b)))
         return b.value
 
     def static_times(self):

@@ -461,6 +461,176 @@ int gatgpu_norm_workspace(gatgpu_ctx* ctx, uint64_t rows, uint32_t width, uint64
  * fixed-p operator has none.  set_layer(layer) drops it. */
 int gatgpu_set_norm(gatgpu_ctx* ctx, int layer, const float* gamma, const float* beta, float eps);
 
+/* ---- norms and rotation of queries and keys ----------------------------- */
+/* No counterpart in the reference.  In front of either attention, for each row and
+ * head:
+ *   n = x / sqrt(mean(x^2) + eps),  t = n gamma   (norm == 0: t = x)
+ *   y = t with the pairs (a, b) of its first `rot` columns turned by the angle
+ *       position freq[i]:  y_a = t_a cos - t_b sin,  y_b = t_b cos + t_a sin
+ * and the gradients of x and gamma.  GATGPU_PAIRS_HALVES: pair i is the columns
+ * (i, i + rot / 2); GATGPU_PAIRS_NEIGHBOURS: (2 i, 2 i + 1).  Angles are formed in
+ * 64 bits, so positions may be far; sums are FP32, y and the gradients are rounded
+ * once.  A NaN or infinity stays in its own row and head.
+ * Device arrays: rows of `heads` (kv_heads) vectors of dim elements side by side,
+ * strides in elements, 16-byte aligned like the bases.  q_out may be q, k_out k, and
+ * dq dq_out, dk dk_out (same strides); else what a call writes shares no memory with
+ * what it reads or else writes.  Stream, capture, device and workspace: as
+ * gatgpu_attention_forward. */
+enum { GATGPU_PAIRS_HALVES = 0, GATGPU_PAIRS_NEIGHBOURS = 1 };
+typedef struct gatgpu_rotate_io {
+    int precision;        /* of the rows: GATGPU_FP32 or GATGPU_BF16             */
+    int heads, kv_heads;  /* heads 1 to 1024, kv_heads 0 (no k) to 1024          */
+    int dim;              /* a multiple of 8, at most 256                        */
+    int norm;
+    int rot;              /* even, 0 (no rotation) to dim                        */
+    int pairs;
+    float eps;            /* >= 0                                                */
+    uint64_t rows;
+    const void *q, *k;
+    uint64_t q_stride, k_stride;
+    const float *gamma_q, *gamma_k; /* [dim], NULL: 1; not read if norm == 0     */
+    const uint32_t* position;       /* [rows]; not read if rot == 0              */
+    const double* freq;             /* [rot / 2] radians a position, 8-byte aligned */
+    void *q_out, *k_out;
+    uint64_t q_out_stride, k_out_stride;
+    const void *dq_out, *dk_out;    /* gradients of q_out and k_out              */
+    uint64_t dq_out_stride, dk_out_stride;
+    void *dq, *dk;                  /* gradients of q and k                      */
+    uint64_t dq_stride, dk_stride;
+    float *dgamma_q, *dgamma_k;     /* [dim], may be NULL; with norm only        */
+} gatgpu_rotate_io;
+
+/* Reads q, k, gamma, position and freq; writes q_out and k_out. */
+int gatgpu_rotate_forward(gatgpu_ctx* ctx, const gatgpu_rotate_io* io);
+/* Reads what the forward call read, dq_out and dk_out; writes dq, dk, dgamma_q and
+ * dgamma_k (sums in one fixed order). */
+int gatgpu_rotate_backward(gatgpu_ctx* ctx, const gatgpu_rotate_io* io, void* workspace, uint64_t bytes);
+/* Bytes of workspace of a backward call that gives dgamma_q or dgamma_k. */
+int gatgpu_rotate_workspace(gatgpu_ctx* ctx, const gatgpu_rotate_io* io, uint64_t* bytes);
+
+/* ---- paged cache ---------------------------------------------------------- */
+/* No counterpart in the reference.  A cache of keys and values in pages of `page`
+ * tokens, for requests that grow token by token.  A request's tokens lie in the
+ * blocks of its row of a block table: token t in page table[r][t / page] at offset
+ * t % page, its slot being page index * page + offset.  A step over a packed batch
+ * (request r has rows q_begin[r] to q_begin[r + 1]) is
+ *   gatgpu_blocks_assign     pages, slots, positions and lengths from the lengths
+ *   gatgpu_rotate_forward    queries and keys (position from the call before)
+ *   gatgpu_cache_append      keys and values into their slots
+ *   gatgpu_cache_attention   the rows' attention over their requests' pages
+ * with every length in device memory, so that one captured graph serves steps of any
+ * lengths (rows behind the last request's are left alone).  Stream, capture, device
+ * and workspace: as gatgpu_attention_forward.  Whatever the arrays of lengths,
+ * slots and pages hold, nothing outside the given arrays is read or written. */
+#define GATGPU_NO_PAGE 0xffffffffu /* in a table: no page; as a slot: no token */
+
+/* Block tables.  All arrays but the counts below are uint32 on the device.
+ * Assign: request r has cached[r] tokens and gets fresh[r] more, for which it takes
+ *   pages from the end of the free list, in the order of requests and blocks: the
+ *   k-th page taken is free[free_count - 1 - k].  Request r is served if
+ *   cached + fresh <= blocks * page, if the pages of requests 0 to r together are there
+ *   (or r needs none; requests too long for the table count none), and if its rows end
+ *   within `rows`.  Writes
+ *     table     the taken pages, in the places of their blocks (nothing else)
+ *     stored    tokens in the cache after the step: cached + fresh, of a request that is
+ *               not served cached.  May be cached
+ *     k_len     cached + fresh, of a request that is not served 0
+ *     q_begin   [requests + 1] sums of fresh, beginning with 0 (2^32 - 1 where they pass that)
+ *     slot      of each row; GATGPU_NO_PAGE behind the last request's rows, in those of a
+ *               request that is not served, and where its table has no page
+ *     position  of each row, 0 in the same places but the last
+ *     free_left pages left in the list.  May be free_count
+ *     unserved  requests that are not served
+ * Release: the pages of the blocks that hold cached[r] tokens are put behind the
+ *   list's free_count pages, in the order of requests and blocks (entries of `pages` or
+ *   more are no pages); free_left: what the list holds then, at most `pages`.
+ * A page belongs to one request, and to it once; equal inputs give equal lists. */
+typedef struct gatgpu_blocks_io {
+    uint32_t requests;     /* at most 2^20                                        */
+    uint32_t page;         /* tokens: 16, 32, 64, 128 or 256                      */
+    uint32_t pages;        /* of the cache, and of the free list; pages * page < 2^32 */
+    uint32_t rows;         /* of slot and position; release: not read             */
+    uint32_t blocks;       /* of a table row; blocks * page < 2^32                */
+    uint64_t table_stride; /* entries from row to row, at least blocks            */
+    const uint32_t *cached, *fresh; /* [requests]; release: cached                */
+    uint32_t *table, *free;
+    const uint32_t* free_count;     /* [1]                                        */
+    uint32_t* free_left;            /* [1]                                        */
+    uint32_t *stored, *k_len, *q_begin, *slot, *position, *unserved; /* release: not written */
+} gatgpu_blocks_io;
+int gatgpu_blocks_assign(gatgpu_ctx* ctx, const gatgpu_blocks_io* io, void* workspace, uint64_t bytes);
+int gatgpu_blocks_release(gatgpu_ctx* ctx, const gatgpu_blocks_io* io, void* workspace, uint64_t bytes);
+/* Bytes of workspace of either call. */
+int gatgpu_blocks_workspace(gatgpu_ctx* ctx, const gatgpu_blocks_io* io, uint64_t* bytes);
+
+/* The cache's device arrays, 16-byte aligned, for the caller to allocate.  Elements
+ * are e4m3 bytes (8-bit floats of 3 mantissa bits, at most 448) times the scale of
+ * their page and head, a power of two from 2^-64 to 2^64. */
+typedef struct gatgpu_cache {
+    uint32_t pages;  /* at least 1; pages * page < 2^32                           */
+    uint32_t page;   /* tokens: 16, 32, 64, 128 or 256                            */
+    int kv_heads;    /* 1 to 64                                                   */
+    int dim;         /* a multiple of 16, at most 128                             */
+    uint8_t* k;      /* [pages][kv_heads][page][dim]                              */
+    uint8_t* v;      /* [pages][kv_heads][dim][page]                              */
+    float *k_scale, *v_scale; /* [pages][kv_heads]                                */
+} gatgpu_cache;
+
+/* Keys and values of new tokens into their slots.  The tokens of a page are
+ * neighbouring rows of one call, in the order of their slots, without gaps.  Those
+ * before the first of them in the page keep their values, those behind the last are
+ * no tokens any more.  The page's scale becomes the smallest power of two that holds
+ * the largest magnitude m of its new tokens (m <= 448 scale), but no less than it was
+ * if tokens stay; where it grows, their bytes are rounded again.  Values round to the
+ * nearest e4m3 value, ties to even, beyond 448 * 2^64 to that; NaN and infinities become NaN
+ * and leave the scale alone.  A slot of pages * page or more is no token: its row is
+ * not read. */
+typedef struct gatgpu_append_io {
+    int precision;        /* of the rows: GATGPU_FP32 or GATGPU_BF16             */
+    uint64_t rows;        /* < 2^27                                              */
+    const void *k, *v;    /* rows of kv_heads vectors, 16-byte aligned           */
+    uint64_t k_stride, v_stride;
+    const uint32_t* slot; /* [rows]                                              */
+} gatgpu_append_io;
+int gatgpu_cache_append(gatgpu_ctx* ctx, const gatgpu_cache* cache, const gatgpu_append_io* io);
+
+/* Attention of the rows over their requests' pages.  Row i of request r, of q_len =
+ * q_begin[r + 1] - q_begin[r] rows, stands at position k_len[r] - q_len + i and sees
+ * the tokens up to it that have a page (a table entry of `pages` or more hides its
+ * block's); heads / kv_heads query heads share a key/value head:
+ *   s = scale q.k,  out = sum p v,  p = softmax of s,  lse = log sum exp s
+ * A row that sees no token of finite score gets out = 0 and lse = -infinity.  What is
+ * not seen adds nothing, whatever its bytes hold; a NaN in a seen value reaches that
+ * row's output.  Rows of no request are neither read nor written; of a request's rows
+ * those beyond the first `most` are not computed.  k_len beyond blocks * page counts
+ * as that, q_begin beyond rows as rows.
+ * GATGPU_BF16: q and out bf16; GATGPU_FP32: both FP32, products of FP32's precision.
+ * Scores, softmax state and sums are FP32.  Sums run in one fixed order: equal inputs
+ * give equal bits. */
+typedef struct gatgpu_cache_attention_io {
+    int precision;
+    int heads;             /* a multiple of kv_heads, at most 64                 */
+    float scale;           /* > 0                                                */
+    uint64_t rows;         /* of q, out and lse: < 2^31 / heads                  */
+    uint32_t requests;     /* at most 2^20                                       */
+    uint32_t most;         /* rows of a request                                  */
+    uint32_t blocks;       /* of a table row; blocks * page < 2^32               */
+    uint64_t table_stride; /* entries from row to row, at least blocks           */
+    const void* q;
+    uint64_t q_stride;
+    const uint32_t* q_begin; /* [requests + 1], not decreasing                   */
+    const uint32_t* k_len;   /* [requests]                                       */
+    const uint32_t* table;
+    void* out;
+    uint64_t out_stride;
+    float* lse;            /* [row][heads], may be NULL                          */
+} gatgpu_cache_attention_io;
+int gatgpu_cache_attention(gatgpu_ctx* ctx, const gatgpu_cache* cache, const gatgpu_cache_attention_io* io,
+                           void* workspace, uint64_t bytes);
+/* Bytes of workspace for a call of these sizes (arrays need not be set). */
+int gatgpu_cache_attention_workspace(gatgpu_ctx* ctx, const gatgpu_cache* cache, const gatgpu_cache_attention_io* io,
+                                     uint64_t* bytes);
+
 /* ---- misc ------------------------------------------------------------ */
 int gatgpu_set_option(gatgpu_ctx* ctx, int key, int64_t value);
 /* Blocks until all work on the context's stream is done. */
