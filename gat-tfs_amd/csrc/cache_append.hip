@@ -5,7 +5,7 @@
 //
 // Bound by bytes: rows read once (two or four bytes a value), one byte a value written.  A block takes the new tokens of
 // one page, key/value head and side (keys or values), reads them into registers, finds their largest magnitude and
-// rounds them from there (what registers do not hold, of pages of 256 tokens, is read again).  Values are turned in LDS,
+// rounds them from there (what registers do not hold, beyond 16 KB, is read again).  Values are turned in LDS,
 // since a page holds them by column: the attention's second product then takes its operands straight from memory.
 #include <algorithm>
 #include <string>
@@ -15,7 +15,7 @@
 namespace gatgpu {
 namespace {
 
-constexpr int kThreads = 256, kHeld = 8;  // 16-byte chunks of rows that a thread keeps
+constexpr int kThreads = 256;
 constexpr int kMaxPage = 256, kMaxDim = 128, kTurnPad = 4;
 
 struct AppendArgs {
@@ -30,12 +30,8 @@ struct AppendArgs {
     float* scale[2] = {};
 };
 
-// Magnitude of a finite value as bits, which order as the values do; 0 of NaN and infinities.
-__device__ inline uint32_t magnitude(uint32_t u) {
-    u &= 0x7fffffffu;
-    return u >= 0x7f800000u ? 0 : u;
-}
-// The least exponent e with m <= 448 2^e = 1.75 2^(8 + e), in the scales' range.
+constexpr uint32_t kInfinity = 0x7f800000u;
+// The least exponent e with m <= 448 2^e = 1.75 2^(8 + e), in the scales' range; m: bits of a finite magnitude.
 __device__ inline int exponent_for(uint32_t m) {
     const int e = int(m >> 23) - 127 - 8 + ((m & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < kLeastScale ? kLeastScale : e > kMostScale ? kMostScale : e;
@@ -46,12 +42,12 @@ __device__ inline uint32_t round4(const uint32_t (&u)[4], float by) {
     uint32_t bad = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        x[i] = fminf(fmaxf(__uint_as_float(u[i]) * by, -448.0f), 448.0f);
-        if ((u[i] & 0x7f800000u) == 0x7f800000u) bad |= 0x7fu << (8 * i);
+        x[i] = __builtin_amdgcn_fmed3f(__uint_as_float(u[i]) * by, -448.0f, 448.0f);
+        if ((u[i] & kInfinity) == kInfinity) bad |= 0x7fu << (8 * i);
     }
     uint32_t w = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false));
     w = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], int(w), true));
-    return bad ? w | bad : w;
+    return w | bad;
 }
 // Four bytes of a page whose scale grows.
 __device__ inline uint32_t round_again(uint32_t w, float by) {
@@ -62,43 +58,84 @@ __device__ inline uint32_t round_again(uint32_t w, float by) {
     u[3] = __float_as_uint(__builtin_amdgcn_cvt_f32_fp8(int(w), 3));
     return round4(u, by);
 }
-// 16 bytes of a row as FP32 bits.
-template <class T>
-struct Bits {
-    uint32_t u[16 / sizeof(T)];
+
+// 16 bytes of four neighbouring tokens' rows, zeros behind the last token.
+struct Quad {
+    uint4 row[4];
 };
 template <class T>
-__device__ inline Bits<T> widen(uint4 w) {
+__device__ inline void widen(uint4 w, uint32_t (&u)[16 / sizeof(T)]) {
     const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-    Bits<T> b;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (sizeof(T) == 2) {
-            b.u[2 * i] = v[i] << 16;
-            b.u[2 * i + 1] = v[i] & 0xffff0000u;
+            u[2 * i] = v[i] << 16;
+            u[2 * i + 1] = v[i] & 0xffff0000u;
         } else {
-            b.u[i] = v[i];
+            u[i] = v[i];
         }
     }
-    return b;
+}
+// The largest magnitude among a quad's values, as FP32 bits, which order as magnitudes do; NaN and infinities beyond kInfinity.
+template <class T>
+__device__ inline uint32_t largest(const Quad& q) {
+    uint32_t top = 0;
+    if constexpr (sizeof(T) == 2) {
+        typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+        u16x2_t m = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, (&q.row[i].x)[k] & 0x7fff7fffu));
+        top = uint32_t(max(m[0], m[1])) << 16;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = max(top, (&q.row[i].x)[k] & 0x7fffffffu);
+    }
+    return top;
+}
+// The same among the finite ones.
+template <class T>
+__device__ inline uint32_t largest_finite(const Quad& q) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t u[16 / sizeof(T)];
+        widen<T>(q.row[i], u);
+#pragma unroll
+        for (int k = 0; k < int(16 / sizeof(T)); ++k) top = max(top, (u[k] & kInfinity) == kInfinity ? 0u : u[k] & 0x7fffffffu);
+    }
+    return top;
+}
+__device__ inline uint32_t block_max(uint32_t x, uint32_t* words) {
+#pragma unroll
+    for (int d = kWave / 2; d; d /= 2) x = max(x, uint32_t(__shfl_xor(int(x), d)));
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) words[threadIdx.x / kWave] = x;
+    __syncthreads();
+    return max(max(words[0], words[1]), max(words[2], words[3]));
 }
 
+// A thread takes 16 bytes of four neighbouring tokens: a row's bytes lie in neighbouring lanes, and four tokens' values of a
+// column make one word of the page's column.
 template <class T>
-__global__ __launch_bounds__(kThreads) void k_cache_append(const AppendArgs a) {
-    constexpr int N = 16 / int(sizeof(T));  // values a chunk
-    extern __shared__ uint8_t turn[];       // values: [dim][page + kTurnPad]
+__global__ __launch_bounds__(kThreads, 4) void k_cache_append(const AppendArgs a) {
+    constexpr int N = 16 / int(sizeof(T));  // values of 16 bytes
+    extern __shared__ uint32_t turn[];      // values: [dim][page + kTurnPad] bytes
     __shared__ uint32_t s_word[kThreads / kWave];
     __shared__ uint64_t s_starts;
     const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
     const int head = int(blockIdx.y), side = int(blockIdx.z);
     const uint64_t first = uint64_t(blockIdx.x) * a.chunk;
-    const uint32_t page = a.page;
+    const uint32_t page = a.page, turn_row = (page + kTurnPad) / 4, per = uint32_t(a.dim) / N;  // words, 16-byte pieces a token
     if (wave == 0) {
         const uint64_t row = first + uint64_t(lane);
         bool start = false;
         if (uint32_t(lane) < a.chunk && row < a.rows) {
-            const uint32_t s = a.slot[row];
-            start = s < a.slots && (row == 0 || s % page == 0 || a.slot[row - 1] + 1 != s);
+            const uint32_t s = a.slot[row], before = row ? a.slot[row - 1] : GATGPU_NO_PAGE;
+            start = s < a.slots && (row == 0 || s % page == 0 || before + 1 != s);
         }
         const uint64_t some = __ballot(start);
         if (lane == 0) s_starts = some;
@@ -107,9 +144,12 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(const AppendArgs a) {
     for (uint64_t starts = s_starts; starts; starts &= starts - 1) {
         const uint64_t row = first + uint64_t(__builtin_ctzll(starts));
         const uint32_t slot = a.slot[row], off = slot % page;
+        const uint64_t place = uint64_t(slot / page) * uint64_t(a.kv_heads) + uint64_t(head);
+        const float scale = a.scale[side][place];
         // Tokens of this page: rows as long as their slots go on.
         const bool more = row + uint64_t(tid) < a.rows && off + uint32_t(tid) < page && a.slot[row + uint64_t(tid)] == slot + uint32_t(tid);
         const uint64_t on = __ballot(more);
+        __syncthreads();
         if (lane == 0) s_word[wave] = ~on ? uint32_t(__builtin_ctzll(~on)) : uint32_t(kWave);
         __syncthreads();
         uint32_t tokens = 0;
@@ -117,33 +157,29 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(const AppendArgs a) {
             tokens += s_word[w];
             if (s_word[w] < uint32_t(kWave)) break;
         }
-        __syncthreads();
-        const uint32_t per = uint32_t(a.dim) / N, chunks = tokens * per;  // chunks a token, and in all
+        const uint32_t quads = (tokens + 3) / 4 * per;
         const T* const x = static_cast<const T*>(a.x[side]) + row * a.xs[side] + uint64_t(head) * uint64_t(a.dim);
-        const auto load = [&](uint32_t i) { return *reinterpret_cast<const uint4*>(x + uint64_t(i / per) * a.xs[side] + uint64_t(i % per) * N); };
-        uint4 held[kHeld];
-        uint32_t top = 0;
-        const auto see = [&](uint4 w) {
-            const Bits<T> b = widen<T>(w);
+        const auto load = [&](uint32_t i) {
+            Quad q;
+            const uint32_t t = i / per * 4;
+            const T* const p = x + uint64_t(t) * a.xs[side] + uint64_t(i % per) * N;
 #pragma unroll
-            for (int j = 0; j < N; ++j) top = max(top, magnitude(b.u[j]));
+            for (uint32_t k = 0; k < 4; ++k)
+                q.row[k] = t + k < tokens ? *reinterpret_cast<const uint4*>(p + k * a.xs[side]) : make_uint4(0, 0, 0, 0);
+            return q;
         };
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            const uint32_t at = uint32_t(tid + i * kThreads);
-            held[i] = at < chunks ? load(at) : make_uint4(0, 0, 0, 0);
+        Quad held{};  // the thread's first one; more than 256 of them are read again
+        if (uint32_t(tid) < quads) held = load(uint32_t(tid));
+        uint32_t top = largest<T>(held);
+        for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) top = max(top, largest<T>(load(i)));
+        top = block_max(top, s_word);
+        if (top >= kInfinity) {  // NaN and infinities leave the scale alone
+            top = largest_finite<T>(held);
+            for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) top = max(top, largest_finite<T>(load(i)));
+            top = block_max(top, s_word);
         }
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) see(held[i]);
-        for (uint32_t at = uint32_t(tid + kHeld * kThreads); at < chunks; at += kThreads) see(load(at));
-#pragma unroll
-        for (int d = kWave / 2; d; d /= 2) top = max(top, uint32_t(__shfl_xor(int(top), d)));
-        if (lane == 0) s_word[wave] = top;
-        __syncthreads();
-        top = max(max(s_word[0], s_word[1]), max(s_word[2], s_word[3]));
-        const uint64_t place = uint64_t(slot / page) * uint64_t(a.kv_heads) + uint64_t(head);
         uint8_t* const to = a.cache[side] + place * page * uint64_t(a.dim);
-        const int had = off ? scale_exponent(a.scale[side][place]) : kLeastScale;
+        const int had = off ? scale_exponent(scale) : kLeastScale;
         const int e = max(exponent_for(top), had);
         if (off && e > had) {  // the page's scale grows under the tokens that stay
             const float by = power_of_two(had - e < -126 ? -126 : had - e);
@@ -163,42 +199,48 @@ __global__ __launch_bounds__(kThreads) void k_cache_append(const AppendArgs a) {
         __syncthreads();  // (the scale has been read, and the words of tokens that stay are written)
         if (tid == 0) a.scale[side][place] = power_of_two(e);
         const float by = power_of_two(-e);
-        const auto put = [&](uint32_t at, uint4 w) {
-            const Bits<T> b = widen<T>(w);
-            const uint32_t token = at / per, col = at % per * N;
-            uint32_t q[N / 4];
+        const auto put = [&](uint32_t i, const Quad& q) {
+            const uint32_t t = i / per * 4, col = i % per * N;
+            uint32_t u[4][N];
 #pragma unroll
-            for (int i = 0; i < N / 4; ++i) {
-                const uint32_t u[4] = {b.u[4 * i], b.u[4 * i + 1], b.u[4 * i + 2], b.u[4 * i + 3]};
-                q[i] = round4(u, by);
-            }
+            for (int k = 0; k < 4; ++k) widen<T>(q.row[k], u[k]);
             if (side == 0) {
-                uint8_t* const p = to + uint64_t(off + token) * uint64_t(a.dim) + col;
-                if constexpr (N == 8) *reinterpret_cast<uint2*>(p) = make_uint2(q[0], q[1]);
-                else *reinterpret_cast<uint32_t*>(p) = q[0];
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    if (t + k >= tokens) break;
+                    uint32_t* const p = reinterpret_cast<uint32_t*>(to + uint64_t(off + t + k) * uint64_t(a.dim) + col);
+                    uint32_t w[N / 4];
+#pragma unroll
+                    for (int c = 0; c < N / 4; ++c) {
+                        const uint32_t v[4] = {u[k][4 * c], u[k][4 * c + 1], u[k][4 * c + 2], u[k][4 * c + 3]};
+                        w[c] = round4(v, by);
+                    }
+                    if constexpr (N == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+                    else *p = w[0];
+                }
             } else {
 #pragma unroll
-                for (int j = 0; j < N; ++j) turn[(col + uint32_t(j)) * (page + kTurnPad) + token] = uint8_t(q[j / 4] >> (8 * (j % 4)));
+                for (int c = 0; c < N; ++c) {
+                    const uint32_t v[4] = {u[0][c], u[1][c], u[2][c], u[3][c]};
+                    turn[(col + uint32_t(c)) * turn_row + t / 4] = round4(v, by);
+                }
             }
         };
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            const uint32_t at = uint32_t(tid + i * kThreads);
-            if (at < chunks) put(at, held[i]);
-        }
-        for (uint32_t at = uint32_t(tid + kHeld * kThreads); at < chunks; at += kThreads) put(at, load(at));
+        if (uint32_t(tid) < quads) put(uint32_t(tid), held);
+        for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) put(i, load(i));
         __syncthreads();
         if (side == 0) continue;
         if (tokens == page) {
-            for (uint32_t i = uint32_t(tid); i < page / 16 * uint32_t(a.dim); i += kThreads) {
-                const uint32_t col = i / (page / 16), at = i % (page / 16) * 16;
-                const uint32_t* const w = reinterpret_cast<const uint32_t*>(turn + col * (page + kTurnPad) + at);
-                *reinterpret_cast<uint4*>(to + uint64_t(col) * page + at) = make_uint4(w[0], w[1], w[2], w[3]);
+            const uint32_t pieces = page / 16;
+            for (uint32_t i = uint32_t(tid); i < pieces * uint32_t(a.dim); i += kThreads) {
+                const uint32_t* const w = turn + i / pieces * turn_row + i % pieces * 4;
+                *reinterpret_cast<uint4*>(to + uint64_t(i) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         } else {
+            const uint8_t* const bytes = reinterpret_cast<const uint8_t*>(turn);
             for (uint32_t i = uint32_t(tid); i < tokens * uint32_t(a.dim); i += kThreads) {
                 const uint32_t col = i / tokens, at = i % tokens;
-                to[uint64_t(col) * page + off + at] = turn[col * (page + kTurnPad) + at];
+                to[uint64_t(col) * page + off + at] = bytes[col * turn_row * 4 + at];
             }
         }
         __syncthreads();

@@ -45,8 +45,7 @@ struct Chunk {
     float x[N];
 };
 template <class T>
-__device__ inline Chunk<T> load_chunk(const T* p) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
+__device__ inline Chunk<T> widen(uint4 w) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
     Chunk<T> c;
 #pragma unroll
@@ -59,6 +58,10 @@ __device__ inline Chunk<T> load_chunk(const T* p) {
         }
     }
     return c;
+}
+template <class T>
+__device__ inline uint4 load16(const T* p) {
+    return *reinterpret_cast<const uint4*>(p);
 }
 // Bits of a NaN may change, nothing else does beside the rounding to nearest even.
 template <class T>
@@ -73,148 +76,264 @@ __device__ inline float load_one(const T* p) {
     if constexpr (sizeof(T) == 2) return bf16_widen(*p);
     else return *p;
 }
+template <int CTRL>
+__device__ inline float add_dpp(float x) {
+    return x + __uint_as_float(uint32_t(__builtin_amdgcn_mov_dpp(int(__float_as_uint(x)), CTRL, 0xf, 0xf, true)));
+}
+// Sum over groups of TPV lanes, in each of them: within quads by quad permutes, then of mirrored halves of 8 and 16 lanes
+// (whose lanes are equal by then), then as the row halves swap.
 template <int TPV>
 __device__ inline float group_sum(float x) {
-#pragma unroll
-    for (int d = TPV / 2; d; d /= 2) x += __shfl_xor(x, d);
+    if (TPV > 1) x = add_dpp<0xb1>(x);
+    if (TPV > 2) x = add_dpp<0x4e>(x);
+    if (TPV > 4) x = add_dpp<0x141>(x);
+    if (TPV > 8) x = add_dpp<0x140>(x);
+    if (TPV > 16) x = xor16_add(x);
+    if (TPV > 32) x = xor32_add(x);
     return x;
 }
+// 1 / sqrt(x): the hardware's, and one step of Newton's method on it.
+__device__ inline float inverse_root(float x) {
+    const float r = __builtin_amdgcn_rsqf(x), h = 0.5f * x * r;
+    return x < INFINITY ? fmaf(r, fmaf(-h, r, 0.5f), r) : r;
+}
 
-// The other columns of a chunk's pairs.
+// A vector's place.
 template <class T>
-__device__ inline Chunk<T> load_partners(const RotateArgs& a, const T* row, int col, const Chunk<T>& own) {
-    constexpr int N = Chunk<T>::N;
-    Chunk<T> p = own;
-    if (!a.half) return p;
-    if (a.neighbours) {
+struct Vector {
+    const T* x;   // what is rotated: the row, or backward the gradient's
+    const T* n;   // backward: the row itself
+    T* to;
+    int which;    // 0 queries, 1 keys
+};
+template <class T, bool BACK>
+__device__ inline Vector<T> vector_at(const RotateArgs& a, uint64_t row, int v) {
+    Vector<T> p;
+    p.which = v >= a.heads;
+    const uint64_t at = uint64_t(p.which ? v - a.heads : v) * uint64_t(a.dim);
+    const T* const x = static_cast<const T*>(a.x[p.which]) + row * a.xs[p.which] + at;
+    p.to = static_cast<T*>(a.y[p.which]) + row * a.ys[p.which] + at;
+    p.n = x;
+    p.x = BACK ? static_cast<const T*>(a.dy[p.which]) + row * a.dys[p.which] + at : x;
+    return p;
+}
+// A lane's 16 bytes of a vector as they come: its columns, those of its pairs' other ones (0 where there are none or they
+// stand in the same chunk), and backward the row's.
+struct Raw {
+    uint4 own, other, n;
+};
+// The other columns of a chunk: kSame: in the chunk itself; kChunk: half a rotation away, a chunk for a chunk; both where
+// a chunk turns as a whole or not at all.  kAny: any.
+enum { kSame = 0, kChunk = 1, kAny = 2 };
+template <class T, bool BACK, int PAIRS>
+__device__ inline Raw fetch(const RotateArgs& a, const Vector<T>& p, int col) {
+    Raw r;
+    r.own = load16(p.x + col);
+    r.other = r.n = make_uint4(0, 0, 0, 0);
+    if (PAIRS == kChunk && col < 2 * a.half) r.other = load16(p.x + (col < a.half ? col + a.half : col - a.half));
+    if (BACK && a.norm) r.n = load16(p.n + col);
+    return r;
+}
+// The other column of column i, or i.
+__device__ inline int partner_of(const RotateArgs& a, int i) {
+    if (i >= 2 * a.half) return i;
+    return a.neighbours ? i ^ 1 : i < a.half ? i + a.half : i - a.half;
+}
+template <class T, int PAIRS>
+__device__ inline Chunk<T> partners(const RotateArgs& a, const Vector<T>& p, const Chunk<T>& own, uint4 other, int col) {
+    if (PAIRS == kChunk) return widen<T>(other);
+    Chunk<T> c;
 #pragma unroll
-        for (int j = 0; j < N; ++j) p.x[j] = own.x[j ^ 1];
-    } else if (a.half % N == 0) {
-        if (col < 2 * a.half) p = load_chunk(row + (col < a.half ? col + a.half : col - a.half));
-    } else {
+    for (int j = 0; j < Chunk<T>::N; ++j) {
+        if (PAIRS == kSame) c.x[j] = col < 2 * a.half ? own.x[j ^ 1] : 0.0f;
+        else c.x[j] = col + j < 2 * a.half ? load_one(p.x + partner_of(a, col + j)) : 0.0f;
+    }
+    return c;
+}
+// A lane's factors of its columns and of their pairs' other ones (forward with gamma in them), and gamma.
+template <class T>
+struct Factors {
+    Chunk<T> own, other, gamma;
+};
+// gamma: of the vector's kind, turn: of its row, both in LDS.
+template <class T, bool BACK, int PAIRS>
+__device__ inline void load_factors(const RotateArgs& a, const float* gamma, const float2* turn, int col, Factors<T>& f) {
+    constexpr int N = Chunk<T>::N;
+    float c[N], s[N], theirs[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        f.gamma.x[j] = theirs[j] = gamma[col + j];
+        c[j] = 1.0f;
+        s[j] = 0.0f;
+    }
+    if (PAIRS == kAny) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int i = col + j;
-            if (i < 2 * a.half) p.x[j] = load_one(row + (i < a.half ? i + a.half : i - a.half));
+            if (i < 2 * a.half) {
+                const bool second = a.neighbours ? i & 1 : i >= a.half;
+                const float2 w = turn[a.neighbours ? i / 2 : second ? i - a.half : i];
+                c[j] = w.x;
+                s[j] = second != BACK ? w.y : -w.y;
+                theirs[j] = gamma[partner_of(a, i)];
+            }
+        }
+    } else if (col < 2 * a.half) {
+        const bool late = PAIRS == kChunk && col >= a.half;
+        const float2* const at = turn + (PAIRS == kSame ? col / 2 : late ? col - a.half : col);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float2 w = at[PAIRS == kSame ? j / 2 : j];
+            c[j] = w.x;
+            s[j] = (PAIRS == kSame ? bool(j & 1) : late) != BACK ? w.y : -w.y;
+            if (!BACK) theirs[j] = PAIRS == kSame ? f.gamma.x[j ^ 1] : gamma[(late ? col - a.half : col + a.half) + j];
         }
     }
-    return p;
-}
-template <class T>
-__device__ inline void load_gamma(const RotateArgs& a, const float* gamma, int col, bool partners, Chunk<T>& own, Chunk<T>& other) {
-    constexpr int N = Chunk<T>::N;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        own.x[j] = gamma ? gamma[col + j] : 1.0f;
-        other.x[j] = 1.0f;
-        if (partners && gamma) {
-            const int i = col + j, p = a.neighbours ? i ^ 1 : i < a.half ? i + a.half : i - a.half;
-            other.x[j] = i < 2 * a.half ? gamma[p] : 0.0f;
-        }
+        f.own.x[j] = BACK ? c[j] : c[j] * f.gamma.x[j];
+        f.other.x[j] = BACK ? s[j] : s[j] * theirs[j];
     }
 }
 
-// T rows of the block's turn at a time; group g of TPV lanes takes heads g % gpt, g % gpt + gpt, ... of row g / gpt.
-template <class T, int TPV, bool BACK>
-__global__ __launch_bounds__(kBlock) void k_rotate(const RotateArgs a) {
+// Rows at once: a group of TPV lanes takes heads g % gpt, g % gpt + gpt, ... of row g / gpt, each vector's bytes requested
+// while the one before is worked on, across the rows that the block takes in turn; the next rows' angles are formed
+// meanwhile, in the other of two buffers.
+template <class T, int TPV, bool BACK, int PAIRS>
+__global__ __launch_bounds__(kBlock, BACK ? 3 : 4) void k_rotate(const RotateArgs a) {
     constexpr int N = Chunk<T>::N, G = kBlock / TPV;
+    constexpr int ANGLES = (G * TPV * N / 2 + kBlock - 1) / kBlock;  // of a thread, at most
     extern __shared__ float lds[];
-    float2* const turn = reinterpret_cast<float2*>(lds);  // [rows at once][half]
-    const int tid = int(threadIdx.x), g = tid / TPV, col = tid % TPV * N;
-    const int at_once = G / a.gpt, vectors = a.heads + a.kv_heads;
-    const bool there = col < a.dim;
+    float* const gamma = lds;                                         // [2][dim]
+    float2* const turn = reinterpret_cast<float2*>(lds + 2 * a.dim);  // [2][rows at once][half]
+    const int tid = int(threadIdx.x), g = tid / TPV, col = tid % TPV * N, mine = g / a.gpt, start = g % a.gpt;
+    const int at_once = G / a.gpt, vectors = a.heads + a.kv_heads, angles = at_once * a.half;
+    const uint64_t stride = uint64_t(gridDim.x) * uint64_t(at_once);
+    const bool there = col < a.dim, any = start < vectors;
+    const float per = 1.0f / float(a.dim);
+    const int step = a.gpt * a.dim;
+    uint64_t first = uint64_t(blockIdx.x) * uint64_t(at_once);
+
+    double freq[ANGLES];  // turns a position
+    uint32_t position[ANGLES];
+    const auto load_positions = [&](uint64_t from) {
+#pragma unroll
+        for (int k = 0; k < ANGLES; ++k) {
+            const int i = tid + k * kBlock;
+            position[k] = 0;
+            if (i < angles && from + uint64_t(i / a.half) < a.rows) position[k] = a.position[from + uint64_t(i / a.half)];
+        }
+    };
+    const auto form_angles = [&](float2* to) {
+#pragma unroll
+        for (int k = 0; k < ANGLES; ++k) {
+            const int i = tid + k * kBlock;
+            if (i >= angles) break;
+            const double t = double(position[k]) * freq[k], part = t - rint(t);
+            // Of a turn: as an FP32 number, and what that lacks, by which the sine and cosine turn on.
+            const float f = float(part), less = float(part - double(f)) * 6.28318530717958648f;
+            float s, c;
+            sincospif(2.0f * f, &s, &c);
+            to[i] = make_float2(fmaf(-less, s, c), fmaf(less, c, s));
+        }
+    };
+    const auto fetch_first = [&](uint64_t row, Vector<T>& at) {
+        Raw r{};
+        if (any && row < a.rows) {
+            at = vector_at<T, BACK>(a, row, start);
+            if (there) r = fetch<T, BACK, PAIRS>(a, at, col);
+        }
+        return r;
+    };
+    for (int i = tid; i < 2 * a.dim; i += kBlock) {
+        const float* const from = a.norm ? a.gamma[i >= a.dim] : nullptr;
+        gamma[i] = from ? from[i >= a.dim ? i - a.dim : i] : 1.0f;
+    }
+    Vector<T> now{};
+    Raw raw = fetch_first(first + uint64_t(mine), now);
+    if (a.half) {
+        load_positions(first);
+#pragma unroll
+        for (int k = 0; k < ANGLES; ++k) {
+            const int i = tid + k * kBlock;
+            freq[k] = i < angles ? a.freq[i % a.half] * 0.15915494309189533577 : 0.0;  // 1 / (2 pi)
+        }
+        form_angles(turn);
+        load_positions(first + stride);
+    } else {
+        __syncthreads();
+    }
     Chunk<T> sum[2];
 #pragma unroll
     for (int j = 0; j < N; ++j) sum[0].x[j] = sum[1].x[j] = 0.0f;
-    for (uint64_t first = uint64_t(blockIdx.x) * at_once; first < a.rows; first += uint64_t(gridDim.x) * at_once) {
+    for (int buffer = 0; first < a.rows; first += stride, buffer ^= 1) {
         if (a.half) {
             __syncthreads();
-            for (int i = tid; i < at_once * a.half; i += kBlock) {
-                const uint64_t row = first + uint64_t(i / a.half);
-                if (row < a.rows) {
-                    const double t = double(a.position[row]) * a.freq[i % a.half] * 0.15915494309189533577;  // 1 / (2 pi)
-                    float s, c;
-                    sincospif(2.0f * float(t - rint(t)), &s, &c);
-                    turn[i] = make_float2(c, BACK ? -s : s);
-                }
-            }
-            __syncthreads();
-        }
-        const uint64_t row = first + uint64_t(g / a.gpt);
-        if (row >= a.rows) continue;
-        Chunk<T> c, s;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int i = col + j;
-            c.x[j] = 1.0f;
-            s.x[j] = 0.0f;
-            if (i < 2 * a.half) {
-                const bool second = a.neighbours ? i & 1 : i >= a.half;
-                const float2 w = turn[g / a.gpt * a.half + (a.neighbours ? i / 2 : second ? i - a.half : i)];
-                c.x[j] = w.x;
-                s.x[j] = second ? w.y : -w.y;
+            if (first + stride < a.rows) {
+                form_angles(turn + (buffer ^ 1) * angles);
+                load_positions(first + 2 * stride);
             }
         }
-        Chunk<T> own, other;
-        int held = -1;  // whose gamma own and other are
-        for (int v = g % a.gpt; v < vectors; v += a.gpt) {
-            const int which = v >= a.heads;
-            const uint64_t at = uint64_t(which ? v - a.heads : v) * uint64_t(a.dim);
-            const T* const x = static_cast<const T*>(a.x[which]) + row * a.xs[which] + at;
-            T* const y = static_cast<T*>(a.y[which]) + row * a.ys[which] + at;
-            Chunk<T> in{}, pair{}, out{};
-            if (there && (!BACK || a.norm)) in = load_chunk(x + col);
-            if constexpr (BACK) {
-                const T* const dy = static_cast<const T*>(a.dy[which]) + row * a.dys[which] + at;
-                if (there) {
-                    out = load_chunk(dy + col);
-                    pair = load_partners(a, dy, col, out);
+        const uint64_t row = first + uint64_t(mine);
+        if (row >= a.rows || !any) continue;
+        Factors<T> f;
+        int held = -1;  // whose factors f are
+        for (int v = start; v < vectors; v += a.gpt) {
+            Vector<T> next = now;
+            Raw ahead{};
+            if (v + a.gpt < vectors) {
+                if ((v + a.gpt >= a.heads) == (v >= a.heads)) {
+                    next.x += step;
+                    next.n += step;
+                    next.to += step;
+                } else {
+                    next = vector_at<T, BACK>(a, row, v + a.gpt);
                 }
-            } else if (there) {
-                pair = load_partners(a, x, col, in);
+                if (there) ahead = fetch<T, BACK, PAIRS>(a, next, col);
+            } else {
+                ahead = fetch_first(row + stride, next);
             }
-            if (a.norm && held != which && there) {
-                load_gamma(a, a.gamma[which], col, !BACK, own, other);
-                held = which;
+            if (held != now.which && there) {
+                load_factors<T, BACK, PAIRS>(a, gamma + now.which * a.dim, turn + buffer * angles + mine * a.half, col, f);
+                held = now.which;
             }
+            const Chunk<T> own = widen<T>(raw.own);
+            Chunk<T> other{}, out;
+            if (there) other = partners<T, PAIRS>(a, now, own, raw.other, col);
             float r = 1.0f;
+            const Chunk<T> in = BACK ? widen<T>(raw.n) : own;
             if (a.norm) {
                 float sq = 0.0f;
 #pragma unroll
                 for (int j = 0; j < N; ++j) sq = fmaf(in.x[j], in.x[j], sq);
-                r = 1.0f / sqrtf(group_sum<TPV>(sq) / float(a.dim) + a.eps);
+                r = inverse_root(fmaf(group_sum<TPV>(sq), per, a.eps));
             }
-            if constexpr (!BACK) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    float t = in.x[j], p = pair.x[j];
-                    if (a.norm) {
-                        t = t * r * own.x[j];
-                        p = p * r * other.x[j];
-                    }
-                    out.x[j] = col + j < 2 * a.half ? fmaf(t, c.x[j], p * s.x[j]) : t;
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (col + j < 2 * a.half) out.x[j] = fmaf(out.x[j], c.x[j], pair.x[j] * s.x[j]);  // dt
+            for (int j = 0; j < N; ++j) {
+                out.x[j] = fmaf(own.x[j], f.own.x[j], other.x[j] * f.other.x[j]);  // backward: dt
+                if (!BACK) out.x[j] *= r;
+            }
+            if constexpr (BACK) {
                 if (a.norm) {
                     float dot = 0.0f;
+                    Chunk<T> n;
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
-                        in.x[j] *= r;  // n
-                        const float add = out.x[j] * in.x[j];
-                        sum[0].x[j] += which ? 0.0f : add;
-                        sum[1].x[j] += which ? add : 0.0f;
-                        out.x[j] = there ? out.x[j] * own.x[j] : 0.0f;
-                        dot = fmaf(out.x[j], in.x[j], dot);
+                        n.x[j] = in.x[j] * r;
+                        const float add = there ? out.x[j] * n.x[j] : 0.0f;
+                        sum[0].x[j] += now.which ? 0.0f : add;
+                        sum[1].x[j] += now.which ? add : 0.0f;
+                        out.x[j] = there ? out.x[j] * f.gamma.x[j] : 0.0f;
+                        dot = fmaf(out.x[j], n.x[j], dot);
                     }
-                    dot = group_sum<TPV>(dot) / float(a.dim);
+                    dot = group_sum<TPV>(dot) * per;
 #pragma unroll
-                    for (int j = 0; j < N; ++j) out.x[j] = r * fmaf(-in.x[j], dot, out.x[j]);
+                    for (int j = 0; j < N; ++j) out.x[j] = r * fmaf(-n.x[j], dot, out.x[j]);
                 }
             }
-            if (there) store_chunk(y + col, out);
+            if (there) store_chunk(now.to + col, out);
+            now = next;
+            raw = ahead;
         }
     }
     if constexpr (BACK) {
@@ -250,18 +369,18 @@ RotateShape rotate_shape(uint64_t rows, int vectors, int dim, bool bf16, int cus
     int gpt = 1;
     while (gpt < groups && gpt < vectors && ((rows * uint64_t(gpt) + uint64_t(groups) - 1) / uint64_t(groups) < uint64_t(4 * cus) || gpt * 8 < vectors)) gpt *= 2;
     const uint64_t at_once = uint64_t(groups / gpt), blocks = std::max<uint64_t>(1, (rows + at_once - 1) / at_once);
-    return {gpt, uint32_t(std::min<uint64_t>(blocks, back ? uint64_t(4 * cus) : uint64_t(1) << 20))};
+    return {gpt, uint32_t(std::min<uint64_t>(blocks, uint64_t(back ? 3 : 4) * uint64_t(cus)))};
 }
 
-template <class T, bool BACK>
-hipError_t launch(RotateArgs a, int cus, hipStream_t st) {
+template <class T, bool BACK, int PAIRS>
+hipError_t launch_pairs(RotateArgs a, int cus, hipStream_t st) {
     const int tpv = lanes(a.dim, sizeof(T) == 2);
     const RotateShape sh = rotate_shape(a.rows, a.heads + a.kv_heads, a.dim, sizeof(T) == 2, cus, BACK);
     a.gpt = sh.gpt;
-    const size_t turns = size_t(kBlock / tpv / sh.gpt) * size_t(a.half) * 8, sums = BACK && a.part ? size_t(kBlock) * Chunk<T>::N * 4 : 0;
+    const size_t turns = size_t(a.dim) * 8 + 2 * size_t(kBlock / tpv / sh.gpt) * size_t(a.half) * 8, sums = BACK && a.part ? size_t(kBlock) * Chunk<T>::N * 4 : 0;
     const size_t bytes = std::max(turns, sums);
     const auto as = [&](auto n) {
-        if (tpv == n) k_rotate<T, decltype(n)::value, BACK><<<sh.blocks, kBlock, bytes, st>>>(a);
+        if (tpv == n) k_rotate<T, decltype(n)::value, BACK, PAIRS><<<sh.blocks, kBlock, bytes, st>>>(a);
     };
     as(std::integral_constant<int, 2>{});
     as(std::integral_constant<int, 4>{});
@@ -271,6 +390,12 @@ hipError_t launch(RotateArgs a, int cus, hipStream_t st) {
     if constexpr (sizeof(T) == 2) as(std::integral_constant<int, 1>{});
     else as(std::integral_constant<int, 64>{});
     return hipGetLastError();
+}
+template <class T, bool BACK>
+hipError_t launch(const RotateArgs& a, int cus, hipStream_t st) {
+    constexpr int N = Chunk<T>::N;
+    if (!a.half || (a.neighbours && 2 * a.half % N == 0)) return launch_pairs<T, BACK, kSame>(a, cus, st);
+    return !a.neighbours && a.half % N == 0 ? launch_pairs<T, BACK, kChunk>(a, cus, st) : launch_pairs<T, BACK, kAny>(a, cus, st);
 }
 
 }  // namespace
