@@ -15,44 +15,23 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 
-// The queries of a wave's 16 rows as operands: PARTS bf16 of each value.
+// The queries of a wave's 16 rows as operands.
 template <class T, int NB>
 struct Queries {
-    static constexpr int PARTS = sizeof(T) == 2 ? 1 : 3;
-    uint4 w[PARTS][NB][2];
+    static constexpr int PARTS = QueryParts<T>::N;
+    QueryParts<T> w[NB][2];
 };
 template <class T, int NB>
 __device__ inline Queries<T, NB> load_queries(const CacheAttnArgs& a, const CacheRequest& rq, uint32_t packed, uint32_t head, int g) {
     Queries<T, NB> q;
     const bool there = packed < rq.rows * a.c.group;
-    const uint32_t i = packed / a.c.group, h = head * a.c.group + packed % a.c.group;
-    const T* const row = static_cast<const T*>(a.q) + uint64_t(rq.begin + (there ? i : 0)) * a.qs + uint64_t(h) * uint64_t(a.c.dim);
+    const T* const row = query_row<T>(a, rq, packed, head);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int col = 64 * b + 16 * g + 8 * s;
-            uint4 zero = make_uint4(0, 0, 0, 0);
-            if constexpr (sizeof(T) == 2) {
-                q.w[0][b][s] = there && uint32_t(col) < a.c.dim ? *reinterpret_cast<const uint4*>(row + col) : zero;
-            } else {
-                float x[8] = {};
-                if (there && uint32_t(col) < a.c.dim) {
-                    const float4 lo = *reinterpret_cast<const float4*>(row + col), hi = *reinterpret_cast<const float4*>(row + col + 4);
-                    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
-                }
-                uint32_t p[3][4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int k = 0; k < 3; ++k) {
-                        p[k][j] = bf16x2(x[2 * j], x[2 * j + 1]);
-                        x[2 * j] -= __uint_as_float(p[k][j] << 16);
-                        x[2 * j + 1] -= __uint_as_float(p[k][j] & 0xffff0000u);
-                    }
-#pragma unroll
-                for (int k = 0; k < 3; ++k) q.w[k][b][s] = make_uint4(p[k][0], p[k][1], p[k][2], p[k][3]);
-            }
+            const uint32_t col = uint32_t(64 * b + 16 * g + 8 * s);
+            q.w[b][s] = load_query8(row, col, there && col < a.c.dim);
         }
     return q;
 }
@@ -118,8 +97,8 @@ __device__ inline void step(const CacheAttnArgs& a, Running<NB>& run, const Quer
             const uint4 lo = keys_operand(t.k[i][b].x, t.k[i][b].y), hi = keys_operand(t.k[i][b].z, t.k[i][b].w);
 #pragma unroll
             for (int p = PARTS - 1; p >= 0; --p) {
-                s[i] = mfma_bf16(lo, q.w[p][b][0], s[i]);
-                s[i] = mfma_bf16(hi, q.w[p][b][1], s[i]);
+                s[i] = mfma_bf16(lo, q.w[b][0].w[p], s[i]);
+                s[i] = mfma_bf16(hi, q.w[b][1].w[p], s[i]);
             }
         }
     }
@@ -221,23 +200,6 @@ __device__ inline void step(const CacheAttnArgs& a, Running<NB>& run, const Quer
         run.o[d] = mfma_f16(lo, w[0], run.o[d]);
         run.o[d] = mfma_f16(hi, w[1], run.o[d]);
     }
-}
-
-// Row n's output: columns 16 d + 4 g ... + 3 from o[d], and its lse (lanes of g = 0).
-template <class T, int NB>
-__device__ inline void store_columns(const CacheAttnArgs& a, const CacheRequest& rq, uint32_t packed, uint32_t head, int d, int g, f32x4_t o, float sum) {
-    if (packed >= rq.rows * a.c.group || uint32_t(16 * d) >= a.c.dim) return;
-    const uint32_t i = packed / a.c.group, h = head * a.c.group + packed % a.c.group;
-    T* const to = static_cast<T*>(a.out) + uint64_t(rq.begin + i) * a.os + uint64_t(h) * uint64_t(a.c.dim) + 16 * d + 4 * g;
-    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (sum == 0.0f) o = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(to) = make_uint2(bf16x2(o[0] * by, o[1] * by), bf16x2(o[2] * by, o[3] * by));
-    else *reinterpret_cast<float4*>(to) = make_float4(o[0] * by, o[1] * by, o[2] * by, o[3] * by);
-}
-__device__ inline void store_lse(const CacheAttnArgs& a, const CacheRequest& rq, uint32_t packed, uint32_t head, float ref, float sum) {
-    if (!a.lse || packed >= rq.rows * a.c.group) return;
-    const uint32_t i = packed / a.c.group, h = head * a.c.group + packed % a.c.group;
-    a.lse[uint64_t(rq.begin + i) * uint64_t(a.c.heads) + h] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
 }
 
 // Sums of the four waves: [wave][columns / 16][lane] columns, [wave][row] references and weights.
@@ -372,7 +334,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_cache_attention(const CacheAttn
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) o += join.o[w][db][lane] * less[w];
             if (cut) *reinterpret_cast<f32x4_t*>(a.part + ((piece * (4 * NB) + uint64_t(db)) * kWave + uint64_t(lane)) * 4) = o;
-            else store_columns<T, NB>(a, rq, packed, head, db, g, o, sum);
+            else store4<T>(a, rq, packed, head, uint32_t(16 * db + 4 * g), o, sum);
         }
         if (wave == 0 && lane < 16) {
             if (cut) {
@@ -434,7 +396,7 @@ __global__ __launch_bounds__(kThreads) void k_cache_join(const CacheAttnArgs a) 
     }
     const CacheRequest rq = request_of(a, meta.x);
     const uint32_t packed = meta.y * kCacheRows + uint32_t(n);
-    store_columns<T, NB>(a, rq, packed, head, int(db), g, o, sum);
+    store4<T>(a, rq, packed, head, 16 * db + 4 * uint32_t(g), o, sum);
     if (db == 0 && lane < 16) store_lse(a, rq, packed, head, top, sum);
 }
 
@@ -455,9 +417,29 @@ uint64_t pad256(uint64_t b) { return (b + 255) / 256 * 256; }
 struct Workspace {
     uint64_t part, stat, meta;
 };
-Workspace workspace_of(const gatgpu_ctx* c, const gatgpu_cache* cache) {
-    const uint64_t blocks = uint64_t(cache_workers(c, cache->kv_heads)) * uint64_t(cache->kv_heads), nb = cache->dim > 64 ? 2 : 1;
+Workspace workspace_of(const gatgpu_ctx* c, const CacheSizes& s) {
+    const uint64_t blocks = uint64_t(cache_workers(c, int(s.kv_heads))) * s.kv_heads, nb = s.dim > 64 ? 2 : 1;
     return {pad256(blocks * 2 * 4 * nb * kWave * 16), pad256(blocks * 2 * 32 * 4), pad256(blocks * 16)};
+}
+CacheSizes sizes_of(const gatgpu_cache* cache, const gatgpu_cache_attention_io* io) {
+    CacheSizes c;
+    c.rows = io->rows;
+    c.requests = io->requests;
+    c.most = io->most;
+    c.blocks = io->blocks;
+    c.pages = cache->pages;
+    while ((1u << c.page_log) < cache->page) ++c.page_log;
+    c.heads = uint32_t(io->heads);
+    c.kv_heads = uint32_t(cache->kv_heads);
+    c.group = uint32_t(io->heads / cache->kv_heads);
+    c.dim = uint32_t(cache->dim);
+    return c;
+}
+// Whether requests have rows enough for tiles of 128 packed ones.
+bool in_chunks(const CacheSizes& c) { return uint64_t(c.most) * c.group > 32; }
+uint64_t workspace_bytes(const gatgpu_ctx* c, const CacheSizes& s) {
+    const Workspace w = workspace_of(c, s);
+    return in_chunks(s) ? chunk_plan(c->cus, s).bytes : w.part + w.stat + w.meta;
 }
 
 }  // namespace
@@ -500,8 +482,7 @@ int gatgpu_cache_attention_workspace(gatgpu_ctx* c, const gatgpu_cache* cache, c
     if (!bytes) return fail(c, GATGPU_EINVAL, "null output");
     if (int r = check_cache(c, cache, false)) return r;
     if (int r = check_sizes(c, cache, io)) return r;
-    const Workspace w = workspace_of(c, cache);
-    *bytes = w.part + w.stat + w.meta;
+    *bytes = workspace_bytes(c, sizes_of(cache, io));
     return GATGPU_OK;
 }
 
@@ -521,22 +502,12 @@ int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgp
         if (int r = check_words(c, "table", io->table)) return r;
     if (io->lse)
         if (int r = check_words(c, "lse", io->lse)) return r;
-    const Workspace w = workspace_of(c, cache);
-    const uint64_t need = w.part + w.stat + w.meta;
+    CacheAttnArgs a;
+    a.c = sizes_of(cache, io);
+    const uint64_t need = workspace_bytes(c, a.c);
     if (bytes < need) return fail(c, GATGPU_EINVAL, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
     if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return fail(c, GATGPU_EINVAL, "workspace must be 16-byte aligned device memory");
     if (int r = check_device_array(c, ws, "workspace")) return r;
-    CacheAttnArgs a;
-    a.c.rows = io->rows;
-    a.c.requests = io->requests;
-    a.c.most = io->most;
-    a.c.blocks = io->blocks;
-    a.c.pages = cache->pages;
-    while ((1u << a.c.page_log) < cache->page) ++a.c.page_log;
-    a.c.heads = uint32_t(io->heads);
-    a.c.kv_heads = uint32_t(cache->kv_heads);
-    a.c.group = uint32_t(io->heads / cache->kv_heads);
-    a.c.dim = uint32_t(cache->dim);
     a.workers = cache_workers(c, cache->kv_heads);
     a.least = 4;
     a.scale = io->scale * 1.44269504088896341f;
@@ -553,10 +524,15 @@ int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgp
     a.v = cache->v;
     a.k_scale = cache->k_scale;
     a.v_scale = cache->v_scale;
+    const bool bf16 = io->precision == GATGPU_BF16, wide = cache->dim > 64;
+    if (in_chunks(a.c)) {
+        HIPCHECK(c, launch_cache_chunk(a, bf16, chunk_plan(c->cus, a.c), ws, c->stream));
+        return GATGPU_OK;
+    }
+    const Workspace w = workspace_of(c, a.c);
     a.part = static_cast<float*>(ws);
     a.stat = reinterpret_cast<float*>(static_cast<char*>(ws) + w.part);
     a.meta = reinterpret_cast<uint4*>(static_cast<char*>(ws) + w.part + w.stat);
-    const bool bf16 = io->precision == GATGPU_BF16, wide = cache->dim > 64;
     HIPCHECK(c, bf16 ? (wide ? launch<uint16_t, 2>(a, c->stream) : launch<uint16_t, 1>(a, c->stream))
                      : (wide ? launch<float, 2>(a, c->stream) : launch<float, 1>(a, c->stream)));
     return GATGPU_OK;

@@ -43,7 +43,13 @@ struct CacheAttnArgs {
     float *part = nullptr, *stat = nullptr;
     uint4* meta = nullptr;  // [worker][head]: request, row tile, pieces (0: none) of the task that begins in the worker and ends in another
 };
-__device__ inline CacheRequest request_of(const CacheAttnArgs& a, uint32_t r) { return cache_request(a.c, a.q_begin[r], a.q_begin[r + 1], a.k_len[r]); }
+// One request's place (by scalar loads where r is the same in all lanes).
+__device__ inline CacheRequest request_of(const CacheAttnArgs& a, uint32_t r) {
+    return cache_request(a.c, read_only(a.q_begin)[r], read_only(a.q_begin)[r + 1], read_only(a.k_len)[r]);
+}
+// A value that is the same in all lanes, in a scalar register.
+__device__ inline uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
+__device__ inline uint64_t uniform(uint64_t x) { return uint64_t(uniform(uint32_t(x >> 32))) << 32 | uniform(uint32_t(x)); }
 
 __device__ inline uint32_t f16x2(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){lo, hi}, f16x2_t));
@@ -77,5 +83,70 @@ __device__ inline uint32_t low_bytes(int n) { return n <= 0 ? 0u : n >= 4 ? 0xff
 // lie before it is raised, and how far below the score it is raised to.  References are whole numbers, so that rescaling
 // is exact and a weight's exponent, x + (ev - ref), is rounded once.
 constexpr float kCacheNoRef = -3.402823466e38f, kCacheRoom = 15.0f, kCacheSet = 7.0f;
+
+// Columns col to col + 3 of a packed row, from the sums of its weights' products and of its weights.
+template <class T>
+__device__ inline void store4(const CacheAttnArgs& a, const CacheRequest& rq, uint32_t packed, uint32_t head, uint32_t col, f32x4_t o, float sum) {
+    if (packed >= rq.rows * a.c.group || col >= a.c.dim) return;
+    const uint32_t i = packed / a.c.group, h = head * a.c.group + packed % a.c.group;
+    T* const to = static_cast<T*>(a.out) + uint64_t(rq.begin + i) * a.os + uint64_t(h) * a.c.dim + col;
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (sum == 0.0f) o = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(to) = make_uint2(bf16x2(o[0] * by, o[1] * by), bf16x2(o[2] * by, o[3] * by));
+    else *reinterpret_cast<float4*>(to) = make_float4(o[0] * by, o[1] * by, o[2] * by, o[3] * by);
+}
+__device__ inline void store_lse(const CacheAttnArgs& a, const CacheRequest& rq, uint32_t packed, uint32_t head, float ref, float sum) {
+    if (!a.lse || packed >= rq.rows * a.c.group) return;
+    const uint32_t i = packed / a.c.group, h = head * a.c.group + packed % a.c.group;
+    a.lse[uint64_t(rq.begin + i) * a.c.heads + h] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Eight values of a query row from `col` on, as PARTS bf16 operands (FP32: three, which hold all its bits).
+template <class T>
+struct QueryParts {
+    static constexpr int N = sizeof(T) == 2 ? 1 : 3;
+    uint4 w[N];
+};
+template <class T>
+__device__ inline QueryParts<T> load_query8(const T* row, uint32_t col, bool there) {
+    QueryParts<T> q;
+    if constexpr (sizeof(T) == 2) {
+        q.w[0] = there ? *reinterpret_cast<const uint4*>(row + col) : make_uint4(0, 0, 0, 0);
+    } else {
+        float x[8] = {};
+        if (there) {
+            const float4 lo = *reinterpret_cast<const float4*>(row + col), hi = *reinterpret_cast<const float4*>(row + col + 4);
+            x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            uint32_t p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                p[j] = bf16x2(x[2 * j], x[2 * j + 1]);
+                x[2 * j] -= __uint_as_float(p[j] << 16);
+                x[2 * j + 1] -= __uint_as_float(p[j] & 0xffff0000u);
+            }
+            q.w[k] = make_uint4(p[0], p[1], p[2], p[3]);
+        }
+    }
+    return q;
+}
+// The queries of a packed row: its first element, the request's first row where there is none.
+template <class T>
+__device__ inline const T* query_row(const CacheAttnArgs& a, const CacheRequest& rq, uint32_t packed, uint32_t head) {
+    const bool there = packed < rq.rows * a.c.group;
+    const uint32_t i = there ? packed / a.c.group : 0, h = head * a.c.group + packed % a.c.group;
+    return static_cast<const T*>(a.q) + uint64_t(rq.begin + i) * a.qs + uint64_t(h) * a.c.dim;
+}
+
+// Many rows a request (cache_attention_chunk.hip): workspace and launches.
+struct ChunkPlan {
+    uint32_t tiles = 0;    // at most, of packed rows
+    uint32_t workers = 0;  // of a key/value head
+    uint64_t begin = 0, request = 0, upto = 0, part = 0, stat = 0, meta = 0, bytes = 0;  // offsets in the workspace
+};
+ChunkPlan chunk_plan(int cus, const CacheSizes& c);
+hipError_t launch_cache_chunk(const CacheAttnArgs& a, bool bf16, const ChunkPlan& plan, void* workspace, hipStream_t s);
 
 }  // namespace gatgpu

@@ -1,0 +1,461 @@
+// Attention over a paged 8-bit cache, many rows a request: chunks of prompts.
+//
+// Bound by matrix and vector instructions (4 products of 64 x 32 x dim a step and wave, an exponential a pair).  A block of
+// four waves takes 128 packed rows, 32 a wave, on v_mfma_f32_32x32x16.  Its threads request a tile of 64 keys two steps
+// ahead, turn its bytes to bf16 keys and fp16 values once for the four waves, and leave them in one of two LDS buffers
+// while the other is worked on; one barrier a step.
+//   S^T = K Q^T: lane (n = lane % 32, h = lane / 32) gets row n's scores of LDS rows 8 i + 4 h + r (register 4 i + r), and LDS
+//   row m of 32 holds key 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that registers 8 s ... 8 s + 7 are keys
+//   16 s + 8 h ... + 7: the second product's operand as they stand.
+// Rows of 16-byte pieces are stored with the piece's index crossed with the row's, so that neighbouring lanes, which read the
+// same piece of neighbouring rows, meet different banks.
+//
+// Work is cut into equal ranges of (row tile, key tile) for two blocks a unit, since lengths are known on the device only:
+// a first launch of one block forms the sums over the tiles, and a last one joins the tiles that a range's end cuts.
+#include <algorithm>
+
+#include "cache_attention.hpp"
+
+namespace gatgpu {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / kWave, kScan = 1024;
+constexpr uint32_t kRows = 128, kWaveRows = 32;  // packed rows of a block and of a wave
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+struct ChunkArgs {
+    CacheAttnArgs a;
+    uint32_t tiles = 0;          // at most
+    uint32_t* begin = nullptr;   // [requests + 1] first row tile of each request
+    uint32_t* request = nullptr; // [tiles]
+    uint64_t* upto = nullptr;    // [tiles + 1] key tiles of the row tiles before each
+};
+
+__device__ inline uint32_t chunk_tiles(const CacheSizes& c, const CacheRequest& q) { return (q.rows * c.group + kRows - 1) / kRows; }
+// Key tiles that the rows of row tile t see (one, if none).
+__device__ inline uint32_t tiles_seen(const CacheSizes& c, const CacheRequest& q, uint32_t t) {
+    const uint32_t last = min(q.rows * c.group, (t + 1) * kRows) - 1, n = cache_seen(q, last / c.group);
+    return n ? (n - 1) / kCacheTile + 1 : 1;
+}
+// The last i of [0, n) with first[i] <= x, for n >= 1, first[0] <= x: 64 places at a time, by a wave.
+template <class V>
+__device__ inline uint32_t last_at_most(const V* first, uint32_t n, V x, int lane) {
+    uint32_t lo = 0;
+    while (n > 1) {
+        const uint32_t step = (n + kWave - 1) / kWave, i = uint32_t(lane) * step;
+        const uint64_t below = __ballot(i < n && first[lo + i] <= x);
+        const uint32_t at = uint32_t(__popcll(below) - 1) * step;  // (sorted: the lanes below are the first ones)
+        lo += at;
+        n = min(step, n - at);
+    }
+    return lo;
+}
+
+__device__ inline uint64_t scan_sums(uint64_t x, uint64_t& total) {
+    __shared__ uint64_t wave_total[kScan / kWave];
+    const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const uint64_t p = __shfl_up(x, d);
+        if (lane >= d) x += p;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) wave_total[wave] = x;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < kScan / kWave; ++w) {
+        if (w < wave) x += wave_total[w];
+        total += wave_total[w];
+    }
+    return x;
+}
+__global__ __launch_bounds__(kScan) void k_cache_plan(const ChunkArgs p) {
+    const CacheAttnArgs& a = p.a;
+    const uint32_t tid = threadIdx.x;
+    uint64_t total, before = 0;
+    for (uint32_t first = 0; first < a.c.requests; first += kScan) {
+        const uint32_t r = first + tid;
+        const uint64_t n = r < a.c.requests ? chunk_tiles(a.c, request_of(a, r)) : 0, sum = scan_sums(n, total);
+        if (r < a.c.requests) p.begin[r] = index_min(before + sum - n, p.tiles);
+        before += total;
+    }
+    const uint32_t tiles = index_min(before, p.tiles);  // (never more, for rows in order)
+    if (tid == 0) {
+        p.begin[a.c.requests] = tiles;
+        p.upto[0] = 0;
+    }
+    __syncthreads();
+    before = 0;
+    for (uint32_t first = 0; first < tiles; first += kScan) {
+        const uint32_t t = first + tid;
+        uint64_t n = 0;
+        if (t < tiles) {
+            uint32_t lo = 0, hi = a.c.requests - 1;  // the last request that begins at or before t
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi + 1) / 2;
+                if (p.begin[mid] <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            p.request[t] = lo;
+            const CacheRequest q = request_of(a, lo);
+            const uint32_t own = t - p.begin[lo];
+            n = own < chunk_tiles(a.c, q) ? tiles_seen(a.c, q, own) : 0;
+        }
+        const uint64_t sum = scan_sums(n, total);
+        if (t < tiles) p.upto[t + 1] = before + sum;
+        before += total;
+    }
+}
+
+// A block's tiles of keys and values: [buffer][row][64 columns of NB], [buffer][column][64 keys]; pieces of 16 bytes.
+template <int NB>
+struct ChunkLds {
+    uint4 k[2][kCacheTile][8 * NB];
+    uint4 v[2][64 * NB][8];
+    uint32_t nan[4];  // the values of tile i (of a piece), in place i % 4, hold one
+};
+
+// What a thread requests of a tile, in 16 bytes: of NB keys each 16 columns, and of NB columns each 16 keys.
+template <int NB>
+struct Bytes {
+    uint4 k[NB], v[NB];
+};
+template <int NB>
+struct Pages {
+    uint32_t k[NB], v;
+};
+__device__ inline f32x16_t mfma32_bf16(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+__device__ inline f32x16_t mfma32_f16(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+// fp16 NaNs among two halves: all ones there, and 1.0 in their places.
+__device__ inline uint32_t nan_halves(uint32_t w) {
+    return ((w & 0x7fffu) > 0x7c00u ? 0xffffu : 0u) | ((w >> 16 & 0x7fffu) > 0x7c00u ? 0xffff0000u : 0u);
+}
+
+template <class T, int NB>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chunk(const ChunkArgs p) {
+    constexpr int PARTS = QueryParts<T>::N, PIECES = 4 * NB;  // 16-byte pieces of a key's bytes
+    __shared__ ChunkLds<NB> lds;
+    const CacheAttnArgs& a = p.a;
+    const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave, n = lane % 32, h = lane / 32;
+    const uint32_t head = blockIdx.x % a.c.kv_heads, worker = blockIdx.x / a.c.kv_heads;
+    const auto upto = read_only(p.upto);
+    const uint32_t tiles = read_only(p.begin)[a.c.requests];
+    const uint64_t total = tiles ? upto[tiles] : 0, share = max(uint64_t(a.least), (total + a.workers - 1) / a.workers);
+    uint64_t at = min(total, uint64_t(worker) * share);
+    const uint64_t end = min(total, at + share);
+    uint4 meta = make_uint4(0, 0, 0, 0);
+    // What this thread brings of a tile: keys k_key + 32 i, columns 16 k_piece; columns v_col + 64 i, keys 16 v_group.
+    const uint32_t k_key = uint32_t(tid) / PIECES, k_piece = uint32_t(tid) % PIECES, v_group = uint32_t(tid) % 4, v_col = uint32_t(tid) / 4;
+    uint32_t tile_at = at < end ? uniform(last_at_most(p.upto, tiles, at, lane)) : 0;
+    for (; at < end; ++tile_at) {
+        const uint64_t base = upto[tile_at], next_base = upto[tile_at + 1];
+        if (at >= next_base) continue;  // (a tile of no work)
+        const uint32_t request = read_only(p.request)[tile_at], row_tile = tile_at - read_only(p.begin)[request];
+        const CacheRequest rq = request_of(a, request);
+        const uint32_t all = uint32_t(next_base - base), lo = uint32_t(at - base), hi = index_min(all, lo + (end - at));
+        const uint32_t packed = row_tile * kRows + uint32_t(wave) * kWaveRows + uint32_t(n), rows = rq.rows * a.c.group;
+        const uint32_t seen = packed < rows ? cache_seen(rq, packed / a.c.group) : 0;
+        // Rows of a wave stand in the order of their positions; a wave without rows sees nothing.
+        const uint32_t first_row = row_tile * kRows + uniform(uint32_t(wave)) * kWaveRows;
+        const uint32_t least = first_row < rows ? cache_seen(rq, first_row / a.c.group) : 0;
+        const uint32_t most = first_row < rows ? cache_seen(rq, (min(rows, first_row + kWaveRows) - 1) / a.c.group) : 0;
+        const uint32_t* const table = a.table + uint64_t(request) * a.ld;
+
+        const auto load_pages = [&](uint32_t tile) {
+            Pages<NB> g;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const uint32_t b = block_of(a.c, rq.keys, tile * kCacheTile + (k_key + uint32_t(i) * (kThreads / PIECES)) / 16 * 16);
+                g.k[i] = b == kNoPage ? b : table[b];
+            }
+            const uint32_t b = block_of(a.c, rq.keys, tile * kCacheTile + 16 * v_group);
+            g.v = b == kNoPage ? b : table[b];
+            return g;
+        };
+        const auto load_bytes = [&](uint32_t tile, const Pages<NB>& g) {
+            Bytes<NB> x;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const uint32_t key = tile * kCacheTile + k_key + uint32_t(i) * (kThreads / PIECES), col = v_col + 64 * uint32_t(i);
+                x.k[i] = 16 * k_piece < a.c.dim ? *reinterpret_cast<const uint4*>(a.k + key_byte(a.c, some_page(a.c, g.k[i]), head, key) + 16 * k_piece) : make_uint4(0, 0, 0, 0);
+                x.v[i] = col < a.c.dim ? *reinterpret_cast<const uint4*>(a.v + value_byte(a.c, some_page(a.c, g.v), head, tile * kCacheTile + 16 * v_group, col)) : make_uint4(0, 0, 0, 0);
+                // Values of no token count as 0.
+                const uint32_t from = tile * kCacheTile + 16 * v_group;
+                const int valid = g.v < a.c.pages ? int(min(rq.keys > from ? rq.keys - from : 0u, 16u)) : 0;
+                if (valid < 16) {
+                    x.v[i].x &= low_bytes(valid);
+                    x.v[i].y &= low_bytes(valid - 4);
+                    x.v[i].z &= low_bytes(valid - 8);
+                    x.v[i].w &= low_bytes(valid - 12);
+                }
+            }
+            return x;
+        };
+        const auto put = [&](int buffer, uint32_t* flag, const Bytes<NB>& x) {
+            uint32_t nan = 0;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const uint32_t key = k_key + uint32_t(i) * (kThreads / PIECES);
+                const uint32_t m = key / 32 * 32 + key / 16 % 2 * 16 + key / 4 % 2 * 8 + key / 8 % 2 * 4 + key % 4, turn = m % (8 * NB);
+                lds.k[buffer][m][(2 * k_piece) ^ turn] = keys_operand(x.k[i].x, x.k[i].y);
+                lds.k[buffer][m][(2 * k_piece + 1) ^ turn] = keys_operand(x.k[i].z, x.k[i].w);
+                const uint32_t col = v_col + 64 * uint32_t(i);
+                lds.v[buffer][col][(2 * v_group) ^ (col % 8)] = values_operand(x.v[i].x, x.v[i].y);
+                lds.v[buffer][col][(2 * v_group + 1) ^ (col % 8)] = values_operand(x.v[i].z, x.v[i].w);
+                nan |= nan_bytes(x.v[i].x) | nan_bytes(x.v[i].y) | nan_bytes(x.v[i].z) | nan_bytes(x.v[i].w);
+            }
+            if (nan) *flag = 1;  // (every writer writes the same)
+        };
+
+        Pages<NB> pages = load_pages(lo);
+        Bytes<NB> bytes = load_bytes(lo, pages);
+        pages = load_pages(lo + 1);
+        QueryParts<T> q[4 * NB];
+        const T* const row = query_row<T>(a, rq, packed, head);
+#pragma unroll
+        for (int s = 0; s < 4 * NB; ++s) {
+            const uint32_t col = uint32_t(16 * s + 8 * h);
+            q[s] = load_query8(row, col, packed < rows && col < a.c.dim);
+        }
+        f32x16_t o[2 * NB];
+#pragma unroll
+        for (int d = 0; d < 2 * NB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+        float ref = kCacheNoRef, sum = 0.0f;
+        if (tid < 4) lds.nan[tid] = 0;
+        __syncthreads();
+        put(0, &lds.nan[0], bytes);
+        if (lo + 1 < hi) {
+            bytes = load_bytes(lo + 1, pages);
+            pages = load_pages(lo + 2);
+        }
+        __syncthreads();
+        for (uint32_t tile = lo; tile < hi; ++tile) {
+            const int buffer = int(tile - lo) & 1;
+            if (tid == 0) lds.nan[(tile - lo + 2) % 4] = 0;  // (read two barriers ago, set again behind the next one)
+            if (tile + 1 < hi) {
+                put(buffer ^ 1, &lds.nan[(tile - lo + 1) % 4], bytes);
+                if (tile + 2 < hi) {
+                    bytes = load_bytes(tile + 2, pages);
+                    pages = load_pages(tile + 3);
+                }
+            }
+            if (tile * kCacheTile < most) {
+                // Scales of the tile's four pages of 16 keys, and which of them there are: the same in all lanes.
+                float by[4], back[4];
+                int ev[4];
+                uint32_t held = 0;
+#pragma unroll
+                for (uint32_t g = 0; g < 4; ++g) {
+                    const uint32_t b = block_of(a.c, rq.keys, tile * kCacheTile + 16 * g);
+                    const uint32_t page = b == kNoPage ? b : read_only(table)[b];
+                    if (page < a.c.pages) held |= 1u << g;
+                    const uint64_t place = uint64_t(some_page(a.c, page)) * a.c.kv_heads + head;
+                    by[g] = a.scale * power_of_two(scale_exponent(read_only(a.k_scale)[place]));
+                    ev[g] = scale_exponent(read_only(a.v_scale)[place]);
+                    back[g] = power_of_two(-ev[g]);
+                }
+                f32x16_t s[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[k][r] = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < 4 * NB; ++c) {
+                        const uint4 keys = lds.k[buffer][32 * k + n][(2 * c + h) ^ (n % (8 * NB))];
+#pragma unroll
+                        for (int part = PARTS - 1; part >= 0; --part) s[k] = mfma32_bf16(keys, q[c].w[part], s[k]);
+                    }
+                }
+                const bool whole = (tile + 1) * kCacheTile <= least && held == 15;
+                if (!whole) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int g = 2 * k + r / 8;
+                            if (!(held >> g & 1) || tile * kCacheTile + uint32_t(16 * g + 8 * h + r % 8) >= seen) s[k][r] = -INFINITY;
+                        }
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float t = s[g / 2][8 * (g % 2)];
+#pragma unroll
+                    for (int r = 1; r < 8; ++r) t = fmaxf(t, s[g / 2][8 * (g % 2) + r]);
+                    top = fmaxf(top, fmaf(t, by[g], float(ev[g])));
+                }
+                if (__any(top > ref + kCacheRoom)) {
+                    const float both = xor32_max(top);
+                    const bool up = both > ref + kCacheRoom;
+                    const float to = up ? ceilf(both) - kCacheSet : ref, less = up ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
+                    ref = to;
+                    sum *= less;
+#pragma unroll
+                    for (int d = 0; d < 2 * NB; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[d][r] *= less;
+                }
+                uint4 w[4], rest[4];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float shift = float(ev[g]) - ref;  // (whole numbers: exact)
+                    float x[8], of = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        x[r] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + r], by[g], shift));
+                        of += x[r];
+                    }
+                    sum = fmaf(of, back[g], sum);
+                    uint32_t u[4], l[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        u[j] = f16x2(x[2 * j], x[2 * j + 1]);
+                        if constexpr (PARTS > 1) {
+                            const f16x2_t up = __builtin_bit_cast(f16x2_t, u[j]);
+                            l[j] = f16x2(x[2 * j] - float(up[0]), x[2 * j + 1] - float(up[1]));
+                        }
+                    }
+                    w[g] = make_uint4(u[0], u[1], u[2], u[3]);
+                    if constexpr (PARTS > 1) rest[g] = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+                const bool care = !whole && lds.nan[(tile - lo) % 4];  // a NaN that some rows see and others may not
+#pragma unroll
+                for (int d = 0; d < 2 * NB; ++d)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        uint4 x = lds.v[buffer][32 * d + n][(2 * g + h) ^ (n % 8)];
+                        if (care) {  // it counts as 0, and marks the rows that see it
+                            const uint4 bad = make_uint4(nan_halves(x.x), nan_halves(x.y), nan_halves(x.z), nan_halves(x.w));
+                            x = make_uint4(x.x & ~bad.x, x.y & ~bad.y, x.z & ~bad.z, x.w & ~bad.w);
+                            uint32_t u[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const uint32_t key = tile * kCacheTile + uint32_t(16 * g + 8 * h + 2 * j);
+                                const bool there = held >> g & 1;
+                                u[j] = (there && key < seen ? 0x3c00u : 0u) | (there && key + 1 < seen ? 0x3c000000u : 0u);
+                            }
+                            f32x16_t count;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) count[r] = 0.0f;
+                            count = mfma32_f16(make_uint4(bad.x & 0x3c003c00u, bad.y & 0x3c003c00u, bad.z & 0x3c003c00u, bad.w & 0x3c003c00u),
+                                               make_uint4(u[0], u[1], u[2], u[3]), count);
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                if (count[r] > 0.0f) o[d][r] = NAN;
+                        }
+                        if constexpr (PARTS > 1) o[d] = mfma32_f16(x, rest[g], o[d]);
+                        o[d] = mfma32_f16(x, w[g], o[d]);
+                    }
+            }
+            __syncthreads();
+        }
+        sum = xor32_add(sum);
+        const bool cut = lo > 0 || hi < all;
+        const uint64_t piece = (uint64_t(blockIdx.x) * 2 + (lo > 0 ? 0 : 1)) * kWaves + uint64_t(wave);
+#pragma unroll
+        for (int d = 0; d < 2 * NB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4_t x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                if (cut) *reinterpret_cast<f32x4_t*>(a.part + ((piece * (8 * NB) + uint64_t(4 * d + i)) * kWave + uint64_t(lane)) * 4) = x;
+                else store4<T>(a, rq, packed, head, uint32_t(32 * d + 8 * i + 4 * h), x, sum);
+            }
+        if (lane < 32) {
+            if (cut) {
+                a.stat[piece * 64 + uint64_t(n)] = ref;
+                a.stat[piece * 64 + 32 + uint64_t(n)] = sum;
+            } else {
+                store_lse(a, rq, packed, head, ref, sum);
+            }
+        }
+        if (lo == 0 && hi < all) meta = make_uint4(request, row_tile, uint32_t((next_base - 1) / share) - worker + 1, 0);
+        at += hi - lo;
+        __syncthreads();
+    }
+    if (tid == 0) a.meta[blockIdx.x] = meta;
+}
+
+// The pieces of the row tile that begins in a worker and ends in another: a wave its 32 rows, four columns of each lane a block.
+template <class T, int NB>
+__global__ __launch_bounds__(kThreads) void k_cache_chunk_join(const ChunkArgs p) {
+    const CacheAttnArgs& a = p.a;
+    const uint4 meta = a.meta[blockIdx.x];
+    if (!meta.z) return;
+    const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave, n = lane % 32, h = lane / 32;
+    const uint32_t head = blockIdx.x % a.c.kv_heads, which = blockIdx.y;
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float ref = kCacheNoRef, sum = 0.0f;
+    for (uint32_t i = 0; i < meta.z; ++i) {
+        const uint64_t piece = ((uint64_t(blockIdx.x) + uint64_t(i) * a.c.kv_heads) * 2 + (i ? 0 : 1)) * kWaves + uint64_t(wave);
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part + ((piece * (8 * NB) + which) * kWave + uint64_t(lane)) * 4);
+        const float r = a.stat[piece * 64 + uint64_t(n)], s = a.stat[piece * 64 + 32 + uint64_t(n)];
+        const float top = fmaxf(ref, r), less = __builtin_amdgcn_exp2f(ref - top), more = __builtin_amdgcn_exp2f(r - top);
+        o = o * less + x * more;
+        sum = sum * less + s * more;
+        ref = top;
+    }
+    const CacheRequest rq = request_of(a, meta.x);
+    const uint32_t packed = meta.y * kRows + uint32_t(wave) * kWaveRows + uint32_t(n);
+    store4<T>(a, rq, packed, head, which / 4 * 32 + which % 4 * 8 + 4 * uint32_t(h), o, sum);
+    if (which == 0 && lane < 32) store_lse(a, rq, packed, head, ref, sum);
+}
+
+uint64_t pad256(uint64_t b) { return (b + 255) / 256 * 256; }
+
+template <class T, int NB>
+hipError_t launch(const ChunkArgs& p, hipStream_t s) {
+    const uint32_t blocks = p.a.workers * p.a.c.kv_heads;
+    k_cache_plan<<<1, kScan, 0, s>>>(p);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    k_cache_chunk<T, NB><<<blocks, kThreads, 0, s>>>(p);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    k_cache_chunk_join<T, NB><<<dim3(blocks, 8 * NB), kThreads, 0, s>>>(p);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+ChunkPlan chunk_plan(int cus, const CacheSizes& c) {
+    ChunkPlan p;
+    p.tiles = uint32_t(c.rows * c.group / kRows + c.requests);  // a request's last tile may be part full
+    p.workers = uint32_t(std::max(1, 2 * cus / int(c.kv_heads)));
+    const uint64_t blocks = uint64_t(p.workers) * c.kv_heads, nb = c.dim > 64 ? 2 : 1;
+    uint64_t at = 0;
+    const auto take = [&](uint64_t bytes) {
+        const uint64_t here = at;
+        at += pad256(bytes);
+        return here;
+    };
+    p.begin = take((uint64_t(c.requests) + 1) * 4);
+    p.request = take(uint64_t(p.tiles) * 4);
+    p.upto = take((uint64_t(p.tiles) + 1) * 8);
+    p.part = take(blocks * 2 * kRows * 64 * nb * 4);
+    p.stat = take(blocks * 2 * kRows * 8);
+    p.meta = take(blocks * 16);
+    p.bytes = at;
+    return p;
+}
+
+hipError_t launch_cache_chunk(const CacheAttnArgs& args, bool bf16, const ChunkPlan& plan, void* workspace, hipStream_t s) {
+    ChunkArgs p;
+    p.a = args;
+    p.a.workers = plan.workers;
+    char* const ws = static_cast<char*>(workspace);
+    p.tiles = plan.tiles;
+    p.begin = reinterpret_cast<uint32_t*>(ws + plan.begin);
+    p.request = reinterpret_cast<uint32_t*>(ws + plan.request);
+    p.upto = reinterpret_cast<uint64_t*>(ws + plan.upto);
+    p.a.part = reinterpret_cast<float*>(ws + plan.part);
+    p.a.stat = reinterpret_cast<float*>(ws + plan.stat);
+    p.a.meta = reinterpret_cast<uint4*>(ws + plan.meta);
+    const bool wide = args.c.dim > 64;
+    return bf16 ? (wide ? launch<uint16_t, 2>(p, s) : launch<uint16_t, 1>(p, s)) : (wide ? launch<float, 2>(p, s) : launch<float, 1>(p, s));
+}
+
+}  // namespace gatgpu
