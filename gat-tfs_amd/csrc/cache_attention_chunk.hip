@@ -7,8 +7,6 @@
 //   S^T = K Q^T: lane (n = lane % 32, h = lane / 32) gets row n's scores of LDS rows 8 i + 4 h + r (register 4 i + r), and LDS
 //   row m of 32 holds key 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that registers 8 s ... 8 s + 7 are keys
 //   16 s + 8 h ... + 7: the second product's operand as they stand.
-// Rows of 16-byte pieces are stored with the piece's index crossed with the row's, so that neighbouring lanes, which read the
-// same piece of neighbouring rows, meet different banks.
 //
 // Work is cut into equal ranges of (row tile, key tile) for two blocks a unit, since lengths are known on the device only:
 // a first launch of one block forms the sums over the tiles, and a last one joins the tiles that a range's end cuts.
@@ -112,14 +110,24 @@ template <int NB>
 struct ChunkLds {
     uint4 k[2][kCacheTile][8 * NB];
     uint4 v[2][64 * NB][8];
-    uint32_t nan[4];  // the values of tile i (of a piece), in place i % 4, hold one
+    float scale[2][4][2];  // of each 16 keys: what a score is multiplied by, and the values' exponent; without a page: -1
+    uint16_t bad[2][64 * NB][4];  // which of each 16 keys' values are NaN (they stand as 0 in v)
+    uint32_t nan[4];       // the values of tile i (of a piece), in place i % 4, hold one
 };
 
 // What a thread requests of a tile, in 16 bytes: of NB keys each 16 columns, and of NB columns each 16 keys.
 template <int NB>
 struct Bytes {
     uint4 k[NB], v[NB];
+    float ks, vs;  // scales of the 16 keys (of the first threads)
+    int tokens;    // among the 16 keys of the values
 };
+// What a row crosses its pieces' indices with, of PIECES of them a row: 16 neighbouring lanes then meet the 16 pieces of 256
+// bytes, all banks of a cycle, both as they write (pieces of a row or of a few) and as they read (a piece of 16 rows).
+template <int PIECES>
+__device__ inline uint32_t turned(uint32_t row) {
+    return PIECES == 16 ? row % 16 : row / 2 % 8;
+}
 template <int NB>
 struct Pages {
     uint32_t k[NB], v;
@@ -130,11 +138,6 @@ __device__ inline f32x16_t mfma32_bf16(uint4 a, uint4 b, f32x16_t c) {
 __device__ inline f32x16_t mfma32_f16(uint4 a, uint4 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
-// fp16 NaNs among two halves: all ones there, and 1.0 in their places.
-__device__ inline uint32_t nan_halves(uint32_t w) {
-    return ((w & 0x7fffu) > 0x7c00u ? 0xffffu : 0u) | ((w >> 16 & 0x7fffu) > 0x7c00u ? 0xffff0000u : 0u);
-}
-
 template <class T, int NB>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chunk(const ChunkArgs p) {
     constexpr int PARTS = QueryParts<T>::N, PIECES = 4 * NB;  // 16-byte pieces of a key's bytes
@@ -165,50 +168,82 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
         const uint32_t most = first_row < rows ? cache_seen(rq, (min(rows, first_row + kWaveRows) - 1) / a.c.group) : 0;
         const uint32_t* const table = a.table + uint64_t(request) * a.ld;
 
+        // Where this thread's bytes lie in a page, but for the tile's place in it (pages of 64 tokens and more).
+        const uint32_t in_page = (1u << a.c.page_log) - 1, all_seen = cache_seen(rq, row_tile * kRows / a.c.group);  // by every row
+        const uint64_t page_bytes = (uint64_t(a.c.kv_heads) << a.c.page_log) * a.c.dim;
+        uint32_t k_at[NB], v_at[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            k_at[i] = uint32_t(key_byte(a.c, 0, head, k_key + uint32_t(i) * (kThreads / PIECES))) + 16 * k_piece;
+            v_at[i] = uint32_t(value_byte(a.c, 0, head, 16 * v_group, v_col + 64 * uint32_t(i)));
+        }
         const auto load_pages = [&](uint32_t tile) {
             Pages<NB> g;
+            const uint32_t first = tile * kCacheTile, block = first >> a.c.page_log;
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
-                const uint32_t b = block_of(a.c, rq.keys, tile * kCacheTile + (k_key + uint32_t(i) * (kThreads / PIECES)) / 16 * 16);
-                g.k[i] = b == kNoPage ? b : table[b];
+                const uint32_t key = (k_key + uint32_t(i) * (kThreads / PIECES)) / 16 * 16;
+                g.k[i] = first + key < rq.keys ? table[block + (key >> a.c.page_log)] : kNoPage;
             }
-            const uint32_t b = block_of(a.c, rq.keys, tile * kCacheTile + 16 * v_group);
-            g.v = b == kNoPage ? b : table[b];
+            g.v = first + 16 * v_group < rq.keys ? table[block + (16 * v_group >> a.c.page_log)] : kNoPage;
             return g;
         };
         const auto load_bytes = [&](uint32_t tile, const Pages<NB>& g) {
             Bytes<NB> x;
+            if (tid < 4) {
+                const uint64_t place = uint64_t(some_page(a.c, g.v)) * a.c.kv_heads + head;
+                x.ks = g.v < a.c.pages ? a.scale * power_of_two(scale_exponent(a.k_scale[place])) : -1.0f;
+                x.vs = float(scale_exponent(a.v_scale[place]));
+            }
+            const uint32_t place = tile * kCacheTile & in_page;
+            const uint8_t* const v = a.v + place + some_page(a.c, g.v) * page_bytes;
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
-                const uint32_t key = tile * kCacheTile + k_key + uint32_t(i) * (kThreads / PIECES), col = v_col + 64 * uint32_t(i);
-                x.k[i] = 16 * k_piece < a.c.dim ? *reinterpret_cast<const uint4*>(a.k + key_byte(a.c, some_page(a.c, g.k[i]), head, key) + 16 * k_piece) : make_uint4(0, 0, 0, 0);
-                x.v[i] = col < a.c.dim ? *reinterpret_cast<const uint4*>(a.v + value_byte(a.c, some_page(a.c, g.v), head, tile * kCacheTile + 16 * v_group, col)) : make_uint4(0, 0, 0, 0);
-                // Values of no token count as 0.
-                const uint32_t from = tile * kCacheTile + 16 * v_group;
-                const int valid = g.v < a.c.pages ? int(min(rq.keys > from ? rq.keys - from : 0u, 16u)) : 0;
-                if (valid < 16) {
-                    x.v[i].x &= low_bytes(valid);
-                    x.v[i].y &= low_bytes(valid - 4);
-                    x.v[i].z &= low_bytes(valid - 8);
-                    x.v[i].w &= low_bytes(valid - 12);
-                }
+                const uint8_t* const k = a.k + place * a.c.dim + some_page(a.c, g.k[i]) * page_bytes;
+                x.k[i] = 16 * k_piece < a.c.dim ? *reinterpret_cast<const uint4*>(k + k_at[i]) : make_uint4(0, 0, 0, 0);
+                x.v[i] = v_col + 64 * uint32_t(i) < a.c.dim ? *reinterpret_cast<const uint4*>(v + v_at[i]) : make_uint4(0, 0, 0, 0);
             }
+            x.tokens = g.v < a.c.pages ? int(min(rq.keys - (tile * kCacheTile + 16 * v_group), 16u)) : 0;
             return x;
         };
-        const auto put = [&](int buffer, uint32_t* flag, const Bytes<NB>& x) {
-            uint32_t nan = 0;
+        const auto put = [&](uint32_t tile, Bytes<NB>& x) {
+            const uint32_t buffer = (tile - lo) % 2;
+            if (tid < 4) {
+                lds.scale[buffer][tid][0] = x.ks;
+                lds.scale[buffer][tid][1] = x.vs;
+            }
+            if (x.tokens < 16) {  // values of no token count as 0
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    x.v[i].x &= low_bytes(x.tokens);
+                    x.v[i].y &= low_bytes(x.tokens - 4);
+                    x.v[i].z &= low_bytes(x.tokens - 8);
+                    x.v[i].w &= low_bytes(x.tokens - 12);
+                }
+            }
+            if ((tile + 1) * kCacheTile > all_seen) {  // some rows do not see all of it: its NaNs stand as 0, and are marked
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    uint4& v = x.v[i];
+                    const uint32_t w[4] = {nan_bytes(v.x) >> 7, nan_bytes(v.y) >> 7, nan_bytes(v.z) >> 7, nan_bytes(v.w) >> 7};  // 1 in each byte
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) bits |= ((w[k] | w[k] >> 7 | w[k] >> 14 | w[k] >> 21) & 15u) << (4 * k);
+                    v = make_uint4(v.x & ~(w[0] * 0xffu), v.y & ~(w[1] * 0xffu), v.z & ~(w[2] * 0xffu), v.w & ~(w[3] * 0xffu));
+                    lds.bad[buffer][v_col + 64 * uint32_t(i)][v_group] = uint16_t(bits);
+                    if (bits) lds.nan[(tile - lo) % 4] = 1;  // (every writer writes the same)
+                }
+            }
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 const uint32_t key = k_key + uint32_t(i) * (kThreads / PIECES);
-                const uint32_t m = key / 32 * 32 + key / 16 % 2 * 16 + key / 4 % 2 * 8 + key / 8 % 2 * 4 + key % 4, turn = m % (8 * NB);
-                lds.k[buffer][m][(2 * k_piece) ^ turn] = keys_operand(x.k[i].x, x.k[i].y);
-                lds.k[buffer][m][(2 * k_piece + 1) ^ turn] = keys_operand(x.k[i].z, x.k[i].w);
+                const uint32_t m = key / 32 * 32 + key / 16 % 2 * 16 + key / 4 % 2 * 8 + key / 8 % 2 * 4 + key % 4;
+                lds.k[buffer][m][(2 * k_piece) ^ turned<8 * NB>(m)] = keys_operand(x.k[i].x, x.k[i].y);
+                lds.k[buffer][m][(2 * k_piece + 1) ^ turned<8 * NB>(m)] = keys_operand(x.k[i].z, x.k[i].w);
                 const uint32_t col = v_col + 64 * uint32_t(i);
-                lds.v[buffer][col][(2 * v_group) ^ (col % 8)] = values_operand(x.v[i].x, x.v[i].y);
-                lds.v[buffer][col][(2 * v_group + 1) ^ (col % 8)] = values_operand(x.v[i].z, x.v[i].w);
-                nan |= nan_bytes(x.v[i].x) | nan_bytes(x.v[i].y) | nan_bytes(x.v[i].z) | nan_bytes(x.v[i].w);
+                lds.v[buffer][col][(2 * v_group) ^ turned<8>(col)] = values_operand(x.v[i].x, x.v[i].y);
+                lds.v[buffer][col][(2 * v_group + 1) ^ turned<8>(col)] = values_operand(x.v[i].z, x.v[i].w);
             }
-            if (nan) *flag = 1;  // (every writer writes the same)
         };
 
         Pages<NB> pages = load_pages(lo);
@@ -229,49 +264,59 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
         float ref = kCacheNoRef, sum = 0.0f;
         if (tid < 4) lds.nan[tid] = 0;
         __syncthreads();
-        put(0, &lds.nan[0], bytes);
+        put(lo, bytes);
         if (lo + 1 < hi) {
             bytes = load_bytes(lo + 1, pages);
             pages = load_pages(lo + 2);
         }
         __syncthreads();
         for (uint32_t tile = lo; tile < hi; ++tile) {
-            const int buffer = int(tile - lo) & 1;
+            const uint32_t buffer = (tile - lo) % 2;
             if (tid == 0) lds.nan[(tile - lo + 2) % 4] = 0;  // (read two barriers ago, set again behind the next one)
             if (tile + 1 < hi) {
-                put(buffer ^ 1, &lds.nan[(tile - lo + 1) % 4], bytes);
+                put(tile + 1, bytes);
                 if (tile + 2 < hi) {
                     bytes = load_bytes(tile + 2, pages);
                     pages = load_pages(tile + 3);
                 }
             }
             if (tile * kCacheTile < most) {
-                // Scales of the tile's four pages of 16 keys, and which of them there are: the same in all lanes.
-                float by[4], back[4];
-                int ev[4];
+                // Of the tile's four 16 keys: scales, and whether they have a page.  The same in all lanes.
+                float by[4], ev[4];
                 uint32_t held = 0;
 #pragma unroll
-                for (uint32_t g = 0; g < 4; ++g) {
-                    const uint32_t b = block_of(a.c, rq.keys, tile * kCacheTile + 16 * g);
-                    const uint32_t page = b == kNoPage ? b : read_only(table)[b];
-                    if (page < a.c.pages) held |= 1u << g;
-                    const uint64_t place = uint64_t(some_page(a.c, page)) * a.c.kv_heads + head;
-                    by[g] = a.scale * power_of_two(scale_exponent(read_only(a.k_scale)[place]));
-                    ev[g] = scale_exponent(read_only(a.v_scale)[place]);
-                    back[g] = power_of_two(-ev[g]);
+                for (int g = 0; g < 4; ++g) {
+                    const uint32_t factor = uniform(__float_as_uint(lds.scale[buffer][g][0]));
+                    by[g] = __uint_as_float(factor & 0x7fffffffu);
+                    ev[g] = __uint_as_float(uniform(__float_as_uint(lds.scale[buffer][g][1])));
+                    if (!(factor >> 31)) held |= 1u << g;
                 }
                 f32x16_t s[2];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
+                for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
+                // Two chains of products; their keys are read two steps ahead.
+                uint4 keys[3][2];
+                const auto read_keys = [&](int c) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[k][r] = 0.0f;
+                    for (int k = 0; k < 2; ++k) keys[c % 3][k] = lds.k[buffer][32 * k + n][uint32_t(2 * c + h) ^ turned<8 * NB>(uint32_t(n))];
+                };
+                read_keys(0);
+                read_keys(1);
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                    for (int c = 0; c < 4 * NB; ++c) {
-                        const uint4 keys = lds.k[buffer][32 * k + n][(2 * c + h) ^ (n % (8 * NB))];
+                for (int c = 0; c < 4 * NB; ++c) {
+                    if (c + 2 < 4 * NB) read_keys(c + 2);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int part = PARTS - 1; part >= 0; --part) s[k] = mfma32_bf16(keys, q[c].w[part], s[k]);
-                    }
+                    for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) s[k] = mfma32_bf16(keys[c % 3][k], q[c].w[part], s[k]);
                 }
+                __builtin_amdgcn_s_setprio(0);
+                uint4 first[4];  // values of the first columns, for the second product
+#pragma unroll
+                for (int g = 0; g < 4; ++g) first[g] = lds.v[buffer][n][uint32_t(2 * g + h) ^ turned<8>(uint32_t(n))];
+                __builtin_amdgcn_sched_barrier(0);
                 const bool whole = (tile + 1) * kCacheTile <= least && held == 15;
                 if (!whole) {
 #pragma unroll
@@ -288,7 +333,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
                     float t = s[g / 2][8 * (g % 2)];
 #pragma unroll
                     for (int r = 1; r < 8; ++r) t = fmaxf(t, s[g / 2][8 * (g % 2) + r]);
-                    top = fmaxf(top, fmaf(t, by[g], float(ev[g])));
+                    top = fmaxf(top, fmaf(t, by[g], ev[g]));
                 }
                 if (__any(top > ref + kCacheRoom)) {
                     const float both = xor32_max(top);
@@ -304,14 +349,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
                 uint4 w[4], rest[4];
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const float shift = float(ev[g]) - ref;  // (whole numbers: exact)
+                    const float shift = ev[g] - ref;  // (whole numbers: exact)
                     float x[8], of = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
                         x[r] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + r], by[g], shift));
                         of += x[r];
                     }
-                    sum = fmaf(of, back[g], sum);
                     uint32_t u[4], l[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -321,37 +365,51 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
                             l[j] = f16x2(x[2 * j] - float(up[0]), x[2 * j + 1] - float(up[1]));
                         }
                     }
+                    sum = fmaf(of, power_of_two(-int(ev[g])), sum);
                     w[g] = make_uint4(u[0], u[1], u[2], u[3]);
                     if constexpr (PARTS > 1) rest[g] = make_uint4(l[0], l[1], l[2], l[3]);
                 }
-                const bool care = !whole && lds.nan[(tile - lo) % 4];  // a NaN that some rows see and others may not
+                if ((tile + 1) * kCacheTile > all_seen && lds.nan[(tile - lo) % 4]) {  // NaNs mark the rows that see them
 #pragma unroll
-                for (int d = 0; d < 2 * NB; ++d)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        uint4 x = lds.v[buffer][32 * d + n][(2 * g + h) ^ (n % 8)];
-                        if (care) {  // it counts as 0, and marks the rows that see it
-                            const uint4 bad = make_uint4(nan_halves(x.x), nan_halves(x.y), nan_halves(x.z), nan_halves(x.w));
-                            x = make_uint4(x.x & ~bad.x, x.y & ~bad.y, x.z & ~bad.z, x.w & ~bad.w);
-                            uint32_t u[4];
+                    for (int d = 0; d < 2 * NB; ++d)
+#pragma unroll 1
+                        for (int g = 0; g < 4; ++g) {
+                            const uint32_t bits = uint32_t(lds.bad[buffer][32 * d + n][g]) >> (8 * h);
+                            uint32_t x[4], u[4];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const uint32_t key = tile * kCacheTile + uint32_t(16 * g + 8 * h + 2 * j);
-                                const bool there = held >> g & 1;
-                                u[j] = (there && key < seen ? 0x3c00u : 0u) | (there && key + 1 < seen ? 0x3c000000u : 0u);
+                                x[j] = (bits >> (2 * j) & 1u ? 0x3c00u : 0u) | (bits >> (2 * j + 1) & 1u ? 0x3c000000u : 0u);
+                                u[j] = (key < seen ? 0x3c00u : 0u) | (key + 1 < seen ? 0x3c000000u : 0u);
                             }
                             f32x16_t count;
 #pragma unroll
                             for (int r = 0; r < 16; ++r) count[r] = 0.0f;
-                            count = mfma32_f16(make_uint4(bad.x & 0x3c003c00u, bad.y & 0x3c003c00u, bad.z & 0x3c003c00u, bad.w & 0x3c003c00u),
-                                               make_uint4(u[0], u[1], u[2], u[3]), count);
+                            count = mfma32_f16(make_uint4(x[0], x[1], x[2], x[3]), make_uint4(u[0], u[1], u[2], u[3]), count);
 #pragma unroll
                             for (int r = 0; r < 16; ++r)
                                 if (count[r] > 0.0f) o[d][r] = NAN;
                         }
-                        if constexpr (PARTS > 1) o[d] = mfma32_f16(x, rest[g], o[d]);
-                        o[d] = mfma32_f16(x, w[g], o[d]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                uint4 values[2][4];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) values[0][g] = first[g];
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int d = 0; d < 2 * NB; ++d) {
+                    if (d + 1 < 2 * NB) {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) values[(d + 1) % 2][g] = lds.v[buffer][32 * (d + 1) + n][uint32_t(2 * g + h) ^ turned<8>(uint32_t(n))];
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        if constexpr (PARTS > 1) o[d] = mfma32_f16(values[d % 2][g], rest[g], o[d]);
+                        o[d] = mfma32_f16(values[d % 2][g], w[g], o[d]);
+                    }
+                }
+                __builtin_amdgcn_s_setprio(0);
             }
             __syncthreads();
         }
