@@ -437,9 +437,9 @@ CacheSizes sizes_of(const gatgpu_cache* cache, const gatgpu_cache_attention_io* 
 }
 // Whether requests have rows enough for tiles of 128 packed ones.
 bool in_chunks(const CacheSizes& c) { return uint64_t(c.most) * c.group > 32; }
-uint64_t workspace_bytes(const gatgpu_ctx* c, const CacheSizes& s) {
+uint64_t workspace_bytes(const gatgpu_ctx* c, const CacheSizes& s, bool bf16) {
     const Workspace w = workspace_of(c, s);
-    return in_chunks(s) ? chunk_plan(c->cus, s).bytes : w.part + w.stat + w.meta;
+    return in_chunks(s) ? chunk_plan(c->cus, s, bf16).bytes : w.part + w.stat + w.meta;
 }
 
 }  // namespace
@@ -482,7 +482,7 @@ int gatgpu_cache_attention_workspace(gatgpu_ctx* c, const gatgpu_cache* cache, c
     if (!bytes) return fail(c, GATGPU_EINVAL, "null output");
     if (int r = check_cache(c, cache, false)) return r;
     if (int r = check_sizes(c, cache, io)) return r;
-    *bytes = workspace_bytes(c, sizes_of(cache, io));
+    *bytes = workspace_bytes(c, sizes_of(cache, io), io->precision == GATGPU_BF16);
     return GATGPU_OK;
 }
 
@@ -504,7 +504,7 @@ int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgp
         if (int r = check_words(c, "lse", io->lse)) return r;
     CacheAttnArgs a;
     a.c = sizes_of(cache, io);
-    const uint64_t need = workspace_bytes(c, a.c);
+    const uint64_t need = workspace_bytes(c, a.c, io->precision == GATGPU_BF16);
     if (bytes < need) return fail(c, GATGPU_EINVAL, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
     if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return fail(c, GATGPU_EINVAL, "workspace must be 16-byte aligned device memory");
     if (int r = check_device_array(c, ws, "workspace")) return r;
@@ -526,7 +526,7 @@ int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgp
     a.v_scale = cache->v_scale;
     const bool bf16 = io->precision == GATGPU_BF16, wide = cache->dim > 64;
     if (in_chunks(a.c)) {
-        HIPCHECK(c, launch_cache_chunk(a, bf16, chunk_plan(c->cus, a.c), ws, c->stream));
+        HIPCHECK(c, launch_cache_chunk(a, bf16, chunk_plan(c->cus, a.c, bf16), ws, c->stream));
         return GATGPU_OK;
     }
     const Workspace w = workspace_of(c, a.c);

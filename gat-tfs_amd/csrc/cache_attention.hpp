@@ -146,7 +146,7 @@ struct ChunkPlan {
     uint32_t workers = 0;  // of a key/value head
     uint64_t begin = 0, request = 0, upto = 0, part = 0, stat = 0, meta = 0, bytes = 0;  // offsets in the workspace
 };
-ChunkPlan chunk_plan(int cus, const CacheSizes& c);
+ChunkPlan chunk_plan(int cus, const CacheSizes& c, bool bf16);
 hipError_t launch_cache_chunk(const CacheAttnArgs& a, bool bf16, const ChunkPlan& plan, void* workspace, hipStream_t s);
 
 }  // namespace gatgpu

@@ -11,28 +11,30 @@
 // Work is cut into equal ranges of (row tile, key tile) for two blocks a unit, since lengths are known on the device only:
 // a first launch of one block forms the sums over the tiles, and a last one joins the tiles that a range's end cuts.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache_attention.hpp"
 
 namespace gatgpu {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / kWave, kScan = 1024;
-constexpr uint32_t kRows = 128, kWaveRows = 32;  // packed rows of a block and of a wave
+constexpr int kScan = 1024;
+constexpr uint32_t kWaveRows = 32;  // packed rows of a wave
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 struct ChunkArgs {
     CacheAttnArgs a;
     uint32_t tiles = 0;          // at most
+    uint32_t tile_rows = 0;      // packed rows of a block
     uint32_t* begin = nullptr;   // [requests + 1] first row tile of each request
     uint32_t* request = nullptr; // [tiles]
     uint64_t* upto = nullptr;    // [tiles + 1] key tiles of the row tiles before each
 };
 
-__device__ inline uint32_t chunk_tiles(const CacheSizes& c, const CacheRequest& q) { return (q.rows * c.group + kRows - 1) / kRows; }
+__device__ inline uint32_t chunk_tiles(const ChunkArgs& p, const CacheRequest& q) { return (q.rows * p.a.c.group + p.tile_rows - 1) / p.tile_rows; }
 // Key tiles that the rows of row tile t see (one, if none).
-__device__ inline uint32_t tiles_seen(const CacheSizes& c, const CacheRequest& q, uint32_t t) {
-    const uint32_t last = min(q.rows * c.group, (t + 1) * kRows) - 1, n = cache_seen(q, last / c.group);
+__device__ inline uint32_t tiles_seen(const ChunkArgs& p, const CacheRequest& q, uint32_t t) {
+    const uint32_t last = min(q.rows * p.a.c.group, (t + 1) * p.tile_rows) - 1, n = cache_seen(q, last / p.a.c.group);
     return n ? (n - 1) / kCacheTile + 1 : 1;
 }
 // The last i of [0, n) with first[i] <= x, for n >= 1, first[0] <= x: 64 places at a time, by a wave.
@@ -73,7 +75,7 @@ __global__ __launch_bounds__(kScan) void k_cache_plan(const ChunkArgs p) {
     uint64_t total, before = 0;
     for (uint32_t first = 0; first < a.c.requests; first += kScan) {
         const uint32_t r = first + tid;
-        const uint64_t n = r < a.c.requests ? chunk_tiles(a.c, request_of(a, r)) : 0, sum = scan_sums(n, total);
+        const uint64_t n = r < a.c.requests ? chunk_tiles(p, request_of(a, r)) : 0, sum = scan_sums(n, total);
         if (r < a.c.requests) p.begin[r] = index_min(before + sum - n, p.tiles);
         before += total;
     }
@@ -97,7 +99,7 @@ __global__ __launch_bounds__(kScan) void k_cache_plan(const ChunkArgs p) {
             p.request[t] = lo;
             const CacheRequest q = request_of(a, lo);
             const uint32_t own = t - p.begin[lo];
-            n = own < chunk_tiles(a.c, q) ? tiles_seen(a.c, q, own) : 0;
+            n = own < chunk_tiles(p, q) ? tiles_seen(p, q, own) : 0;
         }
         const uint64_t sum = scan_sums(n, total);
         if (t < tiles) p.upto[t + 1] = before + sum;
@@ -115,10 +117,10 @@ struct ChunkLds {
     uint32_t nan[4];       // the values of tile i (of a piece), in place i % 4, hold one
 };
 
-// What a thread requests of a tile, in 16 bytes: of NB keys each 16 columns, and of NB columns each 16 keys.
-template <int NB>
+// What a thread requests of a tile, in 16 bytes: of N keys each 16 columns, and of N columns each 16 keys.
+template <int N>
 struct Bytes {
-    uint4 k[NB], v[NB];
+    uint4 k[N], v[N];
     float ks, vs;  // scales of the 16 keys (of the first threads)
     int tokens;    // among the 16 keys of the values
 };
@@ -128,9 +130,9 @@ template <int PIECES>
 __device__ inline uint32_t turned(uint32_t row) {
     return PIECES == 16 ? row % 16 : row / 2 % 8;
 }
-template <int NB>
+template <int N>
 struct Pages {
-    uint32_t k[NB], v;
+    uint32_t k[N], v;
 };
 __device__ inline f32x16_t mfma32_bf16(uint4 a, uint4 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -138,9 +140,11 @@ __device__ inline f32x16_t mfma32_bf16(uint4 a, uint4 b, f32x16_t c) {
 __device__ inline f32x16_t mfma32_f16(uint4 a, uint4 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
-template <class T, int NB>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chunk(const ChunkArgs p) {
+template <class T, int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, sizeof(T) == 2 ? 2 : 1) void k_cache_chunk(const ChunkArgs p) {
     constexpr int PARTS = QueryParts<T>::N, PIECES = 4 * NB;  // 16-byte pieces of a key's bytes
+    constexpr int THREADS = WAVES * kWave, N = NB * 256 > THREADS ? NB * 256 / THREADS : 1;  // pieces of keys (of values) a thread
+    constexpr uint32_t ROWS = WAVES * kWaveRows, KEYS = THREADS / PIECES, COLS = THREADS / 4;  // keys and columns of a pass
     __shared__ ChunkLds<NB> lds;
     const CacheAttnArgs& a = p.a;
     const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave, n = lane % 32, h = lane / 32;
@@ -153,6 +157,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
     uint4 meta = make_uint4(0, 0, 0, 0);
     // What this thread brings of a tile: keys k_key + 32 i, columns 16 k_piece; columns v_col + 64 i, keys 16 v_group.
     const uint32_t k_key = uint32_t(tid) / PIECES, k_piece = uint32_t(tid) % PIECES, v_group = uint32_t(tid) % 4, v_col = uint32_t(tid) / 4;
+    const bool brings = THREADS <= NB * 256 || tid < NB * 256;
     uint32_t tile_at = at < end ? uniform(last_at_most(p.upto, tiles, at, lane)) : 0;
     for (; at < end; ++tile_at) {
         const uint64_t base = upto[tile_at], next_base = upto[tile_at + 1];
@@ -160,36 +165,36 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
         const uint32_t request = read_only(p.request)[tile_at], row_tile = tile_at - read_only(p.begin)[request];
         const CacheRequest rq = request_of(a, request);
         const uint32_t all = uint32_t(next_base - base), lo = uint32_t(at - base), hi = index_min(all, lo + (end - at));
-        const uint32_t packed = row_tile * kRows + uint32_t(wave) * kWaveRows + uint32_t(n), rows = rq.rows * a.c.group;
+        const uint32_t packed = row_tile * ROWS + uint32_t(wave) * kWaveRows + uint32_t(n), rows = rq.rows * a.c.group;
         const uint32_t seen = packed < rows ? cache_seen(rq, packed / a.c.group) : 0;
         // Rows of a wave stand in the order of their positions; a wave without rows sees nothing.
-        const uint32_t first_row = row_tile * kRows + uniform(uint32_t(wave)) * kWaveRows;
+        const uint32_t first_row = row_tile * ROWS + uniform(uint32_t(wave)) * kWaveRows;
         const uint32_t least = first_row < rows ? cache_seen(rq, first_row / a.c.group) : 0;
         const uint32_t most = first_row < rows ? cache_seen(rq, (min(rows, first_row + kWaveRows) - 1) / a.c.group) : 0;
         const uint32_t* const table = a.table + uint64_t(request) * a.ld;
 
         // Where this thread's bytes lie in a page, but for the tile's place in it (pages of 64 tokens and more).
-        const uint32_t in_page = (1u << a.c.page_log) - 1, all_seen = cache_seen(rq, row_tile * kRows / a.c.group);  // by every row
+        const uint32_t in_page = (1u << a.c.page_log) - 1, all_seen = cache_seen(rq, row_tile * ROWS / a.c.group);  // by every row
         const uint64_t page_bytes = (uint64_t(a.c.kv_heads) << a.c.page_log) * a.c.dim;
-        uint32_t k_at[NB], v_at[NB];
+        uint32_t k_at[N], v_at[N];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            k_at[i] = uint32_t(key_byte(a.c, 0, head, k_key + uint32_t(i) * (kThreads / PIECES))) + 16 * k_piece;
-            v_at[i] = uint32_t(value_byte(a.c, 0, head, 16 * v_group, v_col + 64 * uint32_t(i)));
+        for (int i = 0; i < N; ++i) {
+            k_at[i] = uint32_t(key_byte(a.c, 0, head, k_key + uint32_t(i) * KEYS)) + 16 * k_piece;
+            v_at[i] = uint32_t(value_byte(a.c, 0, head, 16 * v_group, v_col + COLS * uint32_t(i)));
         }
         const auto load_pages = [&](uint32_t tile) {
-            Pages<NB> g;
+            Pages<N> g;
             const uint32_t first = tile * kCacheTile, block = first >> a.c.page_log;
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                const uint32_t key = (k_key + uint32_t(i) * (kThreads / PIECES)) / 16 * 16;
+            for (int i = 0; i < N; ++i) {
+                const uint32_t key = (k_key + uint32_t(i) * KEYS) / 16 * 16;
                 g.k[i] = first + key < rq.keys ? table[block + (key >> a.c.page_log)] : kNoPage;
             }
             g.v = first + 16 * v_group < rq.keys ? table[block + (16 * v_group >> a.c.page_log)] : kNoPage;
             return g;
         };
-        const auto load_bytes = [&](uint32_t tile, const Pages<NB>& g) {
-            Bytes<NB> x;
+        const auto load_bytes = [&](uint32_t tile, const Pages<N>& g) {
+            Bytes<N> x;
             if (tid < 4) {
                 const uint64_t place = uint64_t(some_page(a.c, g.v)) * a.c.kv_heads + head;
                 x.ks = g.v < a.c.pages ? a.scale * power_of_two(scale_exponent(a.k_scale[place])) : -1.0f;
@@ -198,15 +203,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
             const uint32_t place = tile * kCacheTile & in_page;
             const uint8_t* const v = a.v + place + some_page(a.c, g.v) * page_bytes;
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
+            for (int i = 0; i < N; ++i) {
                 const uint8_t* const k = a.k + place * a.c.dim + some_page(a.c, g.k[i]) * page_bytes;
-                x.k[i] = 16 * k_piece < a.c.dim ? *reinterpret_cast<const uint4*>(k + k_at[i]) : make_uint4(0, 0, 0, 0);
-                x.v[i] = v_col + 64 * uint32_t(i) < a.c.dim ? *reinterpret_cast<const uint4*>(v + v_at[i]) : make_uint4(0, 0, 0, 0);
+                x.k[i] = brings && 16 * k_piece < a.c.dim ? *reinterpret_cast<const uint4*>(k + k_at[i]) : make_uint4(0, 0, 0, 0);
+                x.v[i] = brings && v_col + COLS * uint32_t(i) < a.c.dim ? *reinterpret_cast<const uint4*>(v + v_at[i]) : make_uint4(0, 0, 0, 0);
             }
             x.tokens = g.v < a.c.pages ? int(min(rq.keys - (tile * kCacheTile + 16 * v_group), 16u)) : 0;
             return x;
         };
-        const auto put = [&](uint32_t tile, Bytes<NB>& x) {
+        const auto put = [&](uint32_t tile, Bytes<N>& x) {
+            if (!brings) return;
             const uint32_t buffer = (tile - lo) % 2;
             if (tid < 4) {
                 lds.scale[buffer][tid][0] = x.ks;
@@ -214,7 +220,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
             }
             if (x.tokens < 16) {  // values of no token count as 0
 #pragma unroll
-                for (int i = 0; i < NB; ++i) {
+                for (int i = 0; i < N; ++i) {
                     x.v[i].x &= low_bytes(x.tokens);
                     x.v[i].y &= low_bytes(x.tokens - 4);
                     x.v[i].z &= low_bytes(x.tokens - 8);
@@ -223,31 +229,31 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
             }
             if ((tile + 1) * kCacheTile > all_seen) {  // some rows do not see all of it: its NaNs stand as 0, and are marked
 #pragma unroll
-                for (int i = 0; i < NB; ++i) {
+                for (int i = 0; i < N; ++i) {
                     uint4& v = x.v[i];
                     const uint32_t w[4] = {nan_bytes(v.x) >> 7, nan_bytes(v.y) >> 7, nan_bytes(v.z) >> 7, nan_bytes(v.w) >> 7};  // 1 in each byte
                     uint32_t bits = 0;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) bits |= ((w[k] | w[k] >> 7 | w[k] >> 14 | w[k] >> 21) & 15u) << (4 * k);
                     v = make_uint4(v.x & ~(w[0] * 0xffu), v.y & ~(w[1] * 0xffu), v.z & ~(w[2] * 0xffu), v.w & ~(w[3] * 0xffu));
-                    lds.bad[buffer][v_col + 64 * uint32_t(i)][v_group] = uint16_t(bits);
+                    lds.bad[buffer][v_col + COLS * uint32_t(i)][v_group] = uint16_t(bits);
                     if (bits) lds.nan[(tile - lo) % 4] = 1;  // (every writer writes the same)
                 }
             }
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                const uint32_t key = k_key + uint32_t(i) * (kThreads / PIECES);
+            for (int i = 0; i < N; ++i) {
+                const uint32_t key = k_key + uint32_t(i) * KEYS;
                 const uint32_t m = key / 32 * 32 + key / 16 % 2 * 16 + key / 4 % 2 * 8 + key / 8 % 2 * 4 + key % 4;
                 lds.k[buffer][m][(2 * k_piece) ^ turned<8 * NB>(m)] = keys_operand(x.k[i].x, x.k[i].y);
                 lds.k[buffer][m][(2 * k_piece + 1) ^ turned<8 * NB>(m)] = keys_operand(x.k[i].z, x.k[i].w);
-                const uint32_t col = v_col + 64 * uint32_t(i);
+                const uint32_t col = v_col + COLS * uint32_t(i);
                 lds.v[buffer][col][(2 * v_group) ^ turned<8>(col)] = values_operand(x.v[i].x, x.v[i].y);
                 lds.v[buffer][col][(2 * v_group + 1) ^ turned<8>(col)] = values_operand(x.v[i].z, x.v[i].w);
             }
         };
 
-        Pages<NB> pages = load_pages(lo);
-        Bytes<NB> bytes = load_bytes(lo, pages);
+        Pages<N> pages = load_pages(lo);
+        Bytes<N> bytes = load_bytes(lo, pages);
         pages = load_pages(lo + 1);
         QueryParts<T> q[4 * NB];
         const T* const row = query_row<T>(a, rq, packed, head);
@@ -294,28 +300,30 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
                 f32x16_t s[2];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
-                // Two chains of products; their keys are read two steps ahead.
-                uint4 keys[3][2];
+                // Two chains of products; their keys are read a step ahead.
+                uint4 keys[2][2];
                 const auto read_keys = [&](int c) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) keys[c % 3][k] = lds.k[buffer][32 * k + n][uint32_t(2 * c + h) ^ turned<8 * NB>(uint32_t(n))];
+                    for (int k = 0; k < 2; ++k) keys[c % 2][k] = lds.k[buffer][32 * k + n][uint32_t(2 * c + h) ^ turned<8 * NB>(uint32_t(n))];
                 };
                 read_keys(0);
-                read_keys(1);
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int c = 0; c < 4 * NB; ++c) {
-                    if (c + 2 < 4 * NB) read_keys(c + 2);
+                    if (c + 1 < 4 * NB) read_keys(c + 1);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int part = PARTS - 1; part >= 0; --part)
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) s[k] = mfma32_bf16(keys[c % 3][k], q[c].w[part], s[k]);
+                        for (int k = 0; k < 2; ++k) s[k] = mfma32_bf16(keys[c % 2][k], q[c].w[part], s[k]);
                 }
                 __builtin_amdgcn_s_setprio(0);
-                uint4 first[4];  // values of the first columns, for the second product
+                uint4 values[2][2 * NB];  // of 16 keys, for the second product: the first ones are there when their weights are
+                const auto read_values = [&](int g) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) first[g] = lds.v[buffer][n][uint32_t(2 * g + h) ^ turned<8>(uint32_t(n))];
+                    for (int d = 0; d < 2 * NB; ++d) values[g % 2][d] = lds.v[buffer][32 * d + n][uint32_t(2 * g + h) ^ turned<8>(uint32_t(n))];
+                };
+                read_values(0);
                 __builtin_amdgcn_sched_barrier(0);
                 const bool whole = (tile + 1) * kCacheTile <= least && held == 15;
                 if (!whole) {
@@ -392,22 +400,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
                         }
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                uint4 values[2][4];
-#pragma unroll
-                for (int g = 0; g < 4; ++g) values[0][g] = first[g];
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int d = 0; d < 2 * NB; ++d) {
-                    if (d + 1 < 2 * NB) {
-#pragma unroll
-                        for (int g = 0; g < 4; ++g) values[(d + 1) % 2][g] = lds.v[buffer][32 * (d + 1) + n][uint32_t(2 * g + h) ^ turned<8>(uint32_t(n))];
-                    }
+                for (int g = 0; g < 4; ++g) {
+                    if (g + 1 < 4) read_values(g + 1);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        if constexpr (PARTS > 1) o[d] = mfma32_f16(values[d % 2][g], rest[g], o[d]);
-                        o[d] = mfma32_f16(values[d % 2][g], w[g], o[d]);
-                    }
+                    for (int part = 0; part < (PARTS > 1 ? 2 : 1); ++part)
+#pragma unroll
+                        for (int d = 0; d < 2 * NB; ++d) o[d] = mfma32_f16(values[g % 2][d], PARTS > 1 && part == 0 ? rest[g] : w[g], o[d]);
                 }
                 __builtin_amdgcn_s_setprio(0);
             }
@@ -415,7 +416,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
         }
         sum = xor32_add(sum);
         const bool cut = lo > 0 || hi < all;
-        const uint64_t piece = (uint64_t(blockIdx.x) * 2 + (lo > 0 ? 0 : 1)) * kWaves + uint64_t(wave);
+        const uint64_t piece = (uint64_t(blockIdx.x) * 2 + (lo > 0 ? 0 : 1)) * WAVES + uint64_t(wave);
 #pragma unroll
         for (int d = 0; d < 2 * NB; ++d)
 #pragma unroll
@@ -440,8 +441,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void k_cache_chun
 }
 
 // The pieces of the row tile that begins in a worker and ends in another: a wave its 32 rows, four columns of each lane a block.
-template <class T, int NB>
-__global__ __launch_bounds__(kThreads) void k_cache_chunk_join(const ChunkArgs p) {
+template <class T, int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void k_cache_chunk_join(const ChunkArgs p) {
     const CacheAttnArgs& a = p.a;
     const uint4 meta = a.meta[blockIdx.x];
     if (!meta.z) return;
@@ -450,7 +451,7 @@ __global__ __launch_bounds__(kThreads) void k_cache_chunk_join(const ChunkArgs p
     f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
     float ref = kCacheNoRef, sum = 0.0f;
     for (uint32_t i = 0; i < meta.z; ++i) {
-        const uint64_t piece = ((uint64_t(blockIdx.x) + uint64_t(i) * a.c.kv_heads) * 2 + (i ? 0 : 1)) * kWaves + uint64_t(wave);
+        const uint64_t piece = ((uint64_t(blockIdx.x) + uint64_t(i) * a.c.kv_heads) * 2 + (i ? 0 : 1)) * WAVES + uint64_t(wave);
         const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part + ((piece * (8 * NB) + which) * kWave + uint64_t(lane)) * 4);
         const float r = a.stat[piece * 64 + uint64_t(n)], s = a.stat[piece * 64 + 32 + uint64_t(n)];
         const float top = fmaxf(ref, r), less = __builtin_amdgcn_exp2f(ref - top), more = __builtin_amdgcn_exp2f(r - top);
@@ -459,30 +460,34 @@ __global__ __launch_bounds__(kThreads) void k_cache_chunk_join(const ChunkArgs p
         ref = top;
     }
     const CacheRequest rq = request_of(a, meta.x);
-    const uint32_t packed = meta.y * kRows + uint32_t(wave) * kWaveRows + uint32_t(n);
+    const uint32_t packed = meta.y * (WAVES * kWaveRows) + uint32_t(wave) * kWaveRows + uint32_t(n);
     store4<T>(a, rq, packed, head, which / 4 * 32 + which % 4 * 8 + 4 * uint32_t(h), o, sum);
     if (which == 0 && lane < 32) store_lse(a, rq, packed, head, ref, sum);
 }
 
 uint64_t pad256(uint64_t b) { return (b + 255) / 256 * 256; }
 
-template <class T, int NB>
+template <class T, int NB, int WAVES>
 hipError_t launch(const ChunkArgs& p, hipStream_t s) {
     const uint32_t blocks = p.a.workers * p.a.c.kv_heads;
     k_cache_plan<<<1, kScan, 0, s>>>(p);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    k_cache_chunk<T, NB><<<blocks, kThreads, 0, s>>>(p);
+    k_cache_chunk<T, NB, WAVES><<<blocks, WAVES * kWave, 0, s>>>(p);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    k_cache_chunk_join<T, NB><<<dim3(blocks, 8 * NB), kThreads, 0, s>>>(p);
+    k_cache_chunk_join<T, NB, WAVES><<<dim3(blocks, 8 * NB), WAVES * kWave, 0, s>>>(p);
     return hipGetLastError();
 }
+// Waves a block: eight where requests may fill them, since a tile is then brought and turned for twice the rows (FP32's
+// products need twice the registers, and leave room for four).
+int waves_of(const CacheSizes& c, bool bf16) { return bf16 && uint64_t(c.most) * c.group > 4 * kWaveRows ? 8 : 4; }
 
 }  // namespace
 
-ChunkPlan chunk_plan(int cus, const CacheSizes& c) {
+ChunkPlan chunk_plan(int cus, const CacheSizes& c, bool bf16) {
     ChunkPlan p;
-    p.tiles = uint32_t(c.rows * c.group / kRows + c.requests);  // a request's last tile may be part full
-    p.workers = uint32_t(std::max(1, 2 * cus / int(c.kv_heads)));
+    const uint32_t tile = uint32_t(waves_of(c, bf16)) * kWaveRows;
+    p.tiles = uint32_t(c.rows * c.group / tile + c.requests);  // a request's last tile may be part full
+    p.workers = uint32_t(std::max(1, (bf16 && waves_of(c, bf16) == 4 ? 2 : 1) * cus / int(c.kv_heads)));
     const uint64_t blocks = uint64_t(p.workers) * c.kv_heads, nb = c.dim > 64 ? 2 : 1;
     uint64_t at = 0;
     const auto take = [&](uint64_t bytes) {
@@ -493,8 +498,8 @@ ChunkPlan chunk_plan(int cus, const CacheSizes& c) {
     p.begin = take((uint64_t(c.requests) + 1) * 4);
     p.request = take(uint64_t(p.tiles) * 4);
     p.upto = take((uint64_t(p.tiles) + 1) * 8);
-    p.part = take(blocks * 2 * kRows * 64 * nb * 4);
-    p.stat = take(blocks * 2 * kRows * 8);
+    p.part = take(blocks * 2 * tile * 64 * nb * 4);
+    p.stat = take(blocks * 2 * tile * 8);
     p.meta = take(blocks * 16);
     p.bytes = at;
     return p;
@@ -506,6 +511,8 @@ hipError_t launch_cache_chunk(const CacheAttnArgs& args, bool bf16, const ChunkP
     p.a.workers = plan.workers;
     char* const ws = static_cast<char*>(workspace);
     p.tiles = plan.tiles;
+    const int waves = waves_of(args.c, bf16);
+    p.tile_rows = uint32_t(waves) * kWaveRows;
     p.begin = reinterpret_cast<uint32_t*>(ws + plan.begin);
     p.request = reinterpret_cast<uint32_t*>(ws + plan.request);
     p.upto = reinterpret_cast<uint64_t*>(ws + plan.upto);
@@ -513,7 +520,12 @@ hipError_t launch_cache_chunk(const CacheAttnArgs& args, bool bf16, const ChunkP
     p.a.stat = reinterpret_cast<float*>(ws + plan.stat);
     p.a.meta = reinterpret_cast<uint4*>(ws + plan.meta);
     const bool wide = args.c.dim > 64;
-    return bf16 ? (wide ? launch<uint16_t, 2>(p, s) : launch<uint16_t, 1>(p, s)) : (wide ? launch<float, 2>(p, s) : launch<float, 1>(p, s));
+    const auto as = [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        return wide ? launch<uint16_t, 2, W>(p, s) : launch<uint16_t, 1, W>(p, s);
+    };
+    if (bf16) return waves == 8 ? as(std::integral_constant<int, 8>{}) : as(std::integral_constant<int, 4>{});
+    return wide ? launch<float, 2, 4>(p, s) : launch<float, 1, 4>(p, s);
 }
 
 }  // namespace gatgpu
