@@ -13,7 +13,7 @@
 namespace gatgpu {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kJoinWaves = 4;
 
 // The queries of a wave's 16 rows as operands.
 template <class T, int NB>
@@ -38,8 +38,12 @@ __device__ inline Queries<T, NB> load_queries(const CacheAttnArgs& a, const Cach
 
 // A tile's bytes as they come: keys [operand][64 columns], values [16 columns], and the scales of the lane's 16 keys.
 template <int NB>
-struct Tile {
-    uint4 k[4][NB], v[4 * NB];
+struct Keys {
+    uint4 w[4][NB];
+};
+template <int NB>
+struct Values {
+    uint4 w[4 * NB];
     float ks, vs;
     bool page;  // the lane's keys have one
 };
@@ -55,24 +59,25 @@ __device__ inline TilePages tile_pages(const CacheAttnArgs& a, const uint32_t* r
     return {own == kNoPage ? own : row[own], load == kNoPage ? load : row[load]};
 }
 template <int NB>
-__device__ inline Tile<NB> load_tile(const CacheAttnArgs& a, TilePages p, uint32_t tile, uint32_t head, int lane) {
-    Tile<NB> t;
-    const uint32_t m = uint32_t(lane % 16), g = uint32_t(lane / 16);
-    t.page = p.own < a.c.pages;
-    const uint32_t own = some_page(a.c, p.own);
-    const uint8_t* const k = a.k + key_byte(a.c, some_page(a.c, p.load), head, loaded_key(tile, lane)) + 16 * g;
+__device__ inline void load_keys(const CacheAttnArgs& a, uint32_t page, uint32_t tile, uint32_t head, int lane, Keys<NB>& t) {
+    const uint32_t g = uint32_t(lane / 16);
+    const uint8_t* const k = a.k + key_byte(a.c, some_page(a.c, page), head, loaded_key(tile, lane)) + 16 * g;
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i)
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b)
-            t.k[i][b] = 64 * b + 16 * g < a.c.dim ? *reinterpret_cast<const uint4*>(k + i * 4 * a.c.dim + 64 * b) : make_uint4(0, 0, 0, 0);
-    const uint8_t* const v = a.v + value_byte(a.c, own, head, own_key(tile, lane), m);
-#pragma unroll
-    for (uint32_t d = 0; d < 4 * NB; ++d)
-        t.v[d] = 16 * d < a.c.dim ? *reinterpret_cast<const uint4*>(v + (uint64_t(16 * d) << a.c.page_log)) : make_uint4(0, 0, 0, 0);
+            t.w[i][b] = 64 * b + 16 * g < a.c.dim ? *reinterpret_cast<const uint4*>(k + i * 4 * a.c.dim + 64 * b) : make_uint4(0, 0, 0, 0);
+}
+template <int NB>
+__device__ inline void load_values(const CacheAttnArgs& a, uint32_t page, uint32_t tile, uint32_t head, int lane, Values<NB>& t) {
+    t.page = page < a.c.pages;
+    const uint32_t own = some_page(a.c, page);
     t.ks = a.k_scale[uint64_t(own) * a.c.kv_heads + head];
     t.vs = a.v_scale[uint64_t(own) * a.c.kv_heads + head];
-    return t;
+    const uint8_t* const v = a.v + value_byte(a.c, own, head, own_key(tile, lane), uint32_t(lane % 16));
+#pragma unroll
+    for (uint32_t d = 0; d < 4 * NB; ++d)
+        t.w[d] = 16 * d < a.c.dim ? *reinterpret_cast<const uint4*>(v + (uint64_t(16 * d) << a.c.page_log)) : make_uint4(0, 0, 0, 0);
 }
 
 // A wave's running softmax: lane (n, g) has row n's reference, the weights' sum of its own keys, and its columns' sums.
@@ -82,37 +87,51 @@ struct Running {
     float ref, sum;
 };
 
-// One step: 64 keys.  seen: keys that the lane's row sees; least, most: of the wave's rows; keys: of the request.
-template <class T, int NB>
-__device__ inline void step(const CacheAttnArgs& a, Running<NB>& run, const Queries<T, NB>& q, Tile<NB>& t, uint32_t tile, uint32_t keys, uint32_t seen,
-                            uint32_t least, int lane) {
-    constexpr int PARTS = Queries<T, NB>::PARTS;
-    const uint32_t first = tile * kCacheTile + 16u * uint32_t(lane / 16);
+// Scores of a tile: keys [operand][register] by the lane's row.
+struct Scores {
     f32x4_t s[4];
+};
+template <class T, int NB>
+__device__ inline Scores scores(const Queries<T, NB>& q, const Keys<NB>& t) {
+    Scores x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        s[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const uint4 lo = keys_operand(t.k[i][b].x, t.k[i][b].y), hi = keys_operand(t.k[i][b].z, t.k[i][b].w);
+            const uint4 lo = keys_operand(t.w[i][b].x, t.w[i][b].y), hi = keys_operand(t.w[i][b].z, t.w[i][b].w);
 #pragma unroll
-            for (int p = PARTS - 1; p >= 0; --p) {
-                s[i] = mfma_bf16(lo, q.w[b][0].w[p], s[i]);
-                s[i] = mfma_bf16(hi, q.w[b][1].w[p], s[i]);
+            for (int p = Queries<T, NB>::PARTS - 1; p >= 0; --p) {
+                s = mfma_bf16(lo, q.w[b][0].w[p], s);
+                s = mfma_bf16(hi, q.w[b][1].w[p], s);
             }
         }
+        x.s[i] = s;
     }
+    return x;
+}
+// The weights of a tile's keys as operands: fp16, and what their rounding took (FP32).
+struct Weights {
+    uint4 w[2], rest[2];
+};
+// seen: keys that the lane's row sees; whole: every row of the wave sees every key of the tile.
+template <int PARTS, int NB>
+__device__ inline Weights weigh(const CacheAttnArgs& a, Running<NB>& run, Scores x, const Values<NB>& t, uint32_t tile, uint32_t seen, bool whole, int lane) {
     const int ev = scale_exponent(t.vs);
     const float by = a.scale * power_of_two(scale_exponent(t.ks));
-    const bool whole = tile * kCacheTile + kCacheTile <= least && __all(t.page);  // every row sees every key
+    if (!whole) {
+        const uint32_t first = own_key(tile, lane), here = t.page && seen > first ? seen - first : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (uint32_t(4 * i + r) >= here) x.s[i][r] = -INFINITY;
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (!whole && !(t.page && first + uint32_t(4 * i + r) < seen)) s[i][r] = -INFINITY;
-            top = fmaxf(top, s[i][r]);
-        }
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, x.s[i][r]);
     top = fmaf(top, by, float(ev));
     if (__any(top > run.ref + kCacheRoom)) {
         const float all = xor32_max(xor16_max(top));
@@ -129,92 +148,93 @@ __device__ inline void step(const CacheAttnArgs& a, Running<NB>& run, const Quer
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], by, shift));
-            sum += s[i][r];
+            x.s[i][r] = __builtin_amdgcn_exp2f(fmaf(x.s[i][r], by, shift));
+            sum += x.s[i][r];
         }
     run.sum = fmaf(sum, power_of_two(-ev), run.sum);
-    uint4 w[2], rest[2];
+    Weights w;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         uint32_t u[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float x = s[2 * h + j / 2][j % 2 * 2], y = s[2 * h + j / 2][j % 2 * 2 + 1];
-            u[j] = f16x2(x, y);
+            const float v0 = x.s[2 * h + j / 2][j % 2 * 2], v1 = x.s[2 * h + j / 2][j % 2 * 2 + 1];
+            u[j] = f16x2(v0, v1);
             if constexpr (PARTS > 1) {
                 const f16x2_t up = __builtin_bit_cast(f16x2_t, u[j]);
-                l[j] = f16x2(x - float(up[0]), y - float(up[1]));
+                l[j] = f16x2(v0 - float(up[0]), v1 - float(up[1]));
             }
         }
-        w[h] = make_uint4(u[0], u[1], u[2], u[3]);
-        if constexpr (PARTS > 1) rest[h] = make_uint4(l[0], l[1], l[2], l[3]);
+        w.w[h] = make_uint4(u[0], u[1], u[2], u[3]);
+        if constexpr (PARTS > 1) w.rest[h] = make_uint4(l[0], l[1], l[2], l[3]);
     }
-    bool bad = false;
-    if (!whole) {
-        // Values of no token count as 0; a NaN that some rows see and others do not needs care.
-        const int valid = t.page ? int(min(keys > first ? keys - first : 0u, 16u)) : 0;
-        uint32_t nan = 0;
-#pragma unroll
-        for (int d = 0; d < 4 * NB; ++d) {
-            t.v[d].x &= low_bytes(valid);
-            t.v[d].y &= low_bytes(valid - 4);
-            t.v[d].z &= low_bytes(valid - 8);
-            t.v[d].w &= low_bytes(valid - 12);
-            nan |= nan_bytes(t.v[d].x) | nan_bytes(t.v[d].y) | nan_bytes(t.v[d].z) | nan_bytes(t.v[d].w);
-        }
-        bad = __any(nan != 0);
-    }
-    if (bad) {
-        uint32_t u[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t at = first + uint32_t(2 * j);
-            u[j] = (t.page && at < seen ? 0x3c00u : 0u) | (t.page && at + 1 < seen ? 0x3c000000u : 0u);
-        }
-        const uint4 one[2] = {make_uint4(u[0], u[1], u[2], u[3]), make_uint4(u[4], u[5], u[6], u[7])};
-#pragma unroll
-        for (int d = 0; d < 4 * NB; ++d) {
-            uint32_t* const c[4] = {&t.v[d].x, &t.v[d].y, &t.v[d].z, &t.v[d].w};
-            uint32_t mark[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t n = nan_bytes(*c[j]) >> 7;  // 1 at each NaN
-                *c[j] &= ~(n * 0xffu);
-                mark[j] = n * 0x38u;  // 1.0 in e4m3
-            }
-            f32x4_t count = {0.0f, 0.0f, 0.0f, 0.0f};
-            count = mfma_f16(values_operand(mark[0], mark[1]), one[0], count);
-            count = mfma_f16(values_operand(mark[2], mark[3]), one[1], count);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (count[r] > 0.0f) run.o[d][r] = NAN;
-        }
-    }
+    return w;
+}
+// A tile that some rows do not see whole: values of no token count as 0, and a NaN that some rows see counts as 0 and marks them.
+template <int NB>
+__device__ inline void clean(Running<NB>& run, Values<NB>& t, uint32_t tile, uint32_t keys, uint32_t seen, int lane) {
+    const uint32_t first = own_key(tile, lane);
+    const int valid = t.page && keys > first ? int(min(keys - first, 16u)) : 0;
+    uint32_t nan = 0;
 #pragma unroll
     for (int d = 0; d < 4 * NB; ++d) {
-        const uint4 lo = values_operand(t.v[d].x, t.v[d].y), hi = values_operand(t.v[d].z, t.v[d].w);
-        if constexpr (PARTS > 1) {
-            run.o[d] = mfma_f16(lo, rest[0], run.o[d]);
-            run.o[d] = mfma_f16(hi, rest[1], run.o[d]);
+        t.w[d].x &= low_bytes(valid);
+        t.w[d].y &= low_bytes(valid - 4);
+        t.w[d].z &= low_bytes(valid - 8);
+        t.w[d].w &= low_bytes(valid - 12);
+        nan |= nan_bytes(t.w[d].x) | nan_bytes(t.w[d].y) | nan_bytes(t.w[d].z) | nan_bytes(t.w[d].w);
+    }
+    if (!__any(nan != 0)) return;
+    const uint32_t here = t.page && seen > first ? seen - first : 0;
+    uint32_t u[8];
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) u[j] = (2 * j < here ? 0x3c00u : 0u) | (2 * j + 1 < here ? 0x3c000000u : 0u);
+#pragma unroll
+    for (int d = 0; d < 4 * NB; ++d) {
+        uint32_t mark[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t& c = (&t.w[d].x)[j];
+            const uint32_t n = nan_bytes(c) >> 7;  // 1 at each NaN
+            c &= ~(n * 0xffu);
+            mark[j] = n * 0x38u;  // 1.0 in e4m3
         }
-        run.o[d] = mfma_f16(lo, w[0], run.o[d]);
-        run.o[d] = mfma_f16(hi, w[1], run.o[d]);
+        f32x4_t count = {0.0f, 0.0f, 0.0f, 0.0f};
+        count = mfma_f16(values_operand(mark[0], mark[1]), make_uint4(u[0], u[1], u[2], u[3]), count);
+        count = mfma_f16(values_operand(mark[2], mark[3]), make_uint4(u[4], u[5], u[6], u[7]), count);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (count[r] > 0.0f) run.o[d][r] = NAN;
+    }
+}
+template <int PARTS, int NB>
+__device__ inline void add_values(Running<NB>& run, const Weights& w, const Values<NB>& t) {
+#pragma unroll
+    for (int d = 0; d < 4 * NB; ++d) {
+        const uint4 lo = values_operand(t.w[d].x, t.w[d].y), hi = values_operand(t.w[d].z, t.w[d].w);
+        if constexpr (PARTS > 1) {
+            run.o[d] = mfma_f16(lo, w.rest[0], run.o[d]);
+            run.o[d] = mfma_f16(hi, w.rest[1], run.o[d]);
+        }
+        run.o[d] = mfma_f16(lo, w.w[0], run.o[d]);
+        run.o[d] = mfma_f16(hi, w.w[1], run.o[d]);
     }
 }
 
-// Sums of the four waves: [wave][columns / 16][lane] columns, [wave][row] references and weights.
-template <int NB>
+// Sums of the waves: [wave][columns / 16][lane] columns, [wave][row] references and weights.
+template <int NB, int WAVES>
 struct JoinLds {
-    f32x4_t o[kWaves][4 * NB][kWave];
-    float ref[kWaves][kCacheRows], sum[kWaves][kCacheRows];
+    f32x4_t o[WAVES][4 * NB][kWave];
+    float ref[WAVES][kCacheRows], sum[WAVES][kCacheRows];
 };
 
-// 8 waves a unit hide their requests behind each other; a wave has a tile's 16 KB (128 columns) in flight while it works
-// on the one before.
-template <class T, int NB>
-__global__ __launch_bounds__(kThreads, 2) void k_cache_attention(const CacheAttnArgs a) {
-    __shared__ JoinLds<NB> join;
-    __shared__ uint64_t s_sum[kWaves], s_start;
+// Two waves a SIMD hide their requests behind each other.  (Three, with 168 registers each, keep a part of them in memory:
+// 142 us against 96 for one token over 260K, 32 heads of 128 on 8.)
+template <class T, int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void k_cache_attention(const CacheAttnArgs a) {
+    constexpr int PARTS = Queries<T, NB>::PARTS;
+    __shared__ JoinLds<NB, WAVES> join;
+    __shared__ uint64_t s_sum[WAVES], s_start;
     __shared__ uint32_t s_request;
     const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
     const uint32_t head = blockIdx.x % a.c.kv_heads;
@@ -222,7 +242,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_cache_attention(const CacheAttn
     uint64_t at = 0, end = 0, base = 0, share = 1;  // the worker's tiles, and those before its request
     uint32_t request = worker;
     if (a.workers) {
-        const uint32_t per = (a.c.requests + kThreads - 1) / kThreads, from = min(a.c.requests, uint32_t(tid) * per), to = min(a.c.requests, from + per);
+        const uint32_t per = (a.c.requests + (WAVES * kWave) - 1) / (WAVES * kWave), from = min(a.c.requests, uint32_t(tid) * per), to = min(a.c.requests, from + per);
         uint64_t own = 0;
         for (uint32_t r = from; r < to; ++r) {
             const CacheRequest q = request_of(a, r);
@@ -238,7 +258,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_cache_attention(const CacheAttn
         __syncthreads();
         uint64_t total = 0;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             if (w < wave) upto += s_sum[w];
             total += s_sum[w];
         }
@@ -296,16 +316,27 @@ __global__ __launch_bounds__(kThreads, 2) void k_cache_attention(const CacheAttn
         const uint32_t stop = min(hi, (most + kCacheTile - 1) / kCacheTile);
         uint32_t tile = lo + uint32_t(wave);
         if (tile < stop) {
-            Tile<NB> now = load_tile<NB>(a, tile_pages(a, row, rq.keys, tile, lane), tile, head, lane);
-            TilePages ahead = tile_pages(a, row, rq.keys, tile + kWaves, lane);
-            for (; tile < stop; tile += kWaves) {
-                Tile<NB> next = now;
-                if (tile + kWaves < stop) {
-                    next = load_tile<NB>(a, ahead, tile + kWaves, head, lane);
-                    ahead = tile_pages(a, row, rq.keys, tile + 2 * kWaves, lane);
-                }
-                step<T, NB>(a, run, q, now, tile, rq.keys, seen, least, lane);
-                now = next;
+            // A tile's keys are requested when the scores of the one before are formed, its values when those are added.
+            TilePages pages = tile_pages(a, row, rq.keys, tile, lane);
+            Keys<NB> k;
+            Values<NB> v;
+            load_keys<NB>(a, pages.load, tile, head, lane, k);
+            load_values<NB>(a, pages.own, tile, head, lane, v);
+            pages = tile_pages(a, row, rq.keys, tile + WAVES, lane);
+            while (true) {
+                const Scores x = scores<T, NB>(q, k);
+                __builtin_amdgcn_sched_barrier(0);
+                const uint32_t next = tile + WAVES;
+                if (next < stop) load_keys<NB>(a, pages.load, next, head, lane, k);
+                const bool whole = tile * kCacheTile + kCacheTile <= least && __all(v.page);  // every row sees every key
+                const Weights w = weigh<PARTS, NB>(a, run, x, v, tile, seen, whole, lane);
+                if (!whole) clean<NB>(run, v, tile, rq.keys, seen, lane);
+                add_values<PARTS, NB>(run, w, v);
+                __builtin_amdgcn_sched_barrier(0);
+                if (next >= stop) break;
+                load_values<NB>(a, pages.own, next, head, lane, v);
+                pages = tile_pages(a, row, rq.keys, next + WAVES, lane);
+                tile = next;
             }
         }
         run.sum = xor32_add(xor16_add(run.sum));
@@ -317,22 +348,21 @@ __global__ __launch_bounds__(kThreads, 2) void k_cache_attention(const CacheAttn
 #pragma unroll
         for (int d = 0; d < 4 * NB; ++d) join.o[wave][d][lane] = run.o[d];
         __syncthreads();
-        float ref = join.ref[0][n], sum = 0.0f, less[kWaves];
+        float ref = join.ref[0][n], sum = 0.0f, less[WAVES];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) ref = fmaxf(ref, join.ref[w][n]);
+        for (int w = 1; w < WAVES; ++w) ref = fmaxf(ref, join.ref[w][n]);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             less[w] = __builtin_amdgcn_exp2f(join.ref[w][n] - ref);
             sum = fmaf(join.sum[w][n], less[w], sum);
         }
         const bool cut = lo > 0 || hi < tiles;
         const uint64_t piece = (uint64_t(blockIdx.x) * 2 + (lo > 0 ? 0 : 1));
 #pragma unroll
-        for (int d = 0; d < NB; ++d) {
-            const int db = wave * NB + d;
+        for (int db = wave; db < 4 * NB; db += WAVES) {
             f32x4_t o = join.o[0][db][lane] * less[0];
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) o += join.o[w][db][lane] * less[w];
+            for (int w = 1; w < WAVES; ++w) o += join.o[w][db][lane] * less[w];
             if (cut) *reinterpret_cast<f32x4_t*>(a.part + ((piece * (4 * NB) + uint64_t(db)) * kWave + uint64_t(lane)) * 4) = o;
             else store4<T>(a, rq, packed, head, uint32_t(16 * db + 4 * g), o, sum);
         }
@@ -356,9 +386,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_cache_attention(const CacheAttn
 
 // The pieces of the task that begins in a worker and ends in another: 16 columns a block, its waves a quarter of the pieces each.
 template <class T, int NB>
-__global__ __launch_bounds__(kThreads) void k_cache_join(const CacheAttnArgs a) {
-    __shared__ f32x4_t s_o[kWaves][kWave];
-    __shared__ float s_ref[kWaves][kCacheRows], s_sum[kWaves][kCacheRows];
+__global__ __launch_bounds__(kJoinWaves * kWave) void k_cache_join(const CacheAttnArgs a) {
+    __shared__ f32x4_t s_o[kJoinWaves][kWave];
+    __shared__ float s_ref[kJoinWaves][kCacheRows], s_sum[kJoinWaves][kCacheRows];
     const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
     const uint32_t block = blockIdx.x, db = blockIdx.y;
     const uint4 meta = a.meta[block];
@@ -367,14 +397,15 @@ __global__ __launch_bounds__(kThreads) void k_cache_join(const CacheAttnArgs a) 
     const auto piece_of = [&](uint32_t p) { return (uint64_t(block) + uint64_t(p) * uint64_t(a.c.kv_heads)) * 2 + (p ? 0 : 1); };
     f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
     float ref = kCacheNoRef, sum = 0.0f;
-    for (uint32_t p = uint32_t(wave); p < meta.z; p += kWaves) {
+#pragma unroll 4
+    for (uint32_t p = uint32_t(wave); p < meta.z; p += kJoinWaves) ref = fmaxf(ref, a.stat[piece_of(p) * 32 + uint64_t(n)]);
+#pragma unroll 4
+    for (uint32_t p = uint32_t(wave); p < meta.z; p += kJoinWaves) {
         const uint64_t piece = piece_of(p);
         const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part + ((piece * (4 * NB) + db) * kWave + uint64_t(lane)) * 4);
-        const float r = a.stat[piece * 32 + uint64_t(n)], s = a.stat[piece * 32 + 16 + uint64_t(n)];
-        const float top = fmaxf(ref, r), less = __builtin_amdgcn_exp2f(ref - top), more = __builtin_amdgcn_exp2f(r - top);
-        o = o * less + x * more;
-        sum = sum * less + s * more;
-        ref = top;
+        const float less = __builtin_amdgcn_exp2f(a.stat[piece * 32 + uint64_t(n)] - ref);
+        o += x * less;
+        sum = fmaf(a.stat[piece * 32 + 16 + uint64_t(n)], less, sum);
     }
     s_o[wave][lane] = o;
     if (lane < 16) {
@@ -385,11 +416,11 @@ __global__ __launch_bounds__(kThreads) void k_cache_join(const CacheAttnArgs a) 
     if (wave) return;
     float top = s_ref[0][n];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_ref[w][n]);
+    for (int w = 1; w < kJoinWaves; ++w) top = fmaxf(top, s_ref[w][n]);
     o = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kJoinWaves; ++w) {
         const float less = __builtin_amdgcn_exp2f(s_ref[w][n] - top);
         o += s_o[w][lane] * less;
         sum = fmaf(s_sum[w][n], less, sum);
@@ -400,16 +431,19 @@ __global__ __launch_bounds__(kThreads) void k_cache_join(const CacheAttnArgs a) 
     if (db == 0 && lane < 16) store_lse(a, rq, packed, head, top, sum);
 }
 
-// Blocks a key/value head: two a unit in all.
+// Blocks a key/value head: three a unit in all.
 uint32_t cache_workers(const gatgpu_ctx* c, int kv_heads) { return uint32_t(std::max(1, 2 * c->cus / kv_heads)); }
 
 template <class T, int NB>
 hipError_t launch(const CacheAttnArgs& a, hipStream_t s) {
     const uint32_t blocks = (a.workers ? a.workers : a.c.requests) * a.c.kv_heads;
-    k_cache_attention<T, NB><<<blocks, kThreads, 0, s>>>(a);
-    if (!a.workers) return hipGetLastError();
+    if (!a.workers) {
+        k_cache_attention<T, NB, 8><<<blocks, 8 * kWave, 0, s>>>(a);
+        return hipGetLastError();
+    }
+    k_cache_attention<T, NB, 4><<<blocks, 4 * kWave, 0, s>>>(a);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    k_cache_join<T, NB><<<dim3(blocks, uint32_t(a.c.dim / 16)), kThreads, 0, s>>>(a);
+    k_cache_join<T, NB><<<dim3(blocks, uint32_t(a.c.dim / 16)), kJoinWaves * kWave, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -508,7 +542,8 @@ int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgp
     if (bytes < need) return fail(c, GATGPU_EINVAL, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
     if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return fail(c, GATGPU_EINVAL, "workspace must be 16-byte aligned device memory");
     if (int r = check_device_array(c, ws, "workspace")) return r;
-    a.workers = cache_workers(c, cache->kv_heads);
+    // Where no request has more than 16 tiles: a block a request, nothing to join.
+    a.workers = uint64_t(a.c.blocks) << a.c.page_log <= 16 * kCacheTile ? 0 : cache_workers(c, cache->kv_heads);
     a.least = 4;
     a.scale = io->scale * 1.44269504088896341f;
     a.ld = io->table_stride;
