@@ -4,20 +4,23 @@
 //   pages of request r: free[count - 1 - k], k from the exclusive sum of need;  slot = table[pos / page] page + pos % page
 //
 // Bound by a launch and its chain of dependent reads (lengths, sums over the requests, a row's request, its page):
-// one block forms the sums over the requests, 1024 at a time, and, where the batch is small, goes on with the
+// one block forms the sums over the requests, 4096 at a time, and, where the batch is small, goes on with the
 // rows from LDS; else a second launch finds each row's request by bisection.  A new block's page is taken from the
 // list by each of its rows, so that no row waits for the table; the row at offset 0 writes it there.
 #include <algorithm>
 #include <string>
 
+#include "cache_index.hpp"
 #include "context.hpp"
 
 namespace gatgpu {
 namespace {
 
-constexpr int kScan = 1024;                        // threads of a block that sums, and requests at a time
+constexpr int kScan = 1024;                        // threads of a block that sums
+constexpr uint32_t kEach = 4;                      // requests of each of them at a time, where there are many
 constexpr uint32_t kOneBlockRows = 8192;           // rows that the block of the sums takes itself
-constexpr uint32_t kOneBlockRelease = 256;         // requests of a release in one block
+constexpr uint32_t kOneBlockRelease = 64;          // requests of a release in one block
+constexpr uint32_t kFewCounts = 16384;             // counts that each block of a release sums itself
 constexpr uint32_t kMaxRequests = 1u << 20;
 
 struct BlocksArgs {
@@ -93,8 +96,8 @@ __device__ inline uint32_t find_request(P begin, uint32_t n, uint32_t row) {
     return lo;
 }
 
-// Sums over the requests; ROWS: the rows as well (at most kScan requests).
-template <bool ROWS>
+// Sums over the requests, EACH of a thread at a time; ROWS: the rows as well (at most kScan requests).
+template <bool ROWS, uint32_t EACH>
 __global__ __launch_bounds__(kScan) void k_blocks_assign(const BlocksArgs a) {
     __shared__ uint32_t s_left, s_unserved;
     __shared__ uint32_t s_begin[ROWS ? kScan + 1 : 1], s_len[ROWS ? kScan : 1], s_behind[ROWS ? kScan : 1];
@@ -108,34 +111,51 @@ __global__ __launch_bounds__(kScan) void k_blocks_assign(const BlocksArgs a) {
     }
     __syncthreads();
     Sums before = {0, 0};
-    for (uint32_t first = 0; first < a.requests; first += kScan) {
-        const uint32_t r = first + tid;
-        const bool there = r < a.requests;
-        const uint64_t c = there ? a.cached[r] : 0, f = there ? a.fresh[r] : 0, page = uint64_t(1) << a.page_log;
-        const bool fits = c + f <= uint64_t(a.blocks) << a.page_log;
-        const uint64_t need = fits ? ((c + f + page - 1) >> a.page_log) - ((c + page - 1) >> a.page_log) : 0;
+    for (uint32_t first = 0; first < a.requests; first += kScan * EACH) {
+        const uint64_t page = uint64_t(1) << a.page_log;
+        uint64_t c[EACH], f[EACH], need[EACH];
+        Sums own = {0, 0};
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) {
+            const uint32_t r = first + tid * EACH + i;
+            c[i] = r < a.requests ? a.cached[r] : 0;
+            f[i] = r < a.requests ? a.fresh[r] : 0;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) {
+            const bool fits = c[i] + f[i] <= uint64_t(a.blocks) << a.page_log;
+            need[i] = fits ? ((c[i] + f[i] + page - 1) >> a.page_log) - ((c[i] + page - 1) >> a.page_log) : 0;
+            own.pages += need[i];
+            own.rows += f[i];
+        }
         Sums total;
-        Sums upto = block_sums({need, f}, total);
-        upto.pages += before.pages;
-        upto.rows += before.rows;
+        const Sums all = block_sums(own, total);
+        Sums upto = {before.pages + all.pages - own.pages, before.rows + all.rows - own.rows};
         before.pages += total.pages;
         before.rows += total.rows;
-        if (!there) continue;
-        const bool served = fits && (need == 0 || upto.pages <= count) && upto.rows <= a.rows;
-        const uint32_t behind = uint32_t(upto.pages - need), len = served ? uint32_t(c + f) : 0;
-        const uint32_t end = upto.rows > 0xffffffffu ? 0xffffffffu : uint32_t(upto.rows);
-        a.stored[r] = uint32_t(served ? c + f : c);
-        a.k_len[r] = len;
-        a.q_begin[r + 1] = end;
-        if (ROWS) {
-            s_begin[r + 1] = end;
-            s_len[r] = len;
-            s_behind[r] = behind;
-        } else {
-            a.behind[r] = behind;
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) {
+            const uint32_t r = first + tid * EACH + i;
+            if (r >= a.requests) break;
+            upto.pages += need[i];
+            upto.rows += f[i];
+            const bool fits = c[i] + f[i] <= uint64_t(a.blocks) << a.page_log;
+            const bool served = fits && (need[i] == 0 || upto.pages <= count) && upto.rows <= a.rows;
+            const uint32_t behind = uint32_t(upto.pages - need[i]), len = served ? uint32_t(c[i] + f[i]) : 0;
+            const uint32_t end = upto.rows > 0xffffffffu ? 0xffffffffu : uint32_t(upto.rows);
+            a.stored[r] = uint32_t(served ? c[i] + f[i] : c[i]);
+            a.k_len[r] = len;
+            a.q_begin[r + 1] = end;
+            if (ROWS) {
+                s_begin[r + 1] = end;
+                s_len[r] = len;
+                s_behind[r] = behind;
+            } else {
+                a.behind[r] = behind;
+            }
+            if (served && need[i]) atomicMin(&s_left, count - uint32_t(upto.pages));
+            if (!served) atomicAdd(&s_unserved, 1u);
         }
-        if (served && need) atomicMin(&s_left, count - uint32_t(upto.pages));
-        if (!served) atomicAdd(&s_unserved, 1u);
     }
     __syncthreads();
     if (tid == 0) {
@@ -184,16 +204,34 @@ __device__ inline uint32_t give_back(const BlocksArgs& a, uint32_t r, uint64_t p
     return found;
 }
 __global__ __launch_bounds__(256) void k_release_count(const BlocksArgs a) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.count = min(*a.free_count, a.pages);
     const uint32_t r = blockIdx.x * 4 + threadIdx.x / kWave;
     if (r >= a.requests) return;
     const uint32_t n = give_back<false>(a, r, 0);
     if (threadIdx.x % kWave == 0) a.behind[r] = n;
 }
+// A block's four requests, behind the sum of the counts before them.
+__global__ __launch_bounds__(256) void k_release_write(const BlocksArgs a) {
+    __shared__ uint64_t s_sum[4];
+    const uint32_t first = blockIdx.x * 4, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    uint64_t sum = 0;
+    for (uint32_t r = threadIdx.x; r < first; r += 256) sum += a.behind[r];
+#pragma unroll
+    for (int d = kWave / 2; d; d /= 2) sum += __shfl_xor(sum, d);
+    if (lane == 0) s_sum[wave] = sum;
+    __syncthreads();
+    uint64_t place = uint64_t(*a.count) + s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+    for (uint32_t r = first; r < a.requests && r < first + 4; ++r) {
+        if (r == first + wave) (void)give_back<true>(a, r, place);
+        place += a.behind[r];
+    }
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *a.free_left = index_min(place, a.pages);
+}
 // Counts to sums; ALL: counts and writes too (at most kOneBlockRelease requests).
 template <bool ALL>
 __global__ __launch_bounds__(kScan) void k_release(const BlocksArgs a) {
     __shared__ uint32_t s_count[ALL ? kOneBlockRelease : 1];
-    const uint32_t tid = threadIdx.x, count = min(*a.free_count, a.pages);
+    const uint32_t tid = threadIdx.x, count = ALL ? min(*a.free_count, a.pages) : *a.count;
     if constexpr (ALL) {
         for (uint32_t r = tid / kWave; r < a.requests; r += kScan / kWave) {
             const uint32_t n = give_back<false>(a, r, 0);
@@ -217,13 +255,13 @@ __global__ __launch_bounds__(kScan) void k_release(const BlocksArgs a) {
     }
     __syncthreads();
     if (tid == 0) {
-        if (!ALL) *a.count = count;
         *a.free_left = uint32_t(min(uint64_t(count) + before, uint64_t(a.pages)));
     }
     if constexpr (ALL)
         for (uint32_t r = tid / kWave; r < a.requests; r += kScan / kWave) (void)give_back<true>(a, r, uint64_t(count) + s_count[r]);
 }
-__global__ __launch_bounds__(256) void k_release_write(const BlocksArgs a) {
+// The same, behind sums that k_release has formed.
+__global__ __launch_bounds__(256) void k_release_place(const BlocksArgs a) {
     const uint32_t r = blockIdx.x * 4 + threadIdx.x / kWave;
     if (r < a.requests) (void)give_back<true>(a, r, uint64_t(*a.count) + a.behind[r]);
 }
@@ -315,11 +353,12 @@ int gatgpu_blocks_assign(gatgpu_ctx* c, const gatgpu_blocks_io* io, void* ws, ui
     if (int r = check_words(c, "unserved", io->unserved)) return r;
     const BlocksArgs a = make_args(io, ws);
     if (a.requests <= uint32_t(kScan) && a.rows <= kOneBlockRows) {
-        k_blocks_assign<true><<<1, kScan, 0, c->stream>>>(a);
+        k_blocks_assign<true, 1><<<1, kScan, 0, c->stream>>>(a);
         HIPCHECK(c, hipGetLastError());
         return GATGPU_OK;
     }
-    k_blocks_assign<false><<<1, kScan, 0, c->stream>>>(a);
+    if (a.requests <= uint32_t(kScan)) k_blocks_assign<false, 1><<<1, kScan, 0, c->stream>>>(a);
+    else k_blocks_assign<false, kEach><<<1, kScan, 0, c->stream>>>(a);
     HIPCHECK(c, hipGetLastError());
     if (!a.rows) return GATGPU_OK;
     k_blocks_rows<<<std::min((a.rows + 255) / 256, 1u << 14), 256, 0, c->stream>>>(a);
@@ -340,9 +379,14 @@ int gatgpu_blocks_release(gatgpu_ctx* c, const gatgpu_blocks_io* io, void* ws, u
     }
     k_release_count<<<(a.requests + 3) / 4, 256, 0, c->stream>>>(a);
     HIPCHECK(c, hipGetLastError());
+    if (a.requests <= kFewCounts) {
+        k_release_write<<<(a.requests + 3) / 4, 256, 0, c->stream>>>(a);
+        HIPCHECK(c, hipGetLastError());
+        return GATGPU_OK;
+    }
     k_release<false><<<1, kScan, 0, c->stream>>>(a);
     HIPCHECK(c, hipGetLastError());
-    k_release_write<<<(a.requests + 3) / 4, 256, 0, c->stream>>>(a);
+    k_release_place<<<(a.requests + 3) / 4, 256, 0, c->stream>>>(a);
     HIPCHECK(c, hipGetLastError());
     return GATGPU_OK;
 }

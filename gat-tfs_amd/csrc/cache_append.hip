@@ -16,6 +16,7 @@ namespace gatgpu {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr uint32_t kShort = 4;  // tokens of a page that a wave takes by itself
 constexpr int kMaxPage = 256, kMaxDim = 128, kTurnPad = 4;
 
 struct AppendArgs {
@@ -118,34 +119,161 @@ __device__ inline uint32_t block_max(uint32_t x, uint32_t* words) {
     return max(max(words[0], words[1]), max(words[2], words[3]));
 }
 
-// A thread takes 16 bytes of four neighbouring tokens: a row's bytes lie in neighbouring lanes, and four tokens' values of a
-// column make one word of the page's column.
+// Where the new tokens of a page go, for one head and side.
+template <class T>
+struct Run {
+    const T* x;       // the first one's row
+    uint64_t stride;  // from row to row
+    uint8_t* to;      // the page's bytes
+    float* scale;
+    uint32_t off;     // tokens before them
+};
+template <class T>
+__device__ inline Run<T> run_at(const AppendArgs& a, uint64_t row, uint32_t slot, int head, int side) {
+    Run<T> r;
+    const uint64_t place = uint64_t(slot / a.page) * uint64_t(a.kv_heads) + uint64_t(head);
+    r.x = static_cast<const T*>(a.x[side]) + row * a.xs[side] + uint64_t(head) * uint64_t(a.dim);
+    r.stride = a.xs[side];
+    r.to = a.cache[side] + place * a.page * uint64_t(a.dim);
+    r.scale = a.scale[side] + place;
+    r.off = slot % a.page;
+    return r;
+}
+// Piece i of four neighbouring tokens' rows: i / per fours, i % per pieces of 16 bytes.
+template <class T>
+__device__ inline Quad load_quad(const Run<T>& r, uint32_t tokens, uint32_t per, uint32_t i) {
+    constexpr uint32_t N = 16 / sizeof(T);
+    Quad q;
+    const uint32_t t = i / per * 4;
+    const T* const p = r.x + uint64_t(t) * r.stride + uint64_t(i % per) * N;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) q.row[k] = t + k < tokens ? *reinterpret_cast<const uint4*>(p + k * r.stride) : make_uint4(0, 0, 0, 0);
+    return q;
+}
+// Bytes of the tokens that stay, from exponent `had` to e, by `threads` threads.
+__device__ inline void grow(uint8_t* to, uint32_t off, uint32_t page, uint32_t dim, int had, int e, int side, uint32_t thread, uint32_t threads) {
+    const float by = power_of_two(had - e < -126 ? -126 : had - e);
+    if (side == 0) {
+        uint32_t* const w = reinterpret_cast<uint32_t*>(to);
+        for (uint32_t i = thread; i < off * dim / 4; i += threads) w[i] = round_again(w[i], by);
+    } else {
+        const uint32_t words = (off + 3) / 4;
+        for (uint32_t i = thread; i < words * dim; i += threads) {
+            const uint32_t at = i % words * 4;
+            uint32_t* const w = reinterpret_cast<uint32_t*>(to + uint64_t(i / words) * page + at);
+            const uint32_t stay = off - at >= 4 ? 0xffffffffu : (1u << (8 * (off - at))) - 1;
+            *w = (round_again(*w, by) & stay) | (*w & ~stay);
+        }
+    }
+}
+// A piece's tokens t ... t + 3 as keys: N columns of a token side by side.
+template <class T>
+__device__ inline void put_keys(uint8_t* to, uint32_t dim, uint32_t tokens, uint32_t t, const uint32_t (&u)[4][16 / sizeof(T)], float by) {
+    constexpr int N = 16 / int(sizeof(T));
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+        if (t + k >= tokens) break;
+        uint32_t w[N / 4];
+#pragma unroll
+        for (int c = 0; c < N / 4; ++c) {
+            const uint32_t v[4] = {u[k][4 * c], u[k][4 * c + 1], u[k][4 * c + 2], u[k][4 * c + 3]};
+            w[c] = round4(v, by);
+        }
+        uint32_t* const p = reinterpret_cast<uint32_t*>(to + uint64_t(k) * dim);
+        if constexpr (N == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        else *p = w[0];
+    }
+}
+
+// A page's few tokens, by a wave: a lane a piece of the rows.
+template <class T>
+__device__ inline void append_short(const AppendArgs& a, uint64_t row, uint32_t tokens, int head, int side) {
+    constexpr int N = 16 / int(sizeof(T));
+    const uint32_t lane = threadIdx.x % kWave, per = uint32_t(a.dim) / N, page = a.page;
+    const Run<T> r = run_at<T>(a, row, a.slot[row], head, side);
+    const float scale = *r.scale;
+    Quad q{};
+    if (lane < per) q = load_quad(r, tokens, per, lane);
+    uint32_t top = largest<T>(q);
+#pragma unroll
+    for (int d = kWave / 2; d; d /= 2) top = max(top, uint32_t(__shfl_xor(int(top), d)));
+    if (top >= kInfinity) {  // NaN and infinities leave the scale alone
+        top = largest_finite<T>(q);
+#pragma unroll
+        for (int d = kWave / 2; d; d /= 2) top = max(top, uint32_t(__shfl_xor(int(top), d)));
+    }
+    const int had = r.off ? scale_exponent(scale) : kLeastScale, e = max(exponent_for(top), had);
+    if (r.off && e > had) {
+        grow(r.to, r.off, page, uint32_t(a.dim), had, e, side, lane, kWave);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");  // (words that hold new tokens too are written before these)
+    }
+    if (lane == 0) *r.scale = power_of_two(e);
+    if (lane >= per) return;
+    const float by = power_of_two(-e);
+    uint32_t u[4][N];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) widen<T>(q.row[k], u[k]);
+    if (side == 0) {
+        put_keys<T>(r.to + uint64_t(r.off) * uint64_t(a.dim) + lane * N, uint32_t(a.dim), tokens, 0, u, by);
+    } else {
+#pragma unroll
+        for (uint32_t c = 0; c < uint32_t(N); ++c) {
+            const uint32_t v[4] = {u[0][c], u[1][c], u[2][c], u[3][c]}, w = round4(v, by);
+            uint8_t* const p = r.to + uint64_t(lane * N + c) * page + r.off;
+            for (uint32_t k = 0; k < tokens; ++k) p[k] = uint8_t(w >> (8 * k));
+        }
+    }
+}
+
+// A block looks for the first tokens of pages among `chunk` rows.  A page's few tokens (a request's new one) are a wave's,
+// others the block's: a thread takes 16 bytes of four neighbouring tokens, a row's bytes lie in neighbouring lanes, and four
+// tokens' values of a column make one word of the page's column.
 template <class T>
 __global__ __launch_bounds__(kThreads, 4) void k_cache_append(const AppendArgs a) {
     constexpr int N = 16 / int(sizeof(T));  // values of 16 bytes
     extern __shared__ uint32_t turn[];      // values: [dim][page + kTurnPad] bytes
     __shared__ uint32_t s_word[kThreads / kWave];
-    __shared__ uint64_t s_starts;
+    __shared__ uint64_t s_starts, s_goes_on;
     const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
     const int head = int(blockIdx.y), side = int(blockIdx.z);
     const uint64_t first = uint64_t(blockIdx.x) * a.chunk;
     const uint32_t page = a.page, turn_row = (page + kTurnPad) / 4, per = uint32_t(a.dim) / N;  // words, 16-byte pieces a token
     if (wave == 0) {
         const uint64_t row = first + uint64_t(lane);
-        bool start = false;
-        if (uint32_t(lane) < a.chunk && row < a.rows) {
+        bool there = false, goes_on = false;  // goes on: the token after that of the row before, in its page
+        if (row < a.rows) {
             const uint32_t s = a.slot[row], before = row ? a.slot[row - 1] : GATGPU_NO_PAGE;
-            start = s < a.slots && (row == 0 || s % page == 0 || before + 1 != s);
+            there = s < a.slots;
+            goes_on = there && row && s % page && before + 1 == s;
         }
-        const uint64_t some = __ballot(start);
-        if (lane == 0) s_starts = some;
+        const uint64_t on = __ballot(goes_on), starts = __ballot(there && !goes_on && uint32_t(lane) < a.chunk);
+        if (lane == 0) {
+            s_starts = starts;
+            s_goes_on = on;
+        }
     }
     __syncthreads();
-    for (uint64_t starts = s_starts; starts; starts &= starts - 1) {
-        const uint64_t row = first + uint64_t(__builtin_ctzll(starts));
-        const uint32_t slot = a.slot[row], off = slot % page;
-        const uint64_t place = uint64_t(slot / page) * uint64_t(a.kv_heads) + uint64_t(head);
-        const float scale = a.scale[side][place];
+    const uint64_t starts = s_starts, goes_on = s_goes_on;
+    uint64_t longer = 0;  // starts of more than kShort tokens: the next kShort rows (there are as many lanes) go on
+    {
+        uint64_t all = starts;
+#pragma unroll
+        for (uint32_t i = 1; i <= kShort; ++i) all &= goes_on >> i;
+        longer = all;
+    }
+    uint32_t number = 0;
+    for (uint64_t left = starts & ~longer; left; left &= left - 1, ++number) {
+        if (int(number % (kThreads / kWave)) != wave) continue;
+        const uint32_t at = uint32_t(__builtin_ctzll(left));
+        const uint32_t tokens = 1 + uint32_t(__builtin_ctzll(~(goes_on >> 1 >> at)));
+        append_short<T>(a, first + at, tokens, head, side);
+    }
+    for (uint64_t left = longer; left; left &= left - 1) {
+        const uint64_t row = first + uint64_t(__builtin_ctzll(left));
+        const uint32_t slot = a.slot[row];
+        const Run<T> r = run_at<T>(a, row, slot, head, side);
+        const uint32_t off = r.off;
+        const float scale = *r.scale;
         // Tokens of this page: rows as long as their slots go on.
         const bool more = row + uint64_t(tid) < a.rows && off + uint32_t(tid) < page && a.slot[row + uint64_t(tid)] == slot + uint32_t(tid);
         const uint64_t on = __ballot(more);
@@ -158,46 +286,20 @@ __global__ __launch_bounds__(kThreads, 4) void k_cache_append(const AppendArgs a
             if (s_word[w] < uint32_t(kWave)) break;
         }
         const uint32_t quads = (tokens + 3) / 4 * per;
-        const T* const x = static_cast<const T*>(a.x[side]) + row * a.xs[side] + uint64_t(head) * uint64_t(a.dim);
-        const auto load = [&](uint32_t i) {
-            Quad q;
-            const uint32_t t = i / per * 4;
-            const T* const p = x + uint64_t(t) * a.xs[side] + uint64_t(i % per) * N;
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k)
-                q.row[k] = t + k < tokens ? *reinterpret_cast<const uint4*>(p + k * a.xs[side]) : make_uint4(0, 0, 0, 0);
-            return q;
-        };
         Quad held{};  // the thread's first one; more than 256 of them are read again
-        if (uint32_t(tid) < quads) held = load(uint32_t(tid));
+        if (uint32_t(tid) < quads) held = load_quad(r, tokens, per, uint32_t(tid));
         uint32_t top = largest<T>(held);
-        for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) top = max(top, largest<T>(load(i)));
+        for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) top = max(top, largest<T>(load_quad(r, tokens, per, i)));
         top = block_max(top, s_word);
-        if (top >= kInfinity) {  // NaN and infinities leave the scale alone
+        if (top >= kInfinity) {
             top = largest_finite<T>(held);
-            for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) top = max(top, largest_finite<T>(load(i)));
+            for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) top = max(top, largest_finite<T>(load_quad(r, tokens, per, i)));
             top = block_max(top, s_word);
         }
-        uint8_t* const to = a.cache[side] + place * page * uint64_t(a.dim);
-        const int had = off ? scale_exponent(scale) : kLeastScale;
-        const int e = max(exponent_for(top), had);
-        if (off && e > had) {  // the page's scale grows under the tokens that stay
-            const float by = power_of_two(had - e < -126 ? -126 : had - e);
-            if (side == 0) {
-                uint32_t* const w = reinterpret_cast<uint32_t*>(to);
-                for (uint32_t i = uint32_t(tid); i < off * uint32_t(a.dim) / 4; i += kThreads) w[i] = round_again(w[i], by);
-            } else {
-                const uint32_t words = (off + 3) / 4;
-                for (uint32_t i = uint32_t(tid); i < words * uint32_t(a.dim); i += kThreads) {
-                    const uint32_t at = i % words * 4;
-                    uint32_t* const w = reinterpret_cast<uint32_t*>(to + uint64_t(i / words) * page + at);
-                    const uint32_t stay = off - at >= 4 ? 0xffffffffu : (1u << (8 * (off - at))) - 1;
-                    *w = (round_again(*w, by) & stay) | (*w & ~stay);
-                }
-            }
-        }
+        const int had = off ? scale_exponent(scale) : kLeastScale, e = max(exponent_for(top), had);
+        if (off && e > had) grow(r.to, off, page, uint32_t(a.dim), had, e, side, uint32_t(tid), kThreads);
         __syncthreads();  // (the scale has been read, and the words of tokens that stay are written)
-        if (tid == 0) a.scale[side][place] = power_of_two(e);
+        if (tid == 0) *r.scale = power_of_two(e);
         const float by = power_of_two(-e);
         const auto put = [&](uint32_t i, const Quad& q) {
             const uint32_t t = i / per * 4, col = i % per * N;
@@ -205,19 +307,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_cache_append(const AppendArgs a
 #pragma unroll
             for (int k = 0; k < 4; ++k) widen<T>(q.row[k], u[k]);
             if (side == 0) {
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) {
-                    if (t + k >= tokens) break;
-                    uint32_t* const p = reinterpret_cast<uint32_t*>(to + uint64_t(off + t + k) * uint64_t(a.dim) + col);
-                    uint32_t w[N / 4];
-#pragma unroll
-                    for (int c = 0; c < N / 4; ++c) {
-                        const uint32_t v[4] = {u[k][4 * c], u[k][4 * c + 1], u[k][4 * c + 2], u[k][4 * c + 3]};
-                        w[c] = round4(v, by);
-                    }
-                    if constexpr (N == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-                    else *p = w[0];
-                }
+                put_keys<T>(r.to + uint64_t(off + t) * uint64_t(a.dim) + col, uint32_t(a.dim), tokens, t, u, by);
             } else {
 #pragma unroll
                 for (int c = 0; c < N; ++c) {
@@ -227,20 +317,20 @@ __global__ __launch_bounds__(kThreads, 4) void k_cache_append(const AppendArgs a
             }
         };
         if (uint32_t(tid) < quads) put(uint32_t(tid), held);
-        for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) put(i, load(i));
+        for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) put(i, load_quad(r, tokens, per, i));
         __syncthreads();
         if (side == 0) continue;
         if (tokens == page) {
             const uint32_t pieces = page / 16;
             for (uint32_t i = uint32_t(tid); i < pieces * uint32_t(a.dim); i += kThreads) {
                 const uint32_t* const w = turn + i / pieces * turn_row + i % pieces * 4;
-                *reinterpret_cast<uint4*>(to + uint64_t(i) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(r.to + uint64_t(i) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         } else {
             const uint8_t* const bytes = reinterpret_cast<const uint8_t*>(turn);
             for (uint32_t i = uint32_t(tid); i < tokens * uint32_t(a.dim); i += kThreads) {
                 const uint32_t col = i / tokens, at = i % tokens;
-                to[uint64_t(col) * page + off + at] = bytes[col * turn_row * 4 + at];
+                r.to[uint64_t(col) * page + off + at] = bytes[col * turn_row * 4 + at];
             }
         }
         __syncthreads();
@@ -314,9 +404,9 @@ extern "C" int gatgpu_cache_append(gatgpu_ctx* c, const gatgpu_cache* cache, con
     a.cache[1] = cache->v;
     a.scale[0] = cache->k_scale;
     a.scale[1] = cache->v_scale;
-    // A block a row where most rows are their page's first (a token of each request), else 16 rows: prompts, in which at
-    // most one or two of them are.
-    a.chunk = io->rows <= 2048 ? 1 : 16;
+    // Rows of a block: as many as waves where calls are small, and at most 64 less those that a look ahead needs.
+    a.chunk = io->rows <= 4096 ? kThreads / kWave : 32;
+    static_assert(32 + kShort < kWave, "a block's first wave sees the tokens of its short runs");
     const dim3 grid(uint32_t((io->rows + a.chunk - 1) / a.chunk), uint32_t(cache->kv_heads), 2);
     const size_t lds = size_t(cache->dim) * (cache->page + kTurnPad);
     if (io->precision == GATGPU_BF16) k_cache_append<uint16_t><<<grid, kThreads, lds, c->stream>>>(a);

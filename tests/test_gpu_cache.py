@@ -67,12 +67,18 @@ def test_append_whole_and_open_pages(ctx, precision, page, dim, heads):
 def test_append_tokens_of_many_requests(ctx, precision):
     """One token each of requests at any offset, rows without a slot between them; and more rows than the kernel takes singly."""
     g = generator(2)
-    for rows, pages in ((90, 100), (2500, 3000)):
-        host = Pages(pages, 16, 2, 32, seed=3)
+    for runs, most in ((90, 1), (700, 9), (4200, 1), (1500, 7)):
+        host = Pages(runs + 10, 16, 2, 32, seed=3)
         d = host.device()
-        slots = [p * 16 + int(o) for p, o in zip(torch.randperm(pages, generator=g).tolist(), torch.randint(0, 16, (rows,), generator=g))]
-        for i, bad in zip(range(0, rows, 11), (NONE, pages * 16, 2 ** 31, NONE) * rows):
-            slots[i] = bad
+        slots = []
+        for p in torch.randperm(runs + 10, generator=g).tolist()[:runs]:  # one to `most` tokens from any offset on
+            n, off = int(torch.randint(1, most + 1, (1,), generator=g)), int(torch.randint(0, 16, (1,), generator=g))
+            slots += [p * 16 + o for o in range(off, min(16, off + n))]
+        rows = len(slots)
+        bad = (NONE, (runs + 10) * 16, 2 ** 31, NONE)
+        for j, i in enumerate(range(0, rows, 11)):
+            if i + 1 == rows or slots[i + 1] != slots[i] + 1:  # (a gap within a page's tokens is none of the operator's)
+                slots[i] = bad[j % 4]
         k, v = rows_of(g, rows, 2, 32, precision)
         host.append(k, v, torch.tensor(slots))
         append(ctx, d, k, v, slots, precision)
