@@ -39,7 +39,7 @@ struct Sums {
 // Inclusive sums over the block's threads; `total`: of all of them.
 __device__ inline Sums block_sums(Sums x, Sums& total) {
     __shared__ Sums wave_total[kScan / kWave];
-    const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
+    const int lane = int(threadIdx.x) % kWave, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
         const uint64_t p = __shfl_up(x.pages, d), r = __shfl_up(x.rows, d);
@@ -51,14 +51,20 @@ __device__ inline Sums block_sums(Sums x, Sums& total) {
     __syncthreads();  // (the totals of the call before have been read)
     if (lane == kWave - 1) wave_total[wave] = x;
     __syncthreads();
-    total = {0, 0};
-    for (int w = 0; w < kScan / kWave; ++w) {
-        if (w < wave) {
-            x.pages += wave_total[w].pages;
-            x.rows += wave_total[w].rows;
+    // A lane a wave's total: sums up to this wave, and of all.
+    Sums t = lane < kScan / kWave ? wave_total[lane] : Sums{0, 0};
+#pragma unroll
+    for (int d = 1; d < kScan / kWave; d *= 2) {
+        const uint64_t p = __shfl_up(t.pages, d), r = __shfl_up(t.rows, d);
+        if (lane >= d) {
+            t.pages += p;
+            t.rows += r;
         }
-        total.pages += wave_total[w].pages;
-        total.rows += wave_total[w].rows;
+    }
+    total = {__shfl(t.pages, kScan / kWave - 1), __shfl(t.rows, kScan / kWave - 1)};
+    if (wave) {
+        x.pages += __shfl(t.pages, wave - 1);
+        x.rows += __shfl(t.rows, wave - 1);
     }
     return x;
 }
@@ -111,6 +117,8 @@ __global__ __launch_bounds__(kScan) void k_blocks_assign(const BlocksArgs a) {
     }
     __syncthreads();
     Sums before = {0, 0};
+    uint32_t left = count, unserved = 0;  // after the thread's requests, and of the wave's
+    bool took = false;
     for (uint32_t first = 0; first < a.requests; first += kScan * EACH) {
         const uint64_t page = uint64_t(1) << a.page_log;
         uint64_t c[EACH], f[EACH], need[EACH];
@@ -136,11 +144,12 @@ __global__ __launch_bounds__(kScan) void k_blocks_assign(const BlocksArgs a) {
 #pragma unroll
         for (uint32_t i = 0; i < EACH; ++i) {
             const uint32_t r = first + tid * EACH + i;
-            if (r >= a.requests) break;
             upto.pages += need[i];
             upto.rows += f[i];
             const bool fits = c[i] + f[i] <= uint64_t(a.blocks) << a.page_log;
             const bool served = fits && (need[i] == 0 || upto.pages <= count) && upto.rows <= a.rows;
+            unserved += uint32_t(__popcll(__ballot(r < a.requests && !served)));
+            if (r >= a.requests) continue;
             const uint32_t behind = uint32_t(upto.pages - need[i]), len = served ? uint32_t(c[i] + f[i]) : 0;
             const uint32_t end = upto.rows > 0xffffffffu ? 0xffffffffu : uint32_t(upto.rows);
             a.stored[r] = uint32_t(served ? c[i] + f[i] : c[i]);
@@ -153,9 +162,17 @@ __global__ __launch_bounds__(kScan) void k_blocks_assign(const BlocksArgs a) {
             } else {
                 a.behind[r] = behind;
             }
-            if (served && need[i]) atomicMin(&s_left, count - uint32_t(upto.pages));
-            if (!served) atomicAdd(&s_unserved, 1u);
+            if (served && need[i]) {
+                left = count - uint32_t(upto.pages);  // (less with each request)
+                took = true;
+            }
         }
+    }
+    const uint64_t some = __ballot(took);
+    if (some) left = __shfl(left, 63 - __builtin_clzll(some));
+    if (tid % kWave == 0) {
+        atomicMin(&s_left, left);
+        atomicAdd(&s_unserved, unserved);
     }
     __syncthreads();
     if (tid == 0) {

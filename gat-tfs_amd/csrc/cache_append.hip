@@ -4,8 +4,8 @@
 //   byte = e4m3(x 2^-e);  a byte that stays becomes e4m3(byte 2^(old e - e))
 //
 // Bound by bytes: rows read once (two or four bytes a value), one byte a value written.  A block takes the new tokens of
-// one page, key/value head and side (keys or values), reads them into registers, finds their largest magnitude and
-// rounds them from there (what registers do not hold, beyond 16 KB, is read again).  Values are turned in LDS,
+// one page and key/value head, reads their keys and values into registers, finds the largest magnitudes and rounds
+// them from there (what registers do not hold, beyond 16 KB of each, is read again).  Values are turned in LDS,
 // since a page holds them by column: the attention's second product then takes its operands straight from memory.
 #include <algorithm>
 #include <string>
@@ -110,13 +110,20 @@ __device__ inline uint32_t largest_finite(const Quad& q) {
     }
     return top;
 }
-__device__ inline uint32_t block_max(uint32_t x, uint32_t* words) {
+__device__ inline void block_max(uint32_t (&x)[2], uint32_t (*words)[kThreads / kWave]) {
 #pragma unroll
-    for (int d = kWave / 2; d; d /= 2) x = max(x, uint32_t(__shfl_xor(int(x), d)));
+    for (int d = kWave / 2; d; d /= 2) {
+        x[0] = max(x[0], uint32_t(__shfl_xor(int(x[0]), d)));
+        x[1] = max(x[1], uint32_t(__shfl_xor(int(x[1]), d)));
+    }
     __syncthreads();
-    if (threadIdx.x % kWave == 0) words[threadIdx.x / kWave] = x;
+    if (threadIdx.x % kWave == 0) {
+        words[0][threadIdx.x / kWave] = x[0];
+        words[1][threadIdx.x / kWave] = x[1];
+    }
     __syncthreads();
-    return max(max(words[0], words[1]), max(words[2], words[3]));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = max(max(words[i][0], words[i][1]), max(words[i][2], words[i][3]));
 }
 
 // Where the new tokens of a page go, for one head and side.
@@ -225,112 +232,145 @@ __device__ inline void append_short(const AppendArgs& a, uint64_t row, uint32_t 
     }
 }
 
-// A block looks for the first tokens of pages among `chunk` rows.  A page's few tokens (a request's new one) are a wave's,
-// others the block's: a thread takes 16 bytes of four neighbouring tokens, a row's bytes lie in neighbouring lanes, and four
-// tokens' values of a column make one word of the page's column.
+// Bits 0 to 63 of a 128-bit word from bit `at` on.
+struct Bits128 {
+    uint64_t lo, hi;
+    __device__ uint64_t from(uint32_t at) const { return at ? lo >> at | hi << (64 - at) : lo; }
+};
+
+// A block looks for the first tokens of pages among `chunk` rows, and sees 128.  A page's few tokens (a request's new one)
+// are a wave's, others the block's, keys and values at once: a thread takes 16 bytes of four neighbouring tokens of each, a
+// row's bytes lie in neighbouring lanes, and four tokens' values of a column make one word of the page's column.
 template <class T>
 __global__ __launch_bounds__(kThreads, 4) void k_cache_append(const AppendArgs a) {
     constexpr int N = 16 / int(sizeof(T));  // values of 16 bytes
     extern __shared__ uint32_t turn[];      // values: [dim][page + kTurnPad] bytes
-    __shared__ uint32_t s_word[kThreads / kWave];
-    __shared__ uint64_t s_starts, s_goes_on;
+    __shared__ uint32_t s_word[2][kThreads / kWave];
+    __shared__ uint64_t s_starts;
+    __shared__ Bits128 s_goes_on;
     const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave;
-    const int head = int(blockIdx.y), side = int(blockIdx.z);
+    const int head = int(blockIdx.y);
     const uint64_t first = uint64_t(blockIdx.x) * a.chunk;
-    const uint32_t page = a.page, turn_row = (page + kTurnPad) / 4, per = uint32_t(a.dim) / N;  // words, 16-byte pieces a token
-    if (wave == 0) {
-        const uint64_t row = first + uint64_t(lane);
+    const uint32_t page = a.page, dim = uint32_t(a.dim), turn_row = (page + kTurnPad) / 4, per = dim / N;  // words, 16-byte pieces a token
+    if (wave < 2) {
+        const uint64_t row = first + uint64_t(tid);
         bool there = false, goes_on = false;  // goes on: the token after that of the row before, in its page
         if (row < a.rows) {
             const uint32_t s = a.slot[row], before = row ? a.slot[row - 1] : GATGPU_NO_PAGE;
             there = s < a.slots;
             goes_on = there && row && s % page && before + 1 == s;
         }
-        const uint64_t on = __ballot(goes_on), starts = __ballot(there && !goes_on && uint32_t(lane) < a.chunk);
+        const uint64_t on = __ballot(goes_on), starts = __ballot(there && !goes_on && uint32_t(tid) < a.chunk);
         if (lane == 0) {
-            s_starts = starts;
-            s_goes_on = on;
+            if (wave == 0) {
+                s_starts = starts;
+                s_goes_on.lo = on;
+            } else {
+                s_goes_on.hi = on;
+            }
         }
     }
     __syncthreads();
-    const uint64_t starts = s_starts, goes_on = s_goes_on;
-    uint64_t longer = 0;  // starts of more than kShort tokens: the next kShort rows (there are as many lanes) go on
-    {
-        uint64_t all = starts;
-#pragma unroll
-        for (uint32_t i = 1; i <= kShort; ++i) all &= goes_on >> i;
-        longer = all;
-    }
     uint32_t number = 0;
-    for (uint64_t left = starts & ~longer; left; left &= left - 1, ++number) {
-        if (int(number % (kThreads / kWave)) != wave) continue;
+    uint64_t longer = 0;
+    for (uint64_t left = s_starts; left; left &= left - 1) {
         const uint32_t at = uint32_t(__builtin_ctzll(left));
-        const uint32_t tokens = 1 + uint32_t(__builtin_ctzll(~(goes_on >> 1 >> at)));
-        append_short<T>(a, first + at, tokens, head, side);
+        const uint64_t on = s_goes_on.from(at) >> 1;
+        const uint32_t tokens = ~on ? 1 + uint32_t(__builtin_ctzll(~on)) : 64;
+        if (tokens > kShort) {
+            longer |= left & (~left + 1);
+        } else {
+            for (int side = 0; side < 2; ++side)
+                if (int(number++ % (kThreads / kWave)) == wave) append_short<T>(a, first + at, tokens, head, side);
+        }
     }
     for (uint64_t left = longer; left; left &= left - 1) {
-        const uint64_t row = first + uint64_t(__builtin_ctzll(left));
-        const uint32_t slot = a.slot[row];
-        const Run<T> r = run_at<T>(a, row, slot, head, side);
-        const uint32_t off = r.off;
-        const float scale = *r.scale;
-        // Tokens of this page: rows as long as their slots go on.
-        const bool more = row + uint64_t(tid) < a.rows && off + uint32_t(tid) < page && a.slot[row + uint64_t(tid)] == slot + uint32_t(tid);
-        const uint64_t on = __ballot(more);
-        __syncthreads();
-        if (lane == 0) s_word[wave] = ~on ? uint32_t(__builtin_ctzll(~on)) : uint32_t(kWave);
-        __syncthreads();
-        uint32_t tokens = 0;
-        for (int w = 0; w < kThreads / kWave; ++w) {
-            tokens += s_word[w];
-            if (s_word[w] < uint32_t(kWave)) break;
+        const uint32_t at = uint32_t(__builtin_ctzll(left));
+        const uint64_t row = first + at, on = s_goes_on.from(at) >> 1;
+        const uint32_t slot = a.slot[row], off = slot % page;
+        const Run<T> runs[2] = {run_at<T>(a, row, slot, head, 0), run_at<T>(a, row, slot, head, 1)};
+        const float scale[2] = {*runs[0].scale, *runs[1].scale};
+        uint32_t tokens = uint32_t(__builtin_ctzll(~on)) + 1;  // (63 bits of `on` are seen)
+        if (!(~on << 1)) {  // 64 tokens are seen, and there may be more: rows as long as their slots go on
+            const bool more = row + uint64_t(tid) < a.rows && off + uint32_t(tid) < page && a.slot[row + uint64_t(tid)] == slot + uint32_t(tid);
+            const uint64_t some = __ballot(more);
+            __syncthreads();
+            if (lane == 0) s_word[0][wave] = ~some ? uint32_t(__builtin_ctzll(~some)) : uint32_t(kWave);
+            __syncthreads();
+            tokens = 0;
+            for (int w = 0; w < kThreads / kWave; ++w) {
+                tokens += s_word[0][w];
+                if (s_word[0][w] < uint32_t(kWave)) break;
+            }
         }
         const uint32_t quads = (tokens + 3) / 4 * per;
-        Quad held{};  // the thread's first one; more than 256 of them are read again
-        if (uint32_t(tid) < quads) held = load_quad(r, tokens, per, uint32_t(tid));
-        uint32_t top = largest<T>(held);
-        for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) top = max(top, largest<T>(load_quad(r, tokens, per, i)));
-        top = block_max(top, s_word);
-        if (top >= kInfinity) {
-            top = largest_finite<T>(held);
-            for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) top = max(top, largest_finite<T>(load_quad(r, tokens, per, i)));
-            top = block_max(top, s_word);
+        Quad held[2] = {};  // the thread's first ones; more than 256 of them are read again
+        uint32_t top[2];
+        if (uint32_t(tid) < quads) {
+            held[0] = load_quad(runs[0], tokens, per, uint32_t(tid));
+            held[1] = load_quad(runs[1], tokens, per, uint32_t(tid));
         }
-        const int had = off ? scale_exponent(scale) : kLeastScale, e = max(exponent_for(top), had);
-        if (off && e > had) grow(r.to, off, page, uint32_t(a.dim), had, e, side, uint32_t(tid), kThreads);
-        __syncthreads();  // (the scale has been read, and the words of tokens that stay are written)
-        if (tid == 0) *r.scale = power_of_two(e);
-        const float by = power_of_two(-e);
-        const auto put = [&](uint32_t i, const Quad& q) {
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            top[side] = largest<T>(held[side]);
+            for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) top[side] = max(top[side], largest<T>(load_quad(runs[side], tokens, per, i)));
+        }
+        block_max(top, s_word);
+        if (max(top[0], top[1]) >= kInfinity) {  // NaN and infinities leave the scale alone
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+                top[side] = largest_finite<T>(held[side]);
+                for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads)
+                    top[side] = max(top[side], largest_finite<T>(load_quad(runs[side], tokens, per, i)));
+            }
+            block_max(top, s_word);
+        }
+        int e[2];
+        bool grows = false;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const int had = off ? scale_exponent(scale[side]) : kLeastScale;
+            e[side] = max(exponent_for(top[side]), had);
+            if (off && e[side] > had) {
+                grow(runs[side].to, off, page, dim, had, e[side], side, uint32_t(tid), kThreads);
+                grows = true;
+            }
+        }
+        if (grows) __syncthreads();  // (words that hold new tokens too are written before these)
+        const float by[2] = {power_of_two(-e[0]), power_of_two(-e[1])};
+        const auto put = [&](int side, uint32_t i, const Quad& q) {
             const uint32_t t = i / per * 4, col = i % per * N;
             uint32_t u[4][N];
 #pragma unroll
             for (int k = 0; k < 4; ++k) widen<T>(q.row[k], u[k]);
             if (side == 0) {
-                put_keys<T>(r.to + uint64_t(off + t) * uint64_t(a.dim) + col, uint32_t(a.dim), tokens, t, u, by);
+                put_keys<T>(runs[0].to + uint64_t(off + t) * dim + col, dim, tokens, t, u, by[0]);
             } else {
 #pragma unroll
                 for (int c = 0; c < N; ++c) {
                     const uint32_t v[4] = {u[0][c], u[1][c], u[2][c], u[3][c]};
-                    turn[(col + uint32_t(c)) * turn_row + t / 4] = round4(v, by);
+                    turn[(col + uint32_t(c)) * turn_row + t / 4] = round4(v, by[1]);
                 }
             }
         };
-        if (uint32_t(tid) < quads) put(uint32_t(tid), held);
-        for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) put(i, load_quad(r, tokens, per, i));
-        __syncthreads();
-        if (side == 0) continue;
+#pragma unroll
+        for (int side = 1; side >= 0; --side) {
+            if (uint32_t(tid) < quads) put(side, uint32_t(tid), held[side]);
+            for (uint32_t i = uint32_t(tid) + kThreads; i < quads; i += kThreads) put(side, i, load_quad(runs[side], tokens, per, i));
+        }
+        __syncthreads();  // (the scales have been read by all, too)
+        if (tid < 2) *(tid ? runs[1].scale : runs[0].scale) = power_of_two(tid ? e[1] : e[0]);
         if (tokens == page) {
             const uint32_t pieces = page / 16;
-            for (uint32_t i = uint32_t(tid); i < pieces * uint32_t(a.dim); i += kThreads) {
+            for (uint32_t i = uint32_t(tid); i < pieces * dim; i += kThreads) {
                 const uint32_t* const w = turn + i / pieces * turn_row + i % pieces * 4;
-                *reinterpret_cast<uint4*>(r.to + uint64_t(i) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(runs[1].to + uint64_t(i) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         } else {
             const uint8_t* const bytes = reinterpret_cast<const uint8_t*>(turn);
-            for (uint32_t i = uint32_t(tid); i < tokens * uint32_t(a.dim); i += kThreads) {
-                const uint32_t col = i / tokens, at = i % tokens;
-                r.to[uint64_t(col) * page + off + at] = bytes[col * turn_row * 4 + at];
+            for (uint32_t i = uint32_t(tid); i < tokens * dim; i += kThreads) {
+                const uint32_t col = i / tokens, of = i % tokens;
+                runs[1].to[uint64_t(col) * page + off + of] = bytes[col * turn_row * 4 + of];
             }
         }
         __syncthreads();
@@ -404,10 +444,10 @@ extern "C" int gatgpu_cache_append(gatgpu_ctx* c, const gatgpu_cache* cache, con
     a.cache[1] = cache->v;
     a.scale[0] = cache->k_scale;
     a.scale[1] = cache->v_scale;
-    // Rows of a block: as many as waves where calls are small, and at most 64 less those that a look ahead needs.
-    a.chunk = io->rows <= 4096 ? kThreads / kWave : 32;
-    static_assert(32 + kShort < kWave, "a block's first wave sees the tokens of its short runs");
-    const dim3 grid(uint32_t((io->rows + a.chunk - 1) / a.chunk), uint32_t(cache->kv_heads), 2);
+    // Rows of a block: two where calls are small (a token of each request: a wave its keys, one its values), else the 64 that
+    // one mask holds.
+    a.chunk = io->rows <= 4096 ? kThreads / kWave / 2 : 64;
+    const dim3 grid(uint32_t((io->rows + a.chunk - 1) / a.chunk), uint32_t(cache->kv_heads));
     const size_t lds = size_t(cache->dim) * (cache->page + kTurnPad);
     if (io->precision == GATGPU_BF16) k_cache_append<uint16_t><<<grid, kThreads, lds, c->stream>>>(a);
     else k_cache_append<float><<<grid, kThreads, lds, c->stream>>>(a);
