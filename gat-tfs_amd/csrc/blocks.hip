@@ -10,8 +10,8 @@
 #include <algorithm>
 #include <string>
 
+#include "cache.hpp"
 #include "cache_index.hpp"
-#include "context.hpp"
 
 namespace gatgpu {
 namespace {
@@ -90,12 +90,11 @@ __device__ inline void assign_row(const BlocksArgs& a, uint32_t row, uint32_t re
     a.slot[row] = slot;
     a.position[row] = pos;
 }
-// The last i of [0, n] with begin[i] <= row (begin[0] = 0; equal begins: the last).
+// The last i of [lo, hi] with begin[i] <= row, for begin[lo] <= row (equal begins: the last).
 template <class P>
-__device__ inline uint32_t find_request(P begin, uint32_t n, uint32_t row) {
-    uint32_t lo = 0, hi = n;
+__device__ inline uint32_t find_request(P begin, uint32_t lo, uint32_t hi, uint32_t row) {
     while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1) / 2;
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
         if (begin[mid] <= row) lo = mid;
         else hi = mid - 1;
     }
@@ -182,19 +181,30 @@ __global__ __launch_bounds__(kScan) void k_blocks_assign(const BlocksArgs a) {
     }
     if constexpr (ROWS) {
         for (uint32_t row = tid; row < a.rows; row += kScan) {
-            const uint32_t q = find_request(s_begin, a.requests, row);
+            const uint32_t q = find_request(s_begin, 0, a.requests, row);
             if (q < a.requests) assign_row(a, row, q, s_begin[q], s_begin[q + 1], s_len[q], s_behind[q], count);
             else assign_row(a, row, 0, 0, 0, 0, 0, count);
         }
     }
 }
 
+// Rows of many requests: the requests of a block's first and last row bound its other rows'.
 __global__ __launch_bounds__(256) void k_blocks_rows(const BlocksArgs a) {
-    const uint32_t count = *a.count;
-    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < a.rows; i += uint64_t(gridDim.x) * 256) {
-        const uint32_t row = uint32_t(i), q = find_request(a.q_begin, a.requests, row);
-        if (q < a.requests) assign_row(a, row, q, a.q_begin[q], a.q_begin[q + 1], a.k_len[q], a.behind[q], count);
-        else assign_row(a, row, 0, 0, 0, 0, 0, count);
+    __shared__ uint32_t s_ends[2];
+    const uint32_t count = *a.count, tid = threadIdx.x;
+    for (uint64_t first = uint64_t(blockIdx.x) * 256; first < a.rows; first += uint64_t(gridDim.x) * 256) {
+        const uint32_t last = index_min(first + 255, a.rows - 1), row = uint32_t(first) + tid;
+        if (tid < 2 * kWave) {
+            const uint32_t end = last_at_most(a.q_begin, a.requests + 1, tid < kWave ? uint32_t(first) : last, int(tid % kWave));
+            if (tid % kWave == 0) s_ends[tid / kWave] = end;
+        }
+        __syncthreads();
+        if (row <= last) {
+            const uint32_t q = find_request(a.q_begin, s_ends[0], s_ends[1], row);
+            if (q < a.requests) assign_row(a, row, q, a.q_begin[q], a.q_begin[q + 1], a.k_len[q], a.behind[q], count);
+            else assign_row(a, row, 0, 0, 0, 0, 0, count);
+        }
+        __syncthreads();
     }
 }
 

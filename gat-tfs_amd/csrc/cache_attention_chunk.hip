@@ -37,20 +37,6 @@ __device__ inline uint32_t tiles_seen(const ChunkArgs& p, const CacheRequest& q,
     const uint32_t last = min(q.rows * p.a.c.group, (t + 1) * p.tile_rows) - 1, n = cache_seen(q, last / p.a.c.group);
     return n ? (n - 1) / kCacheTile + 1 : 1;
 }
-// The last i of [0, n) with first[i] <= x, for n >= 1, first[0] <= x: 64 places at a time, by a wave.
-template <class V>
-__device__ inline uint32_t last_at_most(const V* first, uint32_t n, V x, int lane) {
-    uint32_t lo = 0;
-    while (n > 1) {
-        const uint32_t step = (n + kWave - 1) / kWave, i = uint32_t(lane) * step;
-        const uint64_t below = __ballot(i < n && first[lo + i] <= x);
-        const uint32_t at = uint32_t(__popcll(below) - 1) * step;  // (sorted: the lanes below are the first ones)
-        lo += at;
-        n = min(step, n - at);
-    }
-    return lo;
-}
-
 __device__ inline uint64_t scan_sums(uint64_t x, uint64_t& total) {
     __shared__ uint64_t wave_total[kScan / kWave];
     const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
