@@ -13,7 +13,7 @@
 namespace gatgpu {
 namespace {
 
-constexpr int kJoinWaves = 4;
+constexpr int kJoinWaves = 4, kRequestWaves = 8;
 
 // The queries of a wave's 16 rows as operands.
 template <class T, int NB>
@@ -431,14 +431,14 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_cache_join(const CacheAt
     if (db == 0 && lane < 16) store_lse(a, rq, packed, head, top, sum);
 }
 
-// Blocks a key/value head: three a unit in all.
+// Blocks a key/value head: two a unit in all.
 uint32_t cache_workers(const gatgpu_ctx* c, int kv_heads) { return uint32_t(std::max(1, 2 * c->cus / kv_heads)); }
 
 template <class T, int NB>
 hipError_t launch(const CacheAttnArgs& a, hipStream_t s) {
     const uint32_t blocks = (a.workers ? a.workers : a.c.requests) * a.c.kv_heads;
     if (!a.workers) {
-        k_cache_attention<T, NB, 8><<<blocks, 8 * kWave, 0, s>>>(a);
+        k_cache_attention<T, NB, kRequestWaves><<<blocks, kRequestWaves * kWave, 0, s>>>(a);
         return hipGetLastError();
     }
     k_cache_attention<T, NB, 4><<<blocks, 4 * kWave, 0, s>>>(a);
@@ -471,6 +471,10 @@ CacheSizes sizes_of(const gatgpu_cache* cache, const gatgpu_cache_attention_io* 
 }
 // Whether requests have rows enough for tiles of 128 packed ones.
 bool in_chunks(const CacheSizes& c) { return uint64_t(c.most) * c.group > 32; }
+// Where no request has more than 16 tiles, and one launch takes the blocks' threads: a block a request, nothing to join.
+bool block_a_request(const CacheSizes& c) {
+    return uint64_t(c.blocks) << c.page_log <= 16 * kCacheTile && uint64_t(c.requests) * c.kv_heads * kRequestWaves * kWave < (uint64_t(1) << 32);
+}
 uint64_t workspace_bytes(const gatgpu_ctx* c, const CacheSizes& s, bool bf16) {
     const Workspace w = workspace_of(c, s);
     return in_chunks(s) ? chunk_plan(c->cus, s, bf16).bytes : w.part + w.stat + w.meta;
@@ -542,8 +546,7 @@ int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgp
     if (bytes < need) return fail(c, GATGPU_EINVAL, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
     if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return fail(c, GATGPU_EINVAL, "workspace must be 16-byte aligned device memory");
     if (int r = check_device_array(c, ws, "workspace")) return r;
-    // Where no request has more than 16 tiles: a block a request, nothing to join.
-    a.workers = uint64_t(a.c.blocks) << a.c.page_log <= 16 * kCacheTile ? 0 : cache_workers(c, cache->kv_heads);
+    a.workers = block_a_request(a.c) ? 0 : cache_workers(c, cache->kv_heads);
     a.least = 4;
     a.scale = io->scale * 1.44269504088896341f;
     a.ld = io->table_stride;

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import gatgpu
-from cache_cases import TYPE, Pages, attention, attention_bounds, bytes_of, generator, normal
+from cache_cases import TYPE, Pages, Serving, generator, normal, words
 
 pytestmark = pytest.mark.gpu
 
@@ -19,10 +19,6 @@ def ctx():
     c = gatgpu.Context(0)
     yield c
     c.close()
-
-
-def words(values):
-    return torch.from_numpy(np.asarray(list(values), np.uint64).astype(np.uint32).view(np.int32)).cuda()
 
 
 def append(ctx, d, k, v, slots, precision, gap=0):
@@ -130,82 +126,6 @@ def test_append_writes_the_pages_of_the_slots_only(ctx):
         assert bool(same[[0, 1, 4, 5]].all())
     assert torch.equal(d["k"][3, :, 14:], before["k"][3, :, 14:]) and torch.equal(d["v"][3, :, :, 14:], before["v"][3, :, :, 14:])
     append(ctx, d, k[:0], v[:0], [], BF)  # no rows
-
-
-class Serving:
-    """A cache with whatever bytes, and a packed batch of queries over it."""
-
-    def __init__(self, k_len, q_len, heads, kv_heads, dim, page, precision, seed=0, extra_rows=0, stride=0, size=1.0):
-        g = generator(seed)
-        need = [-(-k // page) for k in k_len]
-        self.blocks = max(need + [1])
-        self.host = Pages(sum(need) + 2, page, kv_heads, dim, seed=seed + 1)
-        order = torch.randperm(sum(need) + 2, generator=g).tolist()
-        self.table = [[order.pop() for _ in range(n)] + [NONE] * (self.blocks + stride - n) for n in need]
-        for r, n in enumerate(k_len):  # tokens' values; behind them whatever was there
-            for (data, scale), s in zip(self.host.sides(), (size, 1.0)):
-                for b in range(need[r]):
-                    p, count = self.table[r][b], min(page, n - b * page)
-                    x = torch.randn(kv_heads, count, dim, generator=g).double() * 100
-                    data[p, :, :count] = bytes_of(x.clamp(-448, 448))
-                    scale[p] = 2.0 ** torch.randint(-8, -5, (kv_heads,), generator=g).float() * s
-        self.k_len, self.q_len, self.precision = list(k_len), list(q_len), precision
-        self.q_begin = [0] + np.cumsum(q_len).tolist()
-        self.rows = self.q_begin[-1] + extra_rows
-        self.q = normal(g, max(1, self.rows), heads, dim).to(TYPE[precision])
-        self.heads, self.dim, self.scale, self.most = heads, dim, dim ** -0.5, max(list(q_len) + [1])
-
-    def device(self, gap=0):
-        d = self.host.device()
-        per = 8 if self.precision == BF else 4
-        q = torch.full((max(1, self.rows), self.heads * self.dim + gap * per), 3.0, dtype=TYPE[self.precision])
-        q[:, :self.heads * self.dim] = self.q.reshape(max(1, self.rows), -1)
-        d.update(q=q.cuda(), q_begin=words(self.q_begin), lens=words(self.k_len), table=words([x for row in self.table for x in row]))
-        d["out"] = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
-        d["lse"] = torch.full((max(1, self.rows), self.heads), 7.0, device="cuda")
-        return d
-
-    def io(self, d, **change):
-        io = gatgpu.CacheAttentionIO(precision=self.precision, heads=self.heads, scale=self.scale, rows=self.rows, requests=len(self.k_len), most=self.most,
-                                     blocks=self.blocks, table_stride=len(self.table[0]), q=d["q"].data_ptr(), q_stride=d["q"].stride(0),
-                                     q_begin=d["q_begin"].data_ptr(), k_len=d["lens"].data_ptr(), table=d["table"].data_ptr(), out=d["out"].data_ptr(),
-                                     out_stride=d["out"].stride(0), lse=d["lse"].data_ptr())
-        for k, v in change.items():
-            setattr(io, k, v)
-        return io
-
-    def run(self, ctx, gap=1, **change):
-        d = self.device(gap)
-        io = self.io(d, **change)
-        need = ctx.cache_attention_workspace(d["cache"], io)
-        work = torch.full((need,), 255, dtype=torch.uint8, device="cuda")  # (NaN, if it were read)
-        torch.cuda.synchronize()
-        ctx.cache_attention(d["cache"], io, work.data_ptr(), need)
-        ctx.synchronize()
-        return d
-
-    def check(self, d, most=None):
-        out, lse, spread, reach = attention(self.host, self.q, self.q_begin, self.k_len, self.table, self.scale, most)
-        wide = self.heads * self.dim
-        got, got_lse = d["out"].cpu()[:, :wide].view(-1, self.heads, self.dim)[:self.rows], d["lse"].cpu()[:self.rows]
-        out, lse, spread, reach = out[:self.rows], lse[:self.rows], spread[:self.rows], reach[:self.rows]
-        assert bool((d["out"][:, wide:] == 7).all())
-        ours = torch.zeros(self.rows, dtype=torch.bool)  # rows that are written
-        for r in range(len(self.k_len)):
-            n = self.q_len[r] if most is None else min(most, self.q_len[r])
-            ours[self.q_begin[r]:self.q_begin[r] + n] = True
-        assert bool((got[~ours] == 7).all()) and bool((got_lse[~ours] == 7).all())
-        got, got_lse, out, lse, spread, reach = (x[ours].double() for x in (got, got_lse, out, lse, spread, reach))
-        assert torch.equal(torch.isnan(got), torch.isnan(out))
-        tol_out, tol_lse = attention_bounds(self.precision, spread, reach, max(self.k_len), out)
-        fine = ~torch.isnan(out)
-        err = ((got - out).abs() / tol_out)[fine]
-        assert err.numel() == 0 or float(err.max()) <= 1, float(err.max())
-        empty = lse == -math.inf
-        assert torch.equal(got_lse == -math.inf, empty) and bool((got[empty] == 0).all())
-        fine = ~empty & ~torch.isnan(lse)
-        err = ((got_lse - lse).abs() / tol_lse)[fine]
-        assert err.numel() == 0 or float(err.max()) <= 1, float(err.max())
 
 
 @pytest.mark.parametrize("precision", [FP, BF])
