@@ -153,6 +153,26 @@ def attention_bounds(precision, spread, reach, keys, want):
     return tol_out, tol_lse
 
 
+def check_attention(pages, q, q_begin, k_len, table, scale, precision, got, got_lse, most=None):
+    """A call's out and lse, which held 7 before."""
+    out, lse, spread, reach = attention(pages, q, q_begin, k_len, table, scale, most)
+    ours = torch.zeros(q.shape[0], dtype=torch.bool)  # rows that are written
+    for lo, hi in zip(q_begin, q_begin[1:]):
+        ours[lo:hi if most is None else min(hi, lo + most)] = True
+    assert bool((got[~ours] == 7).all()) and bool((got_lse[~ours] == 7).all())
+    got, got_lse, out, lse, spread, reach = (x[ours].double() for x in (got, got_lse, out, lse, spread, reach))
+    assert torch.equal(torch.isnan(got), torch.isnan(out))
+    tol_out, tol_lse = attention_bounds(precision, spread, reach, max(k_len), out)
+    fine = ~torch.isnan(out)
+    err = ((got - out).abs() / tol_out)[fine]
+    assert err.numel() == 0 or float(err.max()) <= 1, float(err.max())
+    empty = lse == -math.inf
+    assert torch.equal(got_lse == -math.inf, empty) and bool((got[empty] == 0).all())
+    fine = ~empty & ~torch.isnan(lse)
+    err = ((got_lse - lse).abs() / tol_lse)[fine]
+    assert err.numel() == 0 or float(err.max()) <= 1, float(err.max())
+
+
 # -- calls on the GPU
 def words(values):
     return torch.from_numpy(np.asarray(list(values), np.uint64).astype(np.uint32).view(np.int32)).cuda()
@@ -211,27 +231,10 @@ class Serving:
         return d
 
     def check(self, d, most=None):
-        out, lse, spread, reach = attention(self.host, self.q, self.q_begin, self.k_len, self.table, self.scale, most)
         wide = self.heads * self.dim
         got, got_lse = d["out"].cpu()[:, :wide].view(-1, self.heads, self.dim)[:self.rows], d["lse"].cpu()[:self.rows]
-        out, lse, spread, reach = out[:self.rows], lse[:self.rows], spread[:self.rows], reach[:self.rows]
         assert bool((d["out"][:, wide:] == 7).all())
-        ours = torch.zeros(self.rows, dtype=torch.bool)  # rows that are written
-        for r in range(len(self.k_len)):
-            n = self.q_len[r] if most is None else min(most, self.q_len[r])
-            ours[self.q_begin[r]:self.q_begin[r] + n] = True
-        assert bool((got[~ours] == 7).all()) and bool((got_lse[~ours] == 7).all())
-        got, got_lse, out, lse, spread, reach = (x[ours].double() for x in (got, got_lse, out, lse, spread, reach))
-        assert torch.equal(torch.isnan(got), torch.isnan(out))
-        tol_out, tol_lse = attention_bounds(self.precision, spread, reach, max(self.k_len), out)
-        fine = ~torch.isnan(out)
-        err = ((got - out).abs() / tol_out)[fine]
-        assert err.numel() == 0 or float(err.max()) <= 1, float(err.max())
-        empty = lse == -math.inf
-        assert torch.equal(got_lse == -math.inf, empty) and bool((got[empty] == 0).all())
-        fine = ~empty & ~torch.isnan(lse)
-        err = ((got_lse - lse).abs() / tol_lse)[fine]
-        assert err.numel() == 0 or float(err.max()) <= 1, float(err.max())
+        check_attention(self.host, self.q[:self.rows], self.q_begin, self.k_len, self.table, self.scale, self.precision, got, got_lse, most)
 
 
 # -- norms and rotation
@@ -291,3 +294,17 @@ def release(cached, table, free, count, page, pages, blocks):
                     free[count] = table[r][b]
                 count += 1
     return min(count, pages)
+
+
+def rotate_bound(x, y, gamma, eps, norm, rot, pairs, precision):
+    """How far y = rotate(x) may be off: the norm's factor (a sum of dim squares, a root, a quotient), three products, an angle
+    rounded to 2^-25 of a turn, sine and cosine, each relative to the magnitudes of a pair; then y's own rounding."""
+    r = 1 / torch.sqrt(x.pow(2).mean(-1, keepdim=True) + eps) if norm else torch.ones_like(x[..., :1])
+    m = (x * r * (gamma if gamma is not None and norm else 1.0)).abs()
+    both = m.clone()
+    if rot:
+        first = torch.arange(rot // 2) * (1 if pairs == gatgpu.PAIRS_HALVES else 2)
+        second = first + (rot // 2 if pairs == gatgpu.PAIRS_HALVES else 1)
+        both[..., first] = both[..., second] = m[..., first] + m[..., second]
+    rel = (x.shape[-1] / 2 + 12) * 2.0 ** -24 + 2.0 ** -21
+    return both * rel + y.abs() * EPS[precision] + 1e-37
