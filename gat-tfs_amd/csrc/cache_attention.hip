@@ -469,15 +469,20 @@ CacheSizes sizes_of(const gatgpu_cache* cache, const gatgpu_cache_attention_io* 
     c.dim = uint32_t(cache->dim);
     return c;
 }
-// Whether requests have rows enough for tiles of 128 packed ones.
-bool in_chunks(const CacheSizes& c) { return uint64_t(c.most) * c.group > 32; }
-// Where no request has more than 16 tiles, and one launch takes the blocks' threads: a block a request, nothing to join.
-bool block_a_request(const CacheSizes& c) {
-    return uint64_t(c.blocks) << c.page_log <= 16 * kCacheTile && uint64_t(c.requests) * c.kv_heads * kRequestWaves * kWave < (uint64_t(1) << 32);
+// Whether requests have rows enough for tiles of 128 packed ones and more.  Measured with 32 heads on 8 of 128 columns, tiles
+// of 16 against those: bf16, 32 requests of 4000 keys with 32 packed rows each 58 and 116 us, 48 127 and 125, 128 204 and 130;
+// 64 of 600 keys with 32 43 and 41, 64 79 and 47.  FP32, whose larger tiles are of four waves, one block a unit: 32 of 4000
+// with 64 134 and 228, 128 250 and 236; 64 of 600 with 64 103 and 90, 96 147 and 91.
+bool in_chunks(const CacheSizes& c, bool bf16) { return uint64_t(c.most) * c.group > (bf16 ? 32 : 64); }
+// A block a request, nothing to join, where no request has more than 16 tiles and the blocks are few.  Measured with one row
+// of 32 heads on 8 of 128 columns, bf16, ranges against a block a request: 16 requests of 512 keys 12.5 and 8.5 us, of 1024
+// 18.1 and 12.6; one of 2048 12.2 and 16.9; 64 of 1024 28.7 and 29.0, 256 of them 103 and 121.
+bool block_a_request(const gatgpu_ctx* ctx, const CacheSizes& c) {
+    return uint64_t(c.blocks) << c.page_log <= 16 * kCacheTile && uint64_t(c.requests) * c.kv_heads <= uint64_t(2 * ctx->cus);
 }
 uint64_t workspace_bytes(const gatgpu_ctx* c, const CacheSizes& s, bool bf16) {
     const Workspace w = workspace_of(c, s);
-    return in_chunks(s) ? chunk_plan(c->cus, s, bf16).bytes : w.part + w.stat + w.meta;
+    return in_chunks(s, bf16) ? chunk_plan(c->cus, s, bf16).bytes : w.part + w.stat + w.meta;
 }
 
 }  // namespace
@@ -546,7 +551,7 @@ int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgp
     if (bytes < need) return fail(c, GATGPU_EINVAL, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
     if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return fail(c, GATGPU_EINVAL, "workspace must be 16-byte aligned device memory");
     if (int r = check_device_array(c, ws, "workspace")) return r;
-    a.workers = block_a_request(a.c) ? 0 : cache_workers(c, cache->kv_heads);
+    a.workers = block_a_request(c, a.c) ? 0 : cache_workers(c, cache->kv_heads);
     a.least = 4;
     a.scale = io->scale * 1.44269504088896341f;
     a.ld = io->table_stride;
@@ -563,7 +568,7 @@ int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgp
     a.k_scale = cache->k_scale;
     a.v_scale = cache->v_scale;
     const bool bf16 = io->precision == GATGPU_BF16, wide = cache->dim > 64;
-    if (in_chunks(a.c)) {
+    if (in_chunks(a.c, bf16)) {
         HIPCHECK(c, launch_cache_chunk(a, bf16, chunk_plan(c->cus, a.c, bf16), ws, c->stream));
         return GATGPU_OK;
     }

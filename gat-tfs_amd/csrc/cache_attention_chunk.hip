@@ -464,7 +464,9 @@ hipError_t launch(const ChunkArgs& p, hipStream_t s) {
     return hipGetLastError();
 }
 // Waves a block: eight where requests may fill them, since a tile is then brought and turned for twice the rows (FP32's
-// products need twice the registers, and leave room for four).
+// products need twice the registers, and leave room for four).  Measured with 16 requests of 4000 keys, 32 heads on 8 of 128
+// columns, bf16, four waves against eight: 128 packed rows each 80 and 96 us, 160 114 and 105, 256 117 and 108, 384 162 and
+// 172, 512 197 and 179, 1024 369 and 321.
 int waves_of(const CacheSizes& c, bool bf16) { return bf16 && uint64_t(c.most) * c.group > 4 * kWaveRows ? 8 : 4; }
 
 }  // namespace

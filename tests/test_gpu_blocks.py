@@ -92,7 +92,7 @@ def lengths(n, most, seed, some=True):
 
 
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
-@pytest.mark.parametrize("requests,cached,fresh", [(1, 0, 1), (1, 300, 40), (12, 100, 1), (40, 300, 70), (1000, 40, 5), (1000, 9, 30), (1025, 50, 3), (4097, 30, 30)])
+@pytest.mark.parametrize("requests,cached,fresh", [(1, 0, 1), (1, 300, 40), (12, 100, 1), (40, 300, 70), (1000, 40, 5), (1000, 9, 30), (1025, 50, 3), (4097, 30, 30), (64, 90, 32), (64, 90, 33)])
 def test_steps(ctx, page, requests, cached, fresh):
     p = Problem(lengths(requests, cached, 1) if cached else [0] * requests, lengths(requests, fresh, 2, some=requests > 12), page, seed=requests, stride=3)
     p.check(p.run(ctx))
@@ -152,7 +152,7 @@ def test_bad_pages_and_counts(ctx, rows):
     p.check(p.run(ctx))
 
 
-@pytest.mark.parametrize("requests", [1, 7, 64, 65, 2000, 20_000])
+@pytest.mark.parametrize("requests", [1, 7, 32, 33, 65, 2000, 20_000, 33_000])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_release(ctx, requests, in_place):
     p = Problem(lengths(requests, 400 if requests < 5000 else 40, 14), [0] * requests, seed=15, stride=2)
