@@ -1,9 +1,14 @@
 // Attention over a paged 8-bit cache (cache_attention.hpp says how operands lie).
 //
-// Few rows a request: bound by the cache's bytes.  The calls' keys, in tiles of 64 and over all requests, are cut into
-// equal ranges for a fixed number of blocks a key/value head, since lengths are known on the device only: each block
-// sums the requests' tiles to find its own range, its four waves take its tiles in turn and join their sums in LDS.
-// What is cut between blocks leaves partial sums, which a second launch joins in the order of the keys.
+// Few rows a request: bound by the cache's bytes, short calls by a launch and its chain of dependent reads.  The work, tiles
+// of 64 keys times tiles of 16 rows over all requests, is cut into equal ranges for a fixed number of blocks a key/value
+// head, since lengths are known on the device only: each block sums the requests' work to find its own range.  Its four
+// waves take a request's row tiles side by side, so that keys come from memory once, and the key tiles of a row tile in turn,
+// and join their sums in LDS.  What is cut between blocks leaves partial sums, which a second launch joins in the order of
+// the keys.  Where tables are short, a block takes a row tile alone, and there is nothing to join.
+//
+// One token over 260001 keys, 32 heads on 8 of 128 columns, bf16 rows: 96 us, 5.5 TB/s, and 6.4 for the join; 48 tokens
+// over 200 to 24000 keys: 77 us, 4.6 TB/s, and 5.5.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -13,7 +18,9 @@
 namespace gatgpu {
 namespace {
 
-constexpr int kJoinWaves = 4, kRequestWaves = 8;
+// Waves of a block: of ranges of the work, of a row tile alone, of a join.
+constexpr int kWaves = 4, kAloneWaves = 8, kJoinWaves = 4;
+constexpr uint32_t kSmallShare = 8;  // work of a worker, up to which none takes parts of two requests
 
 // The queries of a wave's 16 rows as operands.
 template <class T, int NB>
@@ -221,6 +228,14 @@ __device__ inline void add_values(Running<NB>& run, const Weights& w, const Valu
     }
 }
 
+// Row tiles that a block takes side by side, as a power of two (at most 4, the most of a request here), and the work of a
+// request.  (64 requests of 4096 keys with 32 packed rows, 32 heads on 8 of 128 columns: 118 us, one row tile after another 189.)
+__device__ inline uint32_t together(uint32_t rows) { return rows > 2 ? 2 : rows > 1 ? 1 : 0; }
+__device__ inline uint64_t work_of(const CacheAttnArgs& a, const CacheRequest& q) {
+    const uint32_t rows = row_tiles(a.c, q);
+    return rows ? uint64_t(key_tiles(q)) << together(rows) : 0;
+}
+
 // Sums of the waves: [wave][columns / 16][lane] columns, [wave][row] references and weights.
 template <int NB, int WAVES>
 struct JoinLds {
@@ -228,84 +243,112 @@ struct JoinLds {
     float ref[WAVES][kCacheRows], sum[WAVES][kCacheRows];
 };
 
+// Parts of a small call's request.
+__device__ inline uint32_t parts_of(uint64_t work, uint64_t share) { return uint32_t(work + share - 1) / uint32_t(share); }
+// Inclusive sums over a block's threads; `total`: of all of them.
+template <int WAVES>
+__device__ inline uint64_t sums_upto(uint64_t x, uint64_t& total) {
+    __shared__ uint64_t s_sum[WAVES];
+    const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const uint64_t p = __shfl_up(x, d);
+        if (lane >= d) x += p;
+    }
+    __syncthreads();  // (the sums of the call before have been read)
+    if (lane == kWave - 1) s_sum[wave] = x;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) x += s_sum[w];
+        total += s_sum[w];
+    }
+    return x;
+}
+
 // Two waves a SIMD hide their requests behind each other.  (Three, with 168 registers each, keep a part of them in memory:
 // 142 us against 96 for one token over 260K, 32 heads of 128 on 8.)
-template <class T, int NB, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, 2) void k_cache_attention(const CacheAttnArgs a) {
-    constexpr int PARTS = Queries<T, NB>::PARTS;
+template <class T, int NB, bool ALONE>
+__global__ __launch_bounds__((ALONE ? kAloneWaves : kWaves) * kWave, 2) void k_cache_attention(const CacheAttnArgs a) {
+    constexpr int PARTS = Queries<T, NB>::PARTS, WAVES = ALONE ? kAloneWaves : kWaves;
     __shared__ JoinLds<NB, WAVES> join;
-    __shared__ uint64_t s_sum[WAVES], s_start;
+    __shared__ uint64_t s_start, s_at, s_end;
     __shared__ uint32_t s_request;
+    bool apart = false;  // each worker's work is of one request
     const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
-    const uint32_t head = blockIdx.x % a.c.kv_heads;
-    const uint32_t worker = blockIdx.x / a.c.kv_heads;
-    uint64_t at = 0, end = 0, base = 0, share = 1;  // the worker's tiles, and those before its request
+    const uint32_t head = blockIdx.x, worker = blockIdx.y, block = worker * a.c.kv_heads + head;
+    uint64_t at = 0, end = 0, base = 0, share = 1;  // the worker's work, and that before its request
     uint32_t request = worker;
-    if (a.workers) {
+    if constexpr (!ALONE) {
         const uint32_t per = (a.c.requests + (WAVES * kWave) - 1) / (WAVES * kWave), from = min(a.c.requests, uint32_t(tid) * per), to = min(a.c.requests, from + per);
         uint64_t own = 0;
-        for (uint32_t r = from; r < to; ++r) {
-            const CacheRequest q = request_of(a, r);
-            own += uint64_t(row_tiles(a.c, q)) * key_tiles(q);
+        for (uint32_t r = from; r < to; ++r) own += work_of(a, request_of(a, r));
+        uint64_t total;
+        const uint64_t upto = sums_upto<WAVES>(own, total);
+        const uint64_t each = total / a.c.requests;  // (a worker takes one short request, not several in turn)
+        share = max(min(max(each, uint64_t(1)), uint64_t(a.least)), (total + a.workers - 1) / a.workers);
+        apart = gridDim.y > a.workers && total <= uint64_t(kSmallShare) * a.workers;
+        uint64_t mine = own, upto_mine = upto, all = total, place = worker;  // the place among all of what is shared out
+        if (apart) {
+            mine = 0;
+            for (uint32_t r = from; r < to; ++r) mine += parts_of(work_of(a, request_of(a, r)), share);
+            upto_mine = sums_upto<WAVES>(mine, all);
+        } else {
+            place = worker < a.workers ? uint64_t(worker) * share : total;
         }
-        uint64_t upto = own;
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) {
-            const uint64_t p = __shfl_up(upto, d);
-            if (lane >= d) upto += p;
-        }
-        if (lane == kWave - 1) s_sum[wave] = upto;
-        __syncthreads();
-        uint64_t total = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            if (w < wave) upto += s_sum[w];
-            total += s_sum[w];
-        }
-        share = max(uint64_t(a.least), (total + a.workers - 1) / a.workers);
-        at = min(total, uint64_t(worker) * share);
-        end = min(total, at + share);
-        if (at < end && at >= upto - own && at < upto) {  // one thread's requests hold the first tile
-            uint64_t sum = upto - own;
+        if (place < all && place >= upto_mine - mine && place < upto_mine) {  // one thread's requests hold it
+            uint64_t sum = upto - own, before = upto_mine - mine;
             for (uint32_t r = from; r < to; ++r) {
-                const CacheRequest q = request_of(a, r);
-                const uint64_t cost = uint64_t(row_tiles(a.c, q)) * key_tiles(q);
-                if (at < sum + cost) {
+                const uint64_t work = work_of(a, request_of(a, r)), places = apart ? parts_of(work, share) : work;
+                if (place < before + places) {
                     s_request = r;
                     s_start = sum;
+                    s_at = apart ? sum + (place - before) * share : place;
+                    s_end = apart ? min(sum + work, s_at + share) : min(total, place + share);
                     break;
                 }
-                sum += cost;
+                sum += work;
+                before += places;
             }
         }
         __syncthreads();
+        if (place < all) {
+            request = s_request;
+            base = s_start;
+            at = s_at;
+            end = s_end;
+        }
         if (at >= end) {
-            if (tid == 0) a.meta[blockIdx.x] = make_uint4(0, 0, 0, 0);
+            if (tid == 0) a.meta[block] = make_uint4(0, 0, 0, 0);
             return;
         }
-        request = s_request;
-        base = s_start;
     }
     uint4 meta = make_uint4(0, 0, 0, 0);
     while (request < a.c.requests) {
         const CacheRequest rq = request_of(a, request);
         const uint32_t tiles = key_tiles(rq), rows = row_tiles(a.c, rq);
-        if (!a.workers) end = uint64_t(rows) * tiles;  // (a block a request)
+        if constexpr (ALONE) {
+            if (end || blockIdx.z >= rows) return;
+            end = tiles;
+        }
         if (at >= end) break;
-        const uint64_t in = at - base;
-        if (in >= uint64_t(rows) * tiles) {  // the next request
-            base += uint64_t(rows) * tiles;
+        // Waves side by side take the request's row tiles, those of one row tile its key tiles in turn.
+        const uint32_t log = ALONE ? 0 : together(rows), per = uint32_t(WAVES) >> log, member = uniform(uint32_t(wave)) % per, group = uniform(uint32_t(wave)) / per;
+        const uint64_t work = ALONE ? tiles : work_of(a, rq), in = at - base, here = min(end - at, work - in);
+        if (in >= work) {  // the next request
+            base += work;
             ++request;
             continue;
         }
-        const uint32_t row_tile = uint32_t(in / tiles), lo = uint32_t(in % tiles);
-        const uint32_t hi = index_min(tiles, lo + (end - at));
+        const uint32_t up = (1u << log) - 1, lo = uint32_t((in + up) >> log), hi = index_min(tiles, (in + here + up) >> log);
+        const uint32_t row_tile = ALONE ? blockIdx.z : group;
         const uint32_t packed = row_tile * kCacheRows + uint32_t(n);
         const bool there = packed < rq.rows * a.c.group;
         const uint32_t seen = there ? cache_seen(rq, packed / a.c.group) : 0;
         // Rows of a tile stand in the order of their positions.
         const uint32_t last = min(rq.rows * a.c.group, (row_tile + 1) * kCacheRows) - 1;
-        const uint32_t least = cache_seen(rq, row_tile * kCacheRows / a.c.group), most = cache_seen(rq, last / a.c.group);
+        const uint32_t least = cache_seen(rq, row_tile * kCacheRows / a.c.group), most = row_tile < rows ? cache_seen(rq, last / a.c.group) : 0;
         const uint32_t* const row = a.table + uint64_t(request) * a.ld;
         const Queries<T, NB> q = load_queries<T, NB>(a, rq, packed, head, g);
         Running<NB> run;
@@ -314,7 +357,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void k_cache_attention(const Cach
         run.ref = kCacheNoRef;
         run.sum = 0.0f;
         const uint32_t stop = min(hi, (most + kCacheTile - 1) / kCacheTile);
-        uint32_t tile = lo + uint32_t(wave);
+        uint32_t tile = lo + member;
         if (tile < stop) {
             // A tile's keys are requested when the scores of the one before are formed, its values when those are added.
             TilePages pages = tile_pages(a, row, rq.keys, tile, lane);
@@ -322,11 +365,11 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void k_cache_attention(const Cach
             Values<NB> v;
             load_keys<NB>(a, pages.load, tile, head, lane, k);
             load_values<NB>(a, pages.own, tile, head, lane, v);
-            pages = tile_pages(a, row, rq.keys, tile + WAVES, lane);
+            pages = tile_pages(a, row, rq.keys, tile + per, lane);
             while (true) {
                 const Scores x = scores<T, NB>(q, k);
                 __builtin_amdgcn_sched_barrier(0);
-                const uint32_t next = tile + WAVES;
+                const uint32_t next = tile + per;
                 if (next < stop) load_keys<NB>(a, pages.load, next, head, lane, k);
                 const bool whole = tile * kCacheTile + kCacheTile <= least && __all(v.page);  // every row sees every key
                 const Weights w = weigh<PARTS, NB>(a, run, x, v, tile, seen, whole, lane);
@@ -335,12 +378,12 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void k_cache_attention(const Cach
                 __builtin_amdgcn_sched_barrier(0);
                 if (next >= stop) break;
                 load_values<NB>(a, pages.own, next, head, lane, v);
-                pages = tile_pages(a, row, rq.keys, next + WAVES, lane);
+                pages = tile_pages(a, row, rq.keys, next + per, lane);
                 tile = next;
             }
         }
         run.sum = xor32_add(xor16_add(run.sum));
-        // The waves' sums to those of the block: each wave joins its share of the columns.
+        // The sums of a row tile's waves to one: each of them joins its share of the columns.
         if (lane < 16) {
             join.ref[wave][n] = run.ref;
             join.sum[wave][n] = run.sum;
@@ -348,25 +391,28 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void k_cache_attention(const Cach
 #pragma unroll
         for (int d = 0; d < 4 * NB; ++d) join.o[wave][d][lane] = run.o[d];
         __syncthreads();
-        float ref = join.ref[0][n], sum = 0.0f, less[WAVES];
+        const uint32_t first = group * per;
+        float ref = join.ref[first][n], sum = 0.0f, less[WAVES];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) ref = fmaxf(ref, join.ref[w][n]);
+        for (uint32_t w = 1; w < uint32_t(WAVES); ++w)
+            if (w < per) ref = fmaxf(ref, join.ref[first + w][n]);
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            less[w] = __builtin_amdgcn_exp2f(join.ref[w][n] - ref);
-            sum = fmaf(join.sum[w][n], less[w], sum);
+        for (uint32_t w = 0; w < uint32_t(WAVES); ++w) {
+            if (w >= per) break;
+            less[w] = __builtin_amdgcn_exp2f(join.ref[first + w][n] - ref);
+            sum = fmaf(join.sum[first + w][n], less[w], sum);
         }
         const bool cut = lo > 0 || hi < tiles;
-        const uint64_t piece = (uint64_t(blockIdx.x) * 2 + (lo > 0 ? 0 : 1));
+        const uint64_t piece = (uint64_t(block) * 2 + (lo > 0 ? 0 : 1)) * a.row_tiles + row_tile;
+        for (uint32_t db = row_tile < rows ? member : 4 * NB; db < 4 * NB; db += per) {
+            f32x4_t o = join.o[first][db][lane] * less[0];
 #pragma unroll
-        for (int db = wave; db < 4 * NB; db += WAVES) {
-            f32x4_t o = join.o[0][db][lane] * less[0];
-#pragma unroll
-            for (int w = 1; w < WAVES; ++w) o += join.o[w][db][lane] * less[w];
+            for (uint32_t w = 1; w < uint32_t(WAVES); ++w)
+                if (w < per) o += join.o[first + w][db][lane] * less[w];
             if (cut) *reinterpret_cast<f32x4_t*>(a.part + ((piece * (4 * NB) + uint64_t(db)) * kWave + uint64_t(lane)) * 4) = o;
             else store4<T>(a, rq, packed, head, uint32_t(16 * db + 4 * g), o, sum);
         }
-        if (wave == 0 && lane < 16) {
+        if (member == 0 && row_tile < rows && lane < 16) {
             if (cut) {
                 a.stat[piece * 32 + uint64_t(n)] = ref;
                 a.stat[piece * 32 + 16 + uint64_t(n)] = sum;
@@ -374,27 +420,27 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void k_cache_attention(const Cach
                 store_lse(a, rq, packed, head, ref, sum);
             }
         }
-        if (lo == 0 && hi < tiles) {
-            const uint64_t task_end = base + uint64_t(row_tile + 1) * tiles;
-            meta = make_uint4(request, row_tile, uint32_t((task_end - 1) / share) - worker + 1, 0);
-        }
-        at += hi - lo;
+        if (lo == 0 && hi < tiles) meta = make_uint4(request, 0, apart ? parts_of(work, share) : uint32_t((base + work - 1) / share) - worker + 1, 0);
+        at += here;
         __syncthreads();
     }
-    if (a.workers && tid == 0) a.meta[blockIdx.x] = meta;
+    if (!ALONE && tid == 0) a.meta[block] = meta;
 }
 
-// The pieces of the task that begins in a worker and ends in another: 16 columns a block, its waves a quarter of the pieces each.
+// The pieces of the request that begins in a worker and ends in another: 16 columns of a row tile a block, its waves a quarter
+// of the pieces each.
 template <class T, int NB>
 __global__ __launch_bounds__(kJoinWaves * kWave) void k_cache_join(const CacheAttnArgs a) {
     __shared__ f32x4_t s_o[kJoinWaves][kWave];
     __shared__ float s_ref[kJoinWaves][kCacheRows], s_sum[kJoinWaves][kCacheRows];
     const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave, n = lane % 16, g = lane / 16;
-    const uint32_t block = blockIdx.x, db = blockIdx.y;
+    const uint32_t block = blockIdx.x, db = blockIdx.y, row_tile = blockIdx.z;
     const uint4 meta = a.meta[block];
     if (!meta.z) return;
     const uint32_t head = block % a.c.kv_heads;
-    const auto piece_of = [&](uint32_t p) { return (uint64_t(block) + uint64_t(p) * uint64_t(a.c.kv_heads)) * 2 + (p ? 0 : 1); };
+    const CacheRequest rq = request_of(a, meta.x);
+    if (row_tile >= row_tiles(a.c, rq)) return;
+    const auto piece_of = [&](uint32_t p) { return ((uint64_t(block) + uint64_t(p) * uint64_t(a.c.kv_heads)) * 2 + (p ? 0 : 1)) * a.row_tiles + row_tile; };
     f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
     float ref = kCacheNoRef, sum = 0.0f;
 #pragma unroll 4
@@ -425,8 +471,7 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_cache_join(const CacheAt
         o += s_o[w][lane] * less;
         sum = fmaf(s_sum[w][n], less, sum);
     }
-    const CacheRequest rq = request_of(a, meta.x);
-    const uint32_t packed = meta.y * kCacheRows + uint32_t(n);
+    const uint32_t packed = row_tile * kCacheRows + uint32_t(n);
     store4<T>(a, rq, packed, head, 16 * db + 4 * uint32_t(g), o, sum);
     if (db == 0 && lane < 16) store_lse(a, rq, packed, head, top, sum);
 }
@@ -434,16 +479,20 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_cache_join(const CacheAt
 // Blocks a key/value head: two a unit in all.
 uint32_t cache_workers(const gatgpu_ctx* c, int kv_heads) { return uint32_t(std::max(1, 2 * c->cus / kv_heads)); }
 
+// With those that calls of little work and few requests take besides, where none takes parts of two requests.  Measured with
+// one row of 32 heads on 8 of 128 columns, bf16, 64 workers a head, parts of two against that: 4 requests of 300 keys 17.0 and
+// 13.0 us, 16 17.4 and 13.8, 64 17.7 and 21.7.
+uint32_t workers_most(uint32_t workers, const CacheSizes& c) { return workers + (c.requests <= workers / 4 ? c.requests : 0); }
+
 template <class T, int NB>
 hipError_t launch(const CacheAttnArgs& a, hipStream_t s) {
-    const uint32_t blocks = (a.workers ? a.workers : a.c.requests) * a.c.kv_heads;
     if (!a.workers) {
-        k_cache_attention<T, NB, kRequestWaves><<<blocks, kRequestWaves * kWave, 0, s>>>(a);
+        k_cache_attention<T, NB, true><<<dim3(a.c.kv_heads, a.c.requests, a.row_tiles), kAloneWaves * kWave, 0, s>>>(a);
         return hipGetLastError();
     }
-    k_cache_attention<T, NB, 4><<<blocks, 4 * kWave, 0, s>>>(a);
+    k_cache_attention<T, NB, false><<<dim3(a.c.kv_heads, workers_most(a.workers, a.c)), kWaves * kWave, 0, s>>>(a);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    k_cache_join<T, NB><<<dim3(blocks, uint32_t(a.c.dim / 16)), kJoinWaves * kWave, 0, s>>>(a);
+    k_cache_join<T, NB><<<dim3(a.c.kv_heads * workers_most(a.workers, a.c), uint32_t(a.c.dim / 16), a.row_tiles), kJoinWaves * kWave, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -451,9 +500,12 @@ uint64_t pad256(uint64_t b) { return (b + 255) / 256 * 256; }
 struct Workspace {
     uint64_t part, stat, meta;
 };
+// Row tiles of a request, at most.
+uint32_t rows_of(const CacheSizes& s, uint32_t tile) { return uint32_t((std::min<uint64_t>(s.most, s.rows) * s.group + tile - 1) / tile); }
 Workspace workspace_of(const gatgpu_ctx* c, const CacheSizes& s) {
-    const uint64_t blocks = uint64_t(cache_workers(c, int(s.kv_heads))) * s.kv_heads, nb = s.dim > 64 ? 2 : 1;
-    return {pad256(blocks * 2 * 4 * nb * kWave * 16), pad256(blocks * 2 * 32 * 4), pad256(blocks * 16)};
+    const uint64_t blocks = uint64_t(workers_most(cache_workers(c, int(s.kv_heads)), s)) * s.kv_heads, nb = s.dim > 64 ? 2 : 1;
+    const uint64_t pieces = blocks * 2 * rows_of(s, kCacheRows);
+    return {pad256(pieces * 4 * nb * kWave * 16), pad256(pieces * 32 * 4), pad256(blocks * 16)};
 }
 CacheSizes sizes_of(const gatgpu_cache* cache, const gatgpu_cache_attention_io* io) {
     CacheSizes c;
@@ -469,20 +521,22 @@ CacheSizes sizes_of(const gatgpu_cache* cache, const gatgpu_cache_attention_io* 
     c.dim = uint32_t(cache->dim);
     return c;
 }
-// Whether requests have rows enough for tiles of 128 packed ones and more.  Measured with 32 heads on 8 of 128 columns, tiles
-// of 16 against those: bf16, 32 requests of 4000 keys with 32 packed rows each 58 and 116 us, 48 127 and 125, 128 204 and 130;
-// 64 of 600 keys with 32 43 and 41, 64 79 and 47.  FP32, whose larger tiles are of four waves, one block a unit: 32 of 4000
-// with 64 134 and 228, 128 250 and 236; 64 of 600 with 64 103 and 90, 96 147 and 91.
-bool in_chunks(const CacheSizes& c, bool bf16) { return uint64_t(c.most) * c.group > (bf16 ? 32 : 64); }
-// A block a request, nothing to join, where no request has more than 16 tiles and the blocks are few.  Measured with one row
-// of 32 heads on 8 of 128 columns, bf16, ranges against a block a request: 16 requests of 512 keys 12.5 and 8.5 us, of 1024
-// 18.1 and 12.6; one of 2048 12.2 and 16.9; 64 of 1024 28.7 and 29.0, 256 of them 103 and 121.
-bool block_a_request(const gatgpu_ctx* ctx, const CacheSizes& c) {
-    return uint64_t(c.blocks) << c.page_log <= 16 * kCacheTile && uint64_t(c.requests) * c.kv_heads <= uint64_t(2 * ctx->cus);
+// Whether requests have more rows than the four tiles of 16 that a block takes side by side.  Measured with 32 heads on 8 of
+// 128 columns, those against the tiles of 128 and more: bf16, 32 requests of 4000 keys with 32 packed rows each 67 and 118 us,
+// with 64 118 and 128; 64 of 600 keys with 64 45 and 48; FP32, 32 of 4000 with 64 134 and 228, 64 of 600 with 64 54 and 89.
+// With 128 rows in tiles of 16, which would read the keys twice: bf16 204 and 130, FP32 250 and 236.
+bool in_chunks(const CacheSizes& c) { return uint64_t(c.most) * c.group > 4 * kCacheRows; }
+// A block a row tile, nothing to join, where no request has more than 16 tiles of keys (many rows: 8) and the blocks are few.
+// Measured with 32 heads on 8 of 128 columns, bf16, ranges of the work against that.  One row each: 16 requests of 300 keys
+// 13.8 and 7.4 us, of 1024 19 and 12; one of 2048 13 and 16; 64 of 1024 29 and 27.  8 rows, two tiles: 64 of 300 22 and 32.
+// 50 rows: 4 of 300 30 and 20, of 1024 30 and 43; 35 of 512 60 and 55, of 1024 80 and 90.
+bool block_a_tile(const gatgpu_ctx* ctx, const CacheSizes& c, uint32_t row_tiles, bool chunks) {
+    const uint64_t tiles = chunks ? 8 : 16, blocks = uint64_t(ctx->cus) * (chunks ? 4 : 2);
+    return uint64_t(c.blocks) << c.page_log <= tiles * kCacheTile && uint64_t(c.requests) * row_tiles * c.kv_heads <= blocks;
 }
 uint64_t workspace_bytes(const gatgpu_ctx* c, const CacheSizes& s, bool bf16) {
     const Workspace w = workspace_of(c, s);
-    return in_chunks(s, bf16) ? chunk_plan(c->cus, s, bf16).bytes : w.part + w.stat + w.meta;
+    return in_chunks(s) ? chunk_plan(c->cus, s, bf16).bytes : w.part + w.stat + w.meta;
 }
 
 }  // namespace
@@ -551,8 +605,6 @@ int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgp
     if (bytes < need) return fail(c, GATGPU_EINVAL, "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
     if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return fail(c, GATGPU_EINVAL, "workspace must be 16-byte aligned device memory");
     if (int r = check_device_array(c, ws, "workspace")) return r;
-    a.workers = block_a_request(c, a.c) ? 0 : cache_workers(c, cache->kv_heads);
-    a.least = 4;
     a.scale = io->scale * 1.44269504088896341f;
     a.ld = io->table_stride;
     a.qs = io->q_stride;
@@ -567,11 +619,18 @@ int gatgpu_cache_attention(gatgpu_ctx* c, const gatgpu_cache* cache, const gatgp
     a.v = cache->v;
     a.k_scale = cache->k_scale;
     a.v_scale = cache->v_scale;
-    const bool bf16 = io->precision == GATGPU_BF16, wide = cache->dim > 64;
-    if (in_chunks(a.c, bf16)) {
-        HIPCHECK(c, launch_cache_chunk(a, bf16, chunk_plan(c->cus, a.c, bf16), ws, c->stream));
+    const bool bf16 = io->precision == GATGPU_BF16, wide = cache->dim > 64, chunks = in_chunks(a.c);
+    a.row_tiles = rows_of(a.c, chunks ? chunk_rows(a.c, bf16) : kCacheRows);
+    const bool alone = block_a_tile(c, a.c, a.row_tiles, chunks);
+    if (chunks) {
+        const ChunkPlan plan = chunk_plan(c->cus, a.c, bf16);
+        a.workers = alone ? 0 : plan.workers;
+        a.least = 4;  // (2 and 8 instead: 16 requests of 50 rows over 1024 keys, 8 heads on 2, 44 and 37 us, 36 with 4; one 22 and 33, 25 with 4)
+        HIPCHECK(c, launch_cache_chunk(a, bf16, plan, ws, c->stream));
         return GATGPU_OK;
     }
+    a.workers = alone ? 0 : cache_workers(c, cache->kv_heads);
+    a.least = 4;  // (a tile a wave; 2 and 8 instead: one row over 4096 keys 13.8 and 14.5 us, 13.1 with 4)
     const Workspace w = workspace_of(c, a.c);
     a.part = static_cast<float*>(ws);
     a.stat = reinterpret_cast<float*>(static_cast<char*>(ws) + w.part);

@@ -29,8 +29,9 @@ typedef __bf16 bf16x2v_t __attribute__((ext_vector_type(2)));
 
 struct CacheAttnArgs {
     CacheSizes c;
-    uint32_t workers = 0;  // of a key/value head; 0: a block a request
-    uint32_t least = 0;    // tiles of a worker
+    uint32_t workers = 0;  // of a key/value head; 0: a block a row tile
+    uint32_t least = 0;    // least work of a worker, where requests have as much: key tiles, times row tiles where these are of 16
+    uint32_t row_tiles = 0;  // of a request, at most; for a block a row tile
     float scale = 0.0f;    // scale log2 e
     uint64_t ld = 0, qs = 0, os = 0;
     const void* q = nullptr;
@@ -39,9 +40,10 @@ struct CacheAttnArgs {
     const uint32_t *q_begin = nullptr, *k_len = nullptr, *table = nullptr;
     const uint8_t *k = nullptr, *v = nullptr;
     const float *k_scale = nullptr, *v_scale = nullptr;
-    // Partial sums, of two pieces a worker and head: [piece][columns / 16][64][4] sums, [piece][2][16] references and weights.
+    // Partial sums, of two pieces a worker and head: [piece][row tile][columns / 16][64][4] sums, [piece][row tile][2][16]
+    // references and weights.
     float *part = nullptr, *stat = nullptr;
-    uint4* meta = nullptr;  // [worker][head]: request, row tile, pieces (0: none) of the task that begins in the worker and ends in another
+    uint4* meta = nullptr;  // [worker][head]: request, row tile, pieces (0: none) of the work that begins in the worker and ends in another
 };
 // One request's place (by scalar loads where r is the same in all lanes).
 __device__ inline CacheRequest request_of(const CacheAttnArgs& a, uint32_t r) {
@@ -147,6 +149,7 @@ struct ChunkPlan {
     uint64_t begin = 0, request = 0, upto = 0, part = 0, stat = 0, meta = 0, bytes = 0;  // offsets in the workspace
 };
 ChunkPlan chunk_plan(int cus, const CacheSizes& c, bool bf16);
+uint32_t chunk_rows(const CacheSizes& c, bool bf16);  // packed rows of a tile
 hipError_t launch_cache_chunk(const CacheAttnArgs& a, bool bf16, const ChunkPlan& plan, void* workspace, hipStream_t s);
 
 }  // namespace gatgpu

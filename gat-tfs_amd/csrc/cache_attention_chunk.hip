@@ -126,7 +126,8 @@ __device__ inline f32x16_t mfma32_bf16(uint4 a, uint4 b, f32x16_t c) {
 __device__ inline f32x16_t mfma32_f16(uint4 a, uint4 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
-template <class T, int NB, int WAVES>
+// ALONE: a block a row tile; else each worker's range of the work.
+template <class T, int NB, int WAVES, bool ALONE>
 __global__ __launch_bounds__(WAVES * kWave, sizeof(T) == 2 ? 2 : 1) void k_cache_chunk(const ChunkArgs p) {
     constexpr int PARTS = QueryParts<T>::N, PIECES = 4 * NB;  // 16-byte pieces of a key's bytes
     constexpr int THREADS = WAVES * kWave, N = NB * 256 > THREADS ? NB * 256 / THREADS : 1;  // pieces of keys (of values) a thread
@@ -134,22 +135,38 @@ __global__ __launch_bounds__(WAVES * kWave, sizeof(T) == 2 ? 2 : 1) void k_cache
     __shared__ ChunkLds<NB> lds;
     const CacheAttnArgs& a = p.a;
     const int tid = int(threadIdx.x), lane = tid % kWave, wave = tid / kWave, n = lane % 32, h = lane / 32;
-    const uint32_t head = blockIdx.x % a.c.kv_heads, worker = blockIdx.x / a.c.kv_heads;
+    const uint32_t head = blockIdx.x, worker = blockIdx.y, block = worker * a.c.kv_heads + head;
     const auto upto = read_only(p.upto);
-    const uint32_t tiles = read_only(p.begin)[a.c.requests];
-    const uint64_t total = tiles ? upto[tiles] : 0, share = max(uint64_t(a.least), (total + a.workers - 1) / a.workers);
-    uint64_t at = min(total, uint64_t(worker) * share);
-    const uint64_t end = min(total, at + share);
+    uint64_t at = 0, end = 1, share = 1;
+    uint32_t tile_at = worker;
+    if constexpr (!ALONE) {
+        const uint32_t tiles = read_only(p.begin)[a.c.requests];
+        const uint64_t total = tiles ? upto[tiles] : 0;
+        const uint64_t each = tiles ? total / tiles : 0;  // (a worker takes one short tile, not several in turn)
+        share = max(min(max(each, uint64_t(1)), uint64_t(a.least)), (total + a.workers - 1) / a.workers);
+        at = min(total, uint64_t(worker) * share);
+        end = min(total, at + share);
+        if (at < end) tile_at = uniform(last_at_most(p.upto, tiles, at, lane));
+    }
     uint4 meta = make_uint4(0, 0, 0, 0);
     // What this thread brings of a tile: keys k_key + 32 i, columns 16 k_piece; columns v_col + 64 i, keys 16 v_group.
     const uint32_t k_key = uint32_t(tid) / PIECES, k_piece = uint32_t(tid) % PIECES, v_group = uint32_t(tid) % 4, v_col = uint32_t(tid) / 4;
     const bool brings = THREADS <= NB * 256 || tid < NB * 256;
-    uint32_t tile_at = at < end ? uniform(last_at_most(p.upto, tiles, at, lane)) : 0;
     for (; at < end; ++tile_at) {
-        const uint64_t base = upto[tile_at], next_base = upto[tile_at + 1];
-        if (at >= next_base) continue;  // (a tile of no work)
-        const uint32_t request = read_only(p.request)[tile_at], row_tile = tile_at - read_only(p.begin)[request];
+        uint64_t base = 0, next_base;
+        uint32_t request = worker, row_tile = blockIdx.z;
+        if constexpr (!ALONE) {
+            base = upto[tile_at];
+            next_base = upto[tile_at + 1];
+            if (at >= next_base) continue;  // (a tile of no work)
+            request = read_only(p.request)[tile_at];
+            row_tile = tile_at - read_only(p.begin)[request];
+        }
         const CacheRequest rq = request_of(a, request);
+        if constexpr (ALONE) {
+            if (row_tile >= chunk_tiles(p, rq)) return;
+            next_base = end = tiles_seen(p, rq, row_tile);
+        }
         const uint32_t all = uint32_t(next_base - base), lo = uint32_t(at - base), hi = index_min(all, lo + (end - at));
         const uint32_t packed = row_tile * ROWS + uint32_t(wave) * kWaveRows + uint32_t(n), rows = rq.rows * a.c.group;
         const uint32_t seen = packed < rows ? cache_seen(rq, packed / a.c.group) : 0;
@@ -402,7 +419,7 @@ __global__ __launch_bounds__(WAVES * kWave, sizeof(T) == 2 ? 2 : 1) void k_cache
         }
         sum = xor32_add(sum);
         const bool cut = lo > 0 || hi < all;
-        const uint64_t piece = (uint64_t(blockIdx.x) * 2 + (lo > 0 ? 0 : 1)) * WAVES + uint64_t(wave);
+        const uint64_t piece = (uint64_t(block) * 2 + (lo > 0 ? 0 : 1)) * WAVES + uint64_t(wave);
 #pragma unroll
         for (int d = 0; d < 2 * NB; ++d)
 #pragma unroll
@@ -423,7 +440,7 @@ __global__ __launch_bounds__(WAVES * kWave, sizeof(T) == 2 ? 2 : 1) void k_cache
         at += hi - lo;
         __syncthreads();
     }
-    if (tid == 0) a.meta[blockIdx.x] = meta;
+    if (!ALONE && tid == 0) a.meta[block] = meta;
 }
 
 // The pieces of the row tile that begins in a worker and ends in another: a wave its 32 rows, four columns of each lane a block.
@@ -455,10 +472,14 @@ uint64_t pad256(uint64_t b) { return (b + 255) / 256 * 256; }
 
 template <class T, int NB, int WAVES>
 hipError_t launch(const ChunkArgs& p, hipStream_t s) {
+    if (!p.a.workers) {
+        k_cache_chunk<T, NB, WAVES, true><<<dim3(p.a.c.kv_heads, p.a.c.requests, p.a.row_tiles), WAVES * kWave, 0, s>>>(p);
+        return hipGetLastError();
+    }
     const uint32_t blocks = p.a.workers * p.a.c.kv_heads;
     k_cache_plan<<<1, kScan, 0, s>>>(p);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    k_cache_chunk<T, NB, WAVES><<<blocks, WAVES * kWave, 0, s>>>(p);
+    k_cache_chunk<T, NB, WAVES, false><<<dim3(p.a.c.kv_heads, p.a.workers), WAVES * kWave, 0, s>>>(p);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     k_cache_chunk_join<T, NB, WAVES><<<dim3(blocks, 8 * NB), WAVES * kWave, 0, s>>>(p);
     return hipGetLastError();
@@ -471,9 +492,11 @@ int waves_of(const CacheSizes& c, bool bf16) { return bf16 && uint64_t(c.most) *
 
 }  // namespace
 
+uint32_t chunk_rows(const CacheSizes& c, bool bf16) { return uint32_t(waves_of(c, bf16)) * kWaveRows; }
+
 ChunkPlan chunk_plan(int cus, const CacheSizes& c, bool bf16) {
     ChunkPlan p;
-    const uint32_t tile = uint32_t(waves_of(c, bf16)) * kWaveRows;
+    const uint32_t tile = chunk_rows(c, bf16);
     p.tiles = uint32_t(c.rows * c.group / tile + c.requests);  // a request's last tile may be part full
     p.workers = uint32_t(std::max(1, (bf16 && waves_of(c, bf16) == 4 ? 2 : 1) * cus / int(c.kv_heads)));
     const uint64_t blocks = uint64_t(p.workers) * c.kv_heads, nb = c.dim > 64 ? 2 : 1;
@@ -496,11 +519,10 @@ ChunkPlan chunk_plan(int cus, const CacheSizes& c, bool bf16) {
 hipError_t launch_cache_chunk(const CacheAttnArgs& args, bool bf16, const ChunkPlan& plan, void* workspace, hipStream_t s) {
     ChunkArgs p;
     p.a = args;
-    p.a.workers = plan.workers;
     char* const ws = static_cast<char*>(workspace);
     p.tiles = plan.tiles;
     const int waves = waves_of(args.c, bf16);
-    p.tile_rows = uint32_t(waves) * kWaveRows;
+    p.tile_rows = chunk_rows(args.c, bf16);
     p.begin = reinterpret_cast<uint32_t*>(ws + plan.begin);
     p.request = reinterpret_cast<uint32_t*>(ws + plan.request);
     p.upto = reinterpret_cast<uint64_t*>(ws + plan.upto);

@@ -41,7 +41,7 @@ GATGPU_INDEX uint32_t cache_seen(const CacheRequest& q, uint32_t i) {
     const int64_t n = q.shift + int64_t(i) + 1;
     return n < 0 ? 0u : uint32_t(n);
 }
-// Tiles of a request's work: its row tiles times its key tiles (one, if it has none).
+// Tiles of a request: of keys (one, if it has none), and of its packed rows.
 GATGPU_INDEX uint32_t key_tiles(const CacheRequest& q) { return q.keys ? (q.keys - 1) / kCacheTile + 1 : 1; }
 GATGPU_INDEX uint32_t row_tiles(const CacheSizes& c, const CacheRequest& q) {
     return uint32_t((uint64_t(q.rows) * c.group + kCacheRows - 1) / kCacheRows);

@@ -255,3 +255,37 @@ def test_two_contexts_at_once(ctx, most):
         torch.cuda.synchronize()
     for (_, _, d), x in zip(held, want):
         assert torch.equal(d["out"], x)
+
+
+@pytest.mark.parametrize("precision", [FP, BF])
+@pytest.mark.parametrize("requests,kv_heads,group,rows,most_keys", [(150, 1, 2, 1, 3000), (70, 4, 4, 16, 1500), (70, 4, 2, 16, 1500), (200, 2, 8, 2, 1500)])
+def test_ranges_over_many_requests(ctx, precision, requests, kv_heads, group, rows, most_keys):
+    """A block's range ends in one request and goes on in others, of one to four row tiles side by side."""
+    g = generator(requests + group)
+    lens = torch.randint(1, most_keys // 8, (requests,), generator=g).tolist()
+    lens[3], lens[40], lens[requests - 1] = most_keys, most_keys - 1, 0
+    q_len = [int(torch.randint(0, min(rows, n) + 1, (1,), generator=g)) for n in lens]
+    q_len[3], q_len[40] = rows, rows
+    p = Serving(lens, q_len, kv_heads * group, kv_heads, 16, 16, precision, seed=requests)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("precision", [FP, BF])
+@pytest.mark.parametrize("group,rows,lens", [(1, 1, [41_000, 3000]), (4, 16, [9000, 5000, 64]), (3, 15, [14_000, 130, 0]), (2, 13, [4100, 4097, 33, 700]), (4, 8, [1100, 90])])
+def test_ranges_of_few_requests(ctx, precision, group, rows, lens):
+    """One to four row tiles side by side, ranges that end between the key tiles of some and of others, in every amount of work."""
+    q_len = [min(rows - i, n) for i, n in enumerate(lens)]
+    p = Serving(lens, [max(0, n) for n in q_len], 8 * group, 8, 16, 16, precision, seed=60 + rows)
+    p.check(p.run(ctx))
+
+
+@pytest.mark.parametrize("keys", [511, 512, 513, 1023, 1024, 1025])
+@forms
+def test_where_a_block_takes_a_row_tile_alone(ctx, precision, most, keys):
+    """Tables at the lengths where the forms change, and one whose blocks are too many for that."""
+    p = Serving([keys, 90], [16, 16], 4, 2, 16, 16, precision, seed=keys)
+    p.check(p.run(ctx, most=most))
+    if keys == 512:
+        p = Serving([keys] + [20] * 300, [16] + [1] * 300, 4, 2, 16, 16, precision, seed=keys)
+        p.check(p.run(ctx, most=most))
+        p.check(p.run(ctx, most=5000))
