@@ -8,7 +8,7 @@
 // the keys.  Where tables are short, a block takes a row tile alone, and there is nothing to join.
 //
 // One token over 260001 keys, 32 heads on 8 of 128 columns, bf16 rows: 96 us, 5.5 TB/s, and 6.4 for the join; 48 tokens
-// over 200 to 24000 keys: 77 us, 4.6 TB/s, and 5.5.
+// over 200 to 24000 keys: 77 us, 4.3 TB/s, and 5.5.
 #include <algorithm>
 #include <cmath>
 #include <string>

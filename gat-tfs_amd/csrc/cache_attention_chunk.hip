@@ -1,15 +1,19 @@
 // Attention over a paged 8-bit cache, many rows a request: chunks of prompts.
 //
 // Bound by matrix and vector instructions (4 products of 64 x 32 x dim a step and wave, an exponential a pair).  A block of
-// four waves takes 128 packed rows, 32 a wave, on v_mfma_f32_32x32x16.  Its threads request a tile of 64 keys two steps
-// ahead, turn its bytes to bf16 keys and fp16 values once for the four waves, and leave them in one of two LDS buffers
+// four or eight waves takes 128 or 256 packed rows, 32 a wave, on v_mfma_f32_32x32x16.  Its threads request a tile of 64 keys
+// two steps ahead, turn its bytes to bf16 keys and fp16 values once for all waves, and leave them in one of two LDS buffers
 // while the other is worked on; one barrier a step.
 //   S^T = K Q^T: lane (n = lane % 32, h = lane / 32) gets row n's scores of LDS rows 8 i + 4 h + r (register 4 i + r), and LDS
 //   row m of 32 holds key 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so that registers 8 s ... 8 s + 7 are keys
 //   16 s + 8 h ... + 7: the second product's operand as they stand.
 //
-// Work is cut into equal ranges of (row tile, key tile) for two blocks a unit, since lengths are known on the device only:
-// a first launch of one block forms the sums over the tiles, and a last one joins the tiles that a range's end cuts.
+// Work is cut into equal ranges of (row tile, key tile) for as many blocks as run at once, since lengths are known on the
+// device only: a first launch of one block forms the sums over the tiles, and a last one joins the tiles that a range's end
+// cuts.  Where tables are short, a block takes a row tile alone, in one launch.
+//
+// 6 requests of 324 to 1649 rows over up to 10392 keys, 16 heads on 4 of 128 columns, bf16: 259 us, 658 TFLOP/s (vector
+// instructions 48 % of the cycles, matrix pipes 35 %, one behind the other in a wave), sums 4.9, join 17.8.
 #include <algorithm>
 #include <type_traits>
 

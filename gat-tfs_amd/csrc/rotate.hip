@@ -11,6 +11,9 @@
 // positions keep an angle's error of 2^-23.  Groups of lanes then take the row's heads in turn with their columns' sines
 // in registers.  The backward pass gives each block a fixed set of rows and keeps its columns' sums for gamma in
 // registers over them; blocks leave one partial row each, added in one fixed order.
+//
+// 20011 rows of 20 heads of 128, bf16: forward 42 us, 4.9 TB/s of the 2 rows, backward 79 us, 3.9 TB/s of 3, the partial
+// rows' sums 4.6.  7 rows of 16 heads of 64: 3.7 us, a launch.
 #include <algorithm>
 #include <cmath>
 #include <string>
