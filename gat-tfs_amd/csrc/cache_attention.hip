@@ -92,6 +92,7 @@ template <int NB>
 struct Running {
     f32x4_t o[4 * NB];
     float ref, sum;
+    uint64_t far;  // lanes of rows whose reference is
 };
 
 // Scores of a tile: keys [operand][register] by the lane's row.
@@ -125,7 +126,7 @@ struct Weights {
 template <int PARTS, int NB>
 __device__ inline Weights weigh(const CacheAttnArgs& a, Running<NB>& run, Scores x, const Values<NB>& t, uint32_t tile, uint32_t seen, bool whole, int lane) {
     const int ev = scale_exponent(t.vs);
-    const float by = a.scale * power_of_two(scale_exponent(t.ks));
+    const float by = score_factor(a.scale, t.ks);
     if (!whole) {
         const uint32_t first = own_key(tile, lane), here = t.page && seen > first ? seen - first : 0;
 #pragma unroll
@@ -145,6 +146,7 @@ __device__ inline Weights weigh(const CacheAttnArgs& a, Running<NB>& run, Scores
         const bool up = all > run.ref + kCacheRoom;
         const float ref = up ? ceilf(all) - kCacheSet : run.ref, less = up ? __builtin_amdgcn_exp2f(run.ref - ref) : 1.0f;
         run.ref = ref;
+        run.far |= __ballot(up && fabsf(ref) >= kCacheFar);
         run.sum *= less;
 #pragma unroll
         for (int d = 0; d < 4 * NB; ++d) run.o[d] *= less;
@@ -226,6 +228,67 @@ __device__ inline void add_values(Running<NB>& run, const Weights& w, const Valu
         run.o[d] = mfma_f16(lo, w.w[0], run.o[d]);
         run.o[d] = mfma_f16(hi, w.w[1], run.o[d]);
     }
+}
+
+// A wave's share of tiles, every `per`-th from `tile` on, with references that follow the scores alone (kCacheFar).
+template <class T, int NB>
+__device__ inline void far_pass(const CacheAttnArgs& a, const uint32_t* row, const Queries<T, NB>& q, uint32_t keys, uint32_t seen, uint32_t tile, uint32_t stop,
+                                      uint32_t per, uint32_t head, int lane, Running<NB>& run) {
+#pragma unroll
+    for (int d = 0; d < 4 * NB; ++d) run.o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    run.ref = kCacheNoRef;
+    run.sum = 0.0f;
+    for (; tile < stop; tile += per) {
+        const TilePages pages = tile_pages(a, row, keys, tile, lane);
+        Keys<NB> k;
+        Values<NB> v;
+        load_keys<NB>(a, pages.load, tile, head, lane, k);
+        load_values<NB>(a, pages.own, tile, head, lane, v);
+        Scores x = scores<T, NB>(q, k);
+        clean<NB>(run, v, tile, keys, seen, lane);
+        const int ev = scale_exponent(v.vs);
+        const float by = score_factor(a.scale, v.ks);
+        const uint32_t first = own_key(tile, lane), here = v.page && seen > first ? seen - first : 0;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                x.s[i][r] = uint32_t(4 * i + r) < here ? far_score(x.s[i][r], by) : -INFINITY;
+                top = fmaxf(top, x.s[i][r]);
+            }
+        top = xor32_max(xor16_max(top));
+        if (top > run.ref + kCacheRoom) {
+            const float ref = ceilf(top) - kCacheSet, less = __builtin_amdgcn_exp2f(run.ref - ref);
+            run.ref = ref;
+            run.sum *= less;
+#pragma unroll
+            for (int d = 0; d < 4 * NB; ++d) run.o[d] *= less;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t u[4], l[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p0 = far_weight(x.s[2 * h + j / 2][j % 2 * 2], run.ref), p1 = far_weight(x.s[2 * h + j / 2][j % 2 * 2 + 1], run.ref);
+                run.sum += p0 + p1;
+                u[j] = f16x2(p0, p1);
+                const f16x2_t up = __builtin_bit_cast(f16x2_t, u[j]);
+                l[j] = f16x2(p0 - float(up[0]), p1 - float(up[1]));
+            }
+            for (int g = 0; g < 4; ++g) {  // (the lanes' keys of one page at a time)
+                const uint32_t keep = lane / 16 == g ? 0xffffffffu : 0u;
+                const uint4 w = make_uint4(u[0] & keep, u[1] & keep, u[2] & keep, u[3] & keep), rest = make_uint4(l[0] & keep, l[1] & keep, l[2] & keep, l[3] & keep);
+                const float scale = power_of_two(__builtin_amdgcn_readlane(ev, 16 * g));
+#pragma unroll
+                for (int d = 0; d < 4 * NB; ++d) {
+                    const uint4 c = h ? values_operand(v.w[d].z, v.w[d].w) : values_operand(v.w[d].x, v.w[d].y);
+                    run.o[d] += mfma_f16(c, w, mfma_f16(c, rest, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f})) * scale;
+                }
+            }
+        }
+    }
+    run.sum = xor32_add(xor16_add(run.sum));
 }
 
 // Row tiles that a block takes side by side, as a power of two (at most 4, the most of a request here), and the work of a
@@ -356,6 +419,7 @@ __global__ __launch_bounds__((ALONE ? kAloneWaves : kWaves) * kWave, 2) void k_c
         for (int d = 0; d < 4 * NB; ++d) run.o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         run.ref = kCacheNoRef;
         run.sum = 0.0f;
+        run.far = 0;
         const uint32_t stop = min(hi, (most + kCacheTile - 1) / kCacheTile);
         uint32_t tile = lo + member;
         if (tile < stop) {
@@ -390,6 +454,17 @@ __global__ __launch_bounds__((ALONE ? kAloneWaves : kWaves) * kWave, 2) void k_c
         }
 #pragma unroll
         for (int d = 0; d < 4 * NB; ++d) join.o[wave][d][lane] = run.o[d];
+        if (run.far) {
+            const bool mine = run.far >> lane & 1;
+            far_pass<T, NB>(a, row, q, rq.keys, seen, lo + member, stop, per, head, lane, run);
+            if (mine && lane < 16) {
+                join.ref[wave][n] = run.ref;
+                join.sum[wave][n] = run.sum;
+            }
+#pragma unroll
+            for (int d = 0; d < 4 * NB; ++d)
+                if (mine) join.o[wave][d][lane] = run.o[d];
+        }
         __syncthreads();
         const uint32_t first = group * per;
         float ref = join.ref[first][n], sum = 0.0f, less[WAVES];

@@ -85,6 +85,27 @@ __device__ inline uint32_t low_bytes(int n) { return n <= 0 ? 0u : n >= 4 ? 0xff
 // lie before it is raised, and how far below the score it is raised to.  References are whole numbers, so that rescaling
 // is exact and a weight's exponent, x + (ev - ref), is rounded once.
 constexpr float kCacheNoRef = -3.402823466e38f, kCacheRoom = 15.0f, kCacheSet = 7.0f;
+// References from this size on are far: an exponent's rounding is a quarter and more of a step of 2, and soon wider than the room
+// and the values' exponents.  What a wave (a block) has of rows whose reference is far is formed again, behind the others: the
+// reference follows the scores alone, which are rounded before it leaves them, so that none passes the largest one, and the
+// values' exponents are applied to the sums, 16 keys at a time.
+constexpr float kCacheFar = 4194304.0f;
+// A far row's score, rounded before anything leaves it, and its weight (NaN stays).
+__device__ inline float far_score(float score, float by) {
+#pragma clang fp contract(off)
+    return score * by;
+}
+__device__ inline float far_weight(float score, float ref) {
+#pragma clang fp contract(off)
+    const float x = score - ref;
+    return __builtin_amdgcn_exp2f(x > kCacheRoom ? kCacheRoom : x);
+}
+
+// What a page's scores are multiplied by: scale log2 e 2^exponent, kept among FP32's normal values, so that a masked score stays
+// -infinity and one of 0 stays 0.
+__device__ inline float score_factor(float scale, float page_scale) {
+    return __builtin_amdgcn_fmed3f(scale * power_of_two(scale_exponent(page_scale)), 1.17549435e-38f, 3.402823466e38f);
+}
 
 // Columns col to col + 3 of a packed row, from the sums of its weights' products and of its weights.
 template <class T>

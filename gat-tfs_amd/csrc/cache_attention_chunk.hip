@@ -105,6 +105,7 @@ struct ChunkLds {
     float scale[2][4][2];  // of each 16 keys: what a score is multiplied by, and the values' exponent; without a page: -1
     uint16_t bad[2][64 * NB][4];  // which of each 16 keys' values are NaN (they stand as 0 in v)
     uint32_t nan[4];       // the values of tile i (of a piece), in place i % 4, hold one
+    uint32_t far;          // some row's reference is
 };
 
 // What a thread requests of a tile, in 16 bytes: of N keys each 16 columns, and of N columns each 16 keys.
@@ -204,7 +205,7 @@ __global__ __launch_bounds__(WAVES * kWave, sizeof(T) == 2 ? 2 : 1) void k_cache
             Bytes<N> x;
             if (tid < 4) {
                 const uint64_t place = uint64_t(some_page(a.c, g.v)) * a.c.kv_heads + head;
-                x.ks = g.v < a.c.pages ? a.scale * power_of_two(scale_exponent(a.k_scale[place])) : -1.0f;
+                x.ks = g.v < a.c.pages ? score_factor(a.scale, a.k_scale[place]) : -1.0f;
                 x.vs = float(scale_exponent(a.v_scale[place]));
             }
             const uint32_t place = tile * kCacheTile & in_page;
@@ -259,186 +260,222 @@ __global__ __launch_bounds__(WAVES * kWave, sizeof(T) == 2 ? 2 : 1) void k_cache
             }
         };
 
-        Pages<N> pages = load_pages(lo);
-        Bytes<N> bytes = load_bytes(lo, pages);
-        pages = load_pages(lo + 1);
         QueryParts<T> q[4 * NB];
-        const T* const row = query_row<T>(a, rq, packed, head);
-#pragma unroll
-        for (int s = 0; s < 4 * NB; ++s) {
-            const uint32_t col = uint32_t(16 * s + 8 * h);
-            q[s] = load_query8(row, col, packed < rows && col < a.c.dim);
-        }
         f32x16_t o[2 * NB];
+        float ref, sum;
+        uint64_t far = 0;  // lanes of rows whose reference is
+        // The tiles' sums; FAR: with references that follow the scores alone (kCacheFar).
+        const auto sums = [&](auto far_pass) {
+            constexpr bool FAR = decltype(far_pass)::value;
+            Pages<N> pages = load_pages(lo);
+            Bytes<N> bytes = load_bytes(lo, pages);
+            pages = load_pages(lo + 1);
+            if constexpr (!FAR) {
+                const T* const row = query_row<T>(a, rq, packed, head);
 #pragma unroll
-        for (int d = 0; d < 2 * NB; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
-        float ref = kCacheNoRef, sum = 0.0f;
-        if (tid < 4) lds.nan[tid] = 0;
-        __syncthreads();
-        put(lo, bytes);
-        if (lo + 1 < hi) {
-            bytes = load_bytes(lo + 1, pages);
-            pages = load_pages(lo + 2);
-        }
-        __syncthreads();
-        for (uint32_t tile = lo; tile < hi; ++tile) {
-            const uint32_t buffer = (tile - lo) % 2;
-            if (tid == 0) lds.nan[(tile - lo + 2) % 4] = 0;  // (read two barriers ago, set again behind the next one)
-            if (tile + 1 < hi) {
-                put(tile + 1, bytes);
-                if (tile + 2 < hi) {
-                    bytes = load_bytes(tile + 2, pages);
-                    pages = load_pages(tile + 3);
+                for (int s = 0; s < 4 * NB; ++s) {
+                    const uint32_t col = uint32_t(16 * s + 8 * h);
+                    q[s] = load_query8(row, col, packed < rows && col < a.c.dim);
                 }
             }
-            if (tile * kCacheTile < most) {
-                // Of the tile's four 16 keys: scales, and whether they have a page.  The same in all lanes.
-                float by[4], ev[4];
-                uint32_t held = 0;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const uint32_t factor = uniform(__float_as_uint(lds.scale[buffer][g][0]));
-                    by[g] = __uint_as_float(factor & 0x7fffffffu);
-                    ev[g] = __uint_as_float(uniform(__float_as_uint(lds.scale[buffer][g][1])));
-                    if (!(factor >> 31)) held |= 1u << g;
-                }
-                f32x16_t s[2];
+            for (int d = 0; d < 2 * NB; ++d)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
-                // Two chains of products; their keys are read a step ahead.
-                uint4 keys[2][2];
-                const auto read_keys = [&](int c) {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) keys[c % 2][k] = lds.k[buffer][32 * k + n][uint32_t(2 * c + h) ^ turned<8 * NB>(uint32_t(n))];
-                };
-                read_keys(0);
-                __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-                for (int c = 0; c < 4 * NB; ++c) {
-                    if (c + 1 < 4 * NB) read_keys(c + 1);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int part = PARTS - 1; part >= 0; --part)
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) s[k] = mfma32_bf16(keys[c % 2][k], q[c].w[part], s[k]);
-                }
-                __builtin_amdgcn_s_setprio(0);
-                uint4 values[2][2 * NB];  // of 16 keys, for the second product: the first ones are there when their weights are
-                const auto read_values = [&](int g) {
-#pragma unroll
-                    for (int d = 0; d < 2 * NB; ++d) values[g % 2][d] = lds.v[buffer][32 * d + n][uint32_t(2 * g + h) ^ turned<8>(uint32_t(n))];
-                };
-                read_values(0);
-                __builtin_amdgcn_sched_barrier(0);
-                const bool whole = (tile + 1) * kCacheTile <= least && held == 15;
-                if (!whole) {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int g = 2 * k + r / 8;
-                            if (!(held >> g & 1) || tile * kCacheTile + uint32_t(16 * g + 8 * h + r % 8) >= seen) s[k][r] = -INFINITY;
-                        }
-                }
-                float top = -INFINITY;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    float t = s[g / 2][8 * (g % 2)];
-#pragma unroll
-                    for (int r = 1; r < 8; ++r) t = fmaxf(t, s[g / 2][8 * (g % 2) + r]);
-                    top = fmaxf(top, fmaf(t, by[g], ev[g]));
-                }
-                if (__any(top > ref + kCacheRoom)) {
-                    const float both = xor32_max(top);
-                    const bool up = both > ref + kCacheRoom;
-                    const float to = up ? ceilf(both) - kCacheSet : ref, less = up ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
-                    ref = to;
-                    sum *= less;
-#pragma unroll
-                    for (int d = 0; d < 2 * NB; ++d)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) o[d][r] *= less;
-                }
-                uint4 w[4], rest[4];
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float shift = ev[g] - ref;  // (whole numbers: exact)
-                    float x[8], of = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        x[r] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + r], by[g], shift));
-                        of += x[r];
-                    }
-                    uint32_t u[4], l[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        u[j] = f16x2(x[2 * j], x[2 * j + 1]);
-                        if constexpr (PARTS > 1) {
-                            const f16x2_t up = __builtin_bit_cast(f16x2_t, u[j]);
-                            l[j] = f16x2(x[2 * j] - float(up[0]), x[2 * j + 1] - float(up[1]));
-                        }
-                    }
-                    sum = fmaf(of, power_of_two(-int(ev[g])), sum);
-                    w[g] = make_uint4(u[0], u[1], u[2], u[3]);
-                    if constexpr (PARTS > 1) rest[g] = make_uint4(l[0], l[1], l[2], l[3]);
-                }
-                if ((tile + 1) * kCacheTile > all_seen && lds.nan[(tile - lo) % 4]) {  // NaNs mark the rows that see them
-#pragma unroll
-                    for (int d = 0; d < 2 * NB; ++d)
-#pragma unroll 1
-                        for (int g = 0; g < 4; ++g) {
-                            const uint32_t bits = uint32_t(lds.bad[buffer][32 * d + n][g]) >> (8 * h);
-                            uint32_t x[4], u[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint32_t key = tile * kCacheTile + uint32_t(16 * g + 8 * h + 2 * j);
-                                x[j] = (bits >> (2 * j) & 1u ? 0x3c00u : 0u) | (bits >> (2 * j + 1) & 1u ? 0x3c000000u : 0u);
-                                u[j] = (key < seen ? 0x3c00u : 0u) | (key + 1 < seen ? 0x3c000000u : 0u);
-                            }
-                            f32x16_t count;
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) count[r] = 0.0f;
-                            count = mfma32_f16(make_uint4(x[0], x[1], x[2], x[3]), make_uint4(u[0], u[1], u[2], u[3]), count);
-#pragma unroll
-                            for (int r = 0; r < 16; ++r)
-                                if (count[r] > 0.0f) o[d][r] = NAN;
-                        }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    if (g + 1 < 4) read_values(g + 1);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int part = 0; part < (PARTS > 1 ? 2 : 1); ++part)
-#pragma unroll
-                        for (int d = 0; d < 2 * NB; ++d) o[d] = mfma32_f16(values[g % 2][d], PARTS > 1 && part == 0 ? rest[g] : w[g], o[d]);
-                }
-                __builtin_amdgcn_s_setprio(0);
+                for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+            ref = kCacheNoRef;
+            sum = 0.0f;
+            if (tid < 4) lds.nan[tid] = 0;
+            if (!FAR && tid == 0) lds.far = 0;
+            __syncthreads();
+            put(lo, bytes);
+            if (lo + 1 < hi) {
+                bytes = load_bytes(lo + 1, pages);
+                pages = load_pages(lo + 2);
             }
             __syncthreads();
-        }
-        sum = xor32_add(sum);
+            for (uint32_t tile = lo; tile < hi; ++tile) {
+                const uint32_t buffer = (tile - lo) % 2;
+                if (tid == 0) lds.nan[(tile - lo + 2) % 4] = 0;  // (read two barriers ago, set again behind the next one)
+                if (tile + 1 < hi) {
+                    put(tile + 1, bytes);
+                    if (tile + 2 < hi) {
+                        bytes = load_bytes(tile + 2, pages);
+                        pages = load_pages(tile + 3);
+                    }
+                }
+                if (tile * kCacheTile < most) {
+                    // Of the tile's four 16 keys: scales, and whether they have a page.  The same in all lanes.
+                    float by[4], ev[4];
+                    uint32_t held = 0;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const uint32_t factor = uniform(__float_as_uint(lds.scale[buffer][g][0]));
+                        by[g] = __uint_as_float(factor & 0x7fffffffu);
+                        ev[g] = __uint_as_float(uniform(__float_as_uint(lds.scale[buffer][g][1])));
+                        if (!(factor >> 31)) held |= 1u << g;
+                    }
+                    f32x16_t s[2];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
+                    // Two chains of products; their keys are read a step ahead.
+                    uint4 keys[2][2];
+                    const auto read_keys = [&](int c) {
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) keys[c % 2][k] = lds.k[buffer][32 * k + n][uint32_t(2 * c + h) ^ turned<8 * NB>(uint32_t(n))];
+                    };
+                    read_keys(0);
+                    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                    for (int c = 0; c < 4 * NB; ++c) {
+                        if (c + 1 < 4 * NB) read_keys(c + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) s[k] = mfma32_bf16(keys[c % 2][k], q[c].w[part], s[k]);
+                    }
+                    __builtin_amdgcn_s_setprio(0);
+                    uint4 values[2][2 * NB];  // of 16 keys, for the second product: the first ones are there when their weights are
+                    const auto read_values = [&](int g) {
+#pragma unroll
+                        for (int d = 0; d < 2 * NB; ++d) values[g % 2][d] = lds.v[buffer][32 * d + n][uint32_t(2 * g + h) ^ turned<8>(uint32_t(n))];
+                    };
+                    if (!FAR) read_values(0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const bool whole = (tile + 1) * kCacheTile <= least && held == 15;
+                    if (!whole) {
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const int g = 2 * k + r / 8;
+                                if (!(held >> g & 1) || tile * kCacheTile + uint32_t(16 * g + 8 * h + r % 8) >= seen) s[k][r] = -INFINITY;
+                            }
+                    }
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        float t = s[g / 2][8 * (g % 2)];
+#pragma unroll
+                        for (int r = 1; r < 8; ++r) t = fmaxf(t, s[g / 2][8 * (g % 2) + r]);
+                        top = fmaxf(top, FAR ? far_score(t, by[g]) : fmaf(t, by[g], ev[g]));
+                    }
+                    if (__any(top > ref + kCacheRoom)) {
+                        const float both = xor32_max(top);
+                        const bool up = both > ref + kCacheRoom;
+                        const float to = up ? ceilf(both) - kCacheSet : ref, less = up ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
+                        ref = to;
+                        if (!FAR) far |= __ballot(up && fabsf(to) >= kCacheFar);
+                        sum *= less;
+#pragma unroll
+                        for (int d = 0; d < 2 * NB; ++d)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[d][r] *= less;
+                    }
+                    uint4 w[4], rest[4];
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float shift = ev[g] - ref;  // (whole numbers: exact)
+                        float x[8], of = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) {
+                            if constexpr (FAR) x[r] = far_weight(far_score(s[g / 2][8 * (g % 2) + r], by[g]), ref);
+                            else x[r] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + r], by[g], shift));
+                            of += x[r];
+                        }
+                        uint32_t u[4], l[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            u[j] = f16x2(x[2 * j], x[2 * j + 1]);
+                            if constexpr (PARTS > 1) {
+                                const f16x2_t up = __builtin_bit_cast(f16x2_t, u[j]);
+                                l[j] = f16x2(x[2 * j] - float(up[0]), x[2 * j + 1] - float(up[1]));
+                            }
+                        }
+                        sum = FAR ? sum + of : fmaf(of, power_of_two(-int(ev[g])), sum);
+                        w[g] = make_uint4(u[0], u[1], u[2], u[3]);
+                        if constexpr (PARTS > 1) rest[g] = make_uint4(l[0], l[1], l[2], l[3]);
+                    }
+                    if ((tile + 1) * kCacheTile > all_seen && lds.nan[(tile - lo) % 4]) {  // NaNs mark the rows that see them
+#pragma unroll
+                        for (int d = 0; d < 2 * NB; ++d)
+#pragma unroll 1
+                            for (int g = 0; g < 4; ++g) {
+                                const uint32_t bits = uint32_t(lds.bad[buffer][32 * d + n][g]) >> (8 * h);
+                                uint32_t x[4], u[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const uint32_t key = tile * kCacheTile + uint32_t(16 * g + 8 * h + 2 * j);
+                                    x[j] = (bits >> (2 * j) & 1u ? 0x3c00u : 0u) | (bits >> (2 * j + 1) & 1u ? 0x3c000000u : 0u);
+                                    u[j] = (key < seen ? 0x3c00u : 0u) | (key + 1 < seen ? 0x3c000000u : 0u);
+                                }
+                                f32x16_t count;
+#pragma unroll
+                                for (int r = 0; r < 16; ++r) count[r] = 0.0f;
+                                count = mfma32_f16(make_uint4(x[0], x[1], x[2], x[3]), make_uint4(u[0], u[1], u[2], u[3]), count);
+#pragma unroll
+                                for (int r = 0; r < 16; ++r)
+                                    if (count[r] > 0.0f) o[d][r] = NAN;
+                            }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        if (FAR) read_values(g);
+                        else if (g + 1 < 4) read_values(g + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if constexpr (FAR) {
+#pragma unroll
+                            for (int d = 0; d < 2 * NB; ++d) {
+                                f32x16_t t;
+#pragma unroll
+                                for (int r = 0; r < 16; ++r) t[r] = 0.0f;
+                                if constexpr (PARTS > 1) t = mfma32_f16(values[g % 2][d], rest[g], t);
+                                o[d] += mfma32_f16(values[g % 2][d], w[g], t) * power_of_two(int(ev[g]));
+                            }
+                            continue;
+                        }
+#pragma unroll
+                        for (int part = 0; part < (PARTS > 1 ? 2 : 1); ++part)
+#pragma unroll
+                            for (int d = 0; d < 2 * NB; ++d) o[d] = mfma32_f16(values[g % 2][d], PARTS > 1 && part == 0 ? rest[g] : w[g], o[d]);
+                    }
+                    __builtin_amdgcn_s_setprio(0);
+                }
+                __syncthreads();
+            }
+            sum = xor32_add(sum);
+        };
+        sums(std::false_type{});
+        if (far) lds.far = 1;  // (every writer writes the same)
+        __syncthreads();
+        const bool again = lds.far != 0;
         const bool cut = lo > 0 || hi < all;
         const uint64_t piece = (uint64_t(block) * 2 + (lo > 0 ? 0 : 1)) * WAVES + uint64_t(wave);
+        const auto leave = [&](bool mine) {
+            if (!mine) return;
 #pragma unroll
-        for (int d = 0; d < 2 * NB; ++d)
+            for (int d = 0; d < 2 * NB; ++d)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4_t x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-                if (cut) *reinterpret_cast<f32x4_t*>(a.part + ((piece * (8 * NB) + uint64_t(4 * d + i)) * kWave + uint64_t(lane)) * 4) = x;
-                else store4<T>(a, rq, packed, head, uint32_t(32 * d + 8 * i + 4 * h), x, sum);
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4_t x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                    if (cut) *reinterpret_cast<f32x4_t*>(a.part + ((piece * (8 * NB) + uint64_t(4 * d + i)) * kWave + uint64_t(lane)) * 4) = x;
+                    else store4<T>(a, rq, packed, head, uint32_t(32 * d + 8 * i + 4 * h), x, sum);
+                }
+            if (lane < 32) {
+                if (cut) {
+                    a.stat[piece * 64 + uint64_t(n)] = ref;
+                    a.stat[piece * 64 + 32 + uint64_t(n)] = sum;
+                } else {
+                    store_lse(a, rq, packed, head, ref, sum);
+                }
             }
-        if (lane < 32) {
-            if (cut) {
-                a.stat[piece * 64 + uint64_t(n)] = ref;
-                a.stat[piece * 64 + 32 + uint64_t(n)] = sum;
-            } else {
-                store_lse(a, rq, packed, head, ref, sum);
-            }
+        };
+        leave(!(far >> lane & 1));
+        if (again) {
+            sums(std::true_type{});
+            leave(far >> lane & 1);
         }
         if (lo == 0 && hi < all) meta = make_uint4(request, row_tile, uint32_t((next_base - 1) / share) - worker + 1, 0);
         at += hi - lo;

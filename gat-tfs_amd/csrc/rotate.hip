@@ -544,6 +544,7 @@ int gatgpu_rotate_backward(gatgpu_ctx* c, const gatgpu_rotate_io* io, void* ws, 
         a.part = static_cast<float*>(ws);
     }
     if (!io->rows && !a.part) return GATGPU_OK;
+    if (!io->rows) a.half = 0;  // (zeros to dgamma: no positions, which may be null)
     HIPCHECK(c, (io->precision == GATGPU_BF16 ? launch<uint16_t, true> : launch<float, true>)(a, c->cus, c->stream));
     if (a.part) {
         const uint32_t blocks = uint32_t(backward_bytes(c, io) / (2 * uint64_t(io->dim) * 4));

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import gatgpu
-from cache_cases import Serving, generator, words
+from cache_cases import EPS, Serving, generator, values, words
 
 pytestmark = pytest.mark.gpu
 
@@ -289,3 +289,57 @@ def test_where_a_block_takes_a_row_tile_alone(ctx, precision, most, keys):
         p = Serving([keys] + [20] * 300, [16] + [1] * 300, 4, 2, 16, 16, precision, seed=keys)
         p.check(p.run(ctx, most=most))
         p.check(p.run(ctx, most=5000))
+
+
+@forms
+@pytest.mark.parametrize("size", [1e5, 3e7, 1e9, 1e12, 1e30])
+def test_far_scores(ctx, precision, most, size):
+    """Scores whose steps in FP32 are wider than the room between a weight and its reference: the largest one's value, of either sign."""
+    p = Serving([70, 300], [16, 16], 4, 2, 32, 16, precision, seed=70)
+    for side in (p.host.k, p.host.k_scale):
+        side.zero_()
+    for r, keys in enumerate(p.k_len):
+        for t in range(keys):
+            page = p.table[r][t // 16]
+            p.host.k[page, :, t % 16] = 0xb8  # -1, and 1 in one column
+            p.host.k[page, :, t % 16, t * 7 % 31] = 0x38
+    p.host.k_scale[:] = 1.0
+    hot = [(3, 1, 0), (9, 2, 12), (20, 0, 30), (31, 3, 5)]  # row, head, column: 1 there, and 0 elsewhere
+    for row, head, c in hot:
+        p.q[row, head] = 0
+        p.q[row, head, c] = size
+    p.q[11] *= size
+    p.q[14] *= -size
+    p.q[25] = -size  # every score is size 30 but for rounding
+    d = p.run(ctx, most=most)
+    p.check(d)
+    out, lse = d["out"].cpu()[:, :128].view(32, 4, 32).double(), d["lse"].cpu().double()
+    assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
+    for row, head, c in hot:
+        r, i = divmod(row, 16)
+        seen = p.k_len[r] - 16 + i + 1
+        kv = head // 2
+        them = [t for t in range(seen) if t * 7 % 31 == c]
+        if not them:
+            continue
+        v = torch.stack([values(p.host.v[p.table[r][t // 16], kv, :, t % 16]) * float(p.host.v_scale[p.table[r][t // 16], kv]) for t in them])
+        # (equal scores: their mean; the weights and their sum are exact but for 2^-21, and fp16's rounding where it is no power of two)
+        tol = v.abs().mean(0) * (2.0 ** -20 + (2.0 ** -11 if precision == BF else 2.0 ** -22)) + v.mean(0).abs() * EPS[precision]
+        assert bool(((out[row, head] - v.mean(0)).abs() <= tol).all())
+        top = p.scale * float(p.q[row, head, c])
+        assert abs(float(lse[row, head]) - top - math.log(len(them))) <= top * 2.0 ** -21
+
+
+@forms
+@pytest.mark.parametrize("scale", [1e-40, 1e-30, 1e30])
+def test_scales_beyond_reason(ctx, precision, most, scale):
+    """Factors of scores that would leave FP32: what is not seen stays so, scores of 0 stay 0."""
+    p = Serving([90, 200], [16, 16], 4, 2, 32, 16, precision, seed=71)
+    for s in (p.host.k_scale, p.host.v_scale):
+        s[:] = 2.0 ** -64 if scale < 1 else 2.0 ** 64
+    p.host.v_scale[:] = 1.0
+    if scale > 1:
+        p.q.zero_()
+    p.table[0][2] = NONE
+    p.scale = scale
+    p.check(p.run(ctx, most=most))

@@ -232,6 +232,22 @@ def test_captured_and_replayed(ctx):
         p.check(p.run(ctx))
 
 
+def test_no_rows_give_zeros(ctx):
+    """Gradients of the norms' weights of no rows; arrays of no rows, and what only they would need, may be null."""
+    p = Problem(1, 4, 2, 64, BF, seed=17)
+    d = p.device()
+    io = p.io(d, True)
+    io.rows = 0
+    for n in ("q", "k", "dq_out", "dk_out", "dq", "dk", "position", "freq"):
+        setattr(io, n, None)
+    work = torch.full((ctx.rotate_workspace(io),), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    ctx.rotate_forward(io)
+    ctx.rotate_backward(io, work.data_ptr(), work.numel())
+    ctx.synchronize()
+    assert all(bool((g == 0).all()) for g in d["dgamma"])
+
+
 def test_refusals(ctx):
     p = Problem(10, 4, 2, 64, BF, seed=16)
     d = p.device()
