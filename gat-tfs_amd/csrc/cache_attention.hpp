@@ -43,8 +43,7 @@ struct CacheAttnArgs {
     // Partial sums, of two pieces a worker and head: [piece][row tile][columns / 16][64][4] sums, [piece][row tile][2][16]
     // references and weights.
     float *part = nullptr, *stat = nullptr;
-    // [worker][head]: request, row tile, pieces (0: none) of the work that begins in the worker and ends in another; whether it has far rows
-    uint4* meta = nullptr;
+    uint4* meta = nullptr;  // [worker][head]: request, row tile, pieces (0: none) of the work that begins in the worker and ends in another
 };
 // One request's place (by scalar loads where r is the same in all lanes).
 __device__ inline CacheRequest request_of(const CacheAttnArgs& a, uint32_t r) {
