@@ -122,8 +122,7 @@ __global__ __launch_bounds__(kScan) void k_blocks_assign(const BlocksArgs a) {
     }
     __syncthreads();
     Sums before = {0, 0};
-    uint32_t left = count, unserved = 0;  // after the thread's requests, and of the wave's
-    bool took = false;
+    uint32_t left = count, unserved = 0;  // after the thread's requests that take pages, and of the wave's
     for (uint32_t first = 0; first < a.requests; first += kScan * EACH) {
         const uint64_t page = uint64_t(1) << a.page_log;
         uint64_t c[EACH], f[EACH], need[EACH];
@@ -167,14 +166,11 @@ __global__ __launch_bounds__(kScan) void k_blocks_assign(const BlocksArgs a) {
             } else {
                 a.behind[r] = behind;
             }
-            if (served && need[i]) {
-                left = count - uint32_t(upto.pages);  // (less with each request)
-                took = true;
-            }
+            if (served && need[i]) left = count - uint32_t(upto.pages);  // (less with each request, so the least of all threads' counts)
         }
     }
-    const uint64_t some = __ballot(took);
-    if (some) left = __shfl(left, 63 - __builtin_clzll(some));
+#pragma unroll
+    for (int d = kWave / 2; d; d /= 2) left = min(left, uint32_t(__shfl_xor(int(left), d)));
     if (tid % kWave == 0) {
         atomicMin(&s_left, left);
         atomicAdd(&s_unserved, unserved);
