@@ -92,8 +92,10 @@ template <int NB>
 struct Running {
     f32x4_t o[4 * NB];
     float ref, sum;
-    uint64_t far;  // lanes of rows whose reference is
+    uint64_t far;  // lanes of rows whose reference is; all, where scales are far apart
+    int first;     // exponent of the first page's values (the same in all lanes), kNoExponent before
 };
+constexpr int kNoExponent = 1000;
 
 // Scores of a tile: keys [operand][register] by the lane's row.
 struct Scores {
@@ -123,10 +125,16 @@ struct Weights {
     uint4 w[2], rest[2];
 };
 // seen: keys that the lane's row sees; whole: every row of the wave sees every key of the tile.
-template <int PARTS, int NB>
+template <class T, int NB>
 __device__ inline Weights weigh(const CacheAttnArgs& a, Running<NB>& run, Scores x, const Values<NB>& t, uint32_t tile, uint32_t seen, bool whole, int lane) {
+    constexpr int PARTS = QueryParts<T>::N, APART = kCacheSpread<T> / 2;
     const int ev = scale_exponent(t.vs);
     const float by = score_factor(a.scale, t.ks);
+    if (run.first == kNoExponent) {
+        const uint64_t some = __ballot(t.page);
+        if (some) run.first = __builtin_amdgcn_readlane(ev, __builtin_ctzll(some));
+    }
+    if (__ballot(t.page && uint32_t(ev - run.first + APART) > uint32_t(2 * APART))) run.far = ~uint64_t(0);
     if (!whole) {
         const uint32_t first = own_key(tile, lane), here = t.page && seen > first ? seen - first : 0;
 #pragma unroll
@@ -230,7 +238,7 @@ __device__ inline void add_values(Running<NB>& run, const Weights& w, const Valu
     }
 }
 
-// A wave's share of tiles, every `per`-th from `tile` on, with references that follow the scores alone (kCacheFar).
+// A wave's share of tiles, every `per`-th from `tile` on, with a reference for each 16 keys (kCacheSpread).
 template <class T, int NB>
 __device__ inline void far_pass(const CacheAttnArgs& a, const uint32_t* row, const Queries<T, NB>& q, uint32_t keys, uint32_t seen, uint32_t tile, uint32_t stop,
                                       uint32_t per, uint32_t head, int lane, Running<NB>& run) {
@@ -246,7 +254,6 @@ __device__ inline void far_pass(const CacheAttnArgs& a, const uint32_t* row, con
         load_values<NB>(a, pages.own, tile, head, lane, v);
         Scores x = scores<T, NB>(q, k);
         clean<NB>(run, v, tile, keys, seen, lane);
-        const int ev = scale_exponent(v.vs);
         const float by = score_factor(a.scale, v.ks);
         const uint32_t first = own_key(tile, lane), here = v.page && seen > first ? seen - first : 0;
         float top = -INFINITY;
@@ -257,36 +264,36 @@ __device__ inline void far_pass(const CacheAttnArgs& a, const uint32_t* row, con
                 x.s[i][r] = uint32_t(4 * i + r) < here ? far_score(x.s[i][r], by) : -INFINITY;
                 top = fmaxf(top, x.s[i][r]);
             }
-        top = xor32_max(xor16_max(top));
-        if (top > run.ref + kCacheRoom) {
-            const float ref = ceilf(top) - kCacheSet, less = __builtin_amdgcn_exp2f(run.ref - ref);
-            run.ref = ref;
-            run.sum *= less;
+        const float own = far_reference(top), ref = fmaxf(run.ref, xor32_max(xor16_max(own)));
+        const int less = shift_of(run.ref, ref), up = shift_of(own, ref) - int(kCacheUp), to = up + scale_exponent(v.vs);
+        run.ref = ref;
+        run.sum = shifted(run.sum, less);
 #pragma unroll
-            for (int d = 0; d < 4 * NB; ++d) run.o[d] *= less;
-        }
+        for (int d = 0; d < 4 * NB; ++d) run.o[d] = shifted_all(run.o[d], less);
+        float sum = 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint32_t u[4], l[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float p0 = far_weight(x.s[2 * h + j / 2][j % 2 * 2], run.ref), p1 = far_weight(x.s[2 * h + j / 2][j % 2 * 2 + 1], run.ref);
-                run.sum += p0 + p1;
+                const float p0 = far_weight(x.s[2 * h + j / 2][j % 2 * 2], own), p1 = far_weight(x.s[2 * h + j / 2][j % 2 * 2 + 1], own);
+                sum += p0 + p1;
                 u[j] = f16x2(p0, p1);
-                const f16x2_t up = __builtin_bit_cast(f16x2_t, u[j]);
-                l[j] = f16x2(p0 - float(up[0]), p1 - float(up[1]));
+                const f16x2_t hi = __builtin_bit_cast(f16x2_t, u[j]);
+                l[j] = f16x2(p0 - float(hi[0]), p1 - float(hi[1]));
             }
             for (int g = 0; g < 4; ++g) {  // (the lanes' keys of one page at a time)
                 const uint32_t keep = lane / 16 == g ? 0xffffffffu : 0u;
                 const uint4 w = make_uint4(u[0] & keep, u[1] & keep, u[2] & keep, u[3] & keep), rest = make_uint4(l[0] & keep, l[1] & keep, l[2] & keep, l[3] & keep);
-                const float scale = power_of_two(__builtin_amdgcn_readlane(ev, 16 * g));
+                const int theirs = __shfl(to, 16 * g + lane % 16);
 #pragma unroll
                 for (int d = 0; d < 4 * NB; ++d) {
                     const uint4 c = h ? values_operand(v.w[d].z, v.w[d].w) : values_operand(v.w[d].x, v.w[d].y);
-                    run.o[d] += mfma_f16(c, w, mfma_f16(c, rest, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f})) * scale;
+                    run.o[d] += shifted_all(mfma_f16(c, w, mfma_f16(c, rest, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f})), theirs);
                 }
             }
         }
+        run.sum += shifted(sum, up);
     }
     run.sum = xor32_add(xor16_add(run.sum));
 }
@@ -420,6 +427,7 @@ __global__ __launch_bounds__((ALONE ? kAloneWaves : kWaves) * kWave, 2) void k_c
         run.ref = kCacheNoRef;
         run.sum = 0.0f;
         run.far = 0;
+        run.first = kNoExponent;
         const uint32_t stop = min(hi, (most + kCacheTile - 1) / kCacheTile);
         uint32_t tile = lo + member;
         if (tile < stop) {
@@ -436,7 +444,7 @@ __global__ __launch_bounds__((ALONE ? kAloneWaves : kWaves) * kWave, 2) void k_c
                 const uint32_t next = tile + per;
                 if (next < stop) load_keys<NB>(a, pages.load, next, head, lane, k);
                 const bool whole = tile * kCacheTile + kCacheTile <= least && __all(v.page);  // every row sees every key
-                const Weights w = weigh<PARTS, NB>(a, run, x, v, tile, seen, whole, lane);
+                const Weights w = weigh<T, NB>(a, run, x, v, tile, seen, whole, lane);
                 if (!whole) clean<NB>(run, v, tile, rq.keys, seen, lane);
                 add_values<PARTS, NB>(run, w, v);
                 __builtin_amdgcn_sched_barrier(0);
@@ -448,12 +456,13 @@ __global__ __launch_bounds__((ALONE ? kAloneWaves : kWaves) * kWave, 2) void k_c
         }
         run.sum = xor32_add(xor16_add(run.sum));
         // The sums of a row tile's waves to one: each of them joins its share of the columns.
+        const int shift = weighed(run.ref, run.sum);
         if (lane < 16) {
             join.ref[wave][n] = run.ref;
             join.sum[wave][n] = run.sum;
         }
 #pragma unroll
-        for (int d = 0; d < 4 * NB; ++d) join.o[wave][d][lane] = run.o[d];
+        for (int d = 0; d < 4 * NB; ++d) join.o[wave][d][lane] = shifted_all(run.o[d], shift);
         if (run.far) {
             const bool mine = run.far >> lane & 1;
             far_pass<T, NB>(a, row, q, rq.keys, seen, lo + member, stop, per, head, lane, run);
@@ -467,23 +476,24 @@ __global__ __launch_bounds__((ALONE ? kAloneWaves : kWaves) * kWave, 2) void k_c
         }
         __syncthreads();
         const uint32_t first = group * per;
-        float ref = join.ref[first][n], sum = 0.0f, less[WAVES];
+        float ref = join.ref[first][n], sum = 0.0f;
+        int less[WAVES];
 #pragma unroll
         for (uint32_t w = 1; w < uint32_t(WAVES); ++w)
             if (w < per) ref = fmaxf(ref, join.ref[first + w][n]);
 #pragma unroll
         for (uint32_t w = 0; w < uint32_t(WAVES); ++w) {
             if (w >= per) break;
-            less[w] = __builtin_amdgcn_exp2f(join.ref[first + w][n] - ref);
-            sum = fmaf(join.sum[first + w][n], less[w], sum);
+            less[w] = shift_of(join.ref[first + w][n], ref);
+            sum += shifted(join.sum[first + w][n], less[w]);
         }
         const bool cut = lo > 0 || hi < tiles;
         const uint64_t piece = (uint64_t(block) * 2 + (lo > 0 ? 0 : 1)) * a.row_tiles + row_tile;
         for (uint32_t db = row_tile < rows ? member : 4 * NB; db < 4 * NB; db += per) {
-            f32x4_t o = join.o[first][db][lane] * less[0];
+            f32x4_t o = shifted_all(join.o[first][db][lane], less[0]);
 #pragma unroll
             for (uint32_t w = 1; w < uint32_t(WAVES); ++w)
-                if (w < per) o += join.o[first + w][db][lane] * less[w];
+                if (w < per) o += shifted_all(join.o[first + w][db][lane], less[w]);
             if (cut) *reinterpret_cast<f32x4_t*>(a.part + ((piece * (4 * NB) + uint64_t(db)) * kWave + uint64_t(lane)) * 4) = o;
             else store4<T>(a, rq, packed, head, uint32_t(16 * db + 4 * g), o, sum);
         }
@@ -524,9 +534,9 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_cache_join(const CacheAt
     for (uint32_t p = uint32_t(wave); p < meta.z; p += kJoinWaves) {
         const uint64_t piece = piece_of(p);
         const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part + ((piece * (4 * NB) + db) * kWave + uint64_t(lane)) * 4);
-        const float less = __builtin_amdgcn_exp2f(a.stat[piece * 32 + uint64_t(n)] - ref);
-        o += x * less;
-        sum = fmaf(a.stat[piece * 32 + 16 + uint64_t(n)], less, sum);
+        const int less = shift_of(a.stat[piece * 32 + uint64_t(n)], ref);
+        o += shifted_all(x, less);
+        sum += shifted(a.stat[piece * 32 + 16 + uint64_t(n)], less);
     }
     s_o[wave][lane] = o;
     if (lane < 16) {
@@ -542,9 +552,9 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void k_cache_join(const CacheAt
     sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < kJoinWaves; ++w) {
-        const float less = __builtin_amdgcn_exp2f(s_ref[w][n] - top);
-        o += s_o[w][lane] * less;
-        sum = fmaf(s_sum[w][n], less, sum);
+        const int less = shift_of(s_ref[w][n], top);
+        o += shifted_all(s_o[w][lane], less);
+        sum += shifted(s_sum[w][n], less);
     }
     const uint32_t packed = row_tile * kCacheRows + uint32_t(n);
     store4<T>(a, rq, packed, head, 16 * db + 4 * uint32_t(g), o, sum);

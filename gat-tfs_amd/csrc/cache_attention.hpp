@@ -14,7 +14,9 @@
 // is off by at most 2^-11 of the weight (bf16: 2^-8, as much as the output's own rounding), and lie below 2^-14 only where
 // they are 2^-21 of the largest; FP32 calls take a second fp16 part for what that rounding took.  The scale of the values'
 // page enters the weight as an exponent, p' = 2^(x + ev - ref), ref following the largest x + ev, so that no page's
-// values leave fp16 or FP32, and the weights' sum takes p' 2^-ev.
+// values leave fp16 or FP32, and the weights' sum takes p' 2^-ev.  That holds where the scales of a wave's (a block's) pages
+// are not far apart: with exponents within kCacheSpread a weight counts in the sum unless it is below 2^-96 of the largest.
+// Sums are joined by references that stand for the weights alone: see weighed.
 #pragma once
 #include "cache.hpp"
 #include "cache_index.hpp"
@@ -86,19 +88,44 @@ __device__ inline uint32_t low_bytes(int n) { return n <= 0 ? 0u : n >= 4 ? 0xff
 // is exact and a weight's exponent, x + (ev - ref), is rounded once.
 constexpr float kCacheNoRef = -3.402823466e38f, kCacheRoom = 15.0f, kCacheSet = 7.0f;
 // References from this size on are far: an exponent's rounding is a quarter and more of a step of 2, and soon wider than the room
-// and the values' exponents.  What a wave (a block) has of rows whose reference is far is formed again, behind the others: the
-// reference follows the scores alone, which are rounded before it leaves them, so that none passes the largest one, and the
-// values' exponents are applied to the sums, 16 keys at a time.
+// and the values' exponents.
 constexpr float kCacheFar = 4194304.0f;
-// A far row's score, rounded before anything leaves it, and its weight (NaN stays).
+// How far apart the exponents of the values' scales may lie: keys of equal weights then have 2^-14 and more of fp16, its 11 bits
+// (FP32: 2^-2 and more of two parts, 23 bits).  Beyond, and for rows whose reference is far, what a wave (a block) has is formed again,
+// behind the others.  There each 16 keys of a row, of one page, have a reference of their own, a whole number at or above their
+// largest score; scores are rounded before it leaves them, and the products with the values are shifted to the row's reference,
+// the largest, and by the page's exponent as they are added.  So a weight is off by 2^-11 (FP32: 2^-22) or by 2^-38 of the 16
+// keys' largest, whatever the pages' scales.
+template <class T>
+constexpr int kCacheSpread = sizeof(T) == 2 ? 20 : 8;
+constexpr float kCacheUp = 14.0f;  // such weights are 2^14 at most
+// A score that is rounded before anything leaves it, and its weight (NaN stays).
 __device__ inline float far_score(float score, float by) {
 #pragma clang fp contract(off)
     return score * by;
 }
 __device__ inline float far_weight(float score, float ref) {
 #pragma clang fp contract(off)
-    const float x = score - ref;
-    return __builtin_amdgcn_exp2f(x > kCacheRoom ? kCacheRoom : x);
+    return __builtin_amdgcn_exp2f((score - ref) + kCacheUp);
+}
+// The reference of keys with this largest score.
+__device__ inline float far_reference(float top) { return top > -INFINITY ? ceilf(top) : kCacheNoRef; }
+// x 2^(from - to), for whole numbers from <= to: by an exponent, since the power alone may lie below FP32's numbers.
+__device__ inline int shift_of(float from, float to) { return int(fmaxf(from - to, -1000.0f)); }
+__device__ inline float shifted(float x, int by) { return __builtin_amdgcn_ldexpf(x, by); }
+template <class V>
+__device__ inline V shifted_all(V x, int by) {
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(V) / 4; ++i) x[i] = shifted(x[i], by);
+    return x;
+}
+// Before sums are joined: a row's reference becomes that of its weights' sum, which is then 0.5 to 1 (the sums of products are a mean of
+// values then).  Returns by what its sums are shifted.
+__device__ inline int weighed(float& ref, float& sum) {
+    const int e = __builtin_amdgcn_frexp_expf(sum);  // (0 for 0, infinity and NaN)
+    ref += float(e);
+    sum = shifted(sum, -e);
+    return -e;
 }
 
 // What a page's scores are multiplied by: scale log2 e 2^exponent, kept among FP32's normal values, so that a masked score stays

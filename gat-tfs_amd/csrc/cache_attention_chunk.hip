@@ -105,14 +105,15 @@ struct ChunkLds {
     float scale[2][4][2];  // of each 16 keys: what a score is multiplied by, and the values' exponent; without a page: -1
     uint16_t bad[2][64 * NB][4];  // which of each 16 keys' values are NaN (they stand as 0 in v)
     uint32_t nan[4];       // the values of tile i (of a piece), in place i % 4, hold one
-    uint32_t far;          // some row's reference is
+    uint32_t far;          // some row is formed again
 };
 
 // What a thread requests of a tile, in 16 bytes: of N keys each 16 columns, and of N columns each 16 keys.
 template <int N>
 struct Bytes {
     uint4 k[N], v[N];
-    float ks, vs;  // scales of the 16 keys (of the first threads)
+    float ks;      // what the 16 keys' scores are multiplied by, and their values' exponent (of the first threads)
+    int vs;
     int tokens;    // among the 16 keys of the values
 };
 // What a row crosses its pieces' indices with, of PIECES of them a row: 16 neighbouring lanes then meet the 16 pieces of 256
@@ -138,7 +139,7 @@ struct Piece {
     uint64_t place;  // where the first wave's sums go then
 };
 // One piece: the rows' sums over its tiles, to the output, or where others are to be joined to them.  `far` becomes the lanes of rows
-// whose references are far; FAR: of those, with references that follow the scores alone (kCacheFar), else of all others.
+// that are to be formed again; FAR: of those, with a reference for each 16 keys (kCacheSpread), else of all others.
 template <class T, int NB, int WAVES, bool FAR>
 __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArgs& p, ChunkLds<NB>& lds, const CacheRequest& rq, const Piece& w, uint64_t& far) {
     constexpr int PARTS = QueryParts<T>::N, PIECES = 4 * NB;  // 16-byte pieces of a key's bytes
@@ -167,6 +168,7 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
         k_at[i] = uint32_t(key_byte(a.c, 0, head, k_key + uint32_t(i) * KEYS)) + 16 * k_piece;
         v_at[i] = uint32_t(value_byte(a.c, 0, head, 16 * v_group, v_col + COLS * uint32_t(i)));
     }
+    int low = kMostScale, high = kLeastScale;  // of the exponents of the values' scales
     const auto load_pages = [&](uint32_t tile) {
         Pages<N> g;
         const uint32_t first = tile * kCacheTile, block = first >> a.c.page_log;
@@ -183,7 +185,7 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
         if (tid < 4) {
             const uint64_t place = uint64_t(some_page(a.c, g.v)) * a.c.kv_heads + head;
             x.ks = g.v < a.c.pages ? score_factor(a.scale, a.k_scale[place]) : -1.0f;
-            x.vs = float(scale_exponent(a.v_scale[place]));
+            x.vs = scale_exponent(a.v_scale[place]);
         }
         const uint32_t place = tile * kCacheTile & in_page;
         const uint8_t* const v = a.v + place + some_page(a.c, g.v) * page_bytes;
@@ -201,7 +203,7 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
         const uint32_t buffer = (tile - lo) % 2;
         if (tid < 4) {
             lds.scale[buffer][tid][0] = x.ks;
-            lds.scale[buffer][tid][1] = x.vs;
+            lds.scale[buffer][tid][1] = __int_as_float(x.vs);
         }
         if (x.tokens < 16) {  // values of no token count as 0
 #pragma unroll
@@ -273,14 +275,19 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
         }
         if (tile * kCacheTile < most) {
             // Of the tile's four 16 keys: scales, and whether they have a page.  The same in all lanes.
-            float by[4], ev[4];
+            float by[4];
+            int ev[4];
             uint32_t held = 0;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const uint32_t factor = uniform(__float_as_uint(lds.scale[buffer][g][0]));
                 by[g] = __uint_as_float(factor & 0x7fffffffu);
-                ev[g] = __uint_as_float(uniform(__float_as_uint(lds.scale[buffer][g][1])));
-                if (!(factor >> 31)) held |= 1u << g;
+                ev[g] = int(uniform(__float_as_uint(lds.scale[buffer][g][1])));
+                if (!(factor >> 31)) {
+                    held |= 1u << g;
+                    low = min(low, ev[g]);
+                    high = max(high, ev[g]);
+                }
             }
             f32x16_t s[2];
 #pragma unroll
@@ -320,35 +327,59 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
                         if (!(held >> g & 1) || tile * kCacheTile + uint32_t(16 * g + 8 * h + r % 8) >= seen) s[k][r] = -INFINITY;
                     }
             }
-            float top = -INFINITY;
+            int far_up[4];  // FAR: by what the sums of each 16 keys' weights are shifted
+            float far_ref[4];
+            if constexpr (FAR) {
+                float to = ref;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                float t = s[g / 2][8 * (g % 2)];
+                for (int g = 0; g < 4; ++g) {
+                    float top = -INFINITY;
 #pragma unroll
-                for (int r = 1; r < 8; ++r) t = fmaxf(t, s[g / 2][8 * (g % 2) + r]);
-                top = fmaxf(top, FAR ? far_score(t, by[g]) : fmaf(t, by[g], ev[g]));
-            }
-            if (__any(top > ref + kCacheRoom)) {
-                const float both = xor32_max(top);
-                const bool up = both > ref + kCacheRoom;
-                const float to = up ? ceilf(both) - kCacheSet : ref, less = up ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
+                    for (int r = 0; r < 8; ++r) {
+                        const float x = far_score(s[g / 2][8 * (g % 2) + r], by[g]);
+                        s[g / 2][8 * (g % 2) + r] = x;
+                        top = fmaxf(top, x);
+                    }
+                    far_ref[g] = far_reference(xor32_max(top));
+                    to = fmaxf(to, far_ref[g]);
+                }
+                const int less = shift_of(ref, to);
                 ref = to;
-                // (FAR: all of the other pass's, whose references have up to 64 of the values' exponents in them)
-                far |= __ballot(up && fabsf(to) >= (FAR ? kCacheFar - 256.0f : kCacheFar));
-                sum *= less;
+                sum = shifted(sum, less);
 #pragma unroll
-                for (int d = 0; d < 2 * NB; ++d)
+                for (int d = 0; d < 2 * NB; ++d) o[d] = shifted_all(o[d], less);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) o[d][r] *= less;
+                for (int g = 0; g < 4; ++g) far_up[g] = shift_of(far_ref[g], ref) - int(kCacheUp);
+            } else {
+                float top = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float t = s[g / 2][8 * (g % 2)];
+#pragma unroll
+                    for (int r = 1; r < 8; ++r) t = fmaxf(t, s[g / 2][8 * (g % 2) + r]);
+                    top = fmaxf(top, fmaf(t, by[g], float(ev[g])));
+                }
+                if (__any(top > ref + kCacheRoom)) {
+                    const float both = xor32_max(top);
+                    const bool up = both > ref + kCacheRoom;
+                    const float to = up ? ceilf(both) - kCacheSet : ref, less = up ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
+                    ref = to;
+                    far |= __ballot(up && fabsf(to) >= kCacheFar);
+                    sum *= less;
+#pragma unroll
+                    for (int d = 0; d < 2 * NB; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[d][r] *= less;
+                }
             }
             uint4 w[4], rest[4];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float shift = ev[g] - ref;  // (whole numbers: exact)
+                const float shift = float(ev[g]) - ref;  // (whole numbers: exact)
                 float x[8], of = 0.0f;
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
-                    if constexpr (FAR) x[r] = far_weight(far_score(s[g / 2][8 * (g % 2) + r], by[g]), ref);
+                    if constexpr (FAR) x[r] = far_weight(s[g / 2][8 * (g % 2) + r], far_ref[g]);
                     else x[r] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + r], by[g], shift));
                     of += x[r];
                 }
@@ -361,7 +392,7 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
                         l[j] = f16x2(x[2 * j] - float(up[0]), x[2 * j + 1] - float(up[1]));
                     }
                 }
-                sum = FAR ? sum + of : fmaf(of, power_of_two(-int(ev[g])), sum);
+                sum = FAR ? sum + shifted(of, far_up[g]) : fmaf(of, power_of_two(-ev[g]), sum);
                 w[g] = make_uint4(u[0], u[1], u[2], u[3]);
                 if constexpr (PARTS > 1) rest[g] = make_uint4(l[0], l[1], l[2], l[3]);
             }
@@ -401,7 +432,7 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
 #pragma unroll
                         for (int r = 0; r < 16; ++r) t[r] = 0.0f;
                         if constexpr (PARTS > 1) t = mfma32_f16(values[g % 2][d], rest[g], t);
-                        o[d] += mfma32_f16(values[g % 2][d], w[g], t) * power_of_two(int(ev[g]));
+                        o[d] += shifted_all(mfma32_f16(values[g % 2][d], w[g], t), far_up[g] + ev[g]);
                     }
                     continue;
                 }
@@ -415,15 +446,17 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
         __syncthreads();
     }
     sum = xor32_add(sum);
+    if (!FAR && high - low > kCacheSpread<T>) far = ~uint64_t(0);
     // A lane's row; both halves of a row are of one mind.
     if ((far >> lane & 1) != uint64_t(FAR)) return;
+    const int shift = w.cut ? weighed(ref, sum) : 0;
     const uint64_t piece = w.place + uint64_t(wave);
 #pragma unroll
     for (int d = 0; d < 2 * NB; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const f32x4_t x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-            if (w.cut) *reinterpret_cast<f32x4_t*>(a.part + ((piece * (8 * NB) + uint64_t(4 * d + i)) * kWave + uint64_t(lane)) * 4) = x;
+            if (w.cut) *reinterpret_cast<f32x4_t*>(a.part + ((piece * (8 * NB) + uint64_t(4 * d + i)) * kWave + uint64_t(lane)) * 4) = shifted_all(x, shift);
             else store4<T>(a, rq, packed, head, uint32_t(32 * d + 8 * i + 4 * h), x, sum);
         }
     if (lane < 32) {
@@ -477,10 +510,7 @@ __global__ __launch_bounds__(WAVES * kWave, sizeof(T) == 2 ? 2 : 1) void k_cache
         chunk_piece<T, NB, WAVES, false>(p, lds, rq, w, far);
         if (far) lds.far = 1;  // (every writer writes the same)
         __syncthreads();
-        if (lds.far) {
-            far = 0;
-            chunk_piece<T, NB, WAVES, true>(p, lds, rq, w, far);
-        }
+        if (lds.far) chunk_piece<T, NB, WAVES, true>(p, lds, rq, w, far);
         if (lo == 0 && hi < all) meta = make_uint4(request, row_tile, uint32_t((next_base - 1) / share) - worker + 1, 0);
         at += hi - lo;
         __syncthreads();
@@ -502,9 +532,10 @@ __global__ __launch_bounds__(WAVES * kWave) void k_cache_chunk_join(const ChunkA
         const uint64_t piece = ((uint64_t(blockIdx.x) + uint64_t(i) * a.c.kv_heads) * 2 + (i ? 0 : 1)) * WAVES + uint64_t(wave);
         const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part + ((piece * (8 * NB) + which) * kWave + uint64_t(lane)) * 4);
         const float r = a.stat[piece * 64 + uint64_t(n)], s = a.stat[piece * 64 + 32 + uint64_t(n)];
-        const float top = fmaxf(ref, r), less = __builtin_amdgcn_exp2f(ref - top), more = __builtin_amdgcn_exp2f(r - top);
-        o = o * less + x * more;
-        sum = sum * less + s * more;
+        const float top = fmaxf(ref, r);
+        const int less = shift_of(ref, top), more = shift_of(r, top);
+        o = shifted_all(o, less) + shifted_all(x, more);
+        sum = shifted(sum, less) + shifted(s, more);
         ref = top;
     }
     const CacheRequest rq = request_of(a, meta.x);
