@@ -26,6 +26,9 @@ namespace gatgpu {
 namespace {
 
 constexpr int kBlock = 256;
+// A vector whose mean square (with eps) lies beyond these is multiplied by a power of two and its squares are formed again, so
+// that they stay among FP32's normal numbers: n is the same, and dx's factor takes the power.
+constexpr float kLeastSquare = 0x1p-100f, kMostSquare = 0x1p120f, kEnlarge = 0x1p96f, kReduce = 0x1p-80f;
 
 struct RotateArgs {
     uint64_t rows = 0;
@@ -95,7 +98,7 @@ __device__ inline float group_sum(float x) {
     if (TPV > 32) x = xor32_add(x);
     return x;
 }
-// 1 / sqrt(x): the hardware's, and one step of Newton's method on it.
+// 1 / sqrt(x), x among FP32's normal numbers: the hardware's, and one step of Newton's method on it.
 __device__ inline float inverse_root(float x) {
     const float r = __builtin_amdgcn_rsqf(x), h = 0.5f * x * r;
     return x < INFINITY ? fmaf(r, fmaf(-h, r, 0.5f), r) : r;
@@ -300,16 +303,31 @@ __global__ __launch_bounds__(kBlock, BACK ? 3 : 4) void k_rotate(const RotateArg
                 load_factors<T, BACK, PAIRS>(a, gamma + now.which * a.dim, turn + buffer * angles + mine * a.half, col, f);
                 held = now.which;
             }
-            const Chunk<T> own = widen<T>(raw.own);
-            Chunk<T> other{}, out;
+            Chunk<T> own = widen<T>(raw.own), other{}, out;
             if (there) other = partners<T, PAIRS>(a, now, own, raw.other, col);
-            float r = 1.0f;
-            const Chunk<T> in = BACK ? widen<T>(raw.n) : own;
+            float r = 1.0f, up = 1.0f;
+            Chunk<T> in = BACK ? widen<T>(raw.n) : own;
             if (a.norm) {
-                float sq = 0.0f;
+                const auto mean_square = [&](float eps) {
+                    float sq = 0.0f;
 #pragma unroll
-                for (int j = 0; j < N; ++j) sq = fmaf(in.x[j], in.x[j], sq);
-                r = inverse_root(fmaf(group_sum<TPV>(sq), per, a.eps));
+                    for (int j = 0; j < N; ++j) sq = fmaf(in.x[j], in.x[j], sq);
+                    return fmaf(group_sum<TPV>(sq), per, eps);
+                };
+                float mean = mean_square(a.eps);
+                if (!(mean >= kLeastSquare && mean <= kMostSquare)) {  // (all lanes of the vector)
+                    up = mean < 1.0f ? kEnlarge : kReduce;
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        in.x[j] *= up;
+                        if (!BACK) {
+                            own.x[j] *= up;
+                            other.x[j] *= up;
+                        }
+                    }
+                    mean = mean_square(a.eps * up * up);
+                }
+                r = inverse_root(mean);
             }
 #pragma unroll
             for (int j = 0; j < N; ++j) {
@@ -332,6 +350,10 @@ __global__ __launch_bounds__(kBlock, BACK ? 3 : 4) void k_rotate(const RotateArg
                     dot = group_sum<TPV>(dot) * per;
 #pragma unroll
                     for (int j = 0; j < N; ++j) out.x[j] = r * fmaf(-n.x[j], dot, out.x[j]);
+                    if (up != 1.0f) {
+#pragma unroll
+                        for (int j = 0; j < N; ++j) out.x[j] *= up;
+                    }
                 }
             }
             if (there) store_chunk(now.to + col, out);
