@@ -151,6 +151,12 @@ __device__ inline void store_lse(const CacheAttnArgs& a, const CacheRequest& rq,
     a.lse[uint64_t(rq.begin + i) * a.c.heads + h] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
 }
 
+// A value's first part before it is rounded to bf16, which is to stay finite, and what a part leaves of it: of an infinity or NaN nothing.
+__device__ inline float first_part(float x) {
+    constexpr float most = 3.38953139e38f;  // bf16's largest number
+    return fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(x, -most, most) : x;
+}
+__device__ inline float rest_of(float x, float part) { return fabsf(x) < INFINITY ? x - part : 0.0f; }
 // Eight values of a query row from `col` on, as PARTS bf16 operands (FP32: three, which hold all its bits).
 template <class T>
 struct QueryParts {
@@ -173,9 +179,9 @@ __device__ inline QueryParts<T> load_query8(const T* row, uint32_t col, bool the
             uint32_t p[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                p[j] = bf16x2(x[2 * j], x[2 * j + 1]);
-                x[2 * j] -= __uint_as_float(p[j] << 16);
-                x[2 * j + 1] -= __uint_as_float(p[j] & 0xffff0000u);
+                p[j] = k ? bf16x2(x[2 * j], x[2 * j + 1]) : bf16x2(first_part(x[2 * j]), first_part(x[2 * j + 1]));
+                x[2 * j] = rest_of(x[2 * j], __uint_as_float(p[j] << 16));
+                x[2 * j + 1] = rest_of(x[2 * j + 1], __uint_as_float(p[j] & 0xffff0000u));
             }
             q.w[k] = make_uint4(p[0], p[1], p[2], p[3]);
         }
