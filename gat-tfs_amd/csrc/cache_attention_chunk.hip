@@ -171,13 +171,14 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
     int low = kMostScale, high = kLeastScale;  // of the exponents of the values' scales
     const auto load_pages = [&](uint32_t tile) {
         Pages<N> g;
-        const uint32_t first = tile * kCacheTile, block = first >> a.c.page_log;
+        const uint32_t first = tile * kCacheTile;
+        const auto page_of = [&](uint32_t key) {
+            const uint32_t block = block_of(a.c, rq.keys, key);
+            return block == kNoPage ? block : table[block];
+        };
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t key = (k_key + uint32_t(i) * KEYS) / 16 * 16;
-            g.k[i] = first + key < rq.keys ? table[block + (key >> a.c.page_log)] : kNoPage;
-        }
-        g.v = first + 16 * v_group < rq.keys ? table[block + (16 * v_group >> a.c.page_log)] : kNoPage;
+        for (int i = 0; i < N; ++i) g.k[i] = page_of(first + (k_key + uint32_t(i) * KEYS) / 16 * 16);
+        g.v = page_of(first + 16 * v_group);
         return g;
     };
     const auto load_bytes = [&](uint32_t tile, const Pages<N>& g) {
