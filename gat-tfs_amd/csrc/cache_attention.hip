@@ -428,7 +428,7 @@ __global__ __launch_bounds__((ALONE ? kAloneWaves : kWaves) * kWave, 2) void k_c
         run.sum = 0.0f;
         run.far = 0;
         run.first = kNoExponent;
-        const uint32_t stop = min(hi, (most + kCacheTile - 1) / kCacheTile);
+        const uint32_t stop = most ? min(hi, (most - 1) / kCacheTile + 1) : 0;
         uint32_t tile = lo + member;
         if (tile < stop) {
             // A tile's keys are requested when the scores of the one before are formed, its values when those are added.
@@ -443,7 +443,7 @@ __global__ __launch_bounds__((ALONE ? kAloneWaves : kWaves) * kWave, 2) void k_c
                 __builtin_amdgcn_sched_barrier(0);
                 const uint32_t next = tile + per;
                 if (next < stop) load_keys<NB>(a, pages.load, next, head, lane, k);
-                const bool whole = tile * kCacheTile + kCacheTile <= least && __all(v.page);  // every row sees every key
+                const bool whole = tile < least / kCacheTile && __all(v.page);  // every row sees every key
                 const Weights w = weigh<T, NB>(a, run, x, v, tile, seen, whole, lane);
                 if (!whole) clean<NB>(run, v, tile, rq.keys, seen, lane);
                 add_values<PARTS, NB>(run, w, v);

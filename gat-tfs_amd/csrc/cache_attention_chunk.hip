@@ -215,7 +215,7 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
                 x.v[i].w &= low_bytes(x.tokens - 12);
             }
         }
-        if ((tile + 1) * kCacheTile > all_seen) {  // some rows do not see all of it: its NaNs stand as 0, and are marked
+        if (tile >= all_seen / kCacheTile) {  // some rows do not see all of it: its NaNs stand as 0, and are marked
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 uint4& v = x.v[i];
@@ -318,7 +318,7 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
             };
             if (!FAR) read_values(0);
             __builtin_amdgcn_sched_barrier(0);
-            const bool whole = (tile + 1) * kCacheTile <= least && held == 15;
+            const bool whole = tile < least / kCacheTile && held == 15;
             if (!whole) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
@@ -397,7 +397,7 @@ __device__ inline __attribute__((always_inline)) void chunk_piece(const ChunkArg
                 w[g] = make_uint4(u[0], u[1], u[2], u[3]);
                 if constexpr (PARTS > 1) rest[g] = make_uint4(l[0], l[1], l[2], l[3]);
             }
-            if ((tile + 1) * kCacheTile > all_seen && lds.nan[(tile - lo) % 4]) {  // NaNs mark the rows that see them
+            if (tile >= all_seen / kCacheTile && lds.nan[(tile - lo) % 4]) {  // NaNs mark the rows that see them
 #pragma unroll
                 for (int d = 0; d < 2 * NB; ++d)
 #pragma unroll 1
