@@ -8,7 +8,7 @@
 // rows from LDS; else a second launch finds each row's request by bisection.  A new block's page is taken from the
 // list by each of its rows, so that no row waits for the table; the row at offset 0 writes it there.
 //
-// A step of 12 requests: 4.7 us.  2500 prompts of 471 thousand rows: sums 6.3 us, rows 5.8; 300 requests that end 2.3 + 3.6.
+// A step of 12 requests: 5.0 us.  2500 prompts of 471 thousand rows: sums 6.9 us, rows 5.6; 300 requests that end 2.5 + 3.5.
 #include <algorithm>
 #include <string>
 

@@ -8,7 +8,7 @@
 // them from there (what registers do not hold, beyond 16 KB of each, is read again).  Values are turned in LDS,
 // since a page holds them by column: the attention's second product then takes its operands straight from memory.
 //
-// 24 prompts of 54 thousand tokens, 8 heads of 128, bf16: 77 us, 4.3 TB/s; 96 requests of one token 5.8 us, a launch and a chain
+// 24 prompts of 54 thousand tokens, 8 heads of 128, bf16: 77 us, 4.3 TB/s; 96 requests of one token 6.1 us, a launch and a chain
 // of reads (slots, scale, row), then a byte of a line for each of a value's columns.
 #include <algorithm>
 #include <string>
@@ -425,7 +425,7 @@ extern "C" int gatgpu_cache_append(gatgpu_ctx* c, const gatgpu_cache* cache, con
     if (int r = check_cache(c, cache, true)) return r;
     if (!io) return fail(c, GATGPU_EINVAL, "null arrays");
     if (io->precision != GATGPU_FP32 && io->precision != GATGPU_BF16) return fail(c, GATGPU_EINVAL, "bad precision");
-    if (io->rows >= (uint64_t(1) << 27)) return fail(c, GATGPU_EOVERFLOW, "more than 2^27 - 1 rows");  // (of a launch: 16 threads a row)
+    if (io->rows >= (uint64_t(1) << 27)) return fail(c, GATGPU_EOVERFLOW, "more than 2^27 - 1 rows");  // (2^21 blocks: a block takes 64 of so many rows)
     if (!io->rows) return GATGPU_OK;
     if (int r = check_rows(c, cache, io, "k", io->k, io->k_stride)) return r;
     if (int r = check_rows(c, cache, io, "v", io->v, io->v_stride)) return r;

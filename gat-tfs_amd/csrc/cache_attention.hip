@@ -7,8 +7,8 @@
 // and join their sums in LDS.  What is cut between blocks leaves partial sums, which a second launch joins in the order of
 // the keys.  Where tables are short, a block takes a row tile alone, and there is nothing to join.
 //
-// One token over 260001 keys, 32 heads on 8 of 128 columns, bf16 rows: 96 us, 5.5 TB/s, and 6.4 for the join; 48 tokens
-// over 200 to 24000 keys: 77 us, 4.3 TB/s, and 5.5.
+// One token over 260001 keys, 32 heads on 8 of 128 columns, bf16 rows: 97 us, 5.5 TB/s, and 6.7 for the join; 48 tokens
+// over 200 to 24000 keys: 80 us, 4.2 TB/s, and 5.7.
 #include <algorithm>
 #include <cmath>
 #include <string>

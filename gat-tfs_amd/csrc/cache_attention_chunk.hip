@@ -12,8 +12,9 @@
 // device only: a first launch of one block forms the sums over the tiles, and a last one joins the tiles that a range's end
 // cuts.  Where tables are short, a block takes a row tile alone, in one launch.
 //
-// 6 requests of 324 to 1649 rows over up to 10392 keys, 16 heads on 4 of 128 columns, bf16: 259 us, 658 TFLOP/s (vector
-// instructions 48 % of the cycles, matrix pipes 35 %, one behind the other in a wave), sums 4.9, join 17.8.
+// 6 requests of 324 to 1649 rows over up to 10392 keys, 16 heads on 4 of 128 columns, bf16: 252 to 260 us, 656 to
+// 676 TFLOP/s, the whole call; under a profiler the kernel alone 261 to 275 (vector instructions 47 % of the cycles, matrix pipes
+// 35 %, one behind the other in a wave), sums 5.2, join 18.
 #include <algorithm>
 #include <type_traits>
 

@@ -5,14 +5,13 @@
 //   dt_i = dy_i c_i - dy_p s_i,  dgamma = sum dt n,  g = dt gamma,  dx = r (g - n mean(g n))
 //
 // Bound by bytes: a head's vector is read once into TPV lanes of 16 bytes each, and written once.  The other column of
-// a pair half a rotation away comes by a second read of the same lines, which the first has just brought (a lane
-// exchange would take one LDS permute an element).  A row's angles are formed once a block, a thread an angle, in 64
+// a pair half a rotation away comes by a second read of the same lines, which the first has just brought.  A row's angles are formed once a block, a thread an angle, in 64
 // bits: position * freq in turns, of which the whole ones go before what is left is rounded to 32 bits, so that far
 // positions keep an angle's error of 2^-23.  Groups of lanes then take the row's heads in turn with their columns' sines
 // in registers.  The backward pass gives each block a fixed set of rows and keeps its columns' sums for gamma in
 // registers over them; blocks leave one partial row each, added in one fixed order.
 //
-// 20011 rows of 20 heads of 128, bf16: forward 42 us, 4.9 TB/s of the 2 rows, backward 79 us, 3.9 TB/s of 3, the partial
+// 20011 rows of 20 heads of 128, bf16: forward 42 us, 4.9 TB/s of the 2 rows, backward 80 us, 3.9 TB/s of 3, the partial
 // rows' sums 4.6.  7 rows of 16 heads of 64: 3.7 us, a launch.
 #include <algorithm>
 #include <cmath>

@@ -469,8 +469,10 @@ int gatgpu_set_norm(gatgpu_ctx* ctx, int layer, const float* gamma, const float*
  *       position freq[i]:  y_a = t_a cos - t_b sin,  y_b = t_b cos + t_a sin
  * and the gradients of x and gamma.  GATGPU_PAIRS_HALVES: pair i is the columns
  * (i, i + rot / 2); GATGPU_PAIRS_NEIGHBOURS: (2 i, 2 i + 1).  Angles are formed in
- * 64 bits, so positions may be far; sums are FP32, y and the gradients are rounded
- * once.  A NaN or infinity stays in its own row and head.
+ * 64 bits, so positions may be far; their sines and cosines (times gamma in a forward
+ * call), products and sums are FP32, y and the gradients are rounded once.  Squares
+ * that would leave FP32 are formed of x times a power of two.  A NaN or infinity stays
+ * in its own row and head, as does the NaN of a vector of zeros with eps 0.
  * Device arrays: rows of `heads` (kv_heads) vectors of dim elements side by side,
  * strides in elements, 16-byte aligned like the bases.  q_out may be q, k_out k, and
  * dq dq_out, dk dk_out (same strides); else what a call writes shares no memory with
@@ -604,9 +606,11 @@ int gatgpu_cache_append(gatgpu_ctx* ctx, const gatgpu_cache* cache, const gatgpu
  * row's output.  Rows of no request are neither read nor written; of a request's rows
  * those beyond the first `most` are not computed.  k_len beyond blocks * page counts
  * as that, q_begin beyond rows as rows.
- * GATGPU_BF16: q and out bf16; GATGPU_FP32: both FP32, products of FP32's precision.
- * Scores, softmax state and sums are FP32.  Sums run in one fixed order: equal inputs
- * give equal bits. */
+ * GATGPU_BF16: q and out bf16; GATGPU_FP32: both FP32.  Scores, softmax state and sums
+ * are FP32; so is the weights' sum, and lse.  Where weights meet the values they are
+ * fp16: one is off by at most 2^-11 of it (FP32 calls, in two parts: 2^-22), or its
+ * product with its page's scale by 2^-31 of the largest such product of the row,
+ * whichever is more.  Sums run in one fixed order: equal inputs give equal bits. */
 typedef struct gatgpu_cache_attention_io {
     int precision;
     int heads;             /* a multiple of kv_heads, at most 64                 */
